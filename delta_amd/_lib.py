@@ -35,6 +35,15 @@ class BudgetRuleC(ctypes.Structure):
 
 
 _BR = ctypes.POINTER(BudgetRuleC)
+
+
+class SharedPrefixC(ctypes.Structure):
+    """``delta_shared_prefix_t``: each row's prefix and the prefixes' page CSR."""
+    _fields_ = [("row_prefix", c_void_p), ("indptr", c_void_p), ("indices", c_void_p), ("indices_len", c_int64),
+                ("num_prefixes", c_int)]
+
+
+_SP = ctypes.POINTER(SharedPrefixC)
 # name -> (restype, argtypes); one entry per function declared in include/delta_hip.h
 SIGNATURES = {
     "delta_last_error": (ctypes.c_char_p, []),
@@ -117,6 +126,15 @@ SIGNATURES = {
     "delta_rope_append": (c_int, [
         _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, c_int64, _P, _P,
         c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_int, c_float, c_float, c_float, _P]),
+    "delta_prefix_attention_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int64]),
+    "delta_paged_decode_prefix": (c_int, [
+        _SP, _P, c_int64, c_int64, _P, c_int64, _P, _P, c_int64, _P, _P, c_int64, c_int64, _P,
+        c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, c_size_t, _P]),
+    "delta_paged_prefill_prefix": (c_int, [
+        _SP, _P, c_int64, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int64, _P,
+        c_int, c_int64, c_int, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
+    "delta_copy_pages": (c_int, [
+        ctypes.POINTER(_P), c_int, c_int64, c_int, c_int, c_int, _P, _P, _P, c_int64, _P]),
 }
 
 _lib = None

@@ -370,6 +370,133 @@ def paged_prefill(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tens
     return out
 
 
+def prefix_attention_workspace_bytes(tokens: int, hq: int, hkv: int, max_pages: int) -> int:
+    """Bytes of workspace of ``paged_decode_prefix`` (``tokens`` = rows, ``max_pages`` = its ``max_pages_per_row``)
+    and ``paged_prefill_prefix`` (``tokens`` = query tokens, ``max_pages`` = entries of ``kv_indices``)."""
+    return int(_lib.query("delta_prefix_attention_workspace_bytes", int(tokens), int(hq), int(hkv), int(max_pages)))
+
+
+def _prefix_struct(row_prefix: torch.Tensor, indptr: torch.Tensor, indices: torch.Tensor, B: int):
+    _check_i32("row_prefix", row_prefix, B)
+    _check_i32("prefix_indptr", indptr, 1)
+    _check_i32("prefix_indices", indices)
+    return _lib.SharedPrefixC(row_prefix.data_ptr(), indptr.data_ptr(), indices.data_ptr(), indices.numel(),
+                              indptr.numel() - 1)
+
+
+def _prefix_outputs(q: torch.Tensor, hq: int, out: Optional[torch.Tensor], lse: Optional[torch.Tensor]):
+    if out is None:
+        out = torch.empty_like(q)
+    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out must match q's shape/dtype with unit inner stride")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], hq)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous fp32 [{q.shape[0]}, {hq}]")
+    return out
+
+
+def _prefix_workspace(workspace: Optional[torch.Tensor], need: int, dev: torch.device) -> torch.Tensor:
+    if workspace is None:  # of this call: safe on any stream, in any capture
+        return torch.empty(need, dtype=torch.uint8, device=dev)
+    if workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace too small: {need} bytes needed")
+    return workspace
+
+
+def paged_decode_prefix(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                        kv_last_page_len: torch.Tensor, row_prefix: torch.Tensor, prefix_indptr: torch.Tensor,
+                        prefix_indices: torch.Tensor, *, max_pages_per_row: int, sm_scale: Optional[float] = None,
+                        out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                        workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_decode`` for a batch whose rows share prefixes (``delta_paged_decode_prefix``): each prefix's pages
+    are read once for all its rows.
+
+    ``row_prefix`` (int32 [B]) names each row's prefix, -1 for none; prefix p's full pages are
+    ``prefix_indices[prefix_indptr[p]:prefix_indptr[p + 1]]``, and the rows' CSR lists them too, first.  A row that
+    its prefix does not fit in attends its own CSR alone.  At most 1024 rows and prefixes."""
+    dev = _check_cuda(q, kv_cache, kv_indptr, kv_indices, kv_last_page_len, row_prefix, prefix_indptr, prefix_indices,
+                      out, lse, workspace)
+    _check_cache(kv_cache)
+    hq, hkv = _check_heads(q, kv_cache)
+    B = q.shape[0]
+    _check_i32("kv_indptr", kv_indptr, B + 1)
+    _check_i32("kv_indices", kv_indices)
+    _check_i32("kv_last_page_len", kv_last_page_len, B)
+    px = _prefix_struct(row_prefix, prefix_indptr, prefix_indices, B)
+    out = _prefix_outputs(q, hq, out, lse)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(HEAD_DIM)
+    workspace = _prefix_workspace(workspace, prefix_attention_workspace_bytes(B, hq, hkv, max_pages_per_row), dev)
+    _lib.call("delta_paged_decode_prefix", ctypes.byref(px), q.data_ptr(), q.stride(0), q.stride(1),
+              kv_cache.data_ptr(), kv_cache.shape[0], kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
+              kv_last_page_len.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), B, hq, hkv,
+              HEAD_DIM, _dtype_code(q), float(sm_scale), int(max_pages_per_row), workspace.data_ptr(),
+              workspace.numel() * workspace.element_size(), _stream(dev))
+    return out
+
+
+def paged_prefill_prefix(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor,
+                         kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, row_prefix: torch.Tensor,
+                         prefix_indptr: torch.Tensor, prefix_indices: torch.Tensor, *, max_qo_len: int,
+                         sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                         lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_prefill`` for prompts that continue shared prefixes (``delta_paged_prefill_prefix``); q/out
+    [nnz, Hq, 128], the prefixes as in ``paged_decode_prefix``.
+
+    A row's prefix applies where it ends before the row's query tokens.  ``max_qo_len`` is the longest row's count of
+    them, as for ``paged_prefill``.  ``out`` and ``lse`` of tokens behind the last row are left as they were."""
+    dev = _check_cuda(q, kv_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, row_prefix, prefix_indptr,
+                      prefix_indices, out, lse, workspace)
+    _check_cache(kv_cache)
+    hq, hkv = _check_heads(q, kv_cache)
+    B = qo_indptr.numel() - 1
+    _check_i32("qo_indptr", qo_indptr, 1)
+    _check_i32("kv_indptr", kv_indptr, B + 1)
+    _check_i32("kv_indices", kv_indices)
+    _check_i32("kv_last_page_len", kv_last_page_len, B)
+    px = _prefix_struct(row_prefix, prefix_indptr, prefix_indices, B)
+    out = _prefix_outputs(q, hq, out, lse)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(HEAD_DIM)
+    need = prefix_attention_workspace_bytes(q.shape[0], hq, hkv, kv_indices.numel())
+    workspace = _prefix_workspace(workspace, need, dev)
+    _lib.call("delta_paged_prefill_prefix", ctypes.byref(px), q.data_ptr(), q.stride(0), q.stride(1),
+              kv_cache.data_ptr(), kv_cache.shape[0], qo_indptr.data_ptr(), kv_indptr.data_ptr(),
+              kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), out.data_ptr(), out.stride(0),
+              out.stride(1), _ptr(lse), B, q.shape[0], hq, hkv, HEAD_DIM, _dtype_code(q), float(sm_scale),
+              workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(dev))
+    return out
+
+
+def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, *,
+               tokens: Optional[torch.Tensor] = None) -> None:
+    """Copy pages in place inside each of ``caches`` (one per layer, one shape) in one launch (``delta_copy_pages``):
+    entry i copies the first ``tokens[i]`` tokens (all 16 without ``tokens``) of page ``src[i]`` to page ``dst[i]``.
+
+    Entries run in no order: a ``dst`` may not be listed twice nor be another entry's ``src``; a ``src`` may be listed
+    any number of times.  An entry with a page id outside the caches copies nothing."""
+    if len(caches) == 0:
+        raise ValueError("no caches")
+    first = caches[0]
+    dev = _check_cuda(src, dst, tokens, *caches)
+    for c in caches:
+        _check_cache(c)
+        if c.shape != first.shape or c.dtype != first.dtype:
+            raise ValueError("the caches must share a shape and a dtype")
+    n = src.numel()
+    _check_i32("src", src)
+    _check_i32("dst", dst)
+    if dst.numel() != n:
+        raise ValueError(f"src names {n} pages, dst {dst.numel()}")
+    if tokens is not None:
+        _check_i32("tokens", tokens)
+        if tokens.numel() != n:
+            raise ValueError(f"src names {n} pages, tokens {tokens.numel()}")
+    ptrs = (ctypes.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
+    _lib.call("delta_copy_pages", ptrs, len(caches), first.shape[0], first.shape[3], HEAD_DIM, _dtype_code(first),
+              src.data_ptr(), dst.data_ptr(), _ptr(tokens), n, _stream(dev))
+
+
 def page_scores_from_logits(logits_dump: torch.Tensor, kv_indptr: torch.Tensor,
                             kv_last_page_len: torch.Tensor, max_pages: int, *,
                             lse: Optional[torch.Tensor] = None,

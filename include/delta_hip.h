@@ -527,6 +527,71 @@ int delta_gemm_rows128(const void *x, int64_t ldx, const void *w, int64_t ldw, c
 int delta_gemm_rows128_silu(const void *x, int64_t ldx, const void *w13, int64_t ldw, void *out, int64_t ldo,
                             int M, int inter, int K, int dtype, delta_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Rows that share a prefix                                                   */
+/* ------------------------------------------------------------------------ */
+
+/* Prefixes that several rows of a batch share.  Prefix p (0 <= p < num_prefixes <= 1024)
+ * holds the pages indices[indptr[p] .. indptr[p + 1]), all full.  A row with
+ * row_prefix[b] = p lists those same pages first in its own CSR (which stays the row's
+ * whole context, so every other entry point reads the same tables); any other value of
+ * row_prefix[b] means no prefix. */
+typedef struct {
+  const int32_t *row_prefix; /* [batch] */
+  const int32_t *indptr;     /* [num_prefixes + 1]; may be NULL with num_prefixes = 0 */
+  const int32_t *indices;    /* [indices_len]; may be NULL with indices_len = 0 */
+  int64_t indices_len;
+  int num_prefixes;
+} delta_shared_prefix_t;
+
+/* Bytes of workspace of the two calls below: `tokens` query tokens (decode: batch),
+ * `max_pages` = the decode call's max_pages_per_row, or the prompt call's kv_indices_len
+ * (no initial contents needed; calls that share a workspace must not overlap).  Grows with
+ * neither argument beyond what 512 blocks write: about 70 MB, or two partials (1040 bytes)
+ * per (query token, q head) where that is more. */
+size_t delta_prefix_attention_workspace_bytes(int64_t tokens, int num_qo_heads, int num_kv_heads,
+                                              int64_t max_pages);
+
+/* delta_paged_decode for a batch whose rows share prefixes: the same o and lse (to
+ * rounding: the softmax is summed in another order), with each prefix's K and V read once
+ * for all its rows instead of once per row.  Row b's prefix applies where its pages fit in
+ * the row (16 * pages <= kv_len_b); a row it does not fit attends its own CSR alone.
+ * batch <= 1024.  No counterpart in the reference. */
+int delta_paged_decode_prefix(const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_b,
+                              int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+                              const int32_t *kv_indptr, const int32_t *kv_indices,
+                              int64_t kv_indices_len, const int32_t *kv_last_page_len,
+                              void *o, int64_t o_stride_b, int64_t o_stride_h, float *lse,
+                              int batch, int num_qo_heads, int num_kv_heads, int head_dim,
+                              int dtype, float sm_scale, int max_pages_per_row,
+                              void *workspace, size_t workspace_bytes, delta_stream_t stream);
+
+/* delta_paged_prefill for prompts that continue shared prefixes: num_tokens query tokens in
+ * rows of qo_indptr, causal.  A row's prefix applies where it lies in front of the row's
+ * query tokens (16 * pages <= kv_len_b - qo_len_b).  o and lse of tokens behind the last
+ * row are left as they were.  batch <= 1024. */
+int delta_paged_prefill_prefix(const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_t,
+                               int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+                               const int32_t *qo_indptr, const int32_t *kv_indptr,
+                               const int32_t *kv_indices, int64_t kv_indices_len,
+                               const int32_t *kv_last_page_len, void *o, int64_t o_stride_t,
+                               int64_t o_stride_h, float *lse, int batch, int64_t num_tokens,
+                               int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
+                               float sm_scale, void *workspace, size_t workspace_bytes,
+                               delta_stream_t stream);
+
+/* Copies pages inside each of num_caches paged caches of one shape (`caches`: a HOST array
+ * of device pointers, one per layer): entry i copies the first tokens[i] tokens (clamped to
+ * [0, 16]; tokens NULL: all 16) of K and V from page src[i] to page dst[i]; the rest of
+ * page dst[i] keeps its contents.  What a sequence forked in the middle of a page needs
+ * (its full pages are shared, the page it goes on filling is copied), or pages that move.
+ * Entries run in no order: a dst may not be listed twice nor be another entry's src (a src
+ * may be listed any number of times).  An entry with a page id outside the caches, or with
+ * src = dst, copies nothing.  num_copies <= 2^23. */
+int delta_copy_pages(void *const *caches, int num_caches, int64_t num_pages, int num_kv_heads,
+                     int head_dim, int dtype, const int32_t *src, const int32_t *dst,
+                     const int32_t *tokens, int64_t num_copies, delta_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
