@@ -9,19 +9,22 @@
 // so a row's softmax splits into its prefix and its own tokens, and each of these into any runs of pages.
 //
 // Work decomposition.  A segment is a prefix with the query tokens of all rows that use it (no mask: all of
-// them come after it), or a row's own pages with its query tokens (causal).  Its (query token, q head of the
-// kv head's G) pairs are cut into tiles of 128, its pages into runs of `chunk` steps of 64 tokens; a block of
-// 4 waves takes one (kv head, segment, tile, run) and writes un-normalised partials (m, l, a), which the
-// merge kernel joins per (token, q head).  The rows' lengths are only on the device, so every block derives
-// the same plan from the tables (plan_unit): it counts the steps of all segments, sets the runs so that
-// they fill the chip's block slots about once, and finds its own unit.
+// them come after it), or a row's own pages with its query tokens (causal).  Its query tokens are cut into
+// tiles of up to 128 (token, q head of the kv head's G) pairs, its pages into steps of 64 tokens.  The steps of
+// all tiles of a kv head form one line, kTileCost more per tile for what a tile costs besides its steps, and
+// block i of the head's `blocks` takes the i-th equal share of it: so the chip's block slots (two per CU)
+// finish together whatever the lengths are, and a tile is cut only where a share ends.  The lengths are only on
+// the device: every block derives the same line from the tables (build_line).
+//   A whole tile of a row without a prefix writes o and lse.  Any other one writes un-normalised partials
+// (m, l, a): a whole tile at its token's place, a cut one into its block's two buffers (a block's first piece may
+// end a cut tile, its last may begin one); the merge kernel joins them per (token, q head).
 //
-// Per block: 4 waves, a 64-token step (four pages) of K and V in LDS, the next one in flight (64 KiB, two
-// blocks per CU).  With more than 64 pairs in the tile every wave owns 32 of them and sweeps the whole step;
-// with 33-64 two waves share 32 pairs and take 32 tokens of the step each; with up to 32 (one decode row's
-// own pages) two waves split the step and the others only load.  Waves that share pairs are joined in LDS.
-// MFMA tiles as in prefill.hip: S^T = K Q^T with lane l holding query row l % 32 and 16 tokens per 32,
-// O^T += V^T P^T, P rounded to the cache's type for the product as there (the sums l stay unrounded fp32).
+// Per block: 4 waves.  Tiles of more than 32 pairs share each step's K and V in LDS, the next step in flight (64 KiB):
+// with more than 64 pairs every wave owns 32 of them and sweeps the whole step, with 33-64 two waves share 32 pairs
+// and take 32 tokens of the step each.  Tiles of up to 32 pairs (a decode row's own pages) are bound by HBM: each wave
+// streams every fourth page through 16 KiB of its own, one page ahead, without barriers, and the waves are joined in
+// LDS at the end.  MFMA tiles as in prefill.hip: S^T = K Q^T with lane l holding query pair l % 32 and 16 tokens per
+// 32, O^T += V^T P^T, P rounded to the cache's type for the product as there (the sums l stay unrounded fp32).
 #include <type_traits>
 
 #include "delta_common.h"
@@ -35,11 +38,12 @@ constexpr int kThreads = 256;
 constexpr int kStep = 64;               // kv tokens per step
 constexpr int kPages = kStep / kPageSize;
 constexpr int kTileB = kStep * 256;     // bytes of a step's K (or V) tile: 64 rows of 256 bytes
-constexpr int kQ = 128;                 // (token, head) pairs of a tile
-constexpr int kMaxRows = 1024;          // rows, and prefixes, of a call (plan_unit's tables)
-constexpr int kMaxSplits = 32;          // runs of a segment
-constexpr int kMinChunk = 2;            // steps of a run, at least
+constexpr int kPageB = kPageSize * 256; // bytes of a page's K (or V) of one head
+constexpr int kQ = 128;                 // (token, head) pairs of a tile, at most
+constexpr int kMaxRows = 1024;          // rows, and prefixes, of a call (the line's tables)
 constexpr int kSlots = 512;             // blocks the chip holds (two per CU)
+constexpr int kTileCost = 2;            // steps that a tile costs besides its own
+constexpr int kMinShare = 4;            // steps of a share, at least
 
 struct PrefixArgs {
   const uint16_t *q;
@@ -59,69 +63,56 @@ struct PrefixArgs {
   uint16_t *o;
   int64_t o_stride_t, o_stride_h;
   float *lse;
-  float *part_ml;      // [slot][token][q head][2]
-  float *part_acc;     // [slot][token][q head][128]; slots [0, splits): prefix runs, then as many: own runs
-  int32_t *tok_runs;   // [token] runs of its prefix | runs of its own tile << 16
+  // Partials: rows (prefix 0 / own 1, token, q head) of whole tiles, then (kv head, block, ends 0 / begins 1 a cut tile,
+  // pair) of cut ones.
+  float *part_ml;   // [row][2]
+  float *part_acc;  // [row][128]
+  int2 *runs;       // [prefix / own][token]: first block of its tile, runs | its first pair in the tile << 16
   int batch, tokens, hq, hkv;
-  int splits;          // slots of a kind
-  int target;          // units per kv head that fill the chip
+  int blocks;       // per kv head
   float sm_scale;
 };
 
-struct RowTable {  // the plan's view of a row
-  int prefix;      // -1: none applies
-  int kv0, pages;  // own pages: first index in kv_indices, count
-  int len;         // own tokens
-  int q0, qn;      // query tokens
-};
-
 // Pages [first, first + n) of CSR entry i, clamped to the index array.
-__device__ __forceinline__ void csr_pages(const int32_t *indptr, int64_t len, int i, int *first, int *n) {
-  int64_t p0 = indptr[i], p1 = indptr[i + 1];
+struct Pages {
+  int first, n;
+};
+__device__ __forceinline__ Pages csr_pages(const int32_t *indptr, int64_t len, int i) {
+  int64_t p0 = ld_scalar(indptr, i), p1 = ld_scalar(indptr, i + 1);
   p0 = p0 < 0 ? 0 : (p0 > len ? len : p0);
   p1 = p1 < p0 ? p0 : (p1 > len ? len : p1);
-  *first = (int)p0;
-  *n = (int)(p1 - p0);
+  return Pages{(int)p0, (int)(p1 - p0)};
 }
 
-__device__ __forceinline__ RowTable row_table(const PrefixArgs &a, int r) {
-  RowTable x;
-  csr_pages(a.kv_indptr, a.kv_indices_len, r, &x.kv0, &x.pages);
-  int last = a.last_page_len[r];
+struct Row {
+  int kv0, pages, len;  // its pages in kv_indices and its tokens, the prefix's included
+  int q0, qn;           // query tokens
+};
+__device__ __forceinline__ Row row_of(const PrefixArgs &a, int r) {
+  Row x;
+  const Pages p = csr_pages(a.kv_indptr, a.kv_indices_len, r);
+  int last = ld_scalar(a.last_page_len, r);
   last = last < 0 ? 0 : (last > kPageSize ? kPageSize : last);
-  x.len = x.pages > 0 ? (x.pages - 1) * kPageSize + last : 0;
+  x.kv0 = p.first;
+  x.pages = p.n;
+  x.len = p.n > 0 ? (p.n - 1) * kPageSize + last : 0;
   x.q0 = r;
   x.qn = 1;
-  int behind = 0;  // query tokens that the prefix has to leave room for
   if (a.qo_indptr) {
-    int q0 = a.qo_indptr[r], q1 = a.qo_indptr[r + 1];
+    int q0 = ld_scalar(a.qo_indptr, r), q1 = ld_scalar(a.qo_indptr, r + 1);
     q0 = q0 < 0 ? 0 : (q0 > a.tokens ? a.tokens : q0);
     q1 = q1 < q0 ? q0 : (q1 > a.tokens ? a.tokens : q1);
     x.q0 = q0;
-    behind = x.qn = q1 - q0;
-  }
-  x.prefix = -1;
-  const int p = a.row_prefix[r];
-  if (p >= 0 && p < a.num_prefixes) {
-    int first, n;
-    csr_pages(a.prefix_indptr, a.prefix_indices_len, p, &first, &n);
-    if (n > 0 && n <= x.pages && n * kPageSize <= x.len - behind) {
-      x.prefix = p;
-      x.kv0 += n;
-      x.pages -= n;
-      x.len -= n * kPageSize;
-    }
+    x.qn = q1 - q0;
   }
   return x;
 }
+// Whether a prefix of n pages applies to the row.
+__device__ __forceinline__ bool prefix_fits(const PrefixArgs &a, const Row &x, int n) {
+  return n > 0 && n <= x.pages && n * kPageSize <= x.len - (a.qo_indptr ? x.qn : 0);
+}
 
 __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
-
-// Steps of a run in a segment of `steps` steps: the plan's, unless that takes more runs than there are slots.
-__device__ __forceinline__ int run_steps(int steps, int chunk, int splits) {
-  const int least = div_up(steps, splits);
-  return least > chunk ? least : chunk;
-}
 
 // A pointer that is the same in every lane, in scalar registers.
 template <typename T>
@@ -131,31 +122,15 @@ __device__ __forceinline__ T *uniform_ptr(T *p) {
                           (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
 }
 
-// What a block works on.
-struct Unit {
-  const int32_t *ids;  // the segment's page ids
-  int pages, len;      // its pages and tokens
-  int pairs0, pairs;   // first (token, head) pair of the tile and how many it has
-  int first_pos;       // segment position of the segment's first query token; >= len: a prefix, no mask
-  int s0, s1;          // steps [s0, s1)
-  int slot;            // partial slot
-};
-
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int x = __shfl_up(v, off, 64);
-    if (lane >= off) v += x;
-  }
-  return v;
-}
-
-// Exclusive sum over the block's threads; *total: the block's sum.  `sums` holds 4 ints; ends with a barrier
-// before it is written again.
+// Exclusive sum over the block's threads; *total: the block's sum.  `sums` holds 4 ints, free again on return.
 __device__ __forceinline__ int block_scan(int v, int *sums, int *total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int incl = wave_scan(v, lane);
+  int incl = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int x = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += x;
+  }
   if (lane == 63) sums[wave] = incl;
   __syncthreads();
   int before = 0, all = 0;
@@ -169,454 +144,585 @@ __device__ __forceinline__ int block_scan(int v, int *sums, int *total) {
   return before + incl - v;
 }
 
-constexpr int kPlanInts = 6 * kMaxRows + 16;
+// The line of a kv head's work, in LDS.
+struct Line {
+  int at[2 * kMaxRows + 1];   // where each segment begins (the prefixes, then the rows), and the end
+  int prefix_toks[kMaxRows];  // query tokens of each prefix
+  int16_t row_prefix[kMaxRows];  // the prefix that applies to each row, -1: none
+  int sums[4];
+  int toks[kQ];               // query tokens of a prefix's tile
+};
 
-// Finds unit u; false past the last one.  `sc` (kPlanInts ints of LDS) is free again on return, toks[i] holds the
-// query token of pair index (pairs0 / G + i) * G.  Writes tok_runs for the tokens of a row's first run (head 0).
-template <int G>
-__device__ bool plan_unit(const PrefixArgs &a, int u, bool head0, int *sc, int *toks, Unit *unit) {
-  int *const cnt = sc;                    // [prefix] query tokens
-  int *const psteps = sc + kMaxRows;      // [prefix] steps
-  int *const rprefix = sc + 2 * kMaxRows; // [row]
-  int *const rsteps = sc + 3 * kMaxRows;
-  int *const rq0 = sc + 4 * kMaxRows;
-  int *const rqn = sc + 5 * kMaxRows;
-  int *const sums = sc + 6 * kMaxRows;    // [4]
-  int *const found = sums + 4;            // item, unit within it
-  const int tid = threadIdx.x;
-  const int P = a.num_prefixes, B = a.batch;
-  for (int p = tid; p < P; p += kThreads) cnt[p] = 0;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  int work = 0;
-  for (int r = tid; r < B; r += kThreads) {
-    const RowTable x = row_table(a, r);
-    const int steps = div_up(x.len, kStep);
-    rprefix[r] = x.prefix;
-    rsteps[r] = steps;
-    rq0[r] = x.q0;
-    rqn[r] = x.qn;
-    if (x.prefix >= 0) atomicAdd(&cnt[x.prefix], x.qn);
-    work += div_up(x.qn * G, kQ) * (steps > 1 ? steps : 1);
-  }
-  __syncthreads();
+// `scratch`: kMaxRows ints of LDS.
+template <int TT>
+__device__ int build_line(const PrefixArgs &a, Line &line, int *scratch) {
+  const int tid = threadIdx.x, P = a.num_prefixes, B = a.batch;
   for (int p = tid; p < P; p += kThreads) {
-    int first, n;
-    csr_pages(a.prefix_indptr, a.prefix_indices_len, p, &first, &n);
-    psteps[p] = div_up(n, kPages);
-    work += div_up(cnt[p] * G, kQ) * psteps[p];
+    line.prefix_toks[p] = 0;
+    scratch[p] = csr_pages(a.prefix_indptr, a.prefix_indices_len, p).n;
   }
-  int total;
-  block_scan(work, sums, &total);
-  int chunk = div_up(total, a.target);
-  chunk = chunk < kMinChunk ? kMinChunk : chunk;
-  // Items: the prefixes, then the rows.
-  auto tiles_of = [&](int i) { return div_up((i < P ? cnt[i] : rqn[i - P]) * G, kQ); };
-  auto steps_of = [&](int i) { return i < P ? psteps[i] : (rsteps[i - P] > 1 ? rsteps[i - P] : 1); };
-  auto runs_of = [&](int steps) { return div_up(steps, run_steps(steps, chunk, a.splits)); };
-  int base = 0;
+  Row x = tid < B ? row_of(a, tid) : Row{0, 0, 0, 0, 0};
+  int want = tid < B ? a.row_prefix[tid] : -1;
+  __syncthreads();
+  for (int r = tid; r < B; r += kThreads) {
+    if (r != tid) {
+      x = row_of(a, r);
+      want = a.row_prefix[r];
+    }
+    const bool fits = want >= 0 && want < P && prefix_fits(a, x, scratch[want >= 0 && want < P ? want : 0]);
+    line.row_prefix[r] = (int16_t)(fits ? want : -1);
+    if (fits) atomicAdd(&line.prefix_toks[want], x.qn);
+    const int own = x.len - (fits ? scratch[want] * kPageSize : 0);
+    line.at[P + r] = div_up(x.qn, TT) * (div_up(own, kStep) + kTileCost);
+  }
+  __syncthreads();
+  int end = 0;
   for (int i0 = 0; i0 < P + B; i0 += kThreads) {
     const int i = i0 + tid;
-    const int n = i < P + B ? tiles_of(i) * runs_of(steps_of(i)) : 0;
-    const int at = base + block_scan(n, sums, &total);
-    if (u >= at && u < at + n) {
-      found[0] = i;
-      found[1] = u - at;
+    int cost = 0, total;
+    if (i < P) {
+      const int tiles = div_up(line.prefix_toks[i], TT);
+      cost = tiles * (div_up(scratch[i], kPages) + kTileCost);
+    } else if (i < P + B) {
+      cost = line.at[i];
     }
-    base += total;
-    if (u < base) break;
+    const int at = end + block_scan(cost, line.sums, &total);
+    if (i < P + B) line.at[i] = at;
+    end += total;
   }
+  if (tid == 0) line.at[P + B] = end;
   __syncthreads();
-  const int item = uniform(found[0]), v = uniform(found[1]);  // (read as scalars: the compiler cannot see it)
-  if (item < 0) return false;
-  const int tiles = tiles_of(item), steps = steps_of(item), each = run_steps(steps, chunk, a.splits);
-  const int run = v / tiles, tile = tiles - 1 - (v - run * tiles);  // a row's last tile attends the most
-  const int nq = (item < P ? cnt[item] : rqn[item - P]) * G;
-  unit->pairs0 = tile * kQ;
-  unit->pairs = min(kQ, nq - tile * kQ);
-  unit->s0 = run * each;
-  unit->s1 = min(steps, unit->s0 + each);
-  const int t0 = unit->pairs0 / G, t1 = (unit->pairs0 + unit->pairs - 1) / G + 1;  // tokens of the tile
-  if (item < P) {
-    int first, n;
-    csr_pages(a.prefix_indptr, a.prefix_indices_len, item, &first, &n);
-    unit->ids = a.prefix_indices + first;
-    unit->pages = n;
-    unit->len = n * kPageSize;
-    unit->first_pos = unit->len;
-    unit->slot = run;
-    // The tile's tokens out of those of the prefix's rows, row by row.
-    int before = 0;
-    for (int r0 = 0; r0 < B; r0 += kThreads) {
-      const int r = r0 + tid;
-      const int n_r = r < B && rprefix[r] == item ? rqn[r] : 0;
-      const int at = before + block_scan(n_r, sums, &total);
-      for (int k = t0 > at ? t0 - at : 0; k < n_r && at + k < t1; ++k) toks[at + k - t0] = rq0[r] + k;
-      before += total;
-      if (before >= t1) break;
-    }
-  } else {
-    const int r = item - P;
-    const RowTable x = row_table(a, r);
-    unit->ids = a.kv_indices + x.kv0;
-    unit->pages = x.pages;
-    unit->len = x.len;
-    unit->first_pos = x.len - x.qn;
-    const int reach = unit->first_pos + t1;  // tokens that the tile's last query token attends
-    unit->s1 = min(unit->s1, reach > 0 ? div_up(min(reach, x.len), kStep) : 0);
-    unit->slot = a.splits + run;
-    const int pruns = x.prefix >= 0 ? runs_of(psteps[x.prefix]) : 0;
-    for (int k = tid; k < t1 - t0; k += kThreads) {
-      toks[k] = x.q0 + t0 + k;
-      if (head0 && run == 0) a.tok_runs[x.q0 + t0 + k] = pruns | (runs_of(steps) << 16);
-    }
-  }
-  __syncthreads();
-  return true;
+  return end;
 }
 
 template <int DT, int G>
 __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArgs a) {
 #pragma clang fp contract(off)
   using MF = Mfma32<DT>;
-  // Step buffers, each the K tile, then the V tile (swizzled rows), shared by the block's waves; the plan's tables
-  // before the first step, the joined waves' accumulators after the last.
+  using E = Elem<DT>;
+  constexpr int TT = kQ / G;  // query tokens of a tile
+  // Two steps' buffers, each the K tile, then the V tile (swizzled rows); or per wave two pages' buffers.  The waves'
+  // accumulators where they are joined.
   __shared__ __attribute__((aligned(1024))) char tiles[2][2 * kTileB];
-  __shared__ int toks[kQ + 2];
-  static_assert(kPlanInts * sizeof(int) <= sizeof(tiles), "the plan's tables lie in the step buffers");
+  __shared__ Line line;
 
-  const int lane = threadIdx.x & 63, hl = lane >> 5, n = lane & 31;
   const int wv = uniform((int)(threadIdx.x >> 6));
-  const int h = blockIdx.x;
-  Unit un;
-  if (!plan_unit<G>(a, (int)(blockIdx.z * gridDim.y + blockIdx.y), h == 0, reinterpret_cast<int *>(&tiles[0][0]), toks,
-                    &un))
-    return;  // whole block
-  const int np = uniform(un.pages), len = uniform(un.len), s0 = uniform(un.s0), s1 = uniform(un.s1);
-  const int pairs = uniform(un.pairs);
+  const int h = blockIdx.x, blk = blockIdx.y;
+  const int total = uniform(build_line<TT>(a, line, reinterpret_cast<int *>(&tiles[0][0])));
+  int share = uniform(div_up(total, a.blocks));
+  share = share < kMinShare ? kMinShare : share;
+  int pos = blk * share;  // (total < 2^30: checked on the host)
+  const int end = min(total, pos + share);
 
-  // The wave's pairs (32 from 32 qsub on) and 32-token halves of each step.
-  const int groups = pairs > 64 ? 4 : (pairs > 32 ? 2 : 1);
-  const int qsub = wv & (groups - 1);
-  const int half = groups == 4 ? 0 : wv / groups;  // the wave's half (groups 4: both)
-  const bool active = half < 2 && 32 * qsub < pairs;
-
-  // This lane's pair: token and head, and the last position of the segment that it attends.
-  const int pair = 32 * qsub + n;
-  const bool row_ok = active && pair < pairs;
-  const int pt = (un.pairs0 + (row_ok ? pair : 0)) / G, g = (un.pairs0 + (row_ok ? pair : 0)) % G;
-  const int t = toks[pt - un.pairs0 / G];
-  const int lim = un.first_pos >= len ? len - 1 : un.first_pos + pt;
-  u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
-  if (row_ok) {
-    // A negative scale flips q's signs, scale 0 clears q: the scale below is then positive.
-    const uint32_t flip = a.sm_scale < 0.f ? 0x80008000u : 0u, keep = a.sm_scale == 0.f ? 0u : 0xffffffffu;
-    const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks)
-      qf[ks] = (ld128(qp + 16 * ks) ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
-  } else {
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qf[ks] = u32x4{0u, 0u, 0u, 0u};
-  }
-  const float scale2 = a.sm_scale == 0.f ? 1.f : fabsf(a.sm_scale) * kLog2e;
-  // Steps that end at or below the position of the wave's first token need no causal mask.
-  const int wpos = un.first_pos >= len ? len - 1 : un.first_pos + (un.pairs0 + 32 * qsub) / G;
-
-  // Step loads: K and V rows go straight to LDS, 1 KiB (4 rows of this head) per load: wave w loads rows 4 w .. + 3 of
-  // each of the step's four pages, K and V.  16-byte chunk ch of K row r sits at slot ch ^ (r % 16) and of V row r at
-  // ch ^ 4 (r % 4), so that the fragment reads cover the banks once.
+  // Loads: K and V rows go straight to LDS, 1 KiB (4 rows of this head) per load.  16-byte chunk ch of K row r sits at
+  // slot ch ^ (r % 16) and of V row r at ch ^ 4 (r % 4), so that the fragment reads cover the banks once.
   const uint32_t row_bytes = (uint32_t)a.hkv * kHeadDim * 2;
   const uint32_t page_bytes = 2 * kPageSize * row_bytes;
-  const int lrow = lane >> 4, lch = lane & 15;
-  const uint32_t koff = (4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * wv + lrow));
-  const uint32_t voff = (kPageSize + 4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&tiles[0][0] + wv * 1024;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&tiles[0][0];
   const char *const kvh = reinterpret_cast<const char *>(a.kv) + (int64_t)h * (kHeadDim * 2);
-  const int32_t *const ids = uniform_ptr(un.ids);
-  auto page_bad = [&](int pid) { return pid < 0 || (int64_t)pid >= a.num_pages; };
-  // Page ids outside the cache are looked for once, over the run's pages.
-  bool run_bad = false;
-  for (int i = s0 * kPages; i < s1 * kPages && i < np; i += 64)
-    run_bad |= __ballot(i + lane < np && i + lane < s1 * kPages && page_bad(ids[i + lane < np ? i + lane : 0])) != 0;
-  // The step's page ids by scalar loads (their waits leave the tile loads in flight), a step ahead; pages past the
-  // segment repeat its last one (masked later).
-  int id[kPages];
-  auto load_ids = [&](int j) {
+  const uint32_t num_pages = a.num_pages < INT32_MAX ? (uint32_t)a.num_pages : (uint32_t)INT32_MAX;
+  const float scale2 = a.sm_scale == 0.f ? 1.f : fabsf(a.sm_scale) * kLog2e;
+  int item = 0;
+  while (pos < end) {
+    // The lane, hidden from the compiler: it would keep every offset that follows from it in registers over all pieces
+    // (55 of them spilled).
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int hl = lane >> 5, n = lane & 31, lrow = lane >> 4, lch = lane & 15;
+    // K fragment of k-slice ks: row n (of 32), chunk 2 ks + hl.
+    uint32_t kfo[8];
 #pragma unroll
-    for (int i = 0; i < kPages; ++i) {
-      const int pg = kPages * j + i;
-      id[i] = ld_scalar(ids, pg < np ? pg : np - 1);
-    }
-  };
-  auto bad_of = [&](int j) {  // bit i: page i of step j lies outside the cache
-    uint32_t r = 0;
+    for (int ks = 0; ks < 8; ++ks) kfo[ks] = (uint32_t)(n * 256 + 16 * ((2 * ks + hl) ^ (n & 15)));
+    // ds_read_b64_tr_b16 of V^T: 16-lane group q16 = lane / 16, t16 = lane % 16 reads rows (kv) base + t16 / 4 at columns
+    // 32 dt + 16 (q16 % 2) + 4 (t16 % 4), and receives its column's four rows.
+    const int q16 = lane >> 4, t16 = lane & 15;
+    uint32_t vfo[4];
 #pragma unroll
-    for (int i = 0; i < kPages; ++i) {
-      const int pg = kPages * j + i;
-      r |= (pg < np && page_bad(ld_scalar(ids, pg < np ? pg : np - 1)) ? 1u : 0u) << i;
-    }
-    return r;
-  };
-  auto issue = [&](int j) {  // step j's loads, then the ids of step j + 1
-#pragma unroll
-    for (int i = 0; i < kPages; ++i) {
-      const char *pbase = uniform_ptr(kvh + (uint64_t)(uint32_t)(run_bad && page_bad(id[i]) ? 0 : id[i]) * page_bytes);
-      const uint32_t dst = lds0 + (uint32_t)(j & 1) * (2 * kTileB) + i * 4096;
-      load_lds_1k(dst, pbase, koff);
-      load_lds_1k(dst + kTileB, pbase, voff);
-    }
-    load_ids(j + 1);
-  };
-  if (s0 < s1) {
-    load_ids(s0);
-    issue(s0);
-  }
+    for (int dt = 0; dt < 4; ++dt)
+      vfo[dt] = (uint32_t)((4 * hl + (t16 >> 2)) * 256 +
+                           16 * ((4 * dt + 2 * (q16 & 1) + ((t16 & 3) >> 1)) ^ (4 * (t16 >> 2))) + 8 * (t16 & 1));
 
-  float m = -INFINITY, l = 0.f;
-  f32x16 acc[4];
-#pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
-  uint32_t kfo[8];  // K fragment of k-slice ks: row n, chunk 2 ks + hl
-#pragma unroll
-  for (int ks = 0; ks < 8; ++ks) kfo[ks] = (uint32_t)(n * 256 + 16 * ((2 * ks + hl) ^ (n & 15)));
-  // ds_read_b64_tr_b16 of V^T: 16-lane group q16 = lane / 16, t16 = lane % 16 reads rows (kv) base + t16 / 4 at columns
-  // 32 dt + 16 (q16 % 2) + 4 (t16 % 4), and receives its column's four rows.
-  const int q16 = lane >> 4, t16 = lane & 15;
-  uint32_t vfo[4];
-#pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
-    vfo[dt] = (uint32_t)(kTileB + (4 * hl + (t16 >> 2)) * 256 +
-                         16 * ((4 * dt + 2 * (q16 & 1) + ((t16 & 3) >> 1)) ^ (4 * (t16 >> 2))) + 8 * (t16 & 1));
-
-  // 32-token halves [h0, h0 + NS) of step j (tile tk): scores, online softmax, P.V.
-  auto sweep = [&](auto ns, int j, const char *tk, int h0, uint32_t bad) {
-    constexpr int NS = decltype(ns)::value;
-    f32x16 S[NS];
-#pragma unroll
-    for (int sb = 0; sb < NS; ++sb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) S[sb][i] = 0.f;
-    const char *tkh = tk + h0 * 8192;
-    auto kfrag = [&](int sb, int ks) { return *reinterpret_cast<const u32x4 *>(tkh + kfo[ks] + sb * 8192); };
-    u32x4 kq[4][NS];
-#pragma unroll
-    for (int s = 0; s < 3; ++s)
-#pragma unroll
-      for (int sb = 0; sb < NS; ++sb) kq[s][sb] = kfrag(sb, s);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      if (ks + 3 < 8) {
-#pragma unroll
-        for (int sb = 0; sb < NS; ++sb) kq[(ks + 3) % 4][sb] = kfrag(sb, ks + 3);
+    // ---- The piece at pos: segment, tile, steps [s0, s1).
+    const int items = a.num_prefixes + a.batch;
+    for (;; item += 64) {  // the first segment that ends past pos
+      const int i = item + lane;
+      const uint64_t past = __ballot(i < items && line.at[i < items ? i + 1 : items] > pos);
+      if (past) {
+        item = uniform(item + __builtin_ctzll(past));
+        break;
       }
-#pragma unroll
-      for (int sb = 0; sb < NS; ++sb) S[sb] = MF::run(kq[ks % 4][sb], qf[ks], S[sb]);
-      __builtin_amdgcn_sched_barrier(0);
     }
-    const int kv0 = j * kStep + 32 * h0;
-    constexpr int NX = 16 * NS;
-    const bool full = kv0 + 32 * NS - 1 <= wpos && kv0 + 32 * NS <= len && bad == 0;
-    float x[NX];
-    float pm = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      x[i] = S[i >> 4][i & 15];
-      if (!full) {
-        const int mm = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * hl + (i & 3);
-        const int tk_i = kv0 + mm;
-        const bool pg_ok = ((bad >> (2 * h0 + (mm >> 4))) & 1u) == 0;
-        x[i] = pg_ok && tk_i <= lim && tk_i < len ? x[i] : -INFINITY;
+    const bool of_prefix = item < a.num_prefixes;
+    const int32_t *ids;  // the segment's page ids
+    int np, len, seg_toks, q0 = 0, px = -1;
+    if (of_prefix) {
+      const Pages p = csr_pages(a.prefix_indptr, a.prefix_indices_len, item);
+      ids = a.prefix_indices + p.first;
+      np = p.n;
+      len = p.n * kPageSize;
+      seg_toks = uniform(line.prefix_toks[item]);
+    } else {
+      const int r = item - a.num_prefixes;
+      const Row x = row_of(a, r);
+      px = uniform(line.row_prefix[r]);
+      const int skip = px >= 0 ? csr_pages(a.prefix_indptr, a.prefix_indices_len, px).n : 0;
+      ids = a.kv_indices + x.kv0 + skip;
+      np = x.pages - skip;
+      len = x.len - skip * kPageSize;
+      seg_toks = x.qn;
+      q0 = x.q0;
+    }
+    const int steps = div_up(len, kStep), cost = steps + kTileCost;
+    const int seg_at = uniform(line.at[item]);
+    const int tile = uniform((pos - seg_at) / cost), tile_at = seg_at + tile * cost;
+    const int stop = min(end, tile_at + cost);
+    const int s0 = max(0, pos - tile_at - kTileCost);
+    int s1 = max(0, stop - tile_at - kTileCost);
+    const int first_blk = uniform(tile_at / share), runs = uniform((tile_at + cost - 1) / share) - first_blk + 1;
+    const int run = blk - first_blk;
+    pos = stop;
+    const int t0 = tile * TT, ntok = min(TT, seg_toks - t0), pairs = ntok * G;
+    // Segment position of query token t0 + i of a row: first_pos + i; a prefix's tokens come behind all of it.
+    const int first_pos = of_prefix ? len : len - seg_toks + t0;
+    if (!of_prefix) {
+      const int reach = first_pos + ntok;  // tokens that the tile's last query token attends
+      s1 = min(s1, reach > 0 ? div_up(min(reach, len), kStep) : 0);
+    }
+    if (of_prefix) {
+      // The tile's tokens out of those of the prefix's rows, row by row.
+      int before = 0, sum;
+      for (int r0 = 0; r0 < a.batch; r0 += kThreads) {
+        const int r = r0 + threadIdx.x;
+        const bool mine = r < a.batch && line.row_prefix[r] == item;
+        int rq0 = r, qn = mine ? 1 : 0;
+        if (a.qo_indptr && mine) {
+          const Row x = row_of(a, r);
+          rq0 = x.q0;
+          qn = x.qn;
+        }
+        const int at = before + block_scan(qn, line.sums, &sum);
+        for (int k = t0 > at ? t0 - at : 0; k < qn && at + k < t0 + ntok; ++k) line.toks[at + k - t0] = rq0 + k;
+        before += sum;
+        if (before >= t0 + ntok) break;
       }
-      pm = fmaxf(pm, x[i]);
     }
-    // m is a reference maximum: it moves only when a score exceeds it by more than 8 (log2), so the exponentials
-    // stay <= 256 and the accumulators are rescaled on few steps.
-    const float smax = halves_max(pm) * scale2;
-    float alpha = 1.f;
-    if (smax > m + 8.f) {  // also the first finite score (m = -inf)
-      alpha = fast_exp2(m - smax);
-      m = smax;
-    }
-    const float nm = m == -INFINITY ? 0.f : -m;
-    float ps = 0.f;
-#pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      x[i] = fast_exp2(fmaf(x[i], scale2, nm));
-      ps += x[i];
-    }
-    l = l * alpha + ps;  // this half-wave's tokens; joined once at the end
-    if (__ballot(alpha != 1.f)) {
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
-    }
-    u32x4 pc[2 * NS];
-#pragma unroll
-    for (int cc = 0; cc < 2 * NS; ++cc)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) pc[cc][w] = pack2<DT>(x[8 * cc + 2 * w], x[8 * cc + 2 * w + 1]);
-    auto vfrag = [&](int i) {  // V^T fragment of 16-token chunk i / 4, d tile i % 4
-      const char *rd = tkh + vfo[i % 4] + (i / 4) * 4096;
-      const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
-      const ps4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)(rd + 2048));
-      const uint2 lo = __builtin_bit_cast(uint2, v0), hi = __builtin_bit_cast(uint2, v1);
-      return u32x4{lo.x, lo.y, hi.x, hi.y};
-    };
-    constexpr int kAhead = 4;
-    u32x4 vq[kAhead + 1];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) vq[i] = vfrag(i);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < 8 * NS; ++i) {
-      if (i + kAhead < 8 * NS) vq[(i + kAhead) % (kAhead + 1)] = vfrag(i + kAhead);
-      acc[i % 4] = MF::run(vq[i % (kAhead + 1)], pc[i / 4], acc[i % 4]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
+    __syncthreads();  // the tile's tokens are listed, the piece before is done with the buffers
 
-  for (int j = s0; j < s1; ++j) {
-    wait_loads<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const uint32_t bad = run_bad ? bad_of(j) : 0u;
-    if (j + 1 < s1) issue(j + 1);
-    if ((j + 1) * kStep > len || bad != 0) {
-      // V rows past the segment and of pages outside the cache meet p = 0 but may hold NaN/Inf: zeros.
-      const int r = (int)threadIdx.x >> 2;
-      if (j * kStep + r >= len || ((bad >> (r >> 4)) & 1u)) {
-        char *vr = &tiles[j & 1][kTileB + r * 256 + 64 * ((int)threadIdx.x & 3)];
+    // ---- The wave's pairs (32 from 32 qsub on), and the 32-token half of each step that it takes.
+    const int groups = pairs > 64 ? 4 : (pairs > 32 ? 2 : 1);
+    const int qsub = wv & (groups - 1);
+    const int half = groups == 2 ? wv >> 1 : 0;
+    const bool active = 32 * qsub < pairs;
+    const int pair = 32 * qsub + n;
+    const bool row_ok = pair < pairs;
+    const int pt = row_ok ? pair / G : 0, g = row_ok ? pair % G : 0;
+    const int t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
+    const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);  // the last position that the lane's pair attends
+    // Steps that end at or below the position of the wave's first token need no mask.
+    const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos + 32 * qsub / G);
+    u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
+    const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-    }
-    if (active) {
-      const char *tk = &tiles[j & 1][0];
-      if (groups == 4)
-        sweep(std::integral_constant<int, 2>(), j, tk, 0, bad);
-      else
-        sweep(std::integral_constant<int, 1>(), j, tk, half, bad);
-    }
-  }
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = row_ok ? ld128(qp + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
 
-  l = halves_sum(l);
-  if (groups < 4) {
-    // Join the waves that took the two halves: the second's (m, l, acc) through LDS.
-    float *const buf = reinterpret_cast<float *>(&tiles[0][0]) + qsub * (66 * 64) + lane;
-    __syncthreads();
-    if (half == 1 && active) {
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) buf[64 * (16 * dt + i)] = acc[dt][i];
-      buf[64 * 64] = m;
-      buf[64 * 65] = l;
-    }
-    __syncthreads();
-    if (half == 0 && active) {
-      const float m2 = buf[64 * 64], l2 = buf[64 * 65];
-      const float M = fmaxf(m, m2), ref = M == -INFINITY ? 0.f : M;
-      const float w1 = fast_exp2(m - ref), w2 = fast_exp2(m2 - ref);
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * w1 + buf[64 * (16 * dt + i)] * w2;
-      l = l * w1 + l2 * w2;
-      m = M;
-    }
-  }
-  if (row_ok && half == 0) {
-    const int64_t at = ((int64_t)un.slot * a.tokens + t) * a.hq + h * G + g;
-    float *op = a.part_acc + at * kHeadDim + 4 * hl;
+    float m = -INFINITY, l = 0.f;
+    f32x16 acc[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4)
-        *reinterpret_cast<f32x4 *>(op + 32 * dt + 8 * q4) =
-            f32x4{acc[dt][4 * q4], acc[dt][4 * q4 + 1], acc[dt][4 * q4 + 2], acc[dt][4 * q4 + 3]};
-    if (hl == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = float2{m, l};
+      for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+
+    // NT tokens from segment position kv0 on, K rows at tk, V rows at tv: scores, online softmax, P.V.  Bit i of bad:
+    // page i of them lies outside the cache.  (NT = 16: fragment rows 16-31 repeat 0-15 and their scores are not used.)
+    auto sweep = [&](auto nt, int kv0, const char *tk, const char *tv, uint32_t bad) {
+      constexpr int NT = decltype(nt)::value, NS = NT >= 32 ? NT / 32 : 1, NX = NT / 2;
+      f32x16 S[NS];
+#pragma unroll
+      for (int sb = 0; sb < NS; ++sb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[sb][i] = 0.f;
+      auto kfrag = [&](int sb, int ks) {
+        return *reinterpret_cast<const u32x4 *>(tk + (NT == 16 ? kfo[ks] & (kPageB - 1) : kfo[ks]) + sb * 8192);
+      };
+      constexpr int kKAhead = 3;
+      u32x4 kq[kKAhead + 1][NS];
+#pragma unroll
+      for (int s = 0; s < kKAhead; ++s)
+#pragma unroll
+        for (int sb = 0; sb < NS; ++sb) kq[s][sb] = kfrag(sb, s);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        if (ks + kKAhead < 8) {
+#pragma unroll
+          for (int sb = 0; sb < NS; ++sb) kq[(ks + kKAhead) % (kKAhead + 1)][sb] = kfrag(sb, ks + kKAhead);
+        }
+#pragma unroll
+        for (int sb = 0; sb < NS; ++sb) S[sb] = MF::run(kq[ks % (kKAhead + 1)][sb], qf[ks], S[sb]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const bool full = kv0 + NT - 1 <= wpos;
+      float x[NX];
+#pragma unroll
+      for (int i = 0; i < NX; ++i) x[i] = S[i >> 4][i & 15];
+      if (!(a.sm_scale > 0.f)) {  // (the scale below is positive)
+        const float sign = a.sm_scale == 0.f ? 0.f : -1.f;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) x[i] *= sign;
+      }
+      auto tok = [&](int i) { return 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3); };  // of x[i], from kv0 + 4 hl on
+      if (!full) {
+        const int last = lim - kv0 - 4 * hl;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) x[i] = tok(i) <= last ? x[i] : -INFINITY;
+      }
+      if (bad) {
+        uint32_t b = bad;  // (in a vector register: selects, not a branch for each value)
+        asm volatile("" : "+v"(b));
+#pragma unroll
+        for (int i = 0; i < NX; ++i) x[i] = (b >> (tok(i) >> 4)) & 1u ? -INFINITY : x[i];
+      }
+      float pm = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NX; ++i) pm = fmaxf(pm, x[i]);
+      // m is a reference maximum: it moves only when a score exceeds it by more than 8 (log2), so the exponentials
+      // stay <= 256 and the accumulators are rescaled on few steps.
+      const float smax = halves_max(pm) * scale2;
+      float alpha = 1.f;
+      if (smax > m + 8.f) {  // also the first finite score (m = -inf)
+        alpha = fast_exp2(m - smax);
+        m = smax;
+      }
+      const float nm = m == -INFINITY ? 0.f : -m;
+      float ps = 0.f;
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        x[i] = fast_exp2(fmaf(x[i], scale2, nm));
+        ps += x[i];
+      }
+      l = l * alpha + ps;  // this half-wave's tokens; joined once at the end
+      if (__ballot(alpha != 1.f)) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+      }
+      constexpr int NC = NT / 16;
+      u32x4 pc[NC];
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) pc[cc][w] = pack2<DT>(x[8 * cc + 2 * w], x[8 * cc + 2 * w + 1]);
+      auto vfrag = [&](int i) {  // V^T fragment of 16-token chunk i / 4, d tile i % 4
+        const char *rd = tv + vfo[i % 4] + (i / 4) * 4096;
+        const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
+        const ps4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)(rd + 2048));
+        const uint2 lo = __builtin_bit_cast(uint2, v0), hi = __builtin_bit_cast(uint2, v1);
+        return u32x4{lo.x, lo.y, hi.x, hi.y};
+      };
+      constexpr int kAhead = 4 * NC < 4 ? 4 * NC : 4;
+      u32x4 vq[kAhead + 1];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) vq[i] = vfrag(i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4 * NC; ++i) {
+        if (i + kAhead < 4 * NC) vq[(i + kAhead) % (kAhead + 1)] = vfrag(i + kAhead);
+        acc[i % 4] = MF::run(vq[i % (kAhead + 1)], pc[i / 4], acc[i % 4]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // Page ids, 64 per register (lane i: the wave's page 64 w + i of `count`); bit i of *bad: outside the cache.
+    auto load_ids = [&](int first, int stride, int count, int w, uint64_t *bad) {
+      const int i = 64 * w + lane;
+      const int id = i < count ? ids[first + stride * i] : 0;
+      const bool ok = (uint32_t)id < num_pages;
+      *bad = __ballot(!ok);
+      return ok ? id : 0;
+    };
+    auto page_base = [&](int id) { return uniform_ptr(kvh + (uint64_t)(uint32_t)id * page_bytes); };
+
+    if (groups == 1) {
+      // Wave-private pages: every fourth of the piece, two buffers.
+      const int p0 = kPages * s0 + wv, p1 = min(np, kPages * s1);
+      const int count = p0 < p1 ? (p1 - p0 + 3) >> 2 : 0;
+      const uint32_t wlds = lds0 + wv * (4 * kPageB);
+      char *const wbuf = &tiles[0][0] + wv * (4 * kPageB);
+      uint32_t koff[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) koff[i] = (4 * i + lrow) * row_bytes + 16 * ((lch ^ lrow) ^ (4 * i));
+      const uint32_t voff = (kPageSize + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
+      auto issue_k = [&](const char *pg, int buf) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_lds_1k(wlds + buf * 2 * kPageB + i * 1024, pg, koff[i]);
+      };
+      auto issue_v = [&](const char *pg, int buf) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          load_lds_1k(wlds + buf * 2 * kPageB + kPageB + i * 1024, pg, voff + (uint32_t)(4 * i) * row_bytes);
+      };
+      uint64_t bad = 0;
+      int idv = load_ids(p0, 4, count, 0, &bad);
+      if (count > 0) {
+        const char *pg = page_base(__builtin_amdgcn_readlane(idv, 0));
+        issue_k(pg, 0);
+        issue_v(pg, 0);
+      }
+      if (count > 1) {
+        const char *pg = page_base(__builtin_amdgcn_readlane(idv, 1));
+        issue_k(pg, 1);
+        issue_v(pg, 1);
+      }
+      uint64_t bad_next = bad;  // of the window of page k + 2
+      for (int k = 0; k < count; ++k) {
+        // (the ids of pages 64 w .. take the place of the last ones' once page 64 w - 2 is under way)
+        if (k + 2 < count && ((k + 2) & 63) == 0) idv = load_ids(p0, 4, count, (k + 2) >> 6, &bad_next);
+        if (k + 1 < count)
+          wait_loads<8>();
+        else
+          wait_loads<0>();
+        const int kv0 = (p0 + 4 * k) * kPageSize;
+        const bool page_bad = (bad >> (k & 63)) & 1u;
+        char *const buf = wbuf + (k & 1) * 2 * kPageB;
+        if (page_bad || kv0 + kPageSize > len) {
+          // V rows past the segment and of pages outside the cache meet p = 0 but may hold NaN/Inf: zeros.
+          const int r = lane >> 2;
+          if (page_bad || kv0 + r >= len) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st128(buf + kPageB + r * 256 + 64 * (lane & 3) + 16 * i, u32x4{0u, 0u, 0u, 0u});
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        sweep(std::integral_constant<int, 16>(), kv0, buf, buf + kPageB, page_bad ? 1u : 0u);
+        if (k + 2 < count) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          const char *pg = page_base(__builtin_amdgcn_readlane(idv, (k + 2) & 63));
+          issue_k(pg, k & 1);
+          issue_v(pg, k & 1);
+        }
+        if (((k + 1) & 63) == 0) bad = bad_next;
+      }
+    } else {
+      // Shared steps: wave w loads rows 4 w .. + 3 of each of the step's four pages, K and V.
+      const uint32_t wlds = lds0 + wv * 1024;
+      const uint32_t koff = (4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * wv + lrow));
+      const uint32_t voff = (kPageSize + 4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
+      const int p0 = kPages * s0, count = min(np, kPages * s1) - p0;  // <= 0: no step
+      uint64_t bad = 0, bad_next = 0;
+      int idv = 0;
+      auto issue = [&](int j) {  // step j of the piece; pages past the segment repeat page 0 of the window (masked later)
+#pragma unroll
+        for (int i = 0; i < kPages; ++i) {
+          const char *pg = page_base(__builtin_amdgcn_readlane(idv, (kPages * j + i) & 63));
+          const uint32_t dst = wlds + (uint32_t)(j & 1) * (2 * kTileB) + i * kPageB;
+          load_lds_1k(dst, pg, koff);
+          load_lds_1k(dst + kTileB, pg, voff);
+        }
+      };
+      const int nst = s1 > s0 ? s1 - s0 : 0;
+      if (nst > 0) {
+        idv = load_ids(p0, 1, count, 0, &bad);
+        bad_next = bad;
+        issue(0);
+      }
+      for (int j = 0; j < nst; ++j) {
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const uint32_t sbad = (uint32_t)(bad >> ((kPages * j) & 63)) & 15u;
+        if (j + 1 < nst) {
+          if (((j + 1) & 15) == 0) idv = load_ids(p0, 1, count, (j + 1) >> 4, &bad_next);
+          issue(j + 1);
+        }
+        const int kv0 = (s0 + j) * kStep;
+        char *const buf = &tiles[j & 1][0];
+        if (kv0 + kStep > len || sbad != 0) {
+          const int r = (int)threadIdx.x >> 2;
+          if (kv0 + r >= len || ((sbad >> (r >> 4)) & 1u)) {
+            char *vr = buf + kTileB + r * 256 + 64 * ((int)threadIdx.x & 3);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        if (active) {
+          if (groups == 4)
+            sweep(std::integral_constant<int, 64>(), kv0, buf, buf + kTileB, sbad);
+          else
+            sweep(std::integral_constant<int, 32>(), kv0 + 32 * half, buf + half * 8192, buf + kTileB + half * 8192,
+                  sbad >> (2 * half));
+        }
+        if (((j + 1) & 15) == 0) bad = bad_next;
+      }
+    }
+
+    l = halves_sum(l);
+    if (groups < 4) {
+      // Join the waves that share pairs: wave qsub + groups k, k > 0, hands (m, l, acc) to wave qsub through LDS.
+      float *const buf = reinterpret_cast<float *>(&tiles[0][0]) + lane;
+      constexpr int kOne = 66 * 64;  // floats of a wave
+      for (int w = 1; w < 4 / groups; ++w) {
+        __syncthreads();
+        float *const at = buf + qsub * kOne;
+        if (wv == qsub + groups * w) {
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) at[64 * (16 * dt + i)] = acc[dt][i];
+          at[64 * 64] = m;
+          at[64 * 65] = l;
+        }
+        __syncthreads();
+        if (wv < groups) {
+          const float m2 = at[64 * 64], l2 = at[64 * 65];
+          const float M = fmaxf(m, m2), ref = M == -INFINITY ? 0.f : M;
+          const float w1 = fast_exp2(m - ref), w2 = fast_exp2(m2 - ref);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * w1 + at[64 * (16 * dt + i)] * w2;
+          l = l * w1 + l2 * w2;
+          m = M;
+        }
+      }
+    }
+    // ---- Results (the lane's pair worked out again: held over the steps it would cost registers).
+    asm volatile("" : "+v"(lane));
+    const int wpair = 32 * qsub + (lane & 31), whl = lane >> 5;
+    const int wpt = wpair < pairs ? wpair / G : 0, wg = wpair - wpt * G;
+    const int wt = of_prefix ? line.toks[wpt] : q0 + t0 + wpt;
+    const bool writes = wpair < pairs && wv < groups;
+    const bool whole = runs == 1 && !of_prefix && px < 0;
+    if (writes && whole) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint16_t *op = a.o + (int64_t)wt * a.o_stride_t + (int64_t)(h * G + wg) * a.o_stride_h + 4 * whl;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t *w = reinterpret_cast<uint32_t *>(op + 32 * dt + 8 * q4);
+          w[0] = pack2<DT>(acc[dt][4 * q4] * inv, acc[dt][4 * q4 + 1] * inv);
+          w[1] = pack2<DT>(acc[dt][4 * q4 + 2] * inv, acc[dt][4 * q4 + 3] * inv);
+        }
+      if (a.lse && whl == 0) a.lse[(int64_t)wt * a.hq + h * G + wg] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    } else if (writes) {
+      const int64_t at = runs == 1 ? ((int64_t)(of_prefix ? 0 : a.tokens) + wt) * a.hq + h * G + wg
+                                   : (int64_t)2 * a.tokens * a.hq +
+                                         (((int64_t)h * a.blocks + blk) * 2 + (run == 0 ? 1 : 0)) * kQ + wpair;
+      float *op = a.part_acc + at * kHeadDim + 4 * whl;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          *reinterpret_cast<f32x4 *>(op + 32 * dt + 8 * q4) =
+              f32x4{acc[dt][4 * q4], acc[dt][4 * q4 + 1], acc[dt][4 * q4 + 2], acc[dt][4 * q4 + 3]};
+      if (whl == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = float2{m, l};
+    }
+    if (h == 0 && run == 0 && (int)threadIdx.x < ntok) {
+      const int i = threadIdx.x, ti = of_prefix ? line.toks[i] : q0 + t0 + i;
+      a.runs[(of_prefix ? 0 : a.tokens) + ti] = int2{first_blk, runs | (i * G) << 16};
+      if (!of_prefix && px < 0) a.runs[ti] = int2{0, 0};
+    }
+    __syncthreads();  // the next piece lists its tokens and loads its pages
   }
 }
 
-// Joins the runs of each (token, q head): one wave each, lane i reading slot i's (m, l) (the prefix's runs from lane
-// 0 on, the row's own from lane kMaxSplits on), then two of the 128 outputs per lane over all runs.
+// Joins the runs of each (token, q head), one wave each: lane e holds entry e's row and (m, l), the prefix's runs
+// first, then the own tile's; then every lane sums two of the 128 outputs over the entries.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) prefix_merge_kernel(PrefixArgs a) {
   using E = Elem<DT>;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (row >= (int64_t)a.tokens * a.hq) return;
   const int t = uniform((int)(row / a.hq)), hq = uniform((int)(row % a.hq));
-  const int lane = threadIdx.x & 63;
-  // (a query token of no row is left as it was; the limits keep a table that is no CSR inside the slots)
+  // A query token of no row is left as it was.
   if (a.qo_indptr && (t < a.qo_indptr[0] || t >= a.qo_indptr[a.batch])) return;
-  const int runs = uniform(a.tok_runs[t]);
-  const int np = min(runs & 0xffff, a.splits), no = min((runs >> 16) & 0xffff, a.splits);
-  const int64_t stride = (int64_t)a.tokens * a.hq, at = (int64_t)t * a.hq + hq;
-  const bool own = lane >= kMaxSplits;
-  const int s = own ? lane - kMaxSplits : lane;
-  const bool have = s < (own ? no : np);
-  float ms = -INFINITY, ls = 0.f;
-  if (have) {
-    const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + ((own ? a.splits + s : s) * stride + at) * 2);
-    ms = ml.x;
-    ls = ml.y;
+  const int lane = threadIdx.x & 63;
+  const int G = a.hq / a.hkv, h = hq / G, g = hq - h * G;
+  int first[2], count[2], pair[2];
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {  // (the limits keep a table that is no CSR inside the partials)
+    const int2 x = a.runs[kind * a.tokens + t];
+    first[kind] = uniform(min(max(x.x, 0), a.blocks - 1));
+    count[kind] = uniform(min(x.y & 0xffff, a.blocks - first[kind]));
+    pair[kind] = uniform(min((x.y >> 16) & 0xffff, kQ - G)) + g;
   }
-  float M = ms;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, shfl_xor(M, off));
-  const float w = fast_exp2(ms - (M == -INFINITY ? 0.f : M));  // 0 where nothing was attended
-  float L = ls * w;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) L += shfl_xor(L, off);
+  const int n = count[0] + count[1];
+  if (count[0] == 0 && count[1] == 1) return;  // written by its tile
+  float M = -INFINITY, L = 0.f;
   float2 A = {0.f, 0.f};
-  auto add = [&](int slot, int from) {
-    const float2 x = *reinterpret_cast<const float2 *>(a.part_acc + (slot * stride + at) * kHeadDim + 2 * lane);
-    const float ws = readlane(w, from);
-    A.x = fmaf(x.x, ws, A.x);
-    A.y = fmaf(x.y, ws, A.y);
-  };
-  for (int i = 0; i < np; ++i) add(i, i);
-  for (int i = 0; i < no; ++i) add(a.splits + i, kMaxSplits + i);
+  for (int e0 = 0; e0 < n; e0 += 64) {
+    const int e = e0 + lane;
+    const bool have = e < n, own = have && e >= count[0];
+    const int r = !have ? 0 : (own ? e - count[0] : e), kind = own || count[0] == 0 ? 1 : 0;
+    const int of = count[kind], b0 = first[kind], pr = pair[kind];
+    const int64_t at = of == 1 ? (int64_t)(kind * a.tokens + t) * a.hq + hq
+                               : (int64_t)2 * a.tokens * a.hq + (((int64_t)h * a.blocks + b0 + r) * 2 + (r == 0)) * kQ + pr;
+    const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
+    const float ms = have ? ml.x : -INFINITY;
+    float cm = fmaxf(M, ms);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) cm = fmaxf(cm, shfl_xor(cm, off));
+    const float ref = cm == -INFINITY ? 0.f : cm, al = fast_exp2(M - ref);
+    const float w = fast_exp2(ms - ref);  // 0 where nothing was attended
+    float s = ml.y * w;
+    s = have ? s : 0.f;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += shfl_xor(s, off);
+    L = L * al + s;
+    A.x *= al;
+    A.y *= al;
+    M = cm;
+    const int lim = min(64, n - e0), at32 = (int)at;  // (rows: below 2^31, checked on the host)
+    for (int i0 = 0; i0 < lim; i0 += 8) {
+      float2 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t from = __builtin_amdgcn_readlane(at32, min(i0 + k, lim - 1));
+        v[k] = *reinterpret_cast<const float2 *>(a.part_acc + from * kHeadDim + 2 * lane);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float ws = i0 + k < lim ? readlane(w, min(i0 + k, 63)) : 0.f;
+        A.x = fmaf(v[k].x, ws, A.x);
+        A.y = fmaf(v[k].y, ws, A.y);
+      }
+    }
+  }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint32_t *op = reinterpret_cast<uint32_t *>(a.o + (int64_t)t * a.o_stride_t + (int64_t)hq * a.o_stride_h);
   op[lane] = E::from_float(A.x * inv) | (E::from_float(A.y * inv) << 16);
-  if (lane == 0 && a.lse) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  if (lane == 0 && a.lse) a.lse[(int64_t)t * a.hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
-// Runs per segment that can be useful: as many as fill the chip when the tokens share one prefix, none shorter than
-// kMinChunk steps.
-int plan_splits(int64_t tokens, int hq, int hkv, int64_t max_pages) {
-  const int64_t tiles = ceil_div(tokens * (hq / hkv), kQ);
-  int64_t n = ceil_div(ceil_div(kSlots, hkv), tiles > 0 ? tiles : 1);
-  const int64_t most = ceil_div(ceil_div(max_pages, kPages), kMinChunk);
-  n = n < most ? n : most;
-  return (int)(n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n));
+// Blocks per kv head: as many as the chip holds, or as the longest line of `tokens` query tokens over rows of
+// `max_pages` fills with kMinShare steps each.
+int plan_blocks(int64_t tokens, int hkv, int64_t max_pages) {
+  const int64_t fill = kSlots / hkv > 0 ? kSlots / hkv : 1;
+  const int64_t steps = ceil_div(max_pages, kPages) + kTileCost;
+  if (steps >= fill * kMinShare || 2 * tokens >= fill * kMinShare) return (int)fill;
+  const int64_t n = ceil_div(2 * tokens * steps, kMinShare);
+  return (int)(n < fill ? n : fill);
 }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-size_t workspace_bytes_for(int64_t tokens, int hq, int splits) {
-  const size_t rows = (size_t)2 * splits * tokens * hq;
+size_t partial_rows(int64_t tokens, int hq, int hkv, int blocks) {
+  return (size_t)2 * tokens * hq + (size_t)hkv * blocks * 2 * kQ;
+}
+
+size_t workspace_bytes_for(int64_t tokens, int hq, int hkv, int blocks) {
+  const size_t rows = partial_rows(tokens, hq, hkv, blocks);
   return align256(rows * 2 * sizeof(float)) + align256(rows * kHeadDim * sizeof(float)) +
-         align256((size_t)tokens * sizeof(int32_t));
+         align256((size_t)2 * tokens * sizeof(int2));
 }
 
 template <int DT, int G>
 void launch_g(const PrefixArgs &a, hipStream_t stream) {
-  // Every unit of plan_unit: at most total / chunk (<= target) and one per (segment, tile).
-  const int64_t tiles = ceil_div((int64_t)a.tokens * G, kQ);
-  const int64_t units = a.target + 2 * tiles + a.batch + (a.num_prefixes < a.batch ? a.num_prefixes : a.batch);
-  const int64_t y = units < 32768 ? units : 32768;
-  hipLaunchKernelGGL((prefix_attention_kernel<DT, G>), dim3((unsigned)a.hkv, (unsigned)y, (unsigned)ceil_div(units, y)),
-                     dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((prefix_attention_kernel<DT, G>), dim3((unsigned)a.hkv, (unsigned)a.blocks), dim3(kThreads), 0, stream,
+                     a);
 }
 
 template <int DT>
@@ -663,7 +769,12 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
   if (num_pages <= 0 || kv_indices_len < 0 || px->indices_len < 0 || kv_indices_len > INT32_MAX / kPageSize ||
       px->indices_len > INT32_MAX / kPageSize)
     return set_error(DELTA_ERR_INVALID, "%s: empty cache or bad table lengths", who);
-  if (tokens * G > INT32_MAX / 2) return set_error(DELTA_ERR_INVALID, "%s: too many query tokens", who);
+  // The line's length and the partials' rows stay below 2^30 (tiles of the rows and of the prefixes, each at most the
+  // longest list's steps).
+  const int64_t longest = kv_indices_len > px->indices_len ? kv_indices_len : px->indices_len;
+  if (tokens > 1 << 23 || 2 * (ceil_div(tokens, kQ / G) + batch) * (ceil_div(longest, kPages) + kTileCost + 1) > 1 << 30 ||
+      partial_rows(tokens, hq, hkv, kSlots) > 1 << 30)
+    return set_error(DELTA_ERR_INVALID, "%s: too many query tokens", who);
   PrefixArgs a;
   a.q = (const uint16_t *)q;
   a.q_stride_t = q_stride_t;
@@ -688,20 +799,19 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
   a.tokens = (int)tokens;
   a.hq = hq;
   a.hkv = hkv;
-  a.splits = plan_splits(tokens, hq, hkv, max_pages);
-  a.target = (int)ceil_div(kSlots, hkv);
+  a.blocks = plan_blocks(tokens, hkv, max_pages);
   a.sm_scale = sm_scale;
-  const size_t need = workspace_bytes_for(tokens, hq, a.splits);
+  const size_t need = workspace_bytes_for(tokens, hq, hkv, a.blocks);
   if (!workspace || workspace_bytes < need)
     return set_error(DELTA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
   if ((uintptr_t)workspace & 255u) return set_error(DELTA_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
-  const size_t rows = (size_t)2 * a.splits * tokens * hq;
+  const size_t rows = partial_rows(tokens, hq, hkv, a.blocks);
   char *ws = (char *)workspace;
   a.part_ml = (float *)ws;
   ws += align256(rows * 2 * sizeof(float));
   a.part_acc = (float *)ws;
   ws += align256(rows * kHeadDim * sizeof(float));
-  a.tok_runs = (int32_t *)ws;
+  a.runs = (int2 *)ws;
   if (dtype == DELTA_BF16)
     launch<DELTA_BF16>(a, G, (hipStream_t)stream);
   else
@@ -715,8 +825,8 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
 extern "C" DELTA_EXPORT size_t delta_prefix_attention_workspace_bytes(int64_t tokens, int num_qo_heads,
                                                                       int num_kv_heads, int64_t max_pages) {
   if (tokens <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads || max_pages < 0) return 0;
-  return delta::workspace_bytes_for(tokens, num_qo_heads,
-                                    delta::plan_splits(tokens, num_qo_heads, num_kv_heads, max_pages));
+  return delta::workspace_bytes_for(tokens, num_qo_heads, num_kv_heads,
+                                    delta::plan_blocks(tokens, num_kv_heads, max_pages));
 }
 
 extern "C" DELTA_EXPORT int delta_paged_decode_prefix(
