@@ -19,9 +19,9 @@
 // (m, l, a): a whole tile at its token's place, a cut one into its block's two buffers (a block's first piece may
 // end a cut tile, its last may begin one); the merge kernel joins them per (token, q head).
 //
-// Per block: 4 waves.  Tiles of more than 32 pairs share each step's K and V in LDS, the next step in flight (64 KiB):
-// with more than 64 pairs every wave owns 32 of them and sweeps the whole step, with 33-64 two waves share 32 pairs
-// and take 32 tokens of the step each.  Tiles of up to 32 pairs (a decode row's own pages) are bound by HBM: each wave
+// Per block: 4 waves.  Tiles of more than 32 pairs share K and V in LDS, in stages of 32 tokens, three under way (64
+// KiB): with more than 64 pairs every wave owns 32 of them and sweeps every stage, with 33-64 two waves share 32 pairs
+// and take every other stage.  Tiles of up to 32 pairs (a decode row's own pages) are bound by HBM: each wave
 // streams every fourth page through 16 KiB of its own, one page ahead, without barriers, and the waves are joined in
 // LDS at the end.  MFMA tiles as in prefill.hip: S^T = K Q^T with lane l holding query pair l % 32 and 16 tokens per
 // 32, O^T += V^T P^T, P rounded to the cache's type for the product as there (the sums l stay unrounded fp32).
@@ -37,8 +37,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kStep = 64;               // kv tokens per step
 constexpr int kPages = kStep / kPageSize;
-constexpr int kTileB = kStep * 256;     // bytes of a step's K (or V) tile: 64 rows of 256 bytes
 constexpr int kPageB = kPageSize * 256; // bytes of a page's K (or V) of one head
+constexpr int kStageB = 4 * kPageB;     // a stage: 32 tokens' K, then their V
+constexpr int kStages = 4;              // stages in LDS
 constexpr int kQ = 128;                 // (token, head) pairs of a tile, at most
 constexpr int kMaxRows = 1024;          // rows, and prefixes, of a call (the line's tables)
 constexpr int kSlots = 512;             // blocks the chip holds (two per CU)
@@ -201,14 +202,14 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   using MF = Mfma32<DT>;
   using E = Elem<DT>;
   constexpr int TT = kQ / G;  // query tokens of a tile
-  // Two steps' buffers, each the K tile, then the V tile (swizzled rows); or per wave two pages' buffers.  The waves'
+  // A ring of stages, each the K tile, then the V tile (swizzled rows); or per wave two pages' buffers.  The waves'
   // accumulators where they are joined.
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2 * kTileB];
+  __shared__ __attribute__((aligned(1024))) char tiles[kStages * kStageB];
   __shared__ Line line;
 
   const int wv = uniform((int)(threadIdx.x >> 6));
   const int h = blockIdx.x, blk = blockIdx.y;
-  const int total = uniform(build_line<TT>(a, line, reinterpret_cast<int *>(&tiles[0][0])));
+  const int total = uniform(build_line<TT>(a, line, reinterpret_cast<int *>(&tiles[0])));
   int share = uniform(div_up(total, a.blocks));
   share = share < kMinShare ? kMinShare : share;
   int pos = blk * share;  // (total < 2^30: checked on the host)
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   // slot ch ^ (r % 16) and of V row r at ch ^ 4 (r % 4), so that the fragment reads cover the banks once.
   const uint32_t row_bytes = (uint32_t)a.hkv * kHeadDim * 2;
   const uint32_t page_bytes = 2 * kPageSize * row_bytes;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&tiles[0][0];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&tiles[0];
   const char *const kvh = reinterpret_cast<const char *>(a.kv) + (int64_t)h * (kHeadDim * 2);
   const uint32_t num_pages = a.num_pages < INT32_MAX ? (uint32_t)a.num_pages : (uint32_t)INT32_MAX;
   const float scale2 = a.sm_scale == 0.f ? 1.f : fabsf(a.sm_scale) * kLog2e;
@@ -447,19 +448,19 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       const int p0 = kPages * s0 + wv, p1 = min(np, kPages * s1);
       const int count = p0 < p1 ? (p1 - p0 + 3) >> 2 : 0;
       const uint32_t wlds = lds0 + wv * (4 * kPageB);
-      char *const wbuf = &tiles[0][0] + wv * (4 * kPageB);
+      char *const wbuf = &tiles[0] + wv * (4 * kPageB);
       uint32_t koff[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) koff[i] = (4 * i + lrow) * row_bytes + 16 * ((lch ^ lrow) ^ (4 * i));
       const uint32_t voff = (kPageSize + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
       auto issue_k = [&](const char *pg, int buf) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load_lds_1k(wlds + buf * 2 * kPageB + i * 1024, pg, koff[i]);
+        for (int i = 0; i < 4; ++i) load_lds_1k<true>(wlds + buf * 2 * kPageB + i * 1024, pg, koff[i]);
       };
       auto issue_v = [&](const char *pg, int buf) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          load_lds_1k(wlds + buf * 2 * kPageB + kPageB + i * 1024, pg, voff + (uint32_t)(4 * i) * row_bytes);
+          load_lds_1k<true>(wlds + buf * 2 * kPageB + kPageB + i * 1024, pg, voff + (uint32_t)(4 * i) * row_bytes);
       };
       uint64_t bad = 0;
       int idv = load_ids(p0, 4, count, 0, &bad);
@@ -503,86 +504,89 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
         if (((k + 1) & 63) == 0) bad = bad_next;
       }
     } else {
-      // Shared steps: wave w loads rows 4 w .. + 3 of each of the step's four pages, K and V.
+      // Shared stages: wave w loads rows 4 w .. + 3 of both of a stage's pages, K and V; three stages are under way
+      // while one is worked on.  (Waves that share pairs take every other stage.)
       const uint32_t wlds = lds0 + wv * 1024;
       const uint32_t koff = (4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * wv + lrow));
       const uint32_t voff = (kPageSize + 4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
-      const int p0 = kPages * s0, count = min(np, kPages * s1) - p0;  // <= 0: no step
-      uint64_t bad = 0, bad_next = 0;
-      int idv = 0;
-      auto issue = [&](int j) {  // step j of the piece; pages past the segment repeat page 0 of the window (masked later)
+      const int p0 = kPages * s0, count = min(np, kPages * s1) - p0;  // <= 0: no page
+      const int nst = count > 0 ? (count + 1) >> 1 : 0;
+      uint64_t bad = 0, bad_next;
+      int idv = load_ids(p0, 1, count, 0, &bad);
+      bad_next = bad;
+      auto issue = [&](int j) {  // stage j of the piece; a page past it is page 0 of the cache (masked later)
+        const uint32_t dst = wlds + (uint32_t)(j & (kStages - 1)) * kStageB;
 #pragma unroll
-        for (int i = 0; i < kPages; ++i) {
-          const char *pg = page_base(__builtin_amdgcn_readlane(idv, (kPages * j + i) & 63));
-          const uint32_t dst = wlds + (uint32_t)(j & 1) * (2 * kTileB) + i * kPageB;
-          load_lds_1k(dst, pg, koff);
-          load_lds_1k(dst + kTileB, pg, voff);
+        for (int i = 0; i < 2; ++i) {
+          const char *pg = page_base(__builtin_amdgcn_readlane(idv, (2 * j + i) & 63));
+          load_lds_1k(dst + i * kPageB, pg, koff);
+          load_lds_1k(dst + 2 * kPageB + i * kPageB, pg, voff);
         }
       };
-      const int nst = s1 > s0 ? s1 - s0 : 0;
-      if (nst > 0) {
-        idv = load_ids(p0, 1, count, 0, &bad);
-        bad_next = bad;
-        issue(0);
-      }
+      for (int j = 0; j < 3 && j < nst; ++j) issue(j);
       for (int j = 0; j < nst; ++j) {
-        wait_loads<0>();
+        if (j + 2 < nst)
+          wait_loads<8>();
+        else if (j + 1 < nst)
+          wait_loads<4>();
+        else
+          wait_loads<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const uint32_t sbad = (uint32_t)(bad >> ((kPages * j) & 63)) & 15u;
-        if (j + 1 < nst) {
-          if (((j + 1) & 15) == 0) idv = load_ids(p0, 1, count, (j + 1) >> 4, &bad_next);
-          issue(j + 1);
+        const uint32_t sbad = (uint32_t)(bad >> ((2 * j) & 63)) & 3u;
+        if (j + 3 < nst) {  // into the buffer of stage j - 1, which every wave has left
+          if (((j + 3) & 31) == 0) idv = load_ids(p0, 1, count, (j + 3) >> 5, &bad_next);
+          issue(j + 3);
         }
-        const int kv0 = (s0 + j) * kStep;
-        char *const buf = &tiles[j & 1][0];
-        if (kv0 + kStep > len || sbad != 0) {
-          const int r = (int)threadIdx.x >> 2;
+        const int kv0 = s0 * kStep + 32 * j;
+        char *const buf = &tiles[(j & (kStages - 1)) * kStageB];
+        if (kv0 + 32 > len || sbad != 0) {
+          // V rows past the segment and of pages outside the cache meet p = 0 but may hold NaN/Inf: zeros.
+          const int r = (int)threadIdx.x >> 3;
           if (kv0 + r >= len || ((sbad >> (r >> 4)) & 1u)) {
-            char *vr = buf + kTileB + r * 256 + 64 * ((int)threadIdx.x & 3);
+            char *vr = buf + 2 * kPageB + r * 256 + 32 * ((int)threadIdx.x & 7);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
+            for (int i = 0; i < 2; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
           }
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
         }
-        if (active) {
-          if (groups == 4)
-            sweep(std::integral_constant<int, 64>(), kv0, buf, buf + kTileB, sbad);
-          else
-            sweep(std::integral_constant<int, 32>(), kv0 + 32 * half, buf + half * 8192, buf + kTileB + half * 8192,
-                  sbad >> (2 * half));
-        }
-        if (((j + 1) & 15) == 0) bad = bad_next;
+        if (active && (groups == 4 || (j & 1) == half))
+          sweep(std::integral_constant<int, 32>(), kv0, buf, buf + 2 * kPageB, sbad);
+        if (((j + 1) & 31) == 0) bad = bad_next;
       }
     }
 
     l = halves_sum(l);
     if (groups < 4) {
-      // Join the waves that share pairs: wave qsub + groups k, k > 0, hands (m, l, acc) to wave qsub through LDS.
-      float *const buf = reinterpret_cast<float *>(&tiles[0][0]) + lane;
-      constexpr int kOne = 66 * 64;  // floats of a wave
-      for (int w = 1; w < 4 / groups; ++w) {
+      // Join the waves that share pairs (wave qsub + groups k), in halves: (m, l, acc) through LDS.
+      constexpr int kOne = 17 * 64;  // f32x4 of a wave
+      f32x4 *const all = reinterpret_cast<f32x4 *>(&tiles[0]) + lane;
+      const int k = wv / groups;
+#pragma unroll 1
+      for (int ks = 1; ks * groups < 4; ks *= 2) {
         __syncthreads();
-        float *const at = buf + qsub * kOne;
-        if (wv == qsub + groups * w) {
+        if ((k & ks) && !(k & (ks - 1))) {
+          f32x4 *const at = all + (wv - ks * groups) * kOne;
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) at[64 * (16 * dt + i)] = acc[dt][i];
-          at[64 * 64] = m;
-          at[64 * 65] = l;
+          for (int i = 0; i < 16; ++i)
+            at[64 * i] = f32x4{acc[i >> 2][4 * (i & 3)], acc[i >> 2][4 * (i & 3) + 1], acc[i >> 2][4 * (i & 3) + 2],
+                               acc[i >> 2][4 * (i & 3) + 3]};
+          at[64 * 16] = f32x4{m, l, 0.f, 0.f};
         }
         __syncthreads();
-        if (wv < groups) {
-          const float m2 = at[64 * 64], l2 = at[64 * 65];
+        if (!(k & (2 * ks - 1))) {
+          const f32x4 *const at = all + wv * kOne;
+          const float m2 = at[64 * 16][0], l2 = at[64 * 16][1];
           const float M = fmaxf(m, m2), ref = M == -INFINITY ? 0.f : M;
           const float w1 = fast_exp2(m - ref), w2 = fast_exp2(m2 - ref);
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt)
+          for (int i = 0; i < 16; ++i) {
+            const f32x4 x = at[64 * i];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * w1 + at[64 * (16 * dt + i)] * w2;
+            for (int e = 0; e < 4; ++e) acc[i >> 2][4 * (i & 3) + e] = acc[i >> 2][4 * (i & 3) + e] * w1 + x[e] * w2;
+          }
           l = l * w1 + l2 * w2;
           m = M;
         }
