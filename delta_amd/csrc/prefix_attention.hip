@@ -19,14 +19,11 @@
 // (m, l, a): a whole tile at its token's place, a cut one into its block's two buffers (a block's first piece may
 // end a cut tile, its last may begin one); the merge kernel joins them per (token, q head).
 //
-// Per block: 4 waves.  Tiles of more than 32 pairs share K and V in LDS, in stages of 32 tokens, three under way (64
-// KiB): with more than 64 pairs every wave owns 32 of them and sweeps every stage, with 33-64 two waves share 32 pairs
-// and take every other stage.  Tiles of up to 32 pairs (a decode row's own pages) are bound by HBM: each wave
-// streams every fourth page through 16 KiB of its own, one page ahead, without barriers, and the waves are joined in
-// LDS at the end.  MFMA tiles as in prefill.hip: S^T = K Q^T with lane l holding query pair l % 32 and 16 tokens per
-// 32, O^T += V^T P^T, P rounded to the cache's type for the product as there (the sums l stay unrounded fp32).
-#include <type_traits>
-
+// Per block: 4 waves, each with 32 of the tile's pairs, share K and V in LDS, in stages of 32 tokens, two or three of
+// them under way (64 KiB, two blocks per CU); waves without pairs (a decode row's own pages have G) only load.  MFMA
+// tiles as in prefill.hip: S^T = K Q^T with lane l holding query pair l % 32 and 16 of the 32 tokens, O^T += V^T P^T, P
+// rounded to the cache's type for the product as there (the sums l stay unrounded fp32).  The S of a stage are computed
+// under the softmax of the stage before.
 #include "delta_common.h"
 #include "mfma32.h"
 
@@ -202,8 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   using MF = Mfma32<DT>;
   using E = Elem<DT>;
   constexpr int TT = kQ / G;  // query tokens of a tile
-  // A ring of stages, each the K tile, then the V tile (swizzled rows); or per wave two pages' buffers.  The waves'
-  // accumulators where they are joined.
+  // A ring of stages, each the K tile, then the V tile (swizzled rows).
   __shared__ __attribute__((aligned(1024))) char tiles[kStages * kStageB];
   __shared__ Line line;
 
@@ -225,8 +221,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   const float scale2 = a.sm_scale == 0.f ? 1.f : fabsf(a.sm_scale) * kLog2e;
   int item = 0;
   while (pos < end) {
-    // The lane, hidden from the compiler: it would keep every offset that follows from it in registers over all pieces
-    // (55 of them spilled).
+    // The lane, hidden from the compiler: it would keep every offset that follows from it in registers over all pieces.
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int hl = lane >> 5, n = lane & 31, lrow = lane >> 4, lch = lane & 15;
@@ -309,22 +304,71 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     }
     __syncthreads();  // the tile's tokens are listed, the piece before is done with the buffers
 
-    // ---- The wave's pairs (32 from 32 qsub on), and the 32-token half of each step that it takes.
-    const int groups = pairs > 64 ? 4 : (pairs > 32 ? 2 : 1);
-    const int qsub = wv & (groups - 1);
-    const int half = groups == 2 ? wv >> 1 : 0;
+    // ---- The wave's pairs: 32 from 32 qsub on.  (Which wave has the first ones goes round with the block: a short tile
+    // keeps one wave, and with it one SIMD, at work.)
+    const int qsub = (wv + blk) & 3;
     const bool active = 32 * qsub < pairs;
     const int pair = 32 * qsub + n;
     const bool row_ok = pair < pairs;
     const int pt = row_ok ? pair / G : 0, g = row_ok ? pair % G : 0;
     const int t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
     const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);  // the last position that the lane's pair attends
-    // Steps that end at or below the position of the wave's first token need no mask.
+    // Stages that end at or below the position of the wave's first token need no mask.
     const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos + 32 * qsub / G);
+
+    // Loads: wave w loads rows 4 w .. + 3 of both of a stage's pages, K and V.  Page ids, 64 per register (lane i: page
+    // 64 w + i of the piece); bit i of *bad: outside the cache.
+    const uint32_t wlds = lds0 + wv * 1024;
+    const uint32_t koff = (4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * wv + lrow));
+    const uint32_t voff = (kPageSize + 4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
+    const int p0 = kPages * s0, count = min(np, kPages * s1) - p0;  // <= 0: no page
+    const int nst = count > 0 ? (count + 1) >> 1 : 0;
+    auto load_ids = [&](int w, uint64_t *bad) {
+      const int i = 64 * w + lane;
+      const int id = i < count ? ids[p0 + i] : 0;
+      const bool ok = (uint32_t)id < num_pages;
+      *bad = __ballot(!ok);
+      return ok ? id : 0;
+    };
     u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
-    const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
+    {
+      const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qf[ks] = row_ok ? ld128(qp + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
+      for (int ks = 0; ks < 8; ++ks) qf[ks] = row_ok ? ld128(qp + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
+    }
+    uint64_t bad = 0, bad_next;
+    int idv = load_ids(0, &bad);
+    // Settles q with the page ids: inside the loop its wait would also drain the stages under way.
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(qf[ks]));
+    bad_next = bad;
+    auto issue = [&](int j) {  // stage j of the piece; a page past it is page 0 of the cache (masked later)
+      const uint32_t dst = wlds + (uint32_t)(j & (kStages - 1)) * kStageB;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const char *pg = uniform_ptr(kvh + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(idv, (2 * j + i) & 63) * page_bytes);
+        if (of_prefix) {
+          load_lds_1k(dst + i * kPageB, pg, koff);
+          load_lds_1k(dst + 2 * kPageB + i * kPageB, pg, voff);
+        } else {  // read once
+          load_lds_1k<true>(dst + i * kPageB, pg, koff);
+          load_lds_1k<true>(dst + 2 * kPageB + i * kPageB, pg, voff);
+        }
+      }
+    };
+    for (int j = 0; j < 3 && j < nst; ++j) issue(j);
+    auto bad_of = [&](int j) { return (uint32_t)(bad >> ((2 * j) & 63)) & 3u; };  // bit i: page i of stage j
+    // V rows past the segment and of pages outside the cache meet p = 0 but may hold NaN/Inf: zeros.
+    auto clear_v = [&](int j, uint32_t sbad) {
+      const int kv0 = s0 * kStep + 32 * j;
+      if (kv0 + 32 <= len && sbad == 0) return;
+      const int r = (int)threadIdx.x >> 3;
+      if (kv0 + r >= len || ((sbad >> (r >> 4)) & 1u)) {
+        char *vr = &tiles[(j & (kStages - 1)) * kStageB + 2 * kPageB] + r * 256 + 32 * ((int)threadIdx.x & 7);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
+      }
+    };
 
     float m = -INFINITY, l = 0.f;
     f32x16 acc[4];
@@ -333,87 +377,99 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
-    // NT tokens from segment position kv0 on, K rows at tk, V rows at tv: scores, online softmax, P.V.  Bit i of bad:
-    // page i of them lies outside the cache.  (NT = 16: fragment rows 16-31 repeat 0-15 and their scores are not used.)
-    auto sweep = [&](auto nt, int kv0, const char *tk, const char *tv, uint32_t bad) {
-      constexpr int NT = decltype(nt)::value, NS = NT >= 32 ? NT / 32 : 1, NX = NT / 2;
-      f32x16 S[NS];
+    // S^T of a stage: K fragments three k-slices ahead of their MFMAs.
+    auto scores = [&](int j, f32x16 &S) {
+      const char *tk = &tiles[(j & (kStages - 1)) * kStageB];
+      u32x4 kq[4];
 #pragma unroll
-      for (int sb = 0; sb < NS; ++sb)
+      for (int s = 0; s < 3; ++s) kq[s] = *reinterpret_cast<const u32x4 *>(tk + kfo[s]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[sb][i] = 0.f;
-      auto kfrag = [&](int sb, int ks) {
-        return *reinterpret_cast<const u32x4 *>(tk + (NT == 16 ? kfo[ks] & (kPageB - 1) : kfo[ks]) + sb * 8192);
-      };
-      constexpr int kKAhead = 3;
-      u32x4 kq[kKAhead + 1][NS];
-#pragma unroll
-      for (int s = 0; s < kKAhead; ++s)
-#pragma unroll
-        for (int sb = 0; sb < NS; ++sb) kq[s][sb] = kfrag(sb, s);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < 16; ++i) S[i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        if (ks + kKAhead < 8) {
-#pragma unroll
-          for (int sb = 0; sb < NS; ++sb) kq[(ks + kKAhead) % (kKAhead + 1)][sb] = kfrag(sb, ks + kKAhead);
-        }
-#pragma unroll
-        for (int sb = 0; sb < NS; ++sb) S[sb] = MF::run(kq[ks % (kKAhead + 1)][sb], qf[ks], S[sb]);
-        __builtin_amdgcn_sched_barrier(0);
+        if (ks + 3 < 8) kq[(ks + 3) & 3] = *reinterpret_cast<const u32x4 *>(tk + kfo[ks + 3]);
+        S = MF::run(kq[ks & 3], qf[ks], S);
       }
-      const bool full = kv0 + NT - 1 <= wpos;
-      float x[NX];
+    };
+    f32x16 S;  // of the stage worked on
+    if (nst > 0) {
+      if (nst > 2)
+        wait_loads<8>();
+      else if (nst > 1)
+        wait_loads<4>();
+      else
+        wait_loads<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      clear_v(0, bad_of(0));
+      if (active) scores(0, S);
+    }
+    for (int j = 0; j < nst; ++j) {
+      // Stage j + 1 has landed, stage j - 1 is left by every wave.
+      if (j + 2 < nst)
+        wait_loads<4>();
+      else
+        wait_loads<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const uint32_t sbad = bad_of(j);
+      if (((j + 1) & 31) == 0) bad = bad_next;
+      if (j + 3 < nst) {
+        if (((j + 3) & 31) == 0) idv = load_ids((j + 3) >> 5, &bad_next);
+        issue(j + 3);
+      }
+      if (j + 1 < nst) clear_v(j + 1, bad_of(j + 1));
+      if (!active) continue;
+      const int kv0 = s0 * kStep + 32 * j;
+      float x[16];
 #pragma unroll
-      for (int i = 0; i < NX; ++i) x[i] = S[i >> 4][i & 15];
+      for (int i = 0; i < 16; ++i) x[i] = S[i];
       if (!(a.sm_scale > 0.f)) {  // (the scale below is positive)
         const float sign = a.sm_scale == 0.f ? 0.f : -1.f;
 #pragma unroll
-        for (int i = 0; i < NX; ++i) x[i] *= sign;
+        for (int i = 0; i < 16; ++i) x[i] *= sign;
       }
-      auto tok = [&](int i) { return 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3); };  // of x[i], from kv0 + 4 hl on
-      if (!full) {
+      auto tok = [&](int i) { return 8 * (i >> 2) + (i & 3); };  // of x[i], from kv0 + 4 hl on
+      if (kv0 + 31 > wpos) {
         const int last = lim - kv0 - 4 * hl;
 #pragma unroll
-        for (int i = 0; i < NX; ++i) x[i] = tok(i) <= last ? x[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) x[i] = tok(i) <= last ? x[i] : -INFINITY;
       }
-      if (bad) {
-        uint32_t b = bad;  // (in a vector register: selects, not a branch for each value)
+      if (sbad) {
+        uint32_t b = sbad;  // (in a vector register: selects, not a branch for each value)
         asm volatile("" : "+v"(b));
 #pragma unroll
-        for (int i = 0; i < NX; ++i) x[i] = (b >> (tok(i) >> 4)) & 1u ? -INFINITY : x[i];
+        for (int i = 0; i < 16; ++i) x[i] = (b >> (i >> 3)) & 1u ? -INFINITY : x[i];
       }
+      // The next stage's S (of no use behind the last stage), an MFMA at a time between pieces of this one's softmax:
+      // each piece runs while its MFMA does.  The fences keep that order.
+      const char *tk = &tiles[((j + 1) & (kStages - 1)) * kStageB];
+      auto kfrag = [&](int ks) { return *reinterpret_cast<const u32x4 *>(tk + kfo[ks]); };
+      u32x4 kq[4];
+#pragma unroll
+      for (int ks = 0; ks < 3; ++ks) kq[ks] = kfrag(ks);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[i] = 0.f;
+      auto mfma_s = [&](int ks) {
+        if (ks + 3 < 8) kq[(ks + 3) & 3] = kfrag(ks + 3);
+        S = MF::run(kq[ks & 3], qf[ks], S);
+        __builtin_amdgcn_sched_barrier(0);
+      };
       float pm = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < NX; ++i) pm = fmaxf(pm, x[i]);
+      for (int i = 0; i < 16; ++i) pm = fmaxf(pm, x[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma_s(0);
       // m is a reference maximum: it moves only when a score exceeds it by more than 8 (log2), so the exponentials
-      // stay <= 256 and the accumulators are rescaled on few steps.
+      // stay <= 256 and the accumulators are rescaled on few stages.
       const float smax = halves_max(pm) * scale2;
-      float alpha = 1.f;
-      if (smax > m + 8.f) {  // also the first finite score (m = -inf)
-        alpha = fast_exp2(m - smax);
-        m = smax;
-      }
+      const bool moves = smax > m + 8.f;  // also the first finite score (m = -inf)
+      const float alpha = moves ? fast_exp2(m - smax) : 1.f;
+      m = moves ? smax : m;
       const float nm = m == -INFINITY ? 0.f : -m;
-      float ps = 0.f;
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        x[i] = fast_exp2(fmaf(x[i], scale2, nm));
-        ps += x[i];
-      }
-      l = l * alpha + ps;  // this half-wave's tokens; joined once at the end
-      if (__ballot(alpha != 1.f)) {
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
-      }
-      constexpr int NC = NT / 16;
-      u32x4 pc[NC];
-#pragma unroll
-      for (int cc = 0; cc < NC; ++cc)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) pc[cc][w] = pack2<DT>(x[8 * cc + 2 * w], x[8 * cc + 2 * w + 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma_s(1);
+      const char *tv = &tiles[(j & (kStages - 1)) * kStageB + 2 * kPageB];
       auto vfrag = [&](int i) {  // V^T fragment of 16-token chunk i / 4, d tile i % 4
         const char *rd = tv + vfo[i % 4] + (i / 4) * 4096;
         const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
@@ -421,183 +477,47 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
         const uint2 lo = __builtin_bit_cast(uint2, v0), hi = __builtin_bit_cast(uint2, v1);
         return u32x4{lo.x, lo.y, hi.x, hi.y};
       };
-      constexpr int kAhead = 4 * NC < 4 ? 4 * NC : 4;
+      constexpr int kAhead = 4;
       u32x4 vq[kAhead + 1];
+      float ps = 0.f;
+      u32x4 pc[2];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) vq[i] = vfrag(i);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int c = 0; c < 8; ++c) {
+        x[2 * c] = fast_exp2(fmaf(x[2 * c], scale2, nm));
+        x[2 * c + 1] = fast_exp2(fmaf(x[2 * c + 1], scale2, nm));
+        if (c > 0) {
+          ps += x[2 * c - 2] + x[2 * c - 1];
+          pc[(c - 1) >> 2][(c - 1) & 3] = pack2<DT>(x[2 * c - 2], x[2 * c - 1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (c < 6) mfma_s(c + 2);
+        if (c >= 4) vq[c - 4] = vfrag(c - 4);
+      }
+      ps += x[14] + x[15];
+      pc[1][3] = pack2<DT>(x[14], x[15]);
+      l = l * alpha + ps;  // this half-wave's tokens; joined once at the end
+      // (used here, or the compiler moves the exponentials behind the rescaling branch, away from the MFMAs)
+      asm volatile("" : "+v"(pc[0]), "+v"(pc[1]), "+v"(l));
+      if (__ballot(alpha != 1.f)) {
 #pragma unroll
-      for (int i = 0; i < 4 * NC; ++i) {
-        if (i + kAhead < 4 * NC) vq[(i + kAhead) % (kAhead + 1)] = vfrag(i + kAhead);
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i + kAhead < 8) vq[(i + kAhead) % (kAhead + 1)] = vfrag(i + kAhead);
         acc[i % 4] = MF::run(vq[i % (kAhead + 1)], pc[i / 4], acc[i % 4]);
         __builtin_amdgcn_sched_barrier(0);
       }
-    };
-    // Page ids, 64 per register (lane i: the wave's page 64 w + i of `count`); bit i of *bad: outside the cache.
-    auto load_ids = [&](int first, int stride, int count, int w, uint64_t *bad) {
-      const int i = 64 * w + lane;
-      const int id = i < count ? ids[first + stride * i] : 0;
-      const bool ok = (uint32_t)id < num_pages;
-      *bad = __ballot(!ok);
-      return ok ? id : 0;
-    };
-    auto page_base = [&](int id) { return uniform_ptr(kvh + (uint64_t)(uint32_t)id * page_bytes); };
-
-    if (groups == 1) {
-      // Wave-private pages: every fourth of the piece, two buffers.
-      const int p0 = kPages * s0 + wv, p1 = min(np, kPages * s1);
-      const int count = p0 < p1 ? (p1 - p0 + 3) >> 2 : 0;
-      const uint32_t wlds = lds0 + wv * (4 * kPageB);
-      char *const wbuf = &tiles[0] + wv * (4 * kPageB);
-      uint32_t koff[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) koff[i] = (4 * i + lrow) * row_bytes + 16 * ((lch ^ lrow) ^ (4 * i));
-      const uint32_t voff = (kPageSize + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
-      auto issue_k = [&](const char *pg, int buf) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_lds_1k<true>(wlds + buf * 2 * kPageB + i * 1024, pg, koff[i]);
-      };
-      auto issue_v = [&](const char *pg, int buf) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          load_lds_1k<true>(wlds + buf * 2 * kPageB + kPageB + i * 1024, pg, voff + (uint32_t)(4 * i) * row_bytes);
-      };
-      uint64_t bad = 0;
-      int idv = load_ids(p0, 4, count, 0, &bad);
-      if (count > 0) {
-        const char *pg = page_base(__builtin_amdgcn_readlane(idv, 0));
-        issue_k(pg, 0);
-        issue_v(pg, 0);
-      }
-      if (count > 1) {
-        const char *pg = page_base(__builtin_amdgcn_readlane(idv, 1));
-        issue_k(pg, 1);
-        issue_v(pg, 1);
-      }
-      uint64_t bad_next = bad;  // of the window of page k + 2
-      for (int k = 0; k < count; ++k) {
-        // (the ids of pages 64 w .. take the place of the last ones' once page 64 w - 2 is under way)
-        if (k + 2 < count && ((k + 2) & 63) == 0) idv = load_ids(p0, 4, count, (k + 2) >> 6, &bad_next);
-        if (k + 1 < count)
-          wait_loads<8>();
-        else
-          wait_loads<0>();
-        const int kv0 = (p0 + 4 * k) * kPageSize;
-        const bool page_bad = (bad >> (k & 63)) & 1u;
-        char *const buf = wbuf + (k & 1) * 2 * kPageB;
-        if (page_bad || kv0 + kPageSize > len) {
-          // V rows past the segment and of pages outside the cache meet p = 0 but may hold NaN/Inf: zeros.
-          const int r = lane >> 2;
-          if (page_bad || kv0 + r >= len) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st128(buf + kPageB + r * 256 + 64 * (lane & 3) + 16 * i, u32x4{0u, 0u, 0u, 0u});
-          }
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
-        sweep(std::integral_constant<int, 16>(), kv0, buf, buf + kPageB, page_bad ? 1u : 0u);
-        if (k + 2 < count) {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          const char *pg = page_base(__builtin_amdgcn_readlane(idv, (k + 2) & 63));
-          issue_k(pg, k & 1);
-          issue_v(pg, k & 1);
-        }
-        if (((k + 1) & 63) == 0) bad = bad_next;
-      }
-    } else {
-      // Shared stages: wave w loads rows 4 w .. + 3 of both of a stage's pages, K and V; three stages are under way
-      // while one is worked on.  (Waves that share pairs take every other stage.)
-      const uint32_t wlds = lds0 + wv * 1024;
-      const uint32_t koff = (4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * wv + lrow));
-      const uint32_t voff = (kPageSize + 4 * wv + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
-      const int p0 = kPages * s0, count = min(np, kPages * s1) - p0;  // <= 0: no page
-      const int nst = count > 0 ? (count + 1) >> 1 : 0;
-      uint64_t bad = 0, bad_next;
-      int idv = load_ids(p0, 1, count, 0, &bad);
-      bad_next = bad;
-      auto issue = [&](int j) {  // stage j of the piece; a page past it is page 0 of the cache (masked later)
-        const uint32_t dst = wlds + (uint32_t)(j & (kStages - 1)) * kStageB;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const char *pg = page_base(__builtin_amdgcn_readlane(idv, (2 * j + i) & 63));
-          load_lds_1k(dst + i * kPageB, pg, koff);
-          load_lds_1k(dst + 2 * kPageB + i * kPageB, pg, voff);
-        }
-      };
-      for (int j = 0; j < 3 && j < nst; ++j) issue(j);
-      for (int j = 0; j < nst; ++j) {
-        if (j + 2 < nst)
-          wait_loads<8>();
-        else if (j + 1 < nst)
-          wait_loads<4>();
-        else
-          wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const uint32_t sbad = (uint32_t)(bad >> ((2 * j) & 63)) & 3u;
-        if (j + 3 < nst) {  // into the buffer of stage j - 1, which every wave has left
-          if (((j + 3) & 31) == 0) idv = load_ids(p0, 1, count, (j + 3) >> 5, &bad_next);
-          issue(j + 3);
-        }
-        const int kv0 = s0 * kStep + 32 * j;
-        char *const buf = &tiles[(j & (kStages - 1)) * kStageB];
-        if (kv0 + 32 > len || sbad != 0) {
-          // V rows past the segment and of pages outside the cache meet p = 0 but may hold NaN/Inf: zeros.
-          const int r = (int)threadIdx.x >> 3;
-          if (kv0 + r >= len || ((sbad >> (r >> 4)) & 1u)) {
-            char *vr = buf + 2 * kPageB + r * 256 + 32 * ((int)threadIdx.x & 7);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
-          }
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          __builtin_amdgcn_s_barrier();
-          asm volatile("" ::: "memory");
-        }
-        if (active && (groups == 4 || (j & 1) == half))
-          sweep(std::integral_constant<int, 32>(), kv0, buf, buf + 2 * kPageB, sbad);
-        if (((j + 1) & 31) == 0) bad = bad_next;
-      }
     }
-
     l = halves_sum(l);
-    if (groups < 4) {
-      // Join the waves that share pairs (wave qsub + groups k), in halves: (m, l, acc) through LDS.
-      constexpr int kOne = 17 * 64;  // f32x4 of a wave
-      f32x4 *const all = reinterpret_cast<f32x4 *>(&tiles[0]) + lane;
-      const int k = wv / groups;
-#pragma unroll 1
-      for (int ks = 1; ks * groups < 4; ks *= 2) {
-        __syncthreads();
-        if ((k & ks) && !(k & (ks - 1))) {
-          f32x4 *const at = all + (wv - ks * groups) * kOne;
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            at[64 * i] = f32x4{acc[i >> 2][4 * (i & 3)], acc[i >> 2][4 * (i & 3) + 1], acc[i >> 2][4 * (i & 3) + 2],
-                               acc[i >> 2][4 * (i & 3) + 3]};
-          at[64 * 16] = f32x4{m, l, 0.f, 0.f};
-        }
-        __syncthreads();
-        if (!(k & (2 * ks - 1))) {
-          const f32x4 *const at = all + wv * kOne;
-          const float m2 = at[64 * 16][0], l2 = at[64 * 16][1];
-          const float M = fmaxf(m, m2), ref = M == -INFINITY ? 0.f : M;
-          const float w1 = fast_exp2(m - ref), w2 = fast_exp2(m2 - ref);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const f32x4 x = at[64 * i];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i >> 2][4 * (i & 3) + e] = acc[i >> 2][4 * (i & 3) + e] * w1 + x[e] * w2;
-          }
-          l = l * w1 + l2 * w2;
-          m = M;
-        }
-      }
-    }
     // ---- Results (the lane's pair worked out again: held over the steps it would cost registers).
     asm volatile("" : "+v"(lane));
     const int wpair = 32 * qsub + (lane & 31), whl = lane >> 5;
     const int wpt = wpair < pairs ? wpair / G : 0, wg = wpair - wpt * G;
     const int wt = of_prefix ? line.toks[wpt] : q0 + t0 + wpt;
-    const bool writes = wpair < pairs && wv < groups;
+    const bool writes = wpair < pairs;
     const bool whole = runs == 1 && !of_prefix && px < 0;
     if (writes && whole) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
