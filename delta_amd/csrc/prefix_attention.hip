@@ -112,6 +112,14 @@ __device__ __forceinline__ bool prefix_fits(const PrefixArgs &a, const Row &x, i
 
 __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
 
+// Whether a row's query tokens leave at most an eighth of its tiles idle: such a row shares no tiles with the others of
+// its prefix, but sweeps the prefix's pages with its own, from one tile's start to its end (the pages come from the L2
+// either way, and nothing has to be joined).
+template <int TT>
+__device__ __forceinline__ bool fills_tiles(int qn) {
+  return 9 * qn >= 8 * TT * div_up(qn, TT);
+}
+
 // A pointer that is the same in every lane, in scalar registers.
 template <typename T>
 __device__ __forceinline__ T *uniform_ptr(T *p) {
@@ -155,19 +163,21 @@ struct Line {
 template <int TT>
 __device__ int build_line(const PrefixArgs &a, Line &line, int *scratch) {
   const int tid = threadIdx.x, P = a.num_prefixes, B = a.batch;
+  // (the rows' tables are asked for before the prefixes' have come)
+  Row x = row_of(a, tid < B ? tid : 0);
+  int want = a.row_prefix[tid < B ? tid : 0];
   for (int p = tid; p < P; p += kThreads) {
     line.prefix_toks[p] = 0;
     scratch[p] = csr_pages(a.prefix_indptr, a.prefix_indices_len, p).n;
   }
-  Row x = tid < B ? row_of(a, tid) : Row{0, 0, 0, 0, 0};
-  int want = tid < B ? a.row_prefix[tid] : -1;
   __syncthreads();
   for (int r = tid; r < B; r += kThreads) {
     if (r != tid) {
       x = row_of(a, r);
       want = a.row_prefix[r];
     }
-    const bool fits = want >= 0 && want < P && prefix_fits(a, x, scratch[want >= 0 && want < P ? want : 0]);
+    const bool fits = want >= 0 && want < P && !fills_tiles<TT>(x.qn) &&
+                      prefix_fits(a, x, scratch[want >= 0 && want < P ? want : 0]);
     line.row_prefix[r] = (int16_t)(fits ? want : -1);
     if (fits) atomicAdd(&line.prefix_toks[want], x.qn);
     const int own = x.len - (fits ? scratch[want] * kPageSize : 0);
@@ -347,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const char *pg = uniform_ptr(kvh + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(idv, (2 * j + i) & 63) * page_bytes);
-        if (of_prefix) {
+        if (of_prefix || a.qo_indptr) {
           load_lds_1k(dst + i * kPageB, pg, koff);
           load_lds_1k(dst + 2 * kPageB + i * kPageB, pg, voff);
         } else {  // read once
@@ -553,17 +563,19 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   }
 }
 
-// Joins the runs of each (token, q head), one wave each: lane e holds entry e's row and (m, l), the prefix's runs
-// first, then the own tile's; then every lane sums two of the 128 outputs over the entries.
-template <int DT>
+// Joins the runs of each (token, q head), W waves each: lane e of wave w holds the row and (m, l) of entry e W + w, the
+// prefix's runs first, then the own tile's; then every lane sums two of the 128 outputs over its wave's entries, and the
+// waves are joined in LDS.
+template <int DT, int W>
 __global__ void __launch_bounds__(kThreads) prefix_merge_kernel(PrefixArgs a) {
   using E = Elem<DT>;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.tokens * a.hq) return;
-  const int t = uniform((int)(row / a.hq)), hq = uniform((int)(row % a.hq));
-  // A query token of no row is left as it was.
-  if (a.qo_indptr && (t < a.qo_indptr[0] || t >= a.qo_indptr[a.batch])) return;
-  const int lane = threadIdx.x & 63;
+  constexpr int kRows = kThreads / 64 / W;
+  __shared__ float s_m[W][kRows], s_l[W][kRows];
+  __shared__ float2 s_a[W][kRows][64];
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), w0 = wave % W, rw = wave / W;
+  const int64_t row = (int64_t)blockIdx.x * kRows + rw;
+  const bool in = row < (int64_t)a.tokens * a.hq;
+  const int t = uniform((int)((in ? row : 0) / a.hq)), hq = uniform((int)((in ? row : 0) % a.hq));
   const int G = a.hq / a.hkv, h = hq / G, g = hq - h * G;
   int first[2], count[2], pair[2];
 #pragma unroll
@@ -574,38 +586,49 @@ __global__ void __launch_bounds__(kThreads) prefix_merge_kernel(PrefixArgs a) {
     pair[kind] = uniform(min((x.y >> 16) & 0xffff, kQ - G)) + g;
   }
   const int n = count[0] + count[1];
-  if (count[0] == 0 && count[1] == 1) return;  // written by its tile
+  // Left as they are: a query token of no row, and one whose tile wrote it.
+  const bool skip = !in || (a.qo_indptr && (t < a.qo_indptr[0] || t >= a.qo_indptr[a.batch])) ||
+                    (count[0] == 0 && count[1] == 1);
+  if (W == 1 && skip) return;  // (W > 1: the block's rows all pass the barrier below)
   float M = -INFINITY, L = 0.f;
   float2 A = {0.f, 0.f};
-  for (int e0 = 0; e0 < n; e0 += 64) {
-    const int e = e0 + lane;
-    const bool have = e < n, own = have && e >= count[0];
+  const int mine = skip ? 0 : (n - w0 + W - 1) / W;  // entries of this wave
+  for (int e0 = 0; e0 < mine; e0 += 64) {
+    const bool have = e0 + lane < mine;
+    const int e = (e0 + lane) * W + w0;
+    const bool own = have && e >= count[0];
     const int r = !have ? 0 : (own ? e - count[0] : e), kind = own || count[0] == 0 ? 1 : 0;
     const int of = count[kind], b0 = first[kind], pr = pair[kind];
     const int64_t at = of == 1 ? (int64_t)(kind * a.tokens + t) * a.hq + hq
                                : (int64_t)2 * a.tokens * a.hq + (((int64_t)h * a.blocks + b0 + r) * 2 + (r == 0)) * kQ + pr;
     const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
+    const int lim = min(64, mine - e0), at32 = (int)at;  // (rows: below 2^30, checked on the host)
+    auto load = [&](int i) {
+      const int64_t from = __builtin_amdgcn_readlane(at32, min(i, lim - 1));
+      return *reinterpret_cast<const float2 *>(a.part_acc + from * kHeadDim + 2 * lane);
+    };
+    float2 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = load(k);  // under the weights' arithmetic
     const float ms = have ? ml.x : -INFINITY;
     float cm = fmaxf(M, ms);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) cm = fmaxf(cm, shfl_xor(cm, off));
     const float ref = cm == -INFINITY ? 0.f : cm, al = fast_exp2(M - ref);
     const float w = fast_exp2(ms - ref);  // 0 where nothing was attended
-    float s = ml.y * w;
-    s = have ? s : 0.f;
+    float s = have ? ml.y * w : 0.f;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += shfl_xor(s, off);
     L = L * al + s;
     A.x *= al;
     A.y *= al;
     M = cm;
-    const int lim = min(64, n - e0), at32 = (int)at;  // (rows: below 2^31, checked on the host)
     for (int i0 = 0; i0 < lim; i0 += 8) {
-      float2 v[8];
+      float2 nx[8];
+      const bool more = i0 + 8 < lim;
+      if (more) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int64_t from = __builtin_amdgcn_readlane(at32, min(i0 + k, lim - 1));
-        v[k] = *reinterpret_cast<const float2 *>(a.part_acc + from * kHeadDim + 2 * lane);
+        for (int k = 0; k < 8; ++k) nx[k] = load(i0 + 8 + k);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -613,6 +636,33 @@ __global__ void __launch_bounds__(kThreads) prefix_merge_kernel(PrefixArgs a) {
         A.x = fmaf(v[k].x, ws, A.x);
         A.y = fmaf(v[k].y, ws, A.y);
       }
+      if (more) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = nx[k];
+      }
+    }
+  }
+  if constexpr (W > 1) {
+    s_a[w0][rw][lane] = A;
+    if (lane == 0) {
+      s_m[w0][rw] = M;
+      s_l[w0][rw] = L;
+    }
+    __syncthreads();
+    if (skip || w0 != 0) return;
+    M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, s_m[w][rw]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    L = 0.f;
+    A = float2{0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float sc = fast_exp2(s_m[w][rw] - ref);
+      const float2 x = s_a[w][rw][lane];
+      L = fmaf(s_l[w][rw], sc, L);
+      A.x = fmaf(x.x, sc, A.x);
+      A.y = fmaf(x.y, sc, A.y);
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -661,8 +711,13 @@ void launch(const PrefixArgs &a, int G, hipStream_t stream) {
     case 7: launch_g<DT, 7>(a, stream); break;
     default: launch_g<DT, 8>(a, stream); break;
   }
+  // Few rows may have many runs each (up to a block's worth): four waves to a row.
   const int64_t rows = (int64_t)a.tokens * a.hq;
-  hipLaunchKernelGGL((prefix_merge_kernel<DT>), dim3((unsigned)ceil_div(rows, kThreads / 64)), dim3(kThreads), 0, stream, a);
+  if (rows <= 4096)
+    hipLaunchKernelGGL((prefix_merge_kernel<DT, 4>), dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((prefix_merge_kernel<DT, 1>), dim3((unsigned)ceil_div(rows, kThreads / 64)), dim3(kThreads), 0,
+                       stream, a);
 }
 
 int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
