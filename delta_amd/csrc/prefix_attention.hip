@@ -38,7 +38,7 @@ constexpr int kPageB = kPageSize * 256; // bytes of a page's K (or V) of one hea
 constexpr int kStageB = 4 * kPageB;     // a stage: 32 tokens' K, then their V
 constexpr int kStages = 4;              // stages in LDS
 constexpr int kQ = 128;                 // (token, head) pairs of a tile, at most
-constexpr int kMaxRows = 1024;          // rows, and prefixes, of a call (the line's tables)
+constexpr int kMaxRows = 1024;          // rows, and prefixes, of a call (the tables: 41 KiB)
 constexpr int kSlots = 512;             // blocks the chip holds (two per CU)
 constexpr int kTileCost = 2;            // steps that a tile costs besides its own
 constexpr int kMinShare = 4;            // steps of a share, at least
@@ -150,25 +150,38 @@ __device__ __forceinline__ int block_scan(int v, int *sums, int *total) {
   return before + incl - v;
 }
 
-// The line of a kv head's work, in LDS.
+// The tables and the line of a kv head's work, in LDS behind the stages.
 struct Line {
-  int at[2 * kMaxRows + 1];   // where each segment begins (the prefixes, then the rows), and the end
-  int prefix_toks[kMaxRows];  // query tokens of each prefix
-  int16_t row_prefix[kMaxRows];  // the prefix that applies to each row, -1: none
-  int sums[4];
-  int toks[kQ];               // query tokens of a prefix's tile
+  int *toks;         // [kQ] query tokens of a prefix's tile
+  int *sums;         // [4]
+  int *at;           // [prefixes + rows + 1] where each segment begins (the prefixes, then the rows), and the end
+  int *prefix_toks;  // [prefixes] query tokens
+  int *prefix_ids;   // [prefixes] first page in prefix_indices
+  int *prefix_pages; // [prefixes]
+  int *row_prefix;   // [rows] the prefix that applies, -1: none
+  int *row_ids;      // [rows] first own page in kv_indices
+  int *row_len;      // [rows] own tokens
+  int *row_q0, *row_qn;  // [rows] query tokens
+  __device__ __forceinline__ Line(int *lds, int prefixes, int rows)
+      : toks(lds), sums(toks + kQ), at(sums + 4), prefix_toks(at + prefixes + rows + 1), prefix_ids(prefix_toks + prefixes),
+        prefix_pages(prefix_ids + prefixes), row_prefix(prefix_pages + prefixes), row_ids(row_prefix + rows),
+        row_len(row_ids + rows), row_q0(row_len + rows), row_qn(row_q0 + rows) {}
+  static size_t bytes(int prefixes, int rows) {
+    return ((size_t)kQ + 4 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
+  }
 };
 
-// `scratch`: kMaxRows ints of LDS.
 template <int TT>
-__device__ int build_line(const PrefixArgs &a, Line &line, int *scratch) {
+__device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line) {
   const int tid = threadIdx.x, P = a.num_prefixes, B = a.batch;
   // (the rows' tables are asked for before the prefixes' have come)
   Row x = row_of(a, tid < B ? tid : 0);
   int want = a.row_prefix[tid < B ? tid : 0];
   for (int p = tid; p < P; p += kThreads) {
+    const Pages pages = csr_pages(a.prefix_indptr, a.prefix_indices_len, p);
     line.prefix_toks[p] = 0;
-    scratch[p] = csr_pages(a.prefix_indptr, a.prefix_indices_len, p).n;
+    line.prefix_ids[p] = pages.first;
+    line.prefix_pages[p] = pages.n;
   }
   __syncthreads();
   for (int r = tid; r < B; r += kThreads) {
@@ -176,24 +189,26 @@ __device__ int build_line(const PrefixArgs &a, Line &line, int *scratch) {
       x = row_of(a, r);
       want = a.row_prefix[r];
     }
-    const bool fits = want >= 0 && want < P && !fills_tiles<TT>(x.qn) &&
-                      prefix_fits(a, x, scratch[want >= 0 && want < P ? want : 0]);
-    line.row_prefix[r] = (int16_t)(fits ? want : -1);
+    const bool named = want >= 0 && want < P;
+    const int n = named ? line.prefix_pages[want] : 0;
+    const bool fits = named && !fills_tiles<TT>(x.qn) && prefix_fits(a, x, n);
     if (fits) atomicAdd(&line.prefix_toks[want], x.qn);
-    const int own = x.len - (fits ? scratch[want] * kPageSize : 0);
-    line.at[P + r] = div_up(x.qn, TT) * (div_up(own, kStep) + kTileCost);
+    const int own = x.len - (fits ? n * kPageSize : 0);
+    line.row_prefix[r] = fits ? want : -1;
+    line.row_ids[r] = x.kv0 + (fits ? n : 0);
+    line.row_len[r] = own;
+    line.row_q0[r] = x.q0;
+    line.row_qn[r] = x.qn;
   }
   __syncthreads();
   int end = 0;
   for (int i0 = 0; i0 < P + B; i0 += kThreads) {
     const int i = i0 + tid;
     int cost = 0, total;
-    if (i < P) {
-      const int tiles = div_up(line.prefix_toks[i], TT);
-      cost = tiles * (div_up(scratch[i], kPages) + kTileCost);
-    } else if (i < P + B) {
-      cost = line.at[i];
-    }
+    if (i < P)
+      cost = div_up(line.prefix_toks[i], TT) * (div_up(line.prefix_pages[i], kPages) + kTileCost);
+    else if (i < P + B)
+      cost = div_up(line.row_qn[i - P], TT) * (div_up(line.row_len[i - P], kStep) + kTileCost);
     const int at = end + block_scan(cost, line.sums, &total);
     if (i < P + B) line.at[i] = at;
     end += total;
@@ -210,12 +225,12 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   using E = Elem<DT>;
   constexpr int TT = kQ / G;  // query tokens of a tile
   // A ring of stages, each the K tile, then the V tile (swizzled rows).
-  __shared__ __attribute__((aligned(1024))) char tiles[kStages * kStageB];
-  __shared__ Line line;
+  extern __shared__ __attribute__((aligned(1024))) char tiles[];
+  const Line line(reinterpret_cast<int *>(tiles + kStages * kStageB), a.num_prefixes, a.batch);
 
   const int wv = uniform((int)(threadIdx.x >> 6));
   const int h = blockIdx.x, blk = blockIdx.y;
-  const int total = uniform(build_line<TT>(a, line, reinterpret_cast<int *>(&tiles[0])));
+  const int total = uniform(build_line<TT>(a, line));
   int share = uniform(div_up(total, a.blocks));
   share = share < kMinShare ? kMinShare : share;
   int pos = blk * share;  // (total < 2^30: checked on the host)
@@ -235,18 +250,13 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int hl = lane >> 5, n = lane & 31, lrow = lane >> 4, lch = lane & 15;
-    // K fragment of k-slice ks: row n (of 32), chunk 2 ks + hl.
-    uint32_t kfo[8];
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) kfo[ks] = (uint32_t)(n * 256 + 16 * ((2 * ks + hl) ^ (n & 15)));
+    // K fragment of k-slice ks: row n, chunk 2 ks + hl (32 ks comes in by xor: the bits above it are the row's).
+    const uint32_t kfo = (uint32_t)(n * 256 + 16 * (hl ^ (n & 15)));
     // ds_read_b64_tr_b16 of V^T: 16-lane group q16 = lane / 16, t16 = lane % 16 reads rows (kv) base + t16 / 4 at columns
-    // 32 dt + 16 (q16 % 2) + 4 (t16 % 4), and receives its column's four rows.
+    // 32 dt + 16 (q16 % 2) + 4 (t16 % 4), and receives its column's four rows (64 dt by xor).
     const int q16 = lane >> 4, t16 = lane & 15;
-    uint32_t vfo[4];
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-      vfo[dt] = (uint32_t)((4 * hl + (t16 >> 2)) * 256 +
-                           16 * ((4 * dt + 2 * (q16 & 1) + ((t16 & 3) >> 1)) ^ (4 * (t16 >> 2))) + 8 * (t16 & 1));
+    const uint32_t vfo = (uint32_t)((4 * hl + (t16 >> 2)) * 256 +
+                                    16 * ((2 * (q16 & 1) + ((t16 & 3) >> 1)) ^ (4 * (t16 >> 2))) + 8 * (t16 & 1));
 
     // ---- The piece at pos: segment, tile, steps [s0, s1).
     const int items = a.num_prefixes + a.batch;
@@ -262,21 +272,18 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     const int32_t *ids;  // the segment's page ids
     int np, len, seg_toks, q0 = 0, px = -1;
     if (of_prefix) {
-      const Pages p = csr_pages(a.prefix_indptr, a.prefix_indices_len, item);
-      ids = a.prefix_indices + p.first;
-      np = p.n;
-      len = p.n * kPageSize;
+      ids = a.prefix_indices + uniform(line.prefix_ids[item]);
+      np = uniform(line.prefix_pages[item]);
+      len = np * kPageSize;
       seg_toks = uniform(line.prefix_toks[item]);
     } else {
       const int r = item - a.num_prefixes;
-      const Row x = row_of(a, r);
       px = uniform(line.row_prefix[r]);
-      const int skip = px >= 0 ? csr_pages(a.prefix_indptr, a.prefix_indices_len, px).n : 0;
-      ids = a.kv_indices + x.kv0 + skip;
-      np = x.pages - skip;
-      len = x.len - skip * kPageSize;
-      seg_toks = x.qn;
-      q0 = x.q0;
+      ids = a.kv_indices + uniform(line.row_ids[r]);
+      len = uniform(line.row_len[r]);
+      np = div_up(len, kPageSize);
+      seg_toks = uniform(line.row_qn[r]);
+      q0 = uniform(line.row_q0[r]);
     }
     const int steps = div_up(len, kStep), cost = steps + kTileCost;
     const int seg_at = uniform(line.at[item]);
@@ -300,12 +307,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       for (int r0 = 0; r0 < a.batch; r0 += kThreads) {
         const int r = r0 + threadIdx.x;
         const bool mine = r < a.batch && line.row_prefix[r] == item;
-        int rq0 = r, qn = mine ? 1 : 0;
-        if (a.qo_indptr && mine) {
-          const Row x = row_of(a, r);
-          rq0 = x.q0;
-          qn = x.qn;
-        }
+        const int qn = mine ? line.row_qn[r] : 0, rq0 = mine ? line.row_q0[r] : 0;
         const int at = before + block_scan(qn, line.sums, &sum);
         for (int k = t0 > at ? t0 - at : 0; k < qn && at + k < t0 + ntok; ++k) line.toks[at + k - t0] = rq0 + k;
         before += sum;
@@ -387,19 +389,12 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
-    // S^T of a stage: K fragments three k-slices ahead of their MFMAs.
-    auto scores = [&](int j, f32x16 &S) {
-      const char *tk = &tiles[(j & (kStages - 1)) * kStageB];
-      u32x4 kq[4];
-#pragma unroll
-      for (int s = 0; s < 3; ++s) kq[s] = *reinterpret_cast<const u32x4 *>(tk + kfo[s]);
+    // S^T of the first stage.
+    auto scores = [&](f32x16 &S) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) S[i] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        if (ks + 3 < 8) kq[(ks + 3) & 3] = *reinterpret_cast<const u32x4 *>(tk + kfo[ks + 3]);
-        S = MF::run(kq[ks & 3], qf[ks], S);
-      }
+      for (int ks = 0; ks < 8; ++ks) S = MF::run(*reinterpret_cast<const u32x4 *>(tiles + (kfo ^ (32u * ks))), qf[ks], S);
     };
     f32x16 S;  // of the stage worked on
     if (nst > 0) {
@@ -412,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       clear_v(0, bad_of(0));
-      if (active) scores(0, S);
+      if (active) scores(S);
     }
     for (int j = 0; j < nst; ++j) {
       // Stage j + 1 has landed, stage j - 1 is left by every wave.
@@ -454,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       // The next stage's S (of no use behind the last stage), an MFMA at a time between pieces of this one's softmax:
       // each piece runs while its MFMA does.  The fences keep that order.
       const char *tk = &tiles[((j + 1) & (kStages - 1)) * kStageB];
-      auto kfrag = [&](int ks) { return *reinterpret_cast<const u32x4 *>(tk + kfo[ks]); };
+      auto kfrag = [&](int ks) { return *reinterpret_cast<const u32x4 *>(tk + (kfo ^ (32u * ks))); };
       u32x4 kq[4];
 #pragma unroll
       for (int ks = 0; ks < 3; ++ks) kq[ks] = kfrag(ks);
@@ -481,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       mfma_s(1);
       const char *tv = &tiles[(j & (kStages - 1)) * kStageB + 2 * kPageB];
       auto vfrag = [&](int i) {  // V^T fragment of 16-token chunk i / 4, d tile i % 4
-        const char *rd = tv + vfo[i % 4] + (i / 4) * 4096;
+        const char *rd = tv + (vfo ^ (64u * (i % 4))) + (i / 4) * 4096;
         const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
         const ps4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)(rd + 2048));
         const uint2 lo = __builtin_bit_cast(uint2, v0), hi = __builtin_bit_cast(uint2, v1);
@@ -563,122 +558,134 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   }
 }
 
-// Joins the runs of each (token, q head), W waves each: lane e of wave w holds the row and (m, l) of entry e W + w, the
-// prefix's runs first, then the own tile's; then every lane sums two of the 128 outputs over its wave's entries, and the
-// waves are joined in LDS.
-template <int DT, int W>
-__global__ void __launch_bounds__(kThreads) prefix_merge_kernel(PrefixArgs a) {
-  using E = Elem<DT>;
-  constexpr int kRows = kThreads / 64 / W;
-  __shared__ float s_m[W][kRows], s_l[W][kRows];
-  __shared__ float2 s_a[W][kRows][64];
-  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), w0 = wave % W, rw = wave / W;
-  const int64_t row = (int64_t)blockIdx.x * kRows + rw;
+// The runs of (token t, q head hq): entry e's row in the partials, the prefix's runs first, then the own tile's.
+struct Runs {
+  int first[2], count[2], pair[2], t, hq, h;
+  bool skip;  // left as they are: a query token of no row, and one whose tile wrote it
+};
+__device__ __forceinline__ Runs runs_of(const PrefixArgs &a, int64_t row) {
+  Runs x;
   const bool in = row < (int64_t)a.tokens * a.hq;
-  const int t = uniform((int)((in ? row : 0) / a.hq)), hq = uniform((int)((in ? row : 0) % a.hq));
-  const int G = a.hq / a.hkv, h = hq / G, g = hq - h * G;
-  int first[2], count[2], pair[2];
+  x.t = (int)((in ? row : 0) / a.hq);
+  x.hq = (int)((in ? row : 0) - (int64_t)x.t * a.hq);
+  const int G = a.hq / a.hkv;
+  x.h = x.hq / G;
 #pragma unroll
   for (int kind = 0; kind < 2; ++kind) {  // (the limits keep a table that is no CSR inside the partials)
-    const int2 x = a.runs[kind * a.tokens + t];
-    first[kind] = uniform(min(max(x.x, 0), a.blocks - 1));
-    count[kind] = uniform(min(x.y & 0xffff, a.blocks - first[kind]));
-    pair[kind] = uniform(min((x.y >> 16) & 0xffff, kQ - G)) + g;
+    const int2 r = a.runs[kind * a.tokens + x.t];
+    x.first[kind] = min(max(r.x, 0), a.blocks - 1);
+    x.count[kind] = min(r.y & 0xffff, a.blocks - x.first[kind]);
+    x.pair[kind] = min((r.y >> 16) & 0xffff, kQ - G) + x.hq - x.h * G;
   }
-  const int n = count[0] + count[1];
-  // Left as they are: a query token of no row, and one whose tile wrote it.
-  const bool skip = !in || (a.qo_indptr && (t < a.qo_indptr[0] || t >= a.qo_indptr[a.batch])) ||
-                    (count[0] == 0 && count[1] == 1);
-  if (W == 1 && skip) return;  // (W > 1: the block's rows all pass the barrier below)
+  x.skip = !in || (a.qo_indptr && (x.t < a.qo_indptr[0] || x.t >= a.qo_indptr[a.batch])) ||
+           (x.count[0] == 0 && x.count[1] == 1);
+  if (x.skip) x.count[0] = x.count[1] = 0;
+  return x;
+}
+// (e >= the runs' number: some row of the partials)
+__device__ __forceinline__ int entry_row(const PrefixArgs &a, const Runs &x, int e) {
+  const bool own = e >= x.count[0];
+  const int kind = own ? 1 : 0, r = min(own ? e - x.count[0] : e, max(x.count[kind] - 1, 0));
+  return x.count[kind] <= 1 ? (kind * a.tokens + x.t) * a.hq + x.hq
+                            : 2 * a.tokens * a.hq + ((x.h * a.blocks + x.first[kind] + r) * 2 + (r == 0)) * kQ + x.pair[kind];
+}
+template <int DT>
+__device__ __forceinline__ void merged(const PrefixArgs &a, const Runs &x, int d, f32x4 A, float M, float L) {
+  using E = Elem<DT>;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint32_t *op = reinterpret_cast<uint32_t *>(a.o + (int64_t)x.t * a.o_stride_t + (int64_t)x.hq * a.o_stride_h + d);
+  op[0] = E::from_float(A[0] * inv) | (E::from_float(A[1] * inv) << 16);
+  op[1] = E::from_float(A[2] * inv) | (E::from_float(A[3] * inv) << 16);
+  if (d == 0 && a.lse) a.lse[(int64_t)x.t * a.hq + x.hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+}
+
+// Joins the runs of each (token, q head), W half-waves each (W = 1: two rows to a wave): lane e of half-wave w holds the
+// row and (m, l) of entry e W + w, then sums four of the 128 outputs over its half-wave's entries; W half-waves are joined
+// in LDS.  A chain of two loads (the runs; partials and statistics together), so what counts is how many are under way.
+template <int DT, int W>
+__global__ void __launch_bounds__(kThreads, 6) prefix_merge_kernel(PrefixArgs a) {
+  constexpr int kHalves = kThreads / 32, kRows = kHalves / W;
+  __shared__ float s_m[kHalves], s_l[kHalves];
+  __shared__ f32x4 s_a[kHalves][32];
+  const int lane = threadIdx.x & 31, half = threadIdx.x >> 5, w0 = half % W;
+  const Runs x = runs_of(a, (int64_t)blockIdx.x * kRows + half / W);
+  const int n = x.count[0] + x.count[1], mine = n > w0 ? (n - w0 + W - 1) / W : 0;  // entries of this half-wave
   float M = -INFINITY, L = 0.f;
-  float2 A = {0.f, 0.f};
-  const int mine = skip ? 0 : (n - w0 + W - 1) / W;  // entries of this wave
-  for (int e0 = 0; e0 < mine; e0 += 64) {
+  f32x4 A = {0.f, 0.f, 0.f, 0.f};
+  const int base = threadIdx.x & 32;  // the half-wave's first lane
+  for (int e0 = 0; __ballot(e0 < mine) != 0; e0 += 32) {
     const bool have = e0 + lane < mine;
-    const int e = (e0 + lane) * W + w0;
-    const bool own = have && e >= count[0];
-    const int r = !have ? 0 : (own ? e - count[0] : e), kind = own || count[0] == 0 ? 1 : 0;
-    const int of = count[kind], b0 = first[kind], pr = pair[kind];
-    const int64_t at = of == 1 ? (int64_t)(kind * a.tokens + t) * a.hq + hq
-                               : (int64_t)2 * a.tokens * a.hq + (((int64_t)h * a.blocks + b0 + r) * 2 + (r == 0)) * kQ + pr;
-    const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
-    const int lim = min(64, mine - e0), at32 = (int)at;  // (rows: below 2^30, checked on the host)
+    const int at = entry_row(a, x, (e0 + lane) * W + w0);
+    const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (int64_t)at * 2);
     auto load = [&](int i) {
-      const int64_t from = __builtin_amdgcn_readlane(at32, min(i, lim - 1));
-      return *reinterpret_cast<const float2 *>(a.part_acc + from * kHeadDim + 2 * lane);
+      const int64_t from = __builtin_amdgcn_ds_bpermute((base + i) << 2, at);
+      return *reinterpret_cast<const f32x4 *>(a.part_acc + from * kHeadDim + 4 * lane);
     };
-    float2 v[8];
+    f32x4 v[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = load(k);  // under the weights' arithmetic
+    for (int k = 0; k < 4; ++k) v[k] = load(k);  // under the weights' arithmetic
     const float ms = have ? ml.x : -INFINITY;
     float cm = fmaxf(M, ms);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) cm = fmaxf(cm, shfl_xor(cm, off));
+    for (int off = 16; off > 0; off >>= 1) cm = fmaxf(cm, shfl_xor(cm, off));
     const float ref = cm == -INFINITY ? 0.f : cm, al = fast_exp2(M - ref);
-    const float w = fast_exp2(ms - ref);  // 0 where nothing was attended
+    const float w = have ? fast_exp2(ms - ref) : 0.f;  // 0 where nothing was attended
     float s = have ? ml.y * w : 0.f;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s += shfl_xor(s, off);
+    for (int off = 16; off > 0; off >>= 1) s += shfl_xor(s, off);
     L = L * al + s;
-    A.x *= al;
-    A.y *= al;
+    A *= al;
     M = cm;
-    for (int i0 = 0; i0 < lim; i0 += 8) {
-      float2 nx[8];
-      const bool more = i0 + 8 < lim;
-      if (more) {
+    const int most = min(32, mine - e0);
+    for (int i0 = 0;;) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) nx[k] = load(i0 + 8 + k);
+      for (int k = 0; k < 4; ++k) {
+        const float ws = shfl(w, base + i0 + k);
+        if (i0 + k < most) A += v[k] * ws;
       }
+      i0 += 4;
+      if (__ballot(i0 < most) == 0) break;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float ws = i0 + k < lim ? readlane(w, min(i0 + k, 63)) : 0.f;
-        A.x = fmaf(v[k].x, ws, A.x);
-        A.y = fmaf(v[k].y, ws, A.y);
-      }
-      if (more) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = nx[k];
-      }
+      for (int k = 0; k < 4; ++k) v[k] = load(i0 + k);
     }
   }
   if constexpr (W > 1) {
-    s_a[w0][rw][lane] = A;
+    s_a[half][lane] = A;
     if (lane == 0) {
-      s_m[w0][rw] = M;
-      s_l[w0][rw] = L;
+      s_m[half] = M;
+      s_l[half] = L;
     }
     __syncthreads();
-    if (skip || w0 != 0) return;
+    if (w0 != 0) return;
     M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, s_m[w][rw]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, s_m[half + w]);
     const float ref = M == -INFINITY ? 0.f : M;
     L = 0.f;
-    A = float2{0.f, 0.f};
+    A = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float sc = fast_exp2(s_m[w][rw] - ref);
-      const float2 x = s_a[w][rw][lane];
-      L = fmaf(s_l[w][rw], sc, L);
-      A.x = fmaf(x.x, sc, A.x);
-      A.y = fmaf(x.y, sc, A.y);
+      const float sc = fast_exp2(s_m[half + w] - ref);
+      L = fmaf(s_l[half + w], sc, L);
+      A += s_a[half + w][lane] * sc;
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint32_t *op = reinterpret_cast<uint32_t *>(a.o + (int64_t)t * a.o_stride_t + (int64_t)hq * a.o_stride_h);
-  op[lane] = E::from_float(A.x * inv) | (E::from_float(A.y * inv) << 16);
-  if (lane == 0 && a.lse) a.lse[(int64_t)t * a.hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  if (!x.skip) merged<DT>(a, x, 4 * lane, A, M, L);
 }
 
 // Blocks per kv head: as many as the chip holds, or as the longest line of `tokens` query tokens over rows of
 // `max_pages` fills with kMinShare steps each.
-int plan_blocks(int64_t tokens, int hkv, int64_t max_pages) {
-  const int64_t fill = kSlots / hkv > 0 ? kSlots / hkv : 1;
+int plan_blocks(int64_t tokens, int hkv, int64_t max_pages, int slots) {
+  const int64_t fill = slots / hkv > 0 ? slots / hkv : 1;
   const int64_t steps = ceil_div(max_pages, kPages) + kTileCost;
   if (steps >= fill * kMinShare || 2 * tokens >= fill * kMinShare) return (int)fill;
   const int64_t n = ceil_div(2 * tokens * steps, kMinShare);
   return (int)(n < fill ? n : fill);
+}
+
+// Blocks the chip holds: two per CU where their LDS (160 KiB per CU) allows.
+int resident_blocks(int prefixes, int rows) {
+  return 2 * (kStages * kStageB + Line::bytes(prefixes, rows)) <= 160 * 1024 ? kSlots : kSlots / 2;
 }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -695,8 +702,8 @@ size_t workspace_bytes_for(int64_t tokens, int hq, int hkv, int blocks) {
 
 template <int DT, int G>
 void launch_g(const PrefixArgs &a, hipStream_t stream) {
-  hipLaunchKernelGGL((prefix_attention_kernel<DT, G>), dim3((unsigned)a.hkv, (unsigned)a.blocks), dim3(kThreads), 0, stream,
-                     a);
+  hipLaunchKernelGGL((prefix_attention_kernel<DT, G>), dim3((unsigned)a.hkv, (unsigned)a.blocks), dim3(kThreads),
+                     kStages * kStageB + Line::bytes(a.num_prefixes, a.batch), stream, a);
 }
 
 template <int DT>
@@ -711,12 +718,12 @@ void launch(const PrefixArgs &a, int G, hipStream_t stream) {
     case 7: launch_g<DT, 7>(a, stream); break;
     default: launch_g<DT, 8>(a, stream); break;
   }
-  // Few rows may have many runs each (up to a block's worth): four waves to a row.
+  // Few rows may have many runs each (up to a block's worth): eight half-waves to a row.
   const int64_t rows = (int64_t)a.tokens * a.hq;
   if (rows <= 4096)
-    hipLaunchKernelGGL((prefix_merge_kernel<DT, 4>), dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((prefix_merge_kernel<DT, 8>), dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((prefix_merge_kernel<DT, 1>), dim3((unsigned)ceil_div(rows, kThreads / 64)), dim3(kThreads), 0,
+    hipLaunchKernelGGL((prefix_merge_kernel<DT, 1>), dim3((unsigned)ceil_div(rows, kThreads / 32)), dim3(kThreads), 0,
                        stream, a);
 }
 
@@ -778,7 +785,7 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
   a.tokens = (int)tokens;
   a.hq = hq;
   a.hkv = hkv;
-  a.blocks = plan_blocks(tokens, hkv, max_pages);
+  a.blocks = plan_blocks(tokens, hkv, max_pages, resident_blocks(px->num_prefixes, batch));
   a.sm_scale = sm_scale;
   const size_t need = workspace_bytes_for(tokens, hq, hkv, a.blocks);
   if (!workspace || workspace_bytes < need)
@@ -805,7 +812,7 @@ extern "C" DELTA_EXPORT size_t delta_prefix_attention_workspace_bytes(int64_t to
                                                                       int num_kv_heads, int64_t max_pages) {
   if (tokens <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads || max_pages < 0) return 0;
   return delta::workspace_bytes_for(tokens, num_qo_heads, num_kv_heads,
-                                    delta::plan_blocks(tokens, num_kv_heads, max_pages));
+                                    delta::plan_blocks(tokens, num_kv_heads, max_pages, delta::kSlots));
 }
 
 extern "C" DELTA_EXPORT int delta_paged_decode_prefix(
