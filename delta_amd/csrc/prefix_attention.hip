@@ -249,15 +249,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     // The lane, hidden from the compiler: it would keep every offset that follows from it in registers over all pieces.
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
-    const int hl = lane >> 5, n = lane & 31, lrow = lane >> 4, lch = lane & 15;
-    // K fragment of k-slice ks: row n, chunk 2 ks + hl (32 ks comes in by xor: the bits above it are the row's).
-    const uint32_t kfo = (uint32_t)(n * 256 + 16 * (hl ^ (n & 15)));
-    // ds_read_b64_tr_b16 of V^T: 16-lane group q16 = lane / 16, t16 = lane % 16 reads rows (kv) base + t16 / 4 at columns
-    // 32 dt + 16 (q16 % 2) + 4 (t16 % 4), and receives its column's four rows (64 dt by xor).
-    const int q16 = lane >> 4, t16 = lane & 15;
-    const uint32_t vfo = (uint32_t)((4 * hl + (t16 >> 2)) * 256 +
-                                    16 * ((2 * (q16 & 1) + ((t16 & 3) >> 1)) ^ (4 * (t16 >> 2))) + 8 * (t16 & 1));
-
+    const int lrow = lane >> 4, lch = lane & 15;
     // ---- The piece at pos: segment, tile, steps [s0, s1).
     const int items = a.num_prefixes + a.batch;
     for (;; item += 64) {  // the first segment that ends past pos
@@ -316,18 +308,6 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     }
     __syncthreads();  // the tile's tokens are listed, the piece before is done with the buffers
 
-    // ---- The wave's pairs: 32 from 32 qsub on.  (Which wave has the first ones goes round with the block: a short tile
-    // keeps one wave, and with it one SIMD, at work.)
-    const int qsub = (wv + blk) & 3;
-    const bool active = 32 * qsub < pairs;
-    const int pair = 32 * qsub + n;
-    const bool row_ok = pair < pairs;
-    const int pt = row_ok ? pair / G : 0, g = row_ok ? pair % G : 0;
-    const int t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
-    const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);  // the last position that the lane's pair attends
-    // Stages that end at or below the position of the wave's first token need no mask.
-    const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos + 32 * qsub / G);
-
     // Loads: wave w loads rows 4 w .. + 3 of both of a stage's pages, K and V.  Page ids, 64 per register (lane i: page
     // 64 w + i of the piece); bit i of *bad: outside the cache.
     const uint32_t wlds = lds0 + wv * 1024;
@@ -342,18 +322,9 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       *bad = __ballot(!ok);
       return ok ? id : 0;
     };
-    u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
-    {
-      const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) qf[ks] = row_ok ? ld128(qp + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
-    }
-    uint64_t bad = 0, bad_next;
-    int idv = load_ids(0, &bad);
-    // Settles q with the page ids: inside the loop its wait would also drain the stages under way.
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(qf[ks]));
-    bad_next = bad;
+    uint64_t bad = 0, bad_next = 0;
+    int idv = 0;
+    auto first_loads = [&]() { idv = load_ids(0, &bad); };
     auto issue = [&](int j) {  // stage j of the piece; a page past it is page 0 of the cache (masked later)
       const uint32_t dst = wlds + (uint32_t)(j & (kStages - 1)) * kStageB;
 #pragma unroll
@@ -368,7 +339,10 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
         }
       }
     };
-    for (int j = 0; j < 3 && j < nst; ++j) issue(j);
+    auto start = [&]() {
+      bad_next = bad;
+      for (int j = 0; j < 3 && j < nst; ++j) issue(j);
+    };
     auto bad_of = [&](int j) { return (uint32_t)(bad >> ((2 * j) & 63)) & 3u; };  // bit i: page i of stage j
     // V rows past the segment and of pages outside the cache meet p = 0 but may hold NaN/Inf: zeros.
     auto clear_v = [&](int j, uint32_t sbad) {
@@ -382,22 +356,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       }
     };
 
-    float m = -INFINITY, l = 0.f;
-    f32x16 acc[4];
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
-
-    // S^T of the first stage.
-    auto scores = [&](f32x16 &S) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) S[i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) S = MF::run(*reinterpret_cast<const u32x4 *>(tiles + (kfo ^ (32u * ks))), qf[ks], S);
-    };
-    f32x16 S;  // of the stage worked on
-    if (nst > 0) {
+    auto enter = [&]() {  // the first stage has landed
       if (nst > 2)
         wait_loads<8>();
       else if (nst > 1)
@@ -406,11 +365,9 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
         wait_loads<0>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      clear_v(0, bad_of(0));
-      if (active) scores(S);
-    }
-    for (int j = 0; j < nst; ++j) {
-      // Stage j + 1 has landed, stage j - 1 is left by every wave.
+      if (nst > 0) clear_v(0, bad_of(0));
+    };
+    auto step = [&](int j) {  // stage j + 1 has landed, stage j - 1 is left by every wave; returns bad_of(j)
       if (j + 2 < nst)
         wait_loads<4>();
       else
@@ -424,130 +381,280 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
         issue(j + 3);
       }
       if (j + 1 < nst) clear_v(j + 1, bad_of(j + 1));
-      if (!active) continue;
-      const int kv0 = s0 * kStep + 32 * j;
-      float x[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = S[i];
-      if (!(a.sm_scale > 0.f)) {  // (the scale below is positive)
-        const float sign = a.sm_scale == 0.f ? 0.f : -1.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= sign;
-      }
-      auto tok = [&](int i) { return 8 * (i >> 2) + (i & 3); };  // of x[i], from kv0 + 4 hl on
-      if (kv0 + 31 > wpos) {
-        const int last = lim - kv0 - 4 * hl;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = tok(i) <= last ? x[i] : -INFINITY;
-      }
-      if (sbad) {
-        uint32_t b = sbad;  // (in a vector register: selects, not a branch for each value)
-        asm volatile("" : "+v"(b));
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = (b >> (i >> 3)) & 1u ? -INFINITY : x[i];
-      }
-      // The next stage's S (of no use behind the last stage), an MFMA at a time between pieces of this one's softmax:
-      // each piece runs while its MFMA does.  The fences keep that order.
-      const char *tk = &tiles[((j + 1) & (kStages - 1)) * kStageB];
-      auto kfrag = [&](int ks) { return *reinterpret_cast<const u32x4 *>(tk + (kfo ^ (32u * ks))); };
-      u32x4 kq[4];
-#pragma unroll
-      for (int ks = 0; ks < 3; ++ks) kq[ks] = kfrag(ks);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) S[i] = 0.f;
-      auto mfma_s = [&](int ks) {
-        if (ks + 3 < 8) kq[(ks + 3) & 3] = kfrag(ks + 3);
-        S = MF::run(kq[ks & 3], qf[ks], S);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      float pm = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) pm = fmaxf(pm, x[i]);
-      __builtin_amdgcn_sched_barrier(0);
-      mfma_s(0);
-      // m is a reference maximum: it moves only when a score exceeds it by more than 8 (log2), so the exponentials
-      // stay <= 256 and the accumulators are rescaled on few stages.
-      const float smax = halves_max(pm) * scale2;
-      const bool moves = smax > m + 8.f;  // also the first finite score (m = -inf)
-      const float alpha = moves ? fast_exp2(m - smax) : 1.f;
-      m = moves ? smax : m;
-      const float nm = m == -INFINITY ? 0.f : -m;
-      __builtin_amdgcn_sched_barrier(0);
-      mfma_s(1);
-      const char *tv = &tiles[(j & (kStages - 1)) * kStageB + 2 * kPageB];
-      auto vfrag = [&](int i) {  // V^T fragment of 16-token chunk i / 4, d tile i % 4
-        const char *rd = tv + (vfo ^ (64u * (i % 4))) + (i / 4) * 4096;
-        const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
-        const ps4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)(rd + 2048));
-        const uint2 lo = __builtin_bit_cast(uint2, v0), hi = __builtin_bit_cast(uint2, v1);
-        return u32x4{lo.x, lo.y, hi.x, hi.y};
-      };
-      constexpr int kAhead = 4;
-      u32x4 vq[kAhead + 1];
-      float ps = 0.f;
-      u32x4 pc[2];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        x[2 * c] = fast_exp2(fmaf(x[2 * c], scale2, nm));
-        x[2 * c + 1] = fast_exp2(fmaf(x[2 * c + 1], scale2, nm));
-        if (c > 0) {
-          ps += x[2 * c - 2] + x[2 * c - 1];
-          pc[(c - 1) >> 2][(c - 1) & 3] = pack2<DT>(x[2 * c - 2], x[2 * c - 1]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (c < 6) mfma_s(c + 2);
-        if (c >= 4) vq[c - 4] = vfrag(c - 4);
-      }
-      ps += x[14] + x[15];
-      pc[1][3] = pack2<DT>(x[14], x[15]);
-      l = l * alpha + ps;  // this half-wave's tokens; joined once at the end
-      // (used here, or the compiler moves the exponentials behind the rescaling branch, away from the MFMAs)
-      asm volatile("" : "+v"(pc[0]), "+v"(pc[1]), "+v"(l));
-      if (__ballot(alpha != 1.f)) {
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i + kAhead < 8) vq[(i + kAhead) % (kAhead + 1)] = vfrag(i + kAhead);
-        acc[i % 4] = MF::run(vq[i % (kAhead + 1)], pc[i / 4], acc[i % 4]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    l = halves_sum(l);
-    // ---- Results (the lane's pair worked out again: held over the steps it would cost registers).
-    asm volatile("" : "+v"(lane));
-    const int wpair = 32 * qsub + (lane & 31), whl = lane >> 5;
-    const int wpt = wpair < pairs ? wpair / G : 0, wg = wpair - wpt * G;
-    const int wt = of_prefix ? line.toks[wpt] : q0 + t0 + wpt;
-    const bool writes = wpair < pairs;
+      return sbad;
+    };
     const bool whole = runs == 1 && !of_prefix && px < 0;
-    if (writes && whole) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t *op = a.o + (int64_t)wt * a.o_stride_t + (int64_t)(h * G + wg) * a.o_stride_h + 4 * whl;
+    // Results of a pair from the lanes that hold it: 4 outputs from d(k) on in v(k), k < N; `one` of the lanes also
+    // writes the statistics.
+    auto put = [&](auto count, int pair, bool one, float m, float l, auto &&v, auto &&d) {
+      constexpr int N = decltype(count)::value;
+      const int pt = pair / G, hq = h * G + pair - pt * G;
+      const int t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t *op = a.o + (int64_t)t * a.o_stride_t + (int64_t)hq * a.o_stride_h;
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          uint32_t *w = reinterpret_cast<uint32_t *>(op + 32 * dt + 8 * q4);
-          w[0] = pack2<DT>(acc[dt][4 * q4] * inv, acc[dt][4 * q4 + 1] * inv);
-          w[1] = pack2<DT>(acc[dt][4 * q4 + 2] * inv, acc[dt][4 * q4 + 3] * inv);
+        for (int k = 0; k < N; ++k) {
+          const f32x4 x = v(k);
+          uint32_t *w = reinterpret_cast<uint32_t *>(op + d(k));
+          w[0] = pack2<DT>(x[0] * inv, x[1] * inv);
+          w[1] = pack2<DT>(x[2] * inv, x[3] * inv);
         }
-      if (a.lse && whl == 0) a.lse[(int64_t)wt * a.hq + h * G + wg] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-    } else if (writes) {
-      const int64_t at = runs == 1 ? ((int64_t)(of_prefix ? 0 : a.tokens) + wt) * a.hq + h * G + wg
-                                   : (int64_t)2 * a.tokens * a.hq +
-                                         (((int64_t)h * a.blocks + blk) * 2 + (run == 0 ? 1 : 0)) * kQ + wpair;
-      float *op = a.part_acc + at * kHeadDim + 4 * whl;
+        if (a.lse && one) a.lse[(int64_t)t * a.hq + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      } else {
+        const int64_t at = runs == 1 ? ((int64_t)(of_prefix ? 0 : a.tokens) + t) * a.hq + hq
+                                     : (int64_t)2 * a.tokens * a.hq +
+                                           (((int64_t)h * a.blocks + blk) * 2 + (run == 0 ? 1 : 0)) * kQ + pair;
+        float *op = a.part_acc + at * kHeadDim;
+#pragma unroll
+        for (int k = 0; k < N; ++k) *reinterpret_cast<f32x4 *>(op + d(k)) = v(k);
+        if (one) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = float2{m, l};
+      }
+    };
+
+    if (pairs <= 16) {
+      // ---- One wave works, on 16x16 tiles: half the MFMA time and half the scores per lane of the 32x32 ones, which for
+      // these tiles would hold the stages up (a decode row's own pages: 0.93 us a stage, above HBM's time for it).
+      // Lane (c, n) = (lane / 16, lane % 16): pair n; scores of tokens 4 c + i and 16 + 4 c + i; outputs d = 16 dt + 4 c + i.
+      const int c = lane >> 4, n = lane & 15;
+      const bool active = ((wv + blk) & 3) == 0, ok = active && n < pairs;
+      const int pt = ok ? n / G : 0, t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
+      const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);
+      const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos);
+      u32x4 qf[4];  // B operand of S^T: d = 32 ks + 8 c + [0, 8)
+      const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + (ok ? n - pt * G : 0)) * a.q_stride_h + 8 * c;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) qf[ks] = ok ? ld128(qp + 32 * ks) : u32x4{0u, 0u, 0u, 0u};
+      first_loads();
+      // Settles q with the page ids: inside the loop its wait would also drain the stages under way.
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) asm volatile("" : "+v"(qf[ks]));
+      start();
+      const uint32_t kfo = (uint32_t)(n * 256 + 16 * (c ^ n));  // K fragment: row n (+ 16), chunk 4 ks + c (64 ks by xor)
+      // V^T fragment of d tile dt: rows 4 c .. + 3 (+ 16) at columns 16 dt + [0, 16) (32 dt by xor)
+      const uint32_t vfo = (uint32_t)((4 * c + (n >> 2)) * 256 + 16 * (((n & 3) >> 1) ^ (4 * (n >> 2))) + 8 * (n & 1));
+      float m = -INFINITY, l = 0.f;
+      f32x4 acc[8], S[2];
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      auto scores = [&](int j) {
+        const char *tk = &tiles[(j & (kStages - 1)) * kStageB];
+        S[0] = S[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            S[u] = E::mfma(*reinterpret_cast<const u32x4 *>(tk + (kfo ^ (64u * ks)) + u * 4096), qf[ks], S[u]);
+      };
+      enter();
+      if (active && nst > 0) scores(0);
+      for (int j = 0; j < nst; ++j) {
+        const uint32_t sbad = step(j);
+        if (!active) continue;
+        const int kv0 = s0 * kStep + 32 * j;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = S[i >> 2][i & 3];
+        if (!(a.sm_scale > 0.f)) {  // (the scale below is positive)
+          const float sign = a.sm_scale == 0.f ? 0.f : -1.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= sign;
+        }
+        if (kv0 + 31 > wpos || sbad) {
+          const int last = lim - kv0 - 4 * c;
+          uint32_t b = sbad;  // (in a vector register: selects, not a branch for each value)
+          asm volatile("" : "+v"(b));
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            x[i] = 16 * (i >> 2) + (i & 3) <= last && !((b >> (i >> 2)) & 1u) ? x[i] : -INFINITY;
+        }
+        scores(j + 1);  // (of no use behind the last stage) under the softmax
+        float pm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pm = fmaxf(pm, x[i]);
+        // (the reference maximum as below)
+        const float smax = rows4_max(pm) * scale2;
+        const bool moves = smax > m + 8.f;
+        const float alpha = moves ? fast_exp2(m - smax) : 1.f;
+        m = moves ? smax : m;
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float ps = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = fast_exp2(fmaf(x[i], scale2, nm));
+          ps += x[i];
+        }
+        l = l * alpha + ps;  // this lane's tokens; joined once at the end
+        const u32x4 pc = {pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]), pack2<DT>(x[4], x[5]), pack2<DT>(x[6], x[7])};
+        if (__ballot(moves)) {
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt) acc[dt] *= alpha;
+        }
+        const char *tv = &tiles[(j & (kStages - 1)) * kStageB + 2 * kPageB];
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          const char *rd = tv + (vfo ^ (32u * dt));
+          const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
+          const ps4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)(rd + 4096));
+          const uint2 lo = __builtin_bit_cast(uint2, v0), hi = __builtin_bit_cast(uint2, v1);
+          acc[dt] = E::mfma(u32x4{lo.x, lo.y, hi.x, hi.y}, pc, acc[dt]);
+        }
+      }
+      l = rows4_sum(l);
+      if (ok)
+        put(std::integral_constant<int, 8>(), n, c == 0, m, l, [&](int k) { return acc[k]; },
+            [&](int k) { return 16 * k + 4 * c; });
+    } else {
+      // ---- The wave's pairs: 32 from 32 qsub on.
+      const int n = lane & 31, hl = lane >> 5, qsub = (wv + blk) & 3;  // (a short tile keeps some SIMDs at work)
+      const bool active = 32 * qsub < pairs;
+      const int pair = 32 * qsub + n;
+      const bool row_ok = pair < pairs;
+      const int pt = row_ok ? pair / G : 0, g = row_ok ? pair % G : 0;
+      const int t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
+      const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);  // the last position that the lane's pair attends
+      // Stages that end at or below the position of the wave's first token need no mask.
+      const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos + 32 * qsub / G);
+      u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
+      {
+        const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) qf[ks] = row_ok ? ld128(qp + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
+      }
+      first_loads();
+      // (see above)
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(qf[ks]));
+      start();
+      // K fragment of k-slice ks: row n, chunk 2 ks + hl (32 ks comes in by xor: the bits above it are the row's).
+      const uint32_t kfo = (uint32_t)(n * 256 + 16 * (hl ^ (n & 15)));
+      // ds_read_b64_tr_b16 of V^T: 16-lane group q16 = lane / 16, t16 = lane % 16 reads rows (kv) base + t16 / 4 at columns
+      // 32 dt + 16 (q16 % 2) + 4 (t16 % 4), and receives its column's four rows (64 dt by xor).
+      const int q16 = lane >> 4, t16 = lane & 15;
+      const uint32_t vfo = (uint32_t)((4 * hl + (t16 >> 2)) * 256 +
+                                      16 * ((2 * (q16 & 1) + ((t16 & 3) >> 1)) ^ (4 * (t16 >> 2))) + 8 * (t16 & 1));
+      float m = -INFINITY, l = 0.f;
+      f32x16 acc[4];
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
-          *reinterpret_cast<f32x4 *>(op + 32 * dt + 8 * q4) =
-              f32x4{acc[dt][4 * q4], acc[dt][4 * q4 + 1], acc[dt][4 * q4 + 2], acc[dt][4 * q4 + 3]};
-      if (whl == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = float2{m, l};
+        for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+
+      // S^T of the first stage.
+      auto scores = [&](f32x16 &S) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) S = MF::run(*reinterpret_cast<const u32x4 *>(tiles + (kfo ^ (32u * ks))), qf[ks], S);
+      };
+      f32x16 S;  // of the stage worked on
+      enter();
+      if (active && nst > 0) scores(S);
+      for (int j = 0; j < nst; ++j) {
+        const uint32_t sbad = step(j);
+        if (!active) continue;
+        const int kv0 = s0 * kStep + 32 * j;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = S[i];
+        if (!(a.sm_scale > 0.f)) {  // (the scale below is positive)
+          const float sign = a.sm_scale == 0.f ? 0.f : -1.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] *= sign;
+        }
+        auto tok = [&](int i) { return 8 * (i >> 2) + (i & 3); };  // of x[i], from kv0 + 4 hl on
+        if (kv0 + 31 > wpos) {
+          const int last = lim - kv0 - 4 * hl;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = tok(i) <= last ? x[i] : -INFINITY;
+        }
+        if (sbad) {
+          uint32_t b = sbad;  // (in a vector register: selects, not a branch for each value)
+          asm volatile("" : "+v"(b));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = (b >> (i >> 3)) & 1u ? -INFINITY : x[i];
+        }
+        // The next stage's S (of no use behind the last stage), an MFMA at a time between pieces of this one's softmax:
+        // each piece runs while its MFMA does.  The fences keep that order.
+        const char *tk = &tiles[((j + 1) & (kStages - 1)) * kStageB];
+        auto kfrag = [&](int ks) { return *reinterpret_cast<const u32x4 *>(tk + (kfo ^ (32u * ks))); };
+        u32x4 kq[4];
+#pragma unroll
+        for (int ks = 0; ks < 3; ++ks) kq[ks] = kfrag(ks);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[i] = 0.f;
+        auto mfma_s = [&](int ks) {
+          if (ks + 3 < 8) kq[(ks + 3) & 3] = kfrag(ks + 3);
+          S = MF::run(kq[ks & 3], qf[ks], S);
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        float pm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pm = fmaxf(pm, x[i]);
+        __builtin_amdgcn_sched_barrier(0);
+        mfma_s(0);
+        // m is a reference maximum: it moves only when a score exceeds it by more than 8 (log2), so the exponentials
+        // stay <= 256 and the accumulators are rescaled on few stages.
+        const float smax = halves_max(pm) * scale2;
+        const bool moves = smax > m + 8.f;  // also the first finite score (m = -inf)
+        const float alpha = moves ? fast_exp2(m - smax) : 1.f;
+        m = moves ? smax : m;
+        const float nm = m == -INFINITY ? 0.f : -m;
+        __builtin_amdgcn_sched_barrier(0);
+        mfma_s(1);
+        const char *tv = &tiles[(j & (kStages - 1)) * kStageB + 2 * kPageB];
+        auto vfrag = [&](int i) {  // V^T fragment of 16-token chunk i / 4, d tile i % 4
+          const char *rd = tv + (vfo ^ (64u * (i % 4))) + (i / 4) * 4096;
+          const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
+          const ps4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)(rd + 2048));
+          const uint2 lo = __builtin_bit_cast(uint2, v0), hi = __builtin_bit_cast(uint2, v1);
+          return u32x4{lo.x, lo.y, hi.x, hi.y};
+        };
+        constexpr int kAhead = 4;
+        u32x4 vq[kAhead + 1];
+        float ps = 0.f;
+        u32x4 pc[2];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          x[2 * c] = fast_exp2(fmaf(x[2 * c], scale2, nm));
+          x[2 * c + 1] = fast_exp2(fmaf(x[2 * c + 1], scale2, nm));
+          if (c > 0) {
+            ps += x[2 * c - 2] + x[2 * c - 1];
+            pc[(c - 1) >> 2][(c - 1) & 3] = pack2<DT>(x[2 * c - 2], x[2 * c - 1]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if (c < 6) mfma_s(c + 2);
+          if (c >= 4) vq[c - 4] = vfrag(c - 4);
+        }
+        ps += x[14] + x[15];
+        pc[1][3] = pack2<DT>(x[14], x[15]);
+        l = l * alpha + ps;  // this half-wave's tokens; joined once at the end
+        // (used here, or the compiler moves the exponentials behind the rescaling branch, away from the MFMAs)
+        asm volatile("" : "+v"(pc[0]), "+v"(pc[1]), "+v"(l));
+        if (__ballot(alpha != 1.f)) {
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i + kAhead < 8) vq[(i + kAhead) % (kAhead + 1)] = vfrag(i + kAhead);
+          acc[i % 4] = MF::run(vq[i % (kAhead + 1)], pc[i / 4], acc[i % 4]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      l = halves_sum(l);
+      // (the lane's pair worked out again: held over the stages it would cost registers)
+      asm volatile("" : "+v"(lane));
+      const int wpair = 32 * qsub + (lane & 31);
+      if (wpair < pairs)
+        put(std::integral_constant<int, 16>(), wpair, (lane >> 5) == 0, m, l,
+            [&](int k) {
+              return f32x4{acc[k >> 2][4 * (k & 3)], acc[k >> 2][4 * (k & 3) + 1], acc[k >> 2][4 * (k & 3) + 2],
+                           acc[k >> 2][4 * (k & 3) + 3]};
+            },
+            [&](int k) { return 32 * (k >> 2) + 8 * (k & 3) + 4 * (lane >> 5); });
     }
     if (h == 0 && run == 0 && (int)threadIdx.x < ntok) {
       const int i = threadIdx.x, ti = of_prefix ? line.toks[i] : q0 + t0 + i;
