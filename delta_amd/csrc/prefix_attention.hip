@@ -65,7 +65,7 @@ struct PrefixArgs {
   // pair) of cut ones.
   float *part_ml;   // [row][2]
   float *part_acc;  // [row][128]
-  int2 *runs;       // [prefix / own][token]: first block of its tile, runs | its first pair in the tile << 16
+  int2 *runs;       // [prefix / own][token][head of the kv head's]: first block of its tile, runs | pair in the tile << 16
   int batch, tokens, hq, hkv;
   int blocks;       // per kv head
   float sm_scale;
@@ -112,12 +112,18 @@ __device__ __forceinline__ bool prefix_fits(const PrefixArgs &a, const Row &x, i
 
 __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
 
+// Tiles of n query tokens.
+template <int G>
+__device__ __forceinline__ int tiles_of(int n) {
+  return div_up(n * G, kQ);
+}
+
 // Whether a row's query tokens leave at most an eighth of its tiles idle: such a row shares no tiles with the others of
 // its prefix, but sweeps the prefix's pages with its own, from one tile's start to its end (the pages come from the L2
 // either way, and nothing has to be joined).
-template <int TT>
+template <int G>
 __device__ __forceinline__ bool fills_tiles(int qn) {
-  return 9 * qn >= 8 * TT * div_up(qn, TT);
+  return 9 * qn * G >= 8 * kQ * tiles_of<G>(qn);
 }
 
 // A pointer that is the same in every lane, in scalar registers.
@@ -152,7 +158,7 @@ __device__ __forceinline__ int block_scan(int v, int *sums, int *total) {
 
 // The tables and the line of a kv head's work, in LDS behind the stages.
 struct Line {
-  int *toks;         // [kQ] query tokens of a prefix's tile
+  int *toks;         // [kQ + 4] query tokens of a prefix's tile
   int *sums;         // [4]
   int *at;           // [prefixes + rows + 1] where each segment begins (the prefixes, then the rows), and the end
   int *prefix_toks;  // [prefixes] query tokens
@@ -163,15 +169,15 @@ struct Line {
   int *row_len;      // [rows] own tokens
   int *row_q0, *row_qn;  // [rows] query tokens
   __device__ __forceinline__ Line(int *lds, int prefixes, int rows)
-      : toks(lds), sums(toks + kQ), at(sums + 4), prefix_toks(at + prefixes + rows + 1), prefix_ids(prefix_toks + prefixes),
+      : toks(lds), sums(toks + kQ + 4), at(sums + 4), prefix_toks(at + prefixes + rows + 1), prefix_ids(prefix_toks + prefixes),
         prefix_pages(prefix_ids + prefixes), row_prefix(prefix_pages + prefixes), row_ids(row_prefix + rows),
         row_len(row_ids + rows), row_q0(row_len + rows), row_qn(row_q0 + rows) {}
   static size_t bytes(int prefixes, int rows) {
-    return ((size_t)kQ + 4 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
+    return ((size_t)kQ + 8 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
   }
 };
 
-template <int TT>
+template <int G>
 __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line) {
   const int tid = threadIdx.x, P = a.num_prefixes, B = a.batch;
   // (the rows' tables are asked for before the prefixes' have come)
@@ -191,7 +197,7 @@ __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line)
     }
     const bool named = want >= 0 && want < P;
     const int n = named ? line.prefix_pages[want] : 0;
-    const bool fits = named && !fills_tiles<TT>(x.qn) && prefix_fits(a, x, n);
+    const bool fits = named && !fills_tiles<G>(x.qn) && prefix_fits(a, x, n);
     if (fits) atomicAdd(&line.prefix_toks[want], x.qn);
     const int own = x.len - (fits ? n * kPageSize : 0);
     line.row_prefix[r] = fits ? want : -1;
@@ -206,9 +212,9 @@ __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line)
     const int i = i0 + tid;
     int cost = 0, total;
     if (i < P)
-      cost = div_up(line.prefix_toks[i], TT) * (div_up(line.prefix_pages[i], kPages) + kTileCost);
+      cost = tiles_of<G>(line.prefix_toks[i]) * (div_up(line.prefix_pages[i], kPages) + kTileCost);
     else if (i < P + B)
-      cost = div_up(line.row_qn[i - P], TT) * (div_up(line.row_len[i - P], kStep) + kTileCost);
+      cost = tiles_of<G>(line.row_qn[i - P]) * (div_up(line.row_len[i - P], kStep) + kTileCost);
     const int at = end + block_scan(cost, line.sums, &total);
     if (i < P + B) line.at[i] = at;
     end += total;
@@ -223,14 +229,13 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
 #pragma clang fp contract(off)
   using MF = Mfma32<DT>;
   using E = Elem<DT>;
-  constexpr int TT = kQ / G;  // query tokens of a tile
   // A ring of stages, each the K tile, then the V tile (swizzled rows).
   extern __shared__ __attribute__((aligned(1024))) char tiles[];
   const Line line(reinterpret_cast<int *>(tiles + kStages * kStageB), a.num_prefixes, a.batch);
 
   const int wv = uniform((int)(threadIdx.x >> 6));
   const int h = blockIdx.x, blk = blockIdx.y;
-  const int total = uniform(build_line<TT>(a, line));
+  const int total = uniform(build_line<G>(a, line));
   int share = uniform(div_up(total, a.blocks));
   share = share < kMinShare ? kMinShare : share;
   int pos = blk * share;  // (total < 2^30: checked on the host)
@@ -286,7 +291,10 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     const int first_blk = uniform(tile_at / share), runs = uniform((tile_at + cost - 1) / share) - first_blk + 1;
     const int run = blk - first_blk;
     pos = stop;
-    const int t0 = tile * TT, ntok = min(TT, seg_toks - t0), pairs = ntok * G;
+    // The tile's pairs, and the query tokens [t0, t0 + ntok) of the segment that they belong to (where G does not divide
+    // 128 a token's heads may lie in two tiles).
+    const int pairs0 = tile * kQ, pairs = min(kQ, seg_toks * G - pairs0);
+    const int t0 = pairs0 / G, ntok = (pairs0 + pairs - 1) / G + 1 - t0, skew = pairs0 - t0 * G;
     // Segment position of query token t0 + i of a row: first_pos + i; a prefix's tokens come behind all of it.
     const int first_pos = of_prefix ? len : len - seg_toks + t0;
     if (!of_prefix) {
@@ -388,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     // writes the statistics.
     auto put = [&](auto count, int pair, bool one, float m, float l, auto &&v, auto &&d) {
       constexpr int N = decltype(count)::value;
-      const int pt = pair / G, hq = h * G + pair - pt * G;
+      const int pt = (skew + pair) / G, hq = h * G + skew + pair - pt * G;
       const int t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -418,11 +426,11 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       // Lane (c, n) = (lane / 16, lane % 16): pair n; scores of tokens 4 c + i and 16 + 4 c + i; outputs d = 16 dt + 4 c + i.
       const int c = lane >> 4, n = lane & 15;
       const bool active = ((wv + blk) & 3) == 0, ok = active && n < pairs;
-      const int pt = ok ? n / G : 0, t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
+      const int pt = ok ? (skew + n) / G : 0, t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
       const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);
       const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos);
       u32x4 qf[4];  // B operand of S^T: d = 32 ks + 8 c + [0, 8)
-      const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + (ok ? n - pt * G : 0)) * a.q_stride_h + 8 * c;
+      const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + (ok ? skew + n - pt * G : 0)) * a.q_stride_h + 8 * c;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) qf[ks] = ok ? ld128(qp + 32 * ks) : u32x4{0u, 0u, 0u, 0u};
       first_loads();
@@ -510,11 +518,11 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       const bool active = 32 * qsub < pairs;
       const int pair = 32 * qsub + n;
       const bool row_ok = pair < pairs;
-      const int pt = row_ok ? pair / G : 0, g = row_ok ? pair % G : 0;
+      const int pt = row_ok ? (skew + pair) / G : 0, g = row_ok ? (skew + pair) % G : 0;
       const int t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
       const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);  // the last position that the lane's pair attends
       // Stages that end at or below the position of the wave's first token need no mask.
-      const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos + 32 * qsub / G);
+      const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos + (skew + 32 * qsub) / G);
       u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
       {
         const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
@@ -656,10 +664,11 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
             },
             [&](int k) { return 32 * (k >> 2) + 8 * (k & 3) + 4 * (lane >> 5); });
     }
-    if (h == 0 && run == 0 && (int)threadIdx.x < ntok) {
-      const int i = threadIdx.x, ti = of_prefix ? line.toks[i] : q0 + t0 + i;
-      a.runs[(of_prefix ? 0 : a.tokens) + ti] = int2{first_blk, runs | (i * G) << 16};
-      if (!of_prefix && px < 0) a.runs[ti] = int2{0, 0};
+    if (h == 0 && run == 0 && (int)threadIdx.x < pairs) {
+      const int pair = threadIdx.x, pt = (skew + pair) / G, g = skew + pair - pt * G;
+      const int ti = of_prefix ? line.toks[pt] : q0 + t0 + pt;
+      a.runs[((of_prefix ? 0 : a.tokens) + ti) * G + g] = int2{first_blk, runs | pair << 16};
+      if (!of_prefix && px < 0) a.runs[ti * G + g] = int2{0, 0};
     }
     __syncthreads();  // the next piece lists its tokens and loads its pages
   }
@@ -679,10 +688,10 @@ __device__ __forceinline__ Runs runs_of(const PrefixArgs &a, int64_t row) {
   x.h = x.hq / G;
 #pragma unroll
   for (int kind = 0; kind < 2; ++kind) {  // (the limits keep a table that is no CSR inside the partials)
-    const int2 r = a.runs[kind * a.tokens + x.t];
+    const int2 r = a.runs[(kind * a.tokens + x.t) * G + x.hq - x.h * G];
     x.first[kind] = min(max(r.x, 0), a.blocks - 1);
     x.count[kind] = min(r.y & 0xffff, a.blocks - x.first[kind]);
-    x.pair[kind] = min((r.y >> 16) & 0xffff, kQ - G) + x.hq - x.h * G;
+    x.pair[kind] = min((r.y >> 16) & 0xffff, kQ - 1);
   }
   x.skip = !in || (a.qo_indptr && (x.t < a.qo_indptr[0] || x.t >= a.qo_indptr[a.batch])) ||
            (x.count[0] == 0 && x.count[1] == 1);
@@ -804,7 +813,7 @@ size_t partial_rows(int64_t tokens, int hq, int hkv, int blocks) {
 size_t workspace_bytes_for(int64_t tokens, int hq, int hkv, int blocks) {
   const size_t rows = partial_rows(tokens, hq, hkv, blocks);
   return align256(rows * 2 * sizeof(float)) + align256(rows * kHeadDim * sizeof(float)) +
-         align256((size_t)2 * tokens * sizeof(int2));
+         align256((size_t)2 * tokens * (hq / hkv) * sizeof(int2));
 }
 
 template <int DT, int G>
@@ -865,7 +874,7 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
   // The line's length and the partials' rows stay below 2^30 (tiles of the rows and of the prefixes, each at most the
   // longest list's steps).
   const int64_t longest = kv_indices_len > px->indices_len ? kv_indices_len : px->indices_len;
-  if (tokens > 1 << 23 || 2 * (ceil_div(tokens, kQ / G) + batch) * (ceil_div(longest, kPages) + kTileCost + 1) > 1 << 30 ||
+  if (tokens > 1 << 23 || 2 * (ceil_div(tokens * G, kQ) + batch) * (ceil_div(longest, kPages) + kTileCost + 1) > 1 << 30 ||
       partial_rows(tokens, hq, hkv, kSlots) > 1 << 30)
     return set_error(DELTA_ERR_INVALID, "%s: too many query tokens", who);
   PrefixArgs a;
