@@ -132,7 +132,7 @@ SIGNATURES = {
         c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, c_size_t, _P]),
     "delta_paged_prefill_prefix": (c_int, [
         _SP, _P, c_int64, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int64, _P,
-        c_int, c_int64, c_int, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
+        c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
     "delta_copy_pages": (c_int, [
         ctypes.POINTER(_P), c_int, c_int64, c_int, c_int, c_int, _P, _P, _P, c_int64, _P]),
 }

@@ -41,7 +41,7 @@ constexpr int kQ = 128;                 // (token, head) pairs of a tile, at mos
 constexpr int kMaxRows = 1024;          // rows, and prefixes, of a call (the tables: 41 KiB)
 constexpr int kSlots = 512;             // blocks the chip holds (two per CU)
 constexpr int kTileCost = 2;            // steps that a tile costs besides its own
-constexpr int kMinShare = 4;            // steps of a share, at least
+constexpr int kMinShare = 2;            // steps of a share, at least
 
 struct PrefixArgs {
   const uint16_t *q;
@@ -822,6 +822,12 @@ void launch_g(const PrefixArgs &a, hipStream_t stream) {
                      kStages * kStageB + Line::bytes(a.num_prefixes, a.batch), stream, a);
 }
 
+template <int DT, int W>
+void launch_merge(const PrefixArgs &a, int64_t rows, hipStream_t stream) {
+  constexpr int kRows = kThreads / 32 / W;
+  hipLaunchKernelGGL((prefix_merge_kernel<DT, W>), dim3((unsigned)ceil_div(rows, kRows)), dim3(kThreads), 0, stream, a);
+}
+
 template <int DT>
 void launch(const PrefixArgs &a, int G, hipStream_t stream) {
   switch (G) {
@@ -834,21 +840,44 @@ void launch(const PrefixArgs &a, int G, hipStream_t stream) {
     case 7: launch_g<DT, 7>(a, stream); break;
     default: launch_g<DT, 8>(a, stream); break;
   }
-  // Few rows may have many runs each (up to a block's worth): eight half-waves to a row.
-  const int64_t rows = (int64_t)a.tokens * a.hq;
-  if (rows <= 4096)
-    hipLaunchKernelGGL((prefix_merge_kernel<DT, 8>), dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+  // Where all tokens share a prefix a row has as many runs as blocks share its tile, about 512 * 128 / rows: about four of
+  // them to a half-wave.
+  const int64_t rows = (int64_t)a.tokens * a.hq, each = ceil_div((int64_t)kSlots * kQ, rows);
+  if (each > 16)
+    launch_merge<DT, 8>(a, rows, stream);
+  else if (each > 8)
+    launch_merge<DT, 4>(a, rows, stream);
+  else if (each > 4)
+    launch_merge<DT, 2>(a, rows, stream);
   else
-    hipLaunchKernelGGL((prefix_merge_kernel<DT, 1>), dim3((unsigned)ceil_div(rows, kThreads / 32)), dim3(kThreads), 0,
-                       stream, a);
+    launch_merge<DT, 1>(a, rows, stream);
 }
 
-int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
-               const int32_t *qo_indptr, const int32_t *kv_indptr, const int32_t *kv_indices, int64_t kv_indices_len,
-               const int32_t *kv_last_page_len, const delta_shared_prefix_t *px, void *o, int64_t o_stride_t,
-               int64_t o_stride_h, float *lse, int batch, int64_t tokens, int hq, int hkv, int head_dim, int dtype,
-               float sm_scale, int64_t max_pages, void *workspace, size_t workspace_bytes, delta_stream_t stream,
-               const char *who) {
+// Whether a decode batch is too small for sharing to pay: one row, or rows that are read in the time that the launches
+// here take besides their work (about 8 us: the line, the pieces' beginnings, the merge).  The ordinary launch reads every
+// row, pages that rows share mostly from the L2 and the Infinity Cache.  (us here / ordinary, 8 kv heads of 4: 4 rows of 2100
+// tokens, 34 MB of K and V, 13.6 / 11.4; 8 of 1100, 36 MB, 13.9 / 11.9; 16 of 4170, 270 MB, 21 / 27; 2 kv heads of 6: 2 of 550, 1
+// MB, 12.5 / 9.5; one row of 4200, 8 kv heads, 15 / 10.8.)
+bool decode_alone(int64_t rows, int hkv, int64_t max_pages) {
+  return hkv <= 16 && (rows == 1 || rows * hkv * max_pages <= 8192);  // page-heads of 8 KiB: 64 MB
+}
+// And a prompt step: the ordinary launch has one block sweep a row's pages for each of its tiles, 0.33 us a page, so only
+// where all rows together are short (3 prompts of up to 17 tokens over 304, 60 pages: 16.7 / 11.4; 2 of up to 20 over 1024, 132
+// pages: 17.4 / 26.7).
+bool prefill_alone(int64_t pages) { return pages <= 64; }
+
+size_t prefix_workspace_bytes(int64_t tokens, int hq, int hkv, int64_t max_pages) {
+  const size_t n = workspace_bytes_for(tokens, hq, hkv, plan_blocks(tokens, hkv, max_pages, kSlots));
+  if (!decode_alone(tokens, hkv, max_pages)) return n;
+  const size_t alone = delta_paged_decode_workspace_bytes((int)tokens, hq, hkv, (int)max_pages);
+  return n > alone ? n : alone;
+}
+
+int check_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+                 const int32_t *kv_indptr, const int32_t *kv_indices, int64_t kv_indices_len,
+                 const int32_t *kv_last_page_len, const delta_shared_prefix_t *px, const void *o, int64_t o_stride_t,
+                 int64_t o_stride_h, int batch, int64_t tokens, int hq, int hkv, int head_dim, int dtype, int64_t max_pages,
+                 const void *workspace, size_t workspace_bytes, const char *who) {
   clear_error();
   if (batch <= 0 || tokens <= 0) return DELTA_OK;
   if (head_dim != kHeadDim) return set_error(DELTA_ERR_INVALID, "%s: head_dim must be 128", who);
@@ -871,12 +900,25 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
   if (num_pages <= 0 || kv_indices_len < 0 || px->indices_len < 0 || kv_indices_len > INT32_MAX / kPageSize ||
       px->indices_len > INT32_MAX / kPageSize)
     return set_error(DELTA_ERR_INVALID, "%s: empty cache or bad table lengths", who);
-  // The line's length and the partials' rows stay below 2^30 (tiles of the rows and of the prefixes, each at most the
-  // longest list's steps).
-  const int64_t longest = kv_indices_len > px->indices_len ? kv_indices_len : px->indices_len;
-  if (tokens > 1 << 23 || 2 * (ceil_div(tokens * G, kQ) + batch) * (ceil_div(longest, kPages) + kTileCost + 1) > 1 << 30 ||
-      partial_rows(tokens, hq, hkv, kSlots) > 1 << 30)
+  // The line's length (each segment's tiles, at most all tokens', times its steps) and the partials' rows stay below 2^30.
+  const int64_t steps = ceil_div(kv_indices_len, kPages) + ceil_div(px->indices_len, kPages) +
+                        (kTileCost + 1) * ((int64_t)batch + px->num_prefixes);
+  if (tokens > 1 << 23 || (ceil_div(tokens * G, kQ) + 1) * steps > 1 << 30 || partial_rows(tokens, hq, hkv, kSlots) > 1 << 30)
     return set_error(DELTA_ERR_INVALID, "%s: too many query tokens", who);
+  const size_t need = prefix_workspace_bytes(tokens, hq, hkv, max_pages);
+  if (!workspace || workspace_bytes < need)
+    return set_error(DELTA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+  if ((uintptr_t)workspace & 255u) return set_error(DELTA_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
+  return DELTA_OK;
+}
+
+// Arguments checked by check_prefix.
+int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+               const int32_t *qo_indptr, const int32_t *kv_indptr, const int32_t *kv_indices, int64_t kv_indices_len,
+               const int32_t *kv_last_page_len, const delta_shared_prefix_t *px, void *o, int64_t o_stride_t,
+               int64_t o_stride_h, float *lse, int batch, int64_t tokens, int hq, int hkv, int dtype, float sm_scale,
+               int64_t max_pages, void *workspace, delta_stream_t stream, const char *who) {
+  const int G = hq / hkv;
   PrefixArgs a;
   a.q = (const uint16_t *)q;
   a.q_stride_t = q_stride_t;
@@ -903,10 +945,6 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
   a.hkv = hkv;
   a.blocks = plan_blocks(tokens, hkv, max_pages, resident_blocks(px->num_prefixes, batch));
   a.sm_scale = sm_scale;
-  const size_t need = workspace_bytes_for(tokens, hq, hkv, a.blocks);
-  if (!workspace || workspace_bytes < need)
-    return set_error(DELTA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
-  if ((uintptr_t)workspace & 255u) return set_error(DELTA_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
   const size_t rows = partial_rows(tokens, hq, hkv, a.blocks);
   char *ws = (char *)workspace;
   a.part_ml = (float *)ws;
@@ -926,9 +964,10 @@ int run_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void
 
 extern "C" DELTA_EXPORT size_t delta_prefix_attention_workspace_bytes(int64_t tokens, int num_qo_heads,
                                                                       int num_kv_heads, int64_t max_pages) {
-  if (tokens <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads || max_pages < 0) return 0;
-  return delta::workspace_bytes_for(tokens, num_qo_heads, num_kv_heads,
-                                    delta::plan_blocks(tokens, num_kv_heads, max_pages, delta::kSlots));
+  if (tokens <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads || max_pages < 0 ||
+      max_pages > INT32_MAX || tokens > INT32_MAX)
+    return 0;
+  return delta::prefix_workspace_bytes(tokens, num_qo_heads, num_kv_heads, max_pages > 1 ? max_pages : 1);
 }
 
 extern "C" DELTA_EXPORT int delta_paged_decode_prefix(
@@ -937,25 +976,45 @@ extern "C" DELTA_EXPORT int delta_paged_decode_prefix(
     const int32_t *kv_last_page_len, void *o, int64_t o_stride_b, int64_t o_stride_h, float *lse, int batch,
     int num_qo_heads, int num_kv_heads, int head_dim, int dtype, float sm_scale, int max_pages_per_row,
     void *workspace, size_t workspace_bytes, delta_stream_t stream) {
+  const char *who = "delta_paged_decode_prefix";
+  if (max_pages_per_row <= 0) max_pages_per_row = 1;
+  const int rc = delta::check_prefix(q, q_stride_b, q_stride_h, kv_cache, num_pages, kv_indptr, kv_indices, kv_indices_len,
+                                     kv_last_page_len, prefix, o, o_stride_b, o_stride_h, batch, batch, num_qo_heads,
+                                     num_kv_heads, head_dim, dtype, max_pages_per_row, workspace, workspace_bytes, who);
+  if (rc != DELTA_OK || batch <= 0) return rc;
+  if (delta::decode_alone(batch, num_kv_heads, max_pages_per_row))
+    return delta_paged_decode(q, q_stride_b, q_stride_h, kv_cache, num_pages, kv_indptr, kv_indices, kv_indices_len,
+                              kv_last_page_len, o, o_stride_b, o_stride_h, lse, nullptr, 0, 0, batch, num_qo_heads,
+                              num_kv_heads, head_dim, dtype, sm_scale, max_pages_per_row, workspace, workspace_bytes,
+                              stream);
   return delta::run_prefix(q, q_stride_b, q_stride_h, kv_cache, num_pages, nullptr, kv_indptr, kv_indices,
                            kv_indices_len, kv_last_page_len, prefix, o, o_stride_b, o_stride_h, lse, batch, batch,
-                           num_qo_heads, num_kv_heads, head_dim, dtype, sm_scale, max_pages_per_row, workspace,
-                           workspace_bytes, stream, "delta_paged_decode_prefix");
+                           num_qo_heads, num_kv_heads, dtype, sm_scale, max_pages_per_row, workspace, stream, who);
 }
 
 extern "C" DELTA_EXPORT int delta_paged_prefill_prefix(
     const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *kv_cache,
     int64_t num_pages, const int32_t *qo_indptr, const int32_t *kv_indptr, const int32_t *kv_indices,
     int64_t kv_indices_len, const int32_t *kv_last_page_len, void *o, int64_t o_stride_t, int64_t o_stride_h,
-    float *lse, int batch, int64_t num_tokens, int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
+    float *lse, int batch, int64_t num_tokens, int max_qo_len, int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
     float sm_scale, void *workspace, size_t workspace_bytes, delta_stream_t stream) {
   const char *who = "delta_paged_prefill_prefix";
+  if (max_qo_len <= 0) num_tokens = 0;
   if (batch > 0 && num_tokens > 0 && !qo_indptr) {
     delta::clear_error();
     return delta::set_error(DELTA_ERR_INVALID, "%s: null pointer", who);
   }
+  const int rc = delta::check_prefix(q, q_stride_t, q_stride_h, kv_cache, num_pages, kv_indptr, kv_indices, kv_indices_len,
+                                     kv_last_page_len, prefix, o, o_stride_t, o_stride_h, batch, num_tokens, num_qo_heads,
+                                     num_kv_heads, head_dim, dtype, kv_indices_len > 1 ? kv_indices_len : 1, workspace,
+                                     workspace_bytes, who);
+  if (rc != DELTA_OK || batch <= 0 || num_tokens <= 0) return rc;
+  if (delta::prefill_alone(kv_indices_len) && !((uintptr_t)o & 7u) && o_stride_t % 4 == 0 && o_stride_h % 4 == 0)
+    return delta_paged_prefill(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices,
+                               kv_indices_len, kv_last_page_len, o, o_stride_t, o_stride_h, lse, batch, num_qo_heads,
+                               num_kv_heads, head_dim, dtype, sm_scale, max_qo_len, stream);
   return delta::run_prefix(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices,
                            kv_indices_len, kv_last_page_len, prefix, o, o_stride_t, o_stride_h, lse, batch, num_tokens,
-                           num_qo_heads, num_kv_heads, head_dim, dtype, sm_scale, kv_indices_len, workspace,
-                           workspace_bytes, stream, who);
+                           num_qo_heads, num_kv_heads, dtype, sm_scale, kv_indices_len > 1 ? kv_indices_len : 1, workspace, stream,
+                           who);
 }

@@ -8,6 +8,7 @@ any graph capture; the kernels themselves never allocate or synchronise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -18,6 +19,7 @@ from . import _lib
 
 PAGE_SIZE = 16
 HEAD_DIM = 128
+_DEFAULT_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 _DTYPES = {torch.bfloat16: _lib.DELTA_BF16, torch.float16: _lib.DELTA_FP16}
 
@@ -370,37 +372,53 @@ def paged_prefill(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tens
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def prefix_attention_workspace_bytes(tokens: int, hq: int, hkv: int, max_pages: int) -> int:
     """Bytes of workspace of ``paged_decode_prefix`` (``tokens`` = rows, ``max_pages`` = its ``max_pages_per_row``)
     and ``paged_prefill_prefix`` (``tokens`` = query tokens, ``max_pages`` = entries of ``kv_indices``)."""
     return int(_lib.query("delta_prefix_attention_workspace_bytes", int(tokens), int(hq), int(hkv), int(max_pages)))
 
 
-def _prefix_struct(row_prefix: torch.Tensor, indptr: torch.Tensor, indices: torch.Tensor, B: int):
-    _check_i32("row_prefix", row_prefix, B)
-    _check_i32("prefix_indptr", indptr, 1)
-    _check_i32("prefix_indices", indices)
-    return _lib.SharedPrefixC(row_prefix.data_ptr(), indptr.data_ptr(), indices.data_ptr(), indices.numel(),
-                              indptr.numel() - 1)
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """``_lib.call`` with ``dev`` as the current device (the launch's stream is one of its)."""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream(dev))
 
 
-def _prefix_outputs(q: torch.Tensor, hq: int, out: Optional[torch.Tensor], lse: Optional[torch.Tensor]):
+def _prefix_call(name: str, q, kv_cache, B: int, tables: tuple, prefix: tuple, out, lse, workspace, max_pages: int,
+                 sm_scale: Optional[float], tail: tuple) -> torch.Tensor:
+    """What the two attention calls over shared prefixes have in common: checks, outputs, workspace, the call.
+    ``tables`` are the row tables in the entry point's order, the page indices next to last; ``tail`` the arguments
+    between the batch and the head counts."""
+    indices, row_prefix, p_indptr, p_indices = tables[-2], *prefix
+    dev = _check_cuda(q, kv_cache, *tables, *prefix, out, lse, workspace)
+    _check_cache(kv_cache)
+    hq, hkv = _check_heads(q, kv_cache)
+    for what, t, n in (("kv_indptr", tables[-3], B + 1), ("kv_indices", indices, 0), ("kv_last_page_len", tables[-1], B),
+                       ("row_prefix", row_prefix, B), ("prefix_indptr", p_indptr, 1), ("prefix_indices", p_indices, 0)):
+        _check_i32(what, t, n)
     if out is None:
         out = torch.empty_like(q)
-    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("out must match q's shape/dtype with unit inner stride")
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], hq)
-                            or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
         raise ValueError(f"lse must be contiguous fp32 [{q.shape[0]}, {hq}]")
-    return out
-
-
-def _prefix_workspace(workspace: Optional[torch.Tensor], need: int, dev: torch.device) -> torch.Tensor:
+    need = prefix_attention_workspace_bytes(q.shape[0], hq, hkv, max_pages)
     if workspace is None:  # of this call: safe on any stream, in any capture
-        return torch.empty(need, dtype=torch.uint8, device=dev)
-    if workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace too small: {need} bytes needed")
-    return workspace
+    px = _lib.SharedPrefixC(row_prefix.data_ptr(), p_indptr.data_ptr(), p_indices.data_ptr(), p_indices.numel(),
+                            p_indptr.numel() - 1)
+    _call_on(dev, name, ctypes.byref(px), q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), kv_cache.shape[0],
+             *[t.data_ptr() for t in tables[:-1]], indices.numel(), tables[-1].data_ptr(), out.data_ptr(), out.stride(0),
+             out.stride(1), _ptr(lse), B, *tail[0], hq, hkv, HEAD_DIM, _DTYPES[q.dtype],
+             _DEFAULT_SCALE if sm_scale is None else float(sm_scale), *tail[1], workspace.data_ptr(),
+             workspace.numel() * workspace.element_size())
+    return out
 
 
 def paged_decode_prefix(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
@@ -413,26 +431,11 @@ def paged_decode_prefix(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torc
 
     ``row_prefix`` (int32 [B]) names each row's prefix, -1 for none; prefix p's full pages are
     ``prefix_indices[prefix_indptr[p]:prefix_indptr[p + 1]]``, and the rows' CSR lists them too, first.  A row that
-    its prefix does not fit in attends its own CSR alone.  At most 1024 rows and prefixes."""
-    dev = _check_cuda(q, kv_cache, kv_indptr, kv_indices, kv_last_page_len, row_prefix, prefix_indptr, prefix_indices,
-                      out, lse, workspace)
-    _check_cache(kv_cache)
-    hq, hkv = _check_heads(q, kv_cache)
-    B = q.shape[0]
-    _check_i32("kv_indptr", kv_indptr, B + 1)
-    _check_i32("kv_indices", kv_indices)
-    _check_i32("kv_last_page_len", kv_last_page_len, B)
-    px = _prefix_struct(row_prefix, prefix_indptr, prefix_indices, B)
-    out = _prefix_outputs(q, hq, out, lse)
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(HEAD_DIM)
-    workspace = _prefix_workspace(workspace, prefix_attention_workspace_bytes(B, hq, hkv, max_pages_per_row), dev)
-    _lib.call("delta_paged_decode_prefix", ctypes.byref(px), q.data_ptr(), q.stride(0), q.stride(1),
-              kv_cache.data_ptr(), kv_cache.shape[0], kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
-              kv_last_page_len.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), B, hq, hkv,
-              HEAD_DIM, _dtype_code(q), float(sm_scale), int(max_pages_per_row), workspace.data_ptr(),
-              workspace.numel() * workspace.element_size(), _stream(dev))
-    return out
+    its prefix does not fit in attends its own CSR alone.  At most 1024 rows and prefixes.  ``workspace``
+    (``prefix_attention_workspace_bytes``) is allocated for the call where none is given."""
+    return _prefix_call("delta_paged_decode_prefix", q, kv_cache, q.shape[0], (kv_indptr, kv_indices, kv_last_page_len),
+                        (row_prefix, prefix_indptr, prefix_indices), out, lse, workspace, int(max_pages_per_row), sm_scale,
+                        ((), (int(max_pages_per_row),)))
 
 
 def paged_prefill_prefix(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor,
@@ -443,29 +446,12 @@ def paged_prefill_prefix(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: tor
     """``paged_prefill`` for prompts that continue shared prefixes (``delta_paged_prefill_prefix``); q/out
     [nnz, Hq, 128], the prefixes as in ``paged_decode_prefix``.
 
-    A row's prefix applies where it ends before the row's query tokens.  ``max_qo_len`` is the longest row's count of
-    them, as for ``paged_prefill``.  ``out`` and ``lse`` of tokens behind the last row are left as they were."""
-    dev = _check_cuda(q, kv_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, row_prefix, prefix_indptr,
-                      prefix_indices, out, lse, workspace)
-    _check_cache(kv_cache)
-    hq, hkv = _check_heads(q, kv_cache)
-    B = qo_indptr.numel() - 1
+    A row's prefix applies where it ends before the row's query tokens.  ``max_qo_len`` is at least the longest row's
+    count of them, as for ``paged_prefill``.  ``out`` and ``lse`` of tokens behind the last row are left as they were."""
     _check_i32("qo_indptr", qo_indptr, 1)
-    _check_i32("kv_indptr", kv_indptr, B + 1)
-    _check_i32("kv_indices", kv_indices)
-    _check_i32("kv_last_page_len", kv_last_page_len, B)
-    px = _prefix_struct(row_prefix, prefix_indptr, prefix_indices, B)
-    out = _prefix_outputs(q, hq, out, lse)
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(HEAD_DIM)
-    need = prefix_attention_workspace_bytes(q.shape[0], hq, hkv, kv_indices.numel())
-    workspace = _prefix_workspace(workspace, need, dev)
-    _lib.call("delta_paged_prefill_prefix", ctypes.byref(px), q.data_ptr(), q.stride(0), q.stride(1),
-              kv_cache.data_ptr(), kv_cache.shape[0], qo_indptr.data_ptr(), kv_indptr.data_ptr(),
-              kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), out.data_ptr(), out.stride(0),
-              out.stride(1), _ptr(lse), B, q.shape[0], hq, hkv, HEAD_DIM, _dtype_code(q), float(sm_scale),
-              workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(dev))
-    return out
+    return _prefix_call("delta_paged_prefill_prefix", q, kv_cache, qo_indptr.numel() - 1,
+                        (qo_indptr, kv_indptr, kv_indices, kv_last_page_len), (row_prefix, prefix_indptr, prefix_indices),
+                        out, lse, workspace, kv_indices.numel(), sm_scale, ((q.shape[0], int(max_qo_len)), ()))
 
 
 def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, *,
@@ -478,11 +464,12 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
     if len(caches) == 0:
         raise ValueError("no caches")
     first = caches[0]
-    dev = _check_cuda(src, dst, tokens, *caches)
-    for c in caches:
-        _check_cache(c)
-        if c.shape != first.shape or c.dtype != first.dtype:
-            raise ValueError("the caches must share a shape and a dtype")
+    dev = _check_cuda(first, src, dst, tokens)
+    _check_cache(first)
+    shape, dtype = first.shape, first.dtype
+    for c in caches:  # (a launch of a few microseconds goes over every layer: no more than is needed for each)
+        if c.shape != shape or c.dtype is not dtype or c.device != dev or not c.is_contiguous():
+            raise ValueError("the caches must be contiguous, on one device, and share a shape and a dtype")
     n = src.numel()
     _check_i32("src", src)
     _check_i32("dst", dst)
@@ -493,8 +480,8 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
         if tokens.numel() != n:
             raise ValueError(f"src names {n} pages, tokens {tokens.numel()}")
     ptrs = (ctypes.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
-    _lib.call("delta_copy_pages", ptrs, len(caches), first.shape[0], first.shape[3], HEAD_DIM, _dtype_code(first),
-              src.data_ptr(), dst.data_ptr(), _ptr(tokens), n, _stream(dev))
+    _call_on(dev, "delta_copy_pages", ptrs, len(caches), shape[0], shape[3], HEAD_DIM, _DTYPES[dtype], src.data_ptr(),
+             dst.data_ptr(), _ptr(tokens), n)
 
 
 def page_scores_from_logits(logits_dump: torch.Tensor, kv_indptr: torch.Tensor,

@@ -546,17 +546,18 @@ typedef struct {
 
 /* Bytes of workspace of the two calls below: `tokens` query tokens (decode: batch),
  * `max_pages` = the decode call's max_pages_per_row, or the prompt call's kv_indices_len
- * (no initial contents needed; calls that share a workspace must not overlap).  Grows with
- * neither argument beyond what 512 blocks write: about 70 MB, or two partials (1040 bytes)
- * per (query token, q head) where that is more. */
+ * (no initial contents needed; calls that share a workspace must not overlap): two partials
+ * (1040 bytes) per (query token, q head), and up to 68 MB for what 512 blocks cut. */
 size_t delta_prefix_attention_workspace_bytes(int64_t tokens, int num_qo_heads, int num_kv_heads,
                                               int64_t max_pages);
 
 /* delta_paged_decode for a batch whose rows share prefixes: the same o and lse (to
  * rounding: the softmax is summed in another order), with each prefix's K and V read once
  * for all its rows instead of once per row.  Row b's prefix applies where its pages fit in
- * the row (16 * pages <= kv_len_b); a row it does not fit attends its own CSR alone.
- * batch <= 1024.  No counterpart in the reference. */
+ * the row (16 * pages <= kv_len_b); a row it does not fit attends its own CSR alone, and so
+ * does every row of a batch too small for sharing to pay.  max_pages_per_row is the planned
+ * maximum of the rows' pages (a longer row is still covered whole).  batch <= 1024.  No
+ * counterpart in the reference. */
 int delta_paged_decode_prefix(const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_b,
                               int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
                               const int32_t *kv_indptr, const int32_t *kv_indices,
@@ -568,17 +569,18 @@ int delta_paged_decode_prefix(const delta_shared_prefix_t *prefix, const void *q
 
 /* delta_paged_prefill for prompts that continue shared prefixes: num_tokens query tokens in
  * rows of qo_indptr, causal.  A row's prefix applies where it lies in front of the row's
- * query tokens (16 * pages <= kv_len_b - qo_len_b).  o and lse of tokens behind the last
- * row are left as they were.  batch <= 1024. */
+ * query tokens (16 * pages <= kv_len_b - qo_len_b).  max_qo_len >= every row's query
+ * tokens, as for delta_paged_prefill.  o and lse of tokens behind the last row are left as
+ * they were.  batch <= 1024. */
 int delta_paged_prefill_prefix(const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_t,
                                int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
                                const int32_t *qo_indptr, const int32_t *kv_indptr,
                                const int32_t *kv_indices, int64_t kv_indices_len,
                                const int32_t *kv_last_page_len, void *o, int64_t o_stride_t,
                                int64_t o_stride_h, float *lse, int batch, int64_t num_tokens,
-                               int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
-                               float sm_scale, void *workspace, size_t workspace_bytes,
-                               delta_stream_t stream);
+                               int max_qo_len, int num_qo_heads, int num_kv_heads,
+                               int head_dim, int dtype, float sm_scale, void *workspace,
+                               size_t workspace_bytes, delta_stream_t stream);
 
 /* Copies pages inside each of num_caches paged caches of one shape (`caches`: a HOST array
  * of device pointers, one per layer): entry i copies the first tokens[i] tokens (clamped to

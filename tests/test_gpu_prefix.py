@@ -31,7 +31,8 @@ def indptr(counts):
 
 
 class Batch:
-    """Rows (prefix or -1, own tokens, query tokens) over prefixes of the given page counts, on shuffled pages."""
+    """Rows (prefix or -1, own tokens, query tokens) over prefixes of the given page counts, on shuffled pages.  Planned
+    for long rows (max_pages_per_row, a long kv_indices), or the small batches here would go to the ordinary kernels."""
 
     def __init__(self, hq, hkv, prefix_pages, rows, dtype="bf16", seed=0, num_pages=None, first_page=0, stale=None):
         g = torch.Generator(device=DEV)
@@ -55,14 +56,14 @@ class Batch:
                     self.cache[pg[-1], :, n:] = stale
         self.q = torch.empty(sum(r[2] for r in rows), hq, D, dtype=DT[dtype], device=DEV).normal_(0, 1, generator=g)
         self.qo = indptr([r[2] for r in rows])
-        self.t = dict(kv_indptr=i32(indptr([len(p) for p in self.pages])), kv_indices=i32([x for p in self.pages for x in p]),
+        self.t = dict(kv_indptr=i32(indptr([len(p) for p in self.pages])), kv_indices=i32([x for p in self.pages for x in p] + [-1] * 65),
                       last=i32(last), row_prefix=i32([p for p, _, _ in rows]), prefix_indptr=i32(indptr(prefix_pages)),
                       prefix_indices=i32([x for s in self.shared for x in s]))
 
     def decode(self, **kw):
         t = self.t
         lse = torch.full((len(self.rows), self.hq), 7.0, device=DEV)
-        kw.setdefault("max_pages_per_row", max(1, max(len(p) for p in self.pages)))
+        kw.setdefault("max_pages_per_row", 8192)
         kw.setdefault("lse", lse)
         o = K.paged_decode_prefix(kw.pop("q", self.q), self.cache, t["kv_indptr"], t["kv_indices"], t["last"],
                                   t["row_prefix"], t["prefix_indptr"], t["prefix_indices"], **kw)
@@ -178,7 +179,7 @@ def test_decode_pages_outside_the_cache_are_dropped(bad):
     rows = [shared + keep[0][12:], shared + keep[1][12:], keep[2]]
     rows[0][14] = bad
     b.t["prefix_indices"] = i32(shared)
-    b.t["kv_indices"] = i32([p for r in rows for p in r])
+    b.t["kv_indices"] = i32([p for r in rows for p in r] + [-1] * 65)
     b.check(b.decode(), b.want(tables=rows))
 
 
@@ -215,8 +216,31 @@ def test_decode_long_prefix_and_a_long_lone_row():
 
 
 def test_decode_more_pages_than_planned():
-    b = Batch(12, 2, [200], [(0, 700, 1), (0, 3, 1)], seed=13)
+    """Rows longer than the planned maximum, in the kernels of a shared batch and of a small one."""
+    b = Batch(12, 2, [200], [(0, 700 - 9 * i, 1) for i in range(70)], seed=13)
+    b.check(b.decode(max_pages_per_row=60), b.want())
     b.check(b.decode(max_pages_per_row=4), b.want())
+
+
+@pytest.mark.parametrize("batch", [1, 2, 7, 30])
+def test_small_batches_on_the_ordinary_kernels(batch):
+    """Planned for what they hold: each row by itself, the same results."""
+    b = Batch(32, 8, [9], [(0 if i % 3 < 2 else -1, 1 + 11 * i % 40, 1) for i in range(batch)], seed=batch)
+    most = max(len(p) for p in b.pages)
+    assert batch * 8 * most <= 8192
+    b.check(b.decode(max_pages_per_row=most), b.want())
+    assert K.prefix_attention_workspace_bytes(batch, 32, 8, most) >= K.decode_workspace_bytes(batch, 32, 8, most)
+
+
+def test_small_prompts_on_the_ordinary_kernel():
+    b = Batch(32, 8, [9], [(0, 17, 17), (0, 1, 1), (-1, 30, 5), (0, 20, 6)], seed=24)
+    b.t["kv_indices"] = b.t["kv_indices"][:-65].clone()
+    assert b.t["kv_indices"].numel() <= 64
+    b.check(b.prefill(), b.want())
+    out = torch.full((29, 33 * D + 2), 2.0, dtype=torch.bfloat16, device=DEV)  # rows that only the shared kernel takes
+    o = torch.as_strided(out, (29, 32, D), (33 * D + 2, D, 1), 2)
+    b.check(b.prefill(out=o), b.want())
+    assert (out[:, :2] == 2).all() and (out[:, 2 + 32 * D:] == 2).all()
 
 
 def test_decode_cache_offsets_past_32_bits():
@@ -302,10 +326,10 @@ def test_captured_decode_follows_the_tables():
 
     def call(out, lse):
         K.paged_decode_prefix(q, cache, room["kv_indptr"], room["kv_indices"], room["last"], room["row_prefix"],
-                              room["prefix_indptr"], room["prefix_indices"], max_pages_per_row=60, out=out, lse=lse,
+                              room["prefix_indptr"], room["prefix_indices"], max_pages_per_row=8192, out=out, lse=lse,
                               workspace=ws)
 
-    ws = torch.empty(K.prefix_attention_workspace_bytes(4, 12, 2, 60), dtype=torch.uint8, device=DEV)
+    ws = torch.empty(K.prefix_attention_workspace_bytes(4, 12, 2, 8192), dtype=torch.uint8, device=DEV)
     out, lse = torch.zeros_like(q), torch.zeros(4, 12, device=DEV)
     load(b)
     call(out, lse)
@@ -443,7 +467,7 @@ def test_fork_then_prompt_then_decode():
         npg = [-(-n // PAGE) for n in lens]
         rows = [pages0[:9] + o[:c - 9] for o, c in zip(own, npg)]
         ap = i32(indptr(new))
-        ip, ind, last = i32(indptr(npg)), i32([p for r in rows for p in r]), i32([(n - 1) % PAGE + 1 for n in lens])
+        ip, ind, last = i32(indptr(npg)), i32([p for r in rows for p in r] + [-1] * 65), i32([(n - 1) % PAGE + 1 for n in lens])
         for cache in caches:
             k = torch.randn(sum(new), hkv, D, device=DEV).to(torch.bfloat16)
             v = torch.randn(sum(new), hkv, D, device=DEV).to(torch.bfloat16)
@@ -454,7 +478,7 @@ def test_fork_then_prompt_then_decode():
                 o = K.paged_prefill_prefix(q, cache, ap, ip, ind, last, *px, max_qo_len=max(new))
                 ref = K.paged_prefill(q, cache, ap, ip, ind, last, max_qo_len=max(new))
             else:
-                o = K.paged_decode_prefix(q, cache, ip, ind, last, *px, max_pages_per_row=max(npg))
+                o = K.paged_decode_prefix(q, cache, ip, ind, last, *px, max_pages_per_row=4096)
                 ref = K.paged_decode(q, cache, ip, ind, last, max_pages_per_row=max(npg))
             # both round P and o once in bf16 (u = 2^-8 of values up to 4)
             assert (o.float() - ref.float()).abs().max() <= 4 * 4 * 2 ** -8

@@ -29,7 +29,7 @@ def decode(p=px(), q=A, sb=4096, sh=128, kv=A, pages=16, ip=A, ind=A, n=16, last
 
 
 def prefill(qo=A, tokens=5, batch=2, p=px(), ws=A, wsb=1 << 40):
-    return (p, A, 4096, 128, A, 16, qo, A, A, 16, A, A, 4096, 128, None, batch, tokens, 32, 8, 128, 0, 1.0, ws, wsb, None)
+    return (p, A, 4096, 128, A, 16, qo, A, A, 16, A, A, 4096, 128, None, batch, tokens, 5, 32, 8, 128, 0, 1.0, ws, wsb, None)
 
 
 def copies(caches, n_caches=None, pages=16, hkv=8, hd=128, dt=0, src=A, dst=A, n=3):
