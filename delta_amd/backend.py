@@ -25,6 +25,7 @@ Out of scope on this build (raise): tensor parallelism, ``torch.compile``
 """
 from __future__ import annotations
 
+import itertools
 import json
 import os
 import time
@@ -40,18 +41,23 @@ from . import model as model_mod
 from .model import Transformer, build_random_model
 from .page_selector_v2 import PageSelectorV2
 from .public_config import FINAL_PUBLIC_DELTA_BACKEND_CONFIG as _CFG
-from .scheduler import BatchSlots, PagePool, ServingRequest
+from .scheduler import BatchSlots, PagePool, ServingRequest, SharedPrefix, shared_prefixes
 
 PAGE_SIZE = 16
+# Page-heads (a page of one kv head, 8 KiB) that sharing has to spare a layer's attention before its rows are served as
+# sharers: 64 MB, what the ordinary launches read in the time that the shared ones take besides their work (8 kv heads: 16
+# rows sharing 256 pages 21 us against 27, 8 sharing 64 14 against 12).
+SHARING_PAYS = 8192
 
 
 class _StepCSR:
     """Page tables the attention ops read during one forward (prefill steps also carry the
     query-token CSR of the rows)."""
 
-    __slots__ = ("mode", "kv_indptr", "kv_indices", "kv_last", "max_pages", "qo_indptr", "max_qo", "single_pages")
+    __slots__ = ("mode", "kv_indptr", "kv_indices", "kv_last", "max_pages", "qo_indptr", "max_qo", "single_pages", "prefix")
 
-    def __init__(self, mode, kv_indptr, kv_indices, kv_last, max_pages, qo_indptr=None, max_qo=1, single_pages=None):
+    def __init__(self, mode, kv_indptr, kv_indices, kv_last, max_pages, qo_indptr=None, max_qo=1, single_pages=None,
+                 prefix=None):
         self.mode = mode
         self.kv_indptr = kv_indptr
         self.kv_indices = kv_indices
@@ -60,6 +66,7 @@ class _StepCSR:
         self.qo_indptr = qo_indptr
         self.max_qo = max_qo
         self.single_pages = single_pages  # pages of each prompt-step row of one new token
+        self.prefix = prefix              # (row_prefix, prefix_indptr, prefix_indices) where rows share pages enough
 
 
 class LMBackend:
@@ -259,6 +266,13 @@ class LMBackend:
                  K.paged_prefill_workspace_bytes(B, hq, hkv, self.max_num_pages), 256)
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
         self._pinned_tokens = torch.zeros(B, dtype=torch.long).pin_memory()
+        # Rows that share their first pages (``_update_sharing``): each slot's prefix and the prefixes' pages, read by a
+        # captured step at every replay; switching them on or off captures it again.
+        self.row_prefix = torch.full((B,), -1, **i32)
+        self.prefix_indptr = torch.zeros(B // 2 + 1, **i32)
+        self.prefix_indices = torch.zeros(max(self.max_num_pages, 1), **i32)
+        self.prefix_workspace = None  # of the first step that shares
+        self._sharing = False
         with torch.device(dev):
             self.model.setup_caches(num_pages=self.num_pages, page_size=PAGE_SIZE, kv_cache_pool=kv_cache_pool)
         self.layer_roles = list(self.model.layer_roles)
@@ -360,6 +374,8 @@ class LMBackend:
 
     def attn_full(self, q, kv_cache, append=None):
         st = self._step
+        if st.prefix is not None:
+            return self._attn_shared(q, kv_cache, append)
         if st.mode == "prefill":  # several query tokens per row: causal prefill kernel
             return self._profile_cuda_section("delta_prefill_attention", lambda: K.paged_prefill(
                 q, kv_cache, st.qo_indptr, st.kv_indptr, st.kv_indices, st.kv_last, max_qo_len=st.max_qo,
@@ -367,6 +383,23 @@ class LMBackend:
         return self._profile_cuda_section("delta_full_attention", lambda: K.paged_decode(
             q, kv_cache, st.kv_indptr, st.kv_indices, st.kv_last, max_pages_per_row=st.max_pages,
             workspace=self.workspace, append=append))
+
+    def _attn_shared(self, q, kv_cache, append=None):
+        """Full attention of a step whose rows share prefixes: every prefix's pages read once for all its rows."""
+        st = self._step
+        if st.mode == "prefill":
+            return self._profile_cuda_section("delta_prefill_attention", lambda: K.paged_prefill_prefix(
+                q, kv_cache, st.qo_indptr, st.kv_indptr, st.kv_indices, st.kv_last, *st.prefix, max_qo_len=st.max_qo))
+
+        def decode():
+            x = q
+            if append is not None:  # the new token's RoPE and KV append, a launch of its own here
+                x = K.rope_append(q, append.k, append.v, self.qo_indptr, append.offsets, kv_cache, append.kv_indices,
+                                  append.kv_indptr, st.kv_last, **self.rope_params())
+            return K.paged_decode_prefix(x, kv_cache, st.kv_indptr, st.kv_indices, st.kv_last, *st.prefix,
+                                         max_pages_per_row=st.max_pages, workspace=self.prefix_workspace)
+
+        return self._profile_cuda_section("delta_full_attention", decode)
 
     def attn_subset(self, q, kv_cache, append=None):
         if not (self.enable_selective_cache and self._decode_mode()):
@@ -511,8 +544,42 @@ class LMBackend:
     # ------------------------------------------------------------ decode step
     def _decode_csr(self) -> _StepCSR:
         sel = self.page_selector
+        prefix = (self.row_prefix, self.prefix_indptr, self.prefix_indices) if self._sharing else None
         return _StepCSR("decode", sel.paged_kv_indptr, sel.paged_kv_indices, sel.paged_kv_last_page_len,
-                        self.pages_per_slot)
+                        self.pages_per_slot, prefix=prefix)
+
+    def _sharing_pays(self, prefixes: List[List[int]], row_prefix: dict, n_rows: int) -> bool:
+        if n_rows > 1024:  # more than the launches take
+            return False
+        users = [0] * len(prefixes)
+        for p in row_prefix.values():
+            users[p] += 1
+        spared = sum((n - 1) * len(pages) for n, pages in zip(users, prefixes))
+        return spared * self.model.config.n_local_heads >= SHARING_PAYS
+
+    @torch.inference_mode()
+    def _update_sharing(self, rows: Optional[dict] = None) -> None:
+        """Find the prefixes that the occupied slots' pages have in common (``rows``: slot -> pages) and hand them to the
+        decode steps: whenever a slot has been filled or released (the pages that rows share do not change in between)."""
+        if rows is None:
+            rows = {s: self.scheduler.request_in(s).pages for s in self.scheduler.occupied()}
+        row_prefix, prefixes = shared_prefixes(rows)
+        on = self._sharing_pays(prefixes, row_prefix, self.batch_size)
+        if on:
+            ip = [0, *itertools.accumulate(len(p) for p in prefixes)]
+            ip += [ip[-1]] * (self.prefix_indptr.numel() - len(ip))
+            flat = [p for pages in prefixes for p in pages]
+            self.row_prefix.copy_(torch.tensor([row_prefix.get(s, -1) for s in range(self.batch_size)], dtype=torch.int32))
+            self.prefix_indptr.copy_(torch.tensor(ip, dtype=torch.int32))
+            self.prefix_indices[:len(flat)].copy_(torch.tensor(flat, dtype=torch.int32))
+            if self.prefix_workspace is None:
+                cfg = self.model.config
+                self.prefix_workspace = torch.empty(
+                    K.prefix_attention_workspace_bytes(self.batch_size, cfg.n_head, cfg.n_local_heads, self.pages_per_slot),
+                    dtype=torch.uint8, device=self.device)
+        if on != self._sharing:
+            self._sharing = on
+            self._decode_graph = None  # captured with the other attention launches
 
     def _decode_body(self, advance: bool):
         """One decode step for all slots; only device work (capturable)."""
@@ -628,12 +695,13 @@ class LMBackend:
     @torch.inference_mode()
     def prepare_synthetic_decode(self, kv_len, decode_budget: int = 256, seed: int = 0,
                                  fill_std: float = 1.0, k_outlier_channels: int = 0,
-                                 k_outlier_scale: float = 8.0):
+                                 k_outlier_scale: float = 8.0, shared_tokens: int = 0):
         """Put every slot in the state "``kv_len`` tokens cached, decoding" (``kv_len`` an int
         or one length per slot): pages for ``kv_len + decode_budget`` tokens from the page
         pool, seeded N(0, fill_std) K/V in every layer, random current tokens.  With
         ``k_outlier_channels`` = n, n seeded head-dim channels of every layer's K are scaled by
-        ``k_outlier_scale`` (per-channel outliers).  The pages an earlier call took go back to
+        ``k_outlier_scale`` (per-channel outliers).  With ``shared_tokens`` the rows share the whole
+        pages of that many first tokens.  The pages an earlier call took go back to
         the pool first.  Used by the benchmark and tests (no prompts, no prefill)."""
         B = self.batch_size
         lens = [int(kv_len)] * B if isinstance(kv_len, int) else [int(x) for x in kv_len]
@@ -647,12 +715,19 @@ class LMBackend:
             self.page_pool.give_back(self._synthetic_pages)
             self._synthetic_pages = []
         bt = self.slot_block_table.cpu()
+        if shared_tokens < 0 or shared_tokens // PAGE_SIZE * PAGE_SIZE > min(lens):
+            raise ValueError(f"rows of {min(lens)} tokens cannot share {shared_tokens}")
+        shared = self.page_pool.take(shared_tokens // PAGE_SIZE)
+        self._synthetic_pages.extend(shared)
+        rows = {}
         for b, n in enumerate(lens):
             need = (n + decode_budget) // PAGE_SIZE + 1
-            pages = self.page_pool.take(need)
-            self._synthetic_pages.extend(pages)
-            bt[b, :need] = torch.tensor(pages, dtype=torch.int32)
+            own = self.page_pool.take(need - len(shared))
+            self._synthetic_pages.extend(own)
+            rows[b] = shared + own
+            bt[b, :need] = torch.tensor(rows[b], dtype=torch.int32)
         self.slot_block_table.copy_(bt)
+        self._update_sharing(rows)
         self._slot_pages = [(n + decode_budget) // PAGE_SIZE + 1 for n in lens]
         self._host_lens = list(lens)
         self._host_active = [1] * B
@@ -679,10 +754,72 @@ class LMBackend:
         self._decode_graph = None
 
     # ------------------------------------------------------ request serving
-    def add_requests(self, input_ids_list: list, max_lengths: list, eot_token_ids: list):
+    def add_requests(self, input_ids_list: list, max_lengths: list, eot_token_ids: list, prefix_ids=None):
+        """Queue requests.  ``prefix_ids`` (a token tensor; an extension): every prompt continues these tokens, whose
+        whole pages are computed once, when the first of the requests is served, held by all of them, and read once for
+        all of them by the full-attention layers.  ``max_lengths`` count the prefix's tokens."""
         if self.scheduler is None:
             raise RuntimeError("Backend not initialized. Call setup_caches first.")
-        self.scheduler.submit(input_ids_list, max_lengths, eot_token_ids)
+        if prefix_ids is not None:
+            prefix_ids = torch.as_tensor(prefix_ids)
+            if prefix_ids.dim() != 1 or prefix_ids.is_floating_point() or prefix_ids.numel() == 0:
+                raise ValueError("prefix_ids must be a non-empty 1-D tensor of token ids")
+        self.scheduler.submit(input_ids_list, max_lengths, eot_token_ids, prefix_ids)
+
+    @torch.inference_mode()
+    def fork_request(self, request_id: int, input_ids, max_length: Optional[int] = None, eot_token_ids=()) -> int:
+        """Branch a request that is being served (an extension; from ``run_scheduler_loop``'s ``on_step``): a new request
+        in a free slot continues its tokens so far with ``input_ids``.  The two share the pages that are full; the page
+        that both go on filling is copied in every layer's cache.  Returns the new request's id; raises when no slot is
+        free.  ``max_length`` (default: the parent's) counts the shared tokens too."""
+        sched = self.scheduler
+        if sched is None or not 0 <= request_id < len(sched.requests):
+            raise ValueError(f"no request {request_id}")
+        parent = sched.requests[request_id]
+        if parent.state != ServingRequest.ACTIVE or not parent.generated:
+            raise RuntimeError(f"request {request_id} is not decoding: it cannot be forked")
+        slot = sched.free_slot()
+        if slot is None:
+            raise RuntimeError("no free slot for a fork")
+        more = torch.as_tensor(input_ids, dtype=torch.long)
+        limit = parent.max_length if max_length is None else int(max_length)
+        total = len(parent.prompt) + len(parent.generated) + len(more)
+        if more.dim() != 1 or total >= limit or limit > self.max_length:
+            raise ValueError(f"a fork of {total} tokens needs 1-D input_ids and a max_length in ({total}, "
+                             f"{self.max_length}], got {limit}")
+        child = parent.fork(len(sched.requests), more, limit, eot_token_ids)
+        sched.place(child)
+        if child.fill:
+            i32 = dict(dtype=torch.int32, device=self.device)
+            K.copy_pages(self._kv_caches(), torch.tensor(parent.pages[-1:], **i32), torch.tensor(child.pages[-1:], **i32),
+                         tokens=torch.tensor([child.fill], **i32))
+        self.slot_block_table[slot].fill_(int(self.scratch_pages[slot]))
+        self._sync_slot_block_table(slot, child, 0)
+        self._update_sharing()
+        return child.rid
+
+    def _kv_caches(self) -> List[torch.Tensor]:
+        """The layers' caches, each physical one once."""
+        caches = {}
+        for layer in self.model.layers:
+            c = layer.attention.kv_cache.kv_cache
+            caches[c.data_ptr()] = c
+        return list(caches.values())
+
+    @torch.inference_mode()
+    def _compute_prefix(self, prefix: SharedPrefix) -> None:
+        """Run the prefix's tokens through the model once, into pages of its own (no slot)."""
+        pages = prefix.reserve()
+        i32 = dict(dtype=torch.int32, device=self.device)
+        n = len(prefix.tokens)
+        ip, ind, last = torch.tensor([0, len(pages)], **i32), torch.tensor(pages, **i32), torch.tensor([PAGE_SIZE], **i32)
+        qo = torch.tensor([0, n], **i32)
+        self._step = _StepCSR("prefill", ip, ind, last, len(pages), qo_indptr=qo, max_qo=n, single_pages=[])
+        try:
+            self._profile_cuda_section("delta_prefill_step", lambda: self.model(
+                prefix.tokens.view(1, -1).to(self.device), torch.zeros(1, **i32), qo, ind, ip, last))
+        finally:
+            self._step = None
 
     @torch.inference_mode()
     def _sync_slot_block_table(self, slot_id: int, request: ServingRequest, old_page_count: int):
@@ -702,8 +839,9 @@ class LMBackend:
         self._slot_pages[slot_id] = self.pages_per_slot  # the scratch page in every column
 
     @torch.inference_mode()
-    def run_scheduler_loop(self):
-        """Serve queued requests until done (backend.py:1486-1553)."""
+    def run_scheduler_loop(self, on_step=None):
+        """Serve queued requests until done (backend.py:1486-1553).  ``on_step(self, i)`` (an extension) is called after
+        step i, with its tokens recorded; it may call ``fork_request`` and ``add_requests``."""
         torch.cuda.synchronize(self.device)
         self.scheduler.t_start = time.perf_counter()
         self._step_records = []
@@ -718,13 +856,20 @@ class LMBackend:
                 break
             for slot_id in finished:
                 self._release_slot(slot_id)
-            for slot_id, req in self.scheduler.fill_free_slots():
+            placed = self.scheduler.fill_free_slots()
+            for slot_id, req in placed:
+                if req.prefix is not None and not req.prefix.pages:
+                    self._compute_prefix(req.prefix)
                 req.admit()
                 self.slot_block_table[slot_id].fill_(int(self.scratch_pages[slot_id]))
                 self._sync_slot_block_table(slot_id, req, 0)
             if not self.scheduler.any_active():
                 break
+            if finished or placed:
+                self._update_sharing()
             self._forward(i)
+            if on_step is not None:
+                on_step(self, i)
             if self.enable_delta_impl_profile:
                 self._flush_delta_impl_profile_events()
         if self.is_main_process:
@@ -736,11 +881,10 @@ class LMBackend:
         for slot_id in self.scheduler.occupied():
             req = self.scheduler.request_in(slot_id)
             if not req.finished:
-                req.state = ServingRequest.FINISHED
-                req.t_end = time.perf_counter()
-                self.page_pool.give_back(req.pages)
+                req.finish()
             self.scheduler.slots[slot_id] = None
             self._release_slot(slot_id)
+        self._update_sharing()
 
     def _active_slots(self) -> List[int]:
         return self.scheduler.occupied()
@@ -851,9 +995,15 @@ class LMBackend:
         row_ip = torch.tensor(kv_indptr, **i32)
         row_ind = torch.tensor(kv_indices, **i32)
         row_last = torch.tensor(rows_last, **i32)
+        row_prefix, prefixes = shared_prefixes(dict(enumerate(rows_pages)))
+        prefix = None
+        if self._sharing_pays(prefixes, row_prefix, len(rows_pages)):
+            prefix = (torch.tensor([row_prefix.get(b, -1) for b in range(len(rows_pages))], **i32),
+                      torch.tensor([0] + list(itertools.accumulate(len(p) for p in prefixes)), **i32),
+                      torch.tensor([p for pages in prefixes for p in pages], **i32))
         self._step = _StepCSR("prefill", row_ip, row_ind, row_last, max(len(p) for p in rows_pages),
                               qo_indptr=qo_indptr, max_qo=max(qo_lens),
-                              single_pages=[len(p) for n, p in zip(qo_lens, rows_pages) if n == 1])
+                              single_pages=[len(p) for n, p in zip(qo_lens, rows_pages) if n == 1], prefix=prefix)
         try:
             out = self.model(tokens, torch.tensor(offsets, **i32), qo_indptr, row_ind, row_ip, row_last)
         finally:

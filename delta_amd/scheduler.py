@@ -14,6 +14,9 @@ both, and are kept exactly:
 * Completion (scheduler.py:83-90): a request ends on a stop token or once prompt plus output
   reach ``max_length``, and its pages go back to the pool.
 
+Requests may share a prefix (``SharedPrefix``: whole pages, computed once) or be forked from one
+another: the pages that several hold are counted, and go back to the pool with the last holder.
+
 Everything else is this build's own: requests live in a flat list indexed by id, slots hold
 request ids (``None`` when free), waiting ids sit in a deque, and the pool reshuffles its
 free ids with its own generator when pages come back (the reference reshuffles with the
@@ -32,7 +35,7 @@ PAGE_SIZE = 16
 
 
 class PagePool:
-    """Shuffled pool of physical KV page ids."""
+    """Shuffled pool of physical KV page ids, with a count of holders for each page that is out."""
 
     def __init__(self, total_pages: int, seed: Optional[int] = None):
         self.total_pages = int(total_pages)
@@ -40,7 +43,7 @@ class PagePool:
         ids = list(range(self.total_pages))
         self._rng.shuffle(ids)
         self._free: List[int] = ids          # handed out from the end
-        self._held = set()
+        self._held: Dict[int, int] = {}      # page -> holders
 
     @property
     def available(self) -> int:
@@ -51,14 +54,111 @@ class PagePool:
         if n > len(self._free):
             raise RuntimeError(f"Out of KV pages: {n} wanted, {len(self._free)} free")
         got = [self._free.pop() for _ in range(n)]
-        self._held.update(got)
+        self._held.update((p, 1) for p in got)
         return got
 
+    def share(self, pages: Sequence[int]) -> List[int]:
+        """One more holder for each of ``pages``, all of them out; returns them as a list."""
+        loose = [p for p in pages if p not in self._held]
+        if loose:
+            raise RuntimeError(f"page {loose[0]} is not held: it cannot be shared")
+        for p in pages:
+            self._held[p] += 1
+        return list(pages)
+
     def give_back(self, pages: Sequence[int]) -> None:
-        back = [p for p in pages if p in self._held]
-        self._held.difference_update(back)
+        """One holder less for each of ``pages``; those without any are free again."""
+        back = []
+        for p in pages:
+            n = self._held.get(p, 0)
+            if n > 1:
+                self._held[p] = n - 1
+            elif n == 1:
+                del self._held[p]
+                back.append(p)
         self._free.extend(back)
         self._rng.shuffle(self._free)
+
+
+class SharedPrefix:
+    """The first tokens of several prompts: whole pages, computed when the first of them is served and held until the
+    last of them has finished."""
+
+    def __init__(self, tokens: torch.Tensor, pool: PagePool, users: int):
+        assert len(tokens) % PAGE_SIZE == 0
+        self.tokens = tokens
+        self.pages: List[int] = []  # once computed
+        self.users = users          # requests that have not finished
+        self._pool = pool
+
+    def reserve(self) -> List[int]:
+        self.pages = self._pool.take(len(self.tokens) // PAGE_SIZE)
+        return self.pages
+
+    def user_finished(self) -> None:
+        self.users -= 1
+        if self.users == 0:
+            self._pool.give_back(self.pages)
+            self.pages = []
+
+
+def shared_prefixes(rows: Dict[int, Sequence[int]]) -> Tuple[Dict[int, int], List[List[int]]]:
+    """Rows (slot -> pages, in order) that begin with the same pages: each sharing slot's prefix, and the prefixes' pages,
+    chosen so that the fewest pages are left to read.
+
+    The rows make a tree of the places where they branch.  A branch at n pages that is taken as a prefix costs n pages once
+    and spares n to every row below it that has no deeper one."""
+    # (n, rows that go on alone from here, branches below, branch above); a branch comes before those below it
+    tree: List[Tuple[int, List[int], List[int], Optional[int]]] = []
+    work: List[Tuple[List[int], int, Optional[int]]] = [(sorted(rows), 0, None)]
+    while work:
+        slots, n, up = work.pop()
+        lo, hi = min((rows[s] for s in slots), default=()), max((rows[s] for s in slots), default=())
+        most = min(len(lo), len(hi))
+        while n < most:  # what the least and the greatest row have in common, all have
+            mid = (n + most + 1) // 2
+            n, most = (mid, most) if lo[n:mid] == hi[n:mid] else (n, mid - 1)
+        by_next: Dict[int, List[int]] = {}
+        alone = []
+        for s in slots:
+            if len(rows[s]) > n:
+                by_next.setdefault(rows[s][n], []).append(s)
+            else:
+                alone.append(s)
+        alone += [g[0] for g in by_next.values() if len(g) == 1]
+        work += [(g, n, len(tree)) for g in by_next.values() if len(g) > 1]
+        if up is not None:
+            tree[up][2].append(len(tree))
+        tree.append((n, alone, [], up))
+
+    # pages spared below branch v by the pages above that its rows have as their prefix, and whether v is worth taking then
+    spared: List[Dict[int, Tuple[int, bool]]] = [{} for _ in tree]
+    for v in reversed(range(len(tree))):
+        n, alone, below, up = tree[v]
+        taken = (len(alone) - 1) * n + sum(spared[c][n][0] for c in below)
+        above = {0}
+        while up is not None:
+            above.add(tree[up][0])
+            up = tree[up][3]
+        for d in above:
+            left = len(alone) * d + sum(spared[c][d][0] for c in below)
+            spared[v][d] = max((left, False), (taken, True), key=lambda x: x[0])
+
+    row_prefix: Dict[int, int] = {}
+    prefixes: List[List[int]] = []
+    inherited: List[Tuple[int, int]] = []  # each branch's (pages, prefix) for the rows that have no deeper one
+    for v, (n, alone, below, up) in enumerate(tree):
+        d, group = inherited[up] if up is not None else (0, -1)
+        if spared[v][d][1]:
+            d, group = n, len(prefixes)
+            first = v
+            while not tree[first][1]:
+                first = tree[first][2][0]
+            prefixes.append(list(rows[tree[first][1][0]][:n]))
+        inherited.append((d, group))
+        if group >= 0:
+            row_prefix.update((s, group) for s in alone)
+    return row_prefix, prefixes
 
 
 class ServingRequest:
@@ -67,7 +167,7 @@ class ServingRequest:
     WAITING, ACTIVE, FINISHED = "waiting", "active", "finished"
 
     def __init__(self, rid: int, prompt: torch.Tensor, max_length: int, stop_ids: Sequence[int],
-                 pool: PagePool):
+                 pool: PagePool, prefix: Optional[SharedPrefix] = None):
         self.rid = rid
         self.prompt = prompt
         self.max_length = int(max_length)
@@ -78,15 +178,35 @@ class ServingRequest:
         self.state = self.WAITING
         self.t_start: Optional[float] = None
         self.t_end: Optional[float] = None
+        self.prefix = prefix           # whose tokens the prompt begins with
+        self.cached = 0                # prompt tokens that were in the cache when serving began
         self._pool = pool
 
     # -- pages
     def admit(self) -> None:
-        """Start serving: one empty page."""
+        """Start serving: one empty page, behind the pages of the prefix (computed by now) if there is one."""
         self.state = self.ACTIVE
         self.t_start = time.perf_counter()
-        self.pages = self._pool.take(1)
+        own = self._pool.take(1)
+        self.pages = own
         self.fill = 0
+        if self.prefix is not None:
+            self.pages = self._pool.share(self.prefix.pages) + own
+            self.cached = len(self.prefix.tokens)
+
+    def fork(self, rid: int, more: torch.Tensor, max_length: int, stop_ids: Sequence[int]) -> "ServingRequest":
+        """A request that continues this one's tokens so far with ``more``, already being served: it shares the full
+        pages and has a page of its own for the ``fill`` tokens of the last one (copied by the caller)."""
+        prompt = torch.cat([self.prompt.to(torch.long), torch.tensor(self.generated, dtype=torch.long),
+                            more.to(torch.long)])
+        child = ServingRequest(rid, prompt, max_length, stop_ids, self._pool)
+        own = self._pool.take(1)
+        child.state = self.ACTIVE
+        child.t_start = time.perf_counter()
+        child.pages = self._pool.share(self.pages[:-1]) + own
+        child.fill = self.fill
+        child.cached = self.kv_len()
+        return child
 
     def reserve(self, n_tokens: int, page_size: int = PAGE_SIZE) -> None:
         """Account for ``n_tokens`` new tokens (the page-growth rule above)."""
@@ -101,18 +221,24 @@ class ServingRequest:
 
     # -- tokens
     def next_input(self) -> torch.Tensor:
-        """The tokens of this request's next forward: the prompt, then the last output."""
-        return self.prompt if not self.generated else torch.tensor([self.generated[-1]], dtype=torch.long)
+        """The tokens of this request's next forward: the prompt's that are not cached, then the last output."""
+        return self.prompt[self.cached:] if not self.generated else torch.tensor([self.generated[-1]], dtype=torch.long)
 
     def record(self, token: int) -> bool:
         """Append an output token; True when the request is now finished."""
         self.generated.append(int(token))
         if int(token) in self.stop_ids or len(self.prompt) + len(self.generated) >= self.max_length:
-            self._pool.give_back(self.pages)
-            self.state = self.FINISHED
-            self.t_end = time.perf_counter()
+            self.finish()
             return True
         return False
+
+    def finish(self) -> None:
+        """End serving: the pages go back to the pool."""
+        self._pool.give_back(self.pages)
+        if self.prefix is not None:
+            self.prefix.user_finished()
+        self.state = self.FINISHED
+        self.t_end = time.perf_counter()
 
     @property
     def finished(self) -> bool:
@@ -150,10 +276,20 @@ class BatchSlots:
         self.tokens_generated = 0
         self.t_start: Optional[float] = None
 
-    def submit(self, prompts: Sequence[torch.Tensor], max_lengths, stop_ids: Sequence[int]) -> None:
+    def submit(self, prompts: Sequence[torch.Tensor], max_lengths, stop_ids: Sequence[int],
+               prefix_tokens: Optional[torch.Tensor] = None) -> None:
+        """Queue requests; with ``prefix_tokens`` each prompt continues them, and their whole pages (short of the last
+        token of a prompt that adds none: every request feeds at least one token of its own) are shared."""
+        prefix = None
+        if prefix_tokens is not None and len(prompts):
+            prefix_tokens = prefix_tokens.to(torch.long)
+            prompts = [torch.cat([prefix_tokens, p.to(torch.long)]) for p in prompts]
+            whole = min(len(prefix_tokens), min(len(p) for p in prompts) - 1) // PAGE_SIZE * PAGE_SIZE
+            if whole > 0:
+                prefix = SharedPrefix(prefix_tokens[:whole], self.pool, len(prompts))
         for i, prompt in enumerate(prompts):
             cap = max_lengths[i] if isinstance(max_lengths, (list, tuple)) else max_lengths
-            req = ServingRequest(len(self.requests), prompt, cap, stop_ids, self.pool)
+            req = ServingRequest(len(self.requests), prompt, cap, stop_ids, self.pool, prefix)
             self.requests.append(req)
             self.waiting.append(req.rid)
         if self.verbose:
@@ -168,6 +304,18 @@ class BatchSlots:
                 self.slots[s] = req.rid
                 placed.append((s, req))
         return placed
+
+    def place(self, req: ServingRequest) -> int:
+        """Put an already served request (a fork) into a free slot."""
+        slot = self.free_slot()
+        if slot is None:
+            raise RuntimeError("no free slot")
+        self.requests.append(req)
+        self.slots[slot] = req.rid
+        return slot
+
+    def free_slot(self) -> Optional[int]:
+        return next((s for s, rid in enumerate(self.slots) if rid is None), None)
 
     def release_finished(self) -> List[int]:
         """Free the slots whose request finished; returns those slot ids."""
