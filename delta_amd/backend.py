@@ -19,6 +19,9 @@ work runs:
   graph also covers partial batches.
 * Prefill / mixed steps run eagerly: all new tokens are appended, then the
   causal paged prefill kernel attends each row's pages.
+* Requests may share a prefix's pages (``add_requests(prefix_ids=)``,
+  ``fork_request``; no counterpart there): full attention then reads them once
+  for all the rows.
 
 Out of scope on this build (raise): tensor parallelism, ``torch.compile``
 (no Triton), the v1 selector, the ``delta_lse`` scorer and an fp16 dump.

@@ -3,7 +3,8 @@
 // Entry i copies the first tokens[i] tokens' K and V of page src[i] to page dst[i], in each of the caches.  A page is
 // [2, 16, Hkv, 128]: its K and its V are contiguous, and so are their first tokens.  A block copies the K or the V of
 // one (entry, cache), up to 16 * Hkv * 256 bytes, 16 bytes per thread and load, all of a thread's loads issued before
-// its stores.  Bound by HBM: every byte is read and written once.
+// its stores.  Bound by HBM: every byte is read and written once (4000 pages of 64 KiB in each of 4 caches: 2.1 GB in 414 us, 5.1
+// TB/s, against 4.85 of a plain copy of 2 GiB; 64 pages in each of 32: 23 us), and by the launch for a single fork (2.9 us).
 #include "delta_common.h"
 
 namespace delta {

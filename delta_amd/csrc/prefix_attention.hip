@@ -9,21 +9,31 @@
 // so a row's softmax splits into its prefix and its own tokens, and each of these into any runs of pages.
 //
 // Work decomposition.  A segment is a prefix with the query tokens of all rows that use it (no mask: all of
-// them come after it), or a row's own pages with its query tokens (causal).  Its query tokens are cut into
-// tiles of up to 128 (token, q head of the kv head's G) pairs, its pages into steps of 64 tokens.  The steps of
+// them come after it), or a row's own pages with its query tokens (causal).  Its (query token, q head of the kv head's G)
+// pairs, in that order, are cut into tiles of 128, its pages into steps of 64 tokens.  The steps of
 // all tiles of a kv head form one line, kTileCost more per tile for what a tile costs besides its steps, and
 // block i of the head's `blocks` takes the i-th equal share of it: so the chip's block slots (two per CU)
-// finish together whatever the lengths are, and a tile is cut only where a share ends.  The lengths are only on
-// the device: every block derives the same line from the tables (build_line).
+// finish together whatever the lengths are (to +-8 %), and a tile is cut only where a share ends.  The lengths are only on
+// the device: every block derives the same line from the tables (build_line, 1.7-2.0 us).
 //   A whole tile of a row without a prefix writes o and lse.  Any other one writes un-normalised partials
 // (m, l, a): a whole tile at its token's place, a cut one into its block's two buffers (a block's first piece may
-// end a cut tile, its last may begin one); the merge kernel joins them per (token, q head).
+// end a cut tile, its last may begin one); the merge kernel joins them per (token, q head).  No atomics: the same call
+// gives the same bits.
 //
 // Per block: 4 waves, each with 32 of the tile's pairs, share K and V in LDS, in stages of 32 tokens, two or three of
-// them under way (64 KiB, two blocks per CU); waves without pairs (a decode row's own pages have G) only load.  MFMA
+// them under way (64 KiB, two blocks per CU); waves without pairs only load.  MFMA
 // tiles as in prefill.hip: S^T = K Q^T with lane l holding query pair l % 32 and 16 of the 32 tokens, O^T += V^T P^T, P
-// rounded to the cache's type for the product as there (the sums l stay unrounded fp32).  The S of a stage are computed
-// under the softmax of the stage before.
+// rounded to the cache's type for the product as there (half a step of it per weight, and the fp32 sums l stay unrounded).
+// The S of a stage are computed under the softmax of the stage before.  Tiles of up to 16 pairs (a decode row's own pages
+// have G) go to one wave on 16x16 MFMA tiles.
+//
+// What bounds it.  Decode reads: 128 rows of 1050 own tokens over a prefix of 16384, 8 kv heads of 5: 630 MB in 149 us, 4.2
+// TB/s (97 us at the 6.5 TB/s of a bare read; the ordinary launch, which reads the prefix for every row, 749); 32 rows of 530
+// over 8192: 33 us against 17 and 101; the line, the pieces' beginnings (2-4 us each) and the merge (6 us with its launch) are
+// the rest.  Prompts compute: 32 prompts of 34 tokens over 8192, 8 kv heads of 4: 195 us, 0.71 PFLOP/s, 1.0 in the loop
+// (1.06 us a stage of two blocks; 116 us at the 1.19 of an 8192^3 product; the ordinary launch 214).  In the loop no single
+// unit is the bound: without the exponentials it would take 95 % of its time, without V's fragments 94, without K's 97,
+// without any of them 84.
 #include "delta_common.h"
 #include "mfma32.h"
 
