@@ -51,6 +51,12 @@ PAGE_SIZE = 16
 # sharers: 64 MB, what the ordinary launches read in the time that the shared ones take besides their work (8 kv heads: 16
 # rows sharing 256 pages 21 us against 27, 8 sharing 64 14 against 12).
 SHARING_PAYS = 8192
+# Prompt steps: a row of more new (token, q head of a kv head) pairs than this fills tiles of its own, so that sharing spares
+# it nothing, and the ordinary launch sweeps such rows faster (8 kv heads of 4 over 8192 tokens, us shared / ordinary: 64
+# rows of 60-70 660 / 720, 32 of 120-130 620 / 680, 8 of 512 626 / 519, 2 of 2048 719 / 561); and a step of more new tokens
+# than this is no sharers' step (the partials take 1 KiB per token and q head).
+SHARING_PAIRS = 1024
+SHARING_TOKENS = 16384
 
 
 class _StepCSR:
@@ -767,6 +773,9 @@ class LMBackend:
             prefix_ids = torch.as_tensor(prefix_ids)
             if prefix_ids.dim() != 1 or prefix_ids.is_floating_point() or prefix_ids.numel() == 0:
                 raise ValueError("prefix_ids must be a non-empty 1-D tensor of token ids")
+            longest = prefix_ids.numel() + max((len(p) for p in input_ids_list), default=0)
+            if longest >= self.max_length:
+                raise ValueError(f"a prompt of {longest} tokens, its prefix included, leaves no room in {self.max_length}")
         self.scheduler.submit(input_ids_list, max_lengths, eot_token_ids, prefix_ids)
 
     @torch.inference_mode()
@@ -784,7 +793,7 @@ class LMBackend:
         slot = sched.free_slot()
         if slot is None:
             raise RuntimeError("no free slot for a fork")
-        more = torch.as_tensor(input_ids, dtype=torch.long)
+        more = torch.as_tensor(input_ids, dtype=torch.long, device=parent.prompt.device)
         limit = parent.max_length if max_length is None else int(max_length)
         total = len(parent.prompt) + len(parent.generated) + len(more)
         if more.dim() != 1 or total >= limit or limit > self.max_length:
@@ -998,9 +1007,11 @@ class LMBackend:
         row_ip = torch.tensor(kv_indptr, **i32)
         row_ind = torch.tensor(kv_indices, **i32)
         row_last = torch.tensor(rows_last, **i32)
-        row_prefix, prefixes = shared_prefixes(dict(enumerate(rows_pages)))
+        cfg = self.model.config
+        group = cfg.n_head // cfg.n_local_heads
+        row_prefix, prefixes = shared_prefixes({b: p for b, p in enumerate(rows_pages) if qo_lens[b] * group <= SHARING_PAIRS})
         prefix = None
-        if self._sharing_pays(prefixes, row_prefix, len(rows_pages)):
+        if sum(qo_lens) <= SHARING_TOKENS and self._sharing_pays(prefixes, row_prefix, len(rows_pages)):
             prefix = (torch.tensor([row_prefix.get(b, -1) for b in range(len(rows_pages))], **i32),
                       torch.tensor([0] + list(itertools.accumulate(len(p) for p in prefixes)), **i32),
                       torch.tensor([p for pages in prefixes for p in pages], **i32))

@@ -197,8 +197,9 @@ class ServingRequest:
     def fork(self, rid: int, more: torch.Tensor, max_length: int, stop_ids: Sequence[int]) -> "ServingRequest":
         """A request that continues this one's tokens so far with ``more``, already being served: it shares the full
         pages and has a page of its own for the ``fill`` tokens of the last one (copied by the caller)."""
-        prompt = torch.cat([self.prompt.to(torch.long), torch.tensor(self.generated, dtype=torch.long),
-                            more.to(torch.long)])
+        prompt = self.prompt.to(torch.long)
+        prompt = torch.cat([prompt, torch.tensor(self.generated, dtype=torch.long, device=prompt.device),
+                            more.to(prompt.device, torch.long)])
         child = ServingRequest(rid, prompt, max_length, stop_ids, self._pool)
         own = self._pool.take(1)
         child.state = self.ACTIVE
@@ -283,7 +284,7 @@ class BatchSlots:
         prefix = None
         if prefix_tokens is not None and len(prompts):
             prefix_tokens = prefix_tokens.to(torch.long)
-            prompts = [torch.cat([prefix_tokens, p.to(torch.long)]) for p in prompts]
+            prompts = [torch.cat([prefix_tokens.to(p.device), p.to(torch.long)]) for p in prompts]
             whole = min(len(prefix_tokens), min(len(p) for p in prompts) - 1) // PAGE_SIZE * PAGE_SIZE
             if whole > 0:
                 prefix = SharedPrefix(prefix_tokens[:whole], self.pool, len(prompts))

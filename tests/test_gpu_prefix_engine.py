@@ -233,3 +233,43 @@ def test_what_cannot_be_forked_is_refused():
     for bad in (torch.tensor([]), torch.tensor([], dtype=torch.long), torch.tensor([[1]]), torch.tensor([1.5])):
         with pytest.raises(ValueError, match="prefix_ids"):
             eng.add_requests([prompt(4, 0)], 20, [], prefix_ids=bad)
+
+
+@pytest.mark.parametrize("limit,value", [("SHARING_TOKENS", 40), ("SHARING_PAIRS", 2)])
+def test_prompt_steps_of_many_tokens_take_the_ordinary_launch(limit, value, calls, monkeypatch):
+    import delta_amd.backend as backend
+    monkeypatch.setattr(backend, limit, value)
+    eng = make_engine(B=16, max_len=5120)
+    eng.add_requests([prompt(3 + i, i) for i in range(16)], PREFIX + 40, [], prefix_ids=prompt(PREFIX, 0))
+    eng.run_scheduler_loop()
+    assert calls["paged_prefill_prefix"] == 0 and calls["paged_decode_prefix"] > 0
+    assert eng.page_pool.available == eng.page_pool.total_pages
+
+
+def test_prompts_that_leave_no_room_are_refused():
+    eng = make_engine(B=3, max_len=256)
+    with pytest.raises(ValueError, match="no room"):
+        eng.add_requests([prompt(3, 0), prompt(56, 1)], 256, [], prefix_ids=prompt(200, 2))
+    assert not eng.scheduler.requests
+    eng.add_requests([prompt(3, 0), prompt(55, 1)], 256, [], prefix_ids=prompt(200, 2))
+    eng.run_scheduler_loop()
+    assert [r.kv_len() for r in eng.scheduler.requests] == [255, 255]
+    assert eng.page_pool.available == eng.page_pool.total_pages
+
+
+def test_requests_added_and_forked_while_others_run():
+    """A prefix group that arrives later, of which one prompt adds nothing, beside forks of a request without a prefix."""
+    eng = make_engine(B=4, max_len=256, graph=True)
+    eng.add_requests([prompt(30, 0)], 80, [])
+    forks = []
+
+    def on_step(e, i):
+        r = e.scheduler.requests[0]
+        if len(r.generated) == 3:
+            e.add_requests([prompt(0, 1), prompt(9, 2), prompt(33, 3), prompt(2, 4)], 120, [], prefix_ids=prompt(48, 5))
+            forks.append(e.fork_request(0, prompt(5, 6), max_length=70))
+
+    results = eng.run_scheduler_loop(on_step=on_step)
+    assert len(results) == 6 and all(r["status"] == "finished" for r in results)
+    assert [len(r.prompt) + len(r.generated) for r in eng.scheduler.requests] == [80] + [120 if i != forks[0] else 70 for i in range(1, 6)]
+    assert eng.page_pool.available == eng.page_pool.total_pages
