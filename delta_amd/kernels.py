@@ -447,7 +447,8 @@ def paged_prefill_prefix(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: tor
     [nnz, Hq, 128], the prefixes as in ``paged_decode_prefix``.
 
     A row's prefix applies where it ends before the row's query tokens.  ``max_qo_len`` is at least the longest row's
-    count of them, as for ``paged_prefill``.  ``out`` and ``lse`` of tokens behind the last row are left as they were."""
+    count of them, as for ``paged_prefill``, which is as fast or faster where the rows bring several hundred tokens each
+    (sharing spares reads, not products).  ``out`` and ``lse`` of tokens behind the last row are left as they were."""
     _check_i32("qo_indptr", qo_indptr, 1)
     return _prefix_call("delta_paged_prefill_prefix", q, kv_cache, qo_indptr.numel() - 1,
                         (qo_indptr, kv_indptr, kv_indices, kv_last_page_len), (row_prefix, prefix_indptr, prefix_indices),
