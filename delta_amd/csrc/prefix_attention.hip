@@ -24,8 +24,8 @@
 // them under way (64 KiB, two blocks per CU); waves without pairs only load.  MFMA
 // tiles as in prefill.hip: S^T = K Q^T with lane l holding query pair l % 32 and 16 of the 32 tokens, O^T += V^T P^T, P
 // rounded to the cache's type for the product as there (half a step of it per weight, and the fp32 sums l stay unrounded).
-// The S of a stage are computed under the softmax of the stage before.  Tiles of up to 16 pairs (a decode row's own pages
-// have G) go to one wave on 16x16 MFMA tiles.
+// The S of a stage are computed under the softmax of the stage before.  Tiles of up to 64 pairs (a decode row's own pages
+// have G) have 16 to a wave, on 16x16 MFMA tiles.
 //
 // What bounds it.  Decode reads: 128 rows of 1050 own tokens over a prefix of 16384, 8 kv heads of 5: 630 MB in 149 us, 4.2
 // TB/s (97 us at the 6.5 TB/s of a bare read; the ordinary launch, which reads the prefix for every row, 749); 32 rows of 530
@@ -430,17 +430,19 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       }
     };
 
-    if (pairs <= 16) {
-      // ---- One wave works, on 16x16 tiles: half the MFMA time and half the scores per lane of the 32x32 ones, which for
-      // these tiles would hold the stages up (a decode row's own pages: 0.93 us a stage, above HBM's time for it).
+    if (pairs <= 64) {
+      // ---- 16 pairs per wave, on 16x16 tiles: half the MFMA time and half the scores per lane of the 32x32 ones, and more
+      // of the SIMDs at work (a decode row's own pages, one wave: 0.93 us a stage on 32x32 tiles, 0.85 here; us for 64 prompts of 5
+      // tokens behind up to 1500 own, 25 pairs, 81.3 / 78.0; for 8 rows of 7 heads over 16384, 56 pairs, 23.8 / 22.7).
       // Lane (c, n) = (lane / 16, lane % 16): pair n; scores of tokens 4 c + i and 16 + 4 c + i; outputs d = 16 dt + 4 c + i.
       const int c = lane >> 4, n = lane & 15;
-      const bool active = ((wv + blk) & 3) == 0, ok = active && n < pairs;
-      const int pt = ok ? (skew + n) / G : 0, t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
+      const int qsub = (wv + blk) & 3, pair = 16 * qsub + n;
+      const bool active = 16 * qsub < pairs, ok = pair < pairs;
+      const int pt = ok ? (skew + pair) / G : 0, t = of_prefix ? line.toks[pt] : q0 + t0 + pt;
       const int lim = of_prefix ? len - 1 : min(len - 1, first_pos + pt);
-      const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos);
+      const int wpos = of_prefix ? len - 1 : min(len - 1, first_pos + (skew + 16 * qsub) / G);
       u32x4 qf[4];  // B operand of S^T: d = 32 ks + 8 c + [0, 8)
-      const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + (ok ? skew + n - pt * G : 0)) * a.q_stride_h + 8 * c;
+      const uint16_t *qp = a.q + (int64_t)t * a.q_stride_t + (int64_t)(h * G + (ok ? skew + pair - pt * G : 0)) * a.q_stride_h + 8 * c;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) qf[ks] = ok ? ld128(qp + 32 * ks) : u32x4{0u, 0u, 0u, 0u};
       first_loads();
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       }
       l = rows4_sum(l);
       if (ok)
-        put(std::integral_constant<int, 8>(), n, c == 0, m, l, [&](int k) { return acc[k]; },
+        put(std::integral_constant<int, 8>(), pair, c == 0, m, l, [&](int k) { return acc[k]; },
             [&](int k) { return 16 * k + 4 * c; });
     } else {
       // ---- The wave's pairs: 32 from 32 qsub on.
