@@ -10,8 +10,8 @@
 //
 // Work decomposition.  A segment is a prefix with the query tokens of all rows that use it (no mask: all of
 // them come after it), or a row's own pages with its query tokens (causal).  Its (query token, q head of the kv head's G)
-// pairs, in that order, are cut into tiles of 128, its pages into steps of 64 tokens.  The steps of
-// all tiles of a kv head form one line, kTileCost more per tile for what a tile costs besides its steps, and
+// pairs, in that order, are cut into tiles of 128, its pages into stages of 32 tokens.  The stages of
+// all tiles of a kv head form one line, kTileCost more per tile for what a tile costs besides them, and
 // block i of the head's `blocks` takes the i-th equal share of it: so the chip's block slots (two per CU)
 // finish together whatever the lengths are (to +-8 %), and a tile is cut only where a share ends.  The lengths are only on
 // the device: every block derives the same line from the tables (build_line, 1.7-2.0 us).
@@ -27,11 +27,11 @@
 // The S of a stage are computed under the softmax of the stage before.  Tiles of up to 64 pairs (a decode row's own pages
 // have G) have 16 to a wave, on 16x16 MFMA tiles.
 //
-// What bounds it.  Decode reads: 128 rows of 1050 own tokens over a prefix of 16384, 8 kv heads of 5: 630 MB in 149 us, 4.2
-// TB/s (97 us at the 6.5 TB/s of a bare read; the ordinary launch, which reads the prefix for every row, 749); 32 rows of 530
+// What bounds it.  Decode reads: 128 rows of 1050 own tokens over a prefix of 16384, 8 kv heads of 5: 632 MB in 148 us, 4.3
+// TB/s (97 us at the 6.5 TB/s of a bare read; the ordinary launch, which reads the prefix for every row, 752); 32 rows of 530
 // over 8192: 33 us against 17 and 101; the line, the pieces' beginnings (2-4 us each) and the merge (6 us with its launch) are
-// the rest.  Prompts compute: 32 prompts of 34 tokens over 8192, 8 kv heads of 4: 195 us, 0.71 PFLOP/s, 1.0 in the loop
-// (1.06 us a stage of two blocks; 116 us at the 1.19 of an 8192^3 product; the ordinary launch 214).  In the loop no single
+// the rest.  Prompts compute: 32 prompts of 34 tokens over 8192, 8 kv heads of 4: 196 us, 0.70 PFLOP/s, 1.0 in the loop
+// (1.06 us a stage of two blocks; 116 us at the 1.19 of an 8192^3 product; the ordinary launch 217).  In the loop no single
 // unit is the bound: without the exponentials it would take 95 % of its time, without V's fragments 94, without K's 97,
 // without any of them 84.
 #include "delta_common.h"
@@ -42,7 +42,7 @@ namespace delta {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kStep = 64;               // kv tokens per step
+constexpr int kStep = 32;               // kv tokens per stage, the unit of the line
 constexpr int kPages = kStep / kPageSize;
 constexpr int kPageB = kPageSize * 256; // bytes of a page's K (or V) of one head
 constexpr int kStageB = 4 * kPageB;     // a stage: 32 tokens' K, then their V
@@ -50,8 +50,10 @@ constexpr int kStages = 4;              // stages in LDS
 constexpr int kQ = 128;                 // (token, head) pairs of a tile, at most
 constexpr int kMaxRows = 1024;          // rows, and prefixes, of a call (the tables: 41 KiB)
 constexpr int kSlots = 512;             // blocks the chip holds (two per CU)
-constexpr int kTileCost = 2;            // steps that a tile costs besides its own
-constexpr int kMinShare = 2;            // steps of a share, at least
+// Stages that a tile costs besides its own, and those of a share, at least: geometric means over 25 batches against units
+// of 64 tokens, tile cost 2, shares of 2: (5, 6) -0.5 %, (5, 4) -0.4, (4, 4) +0.3, (6, 6) +0.2, (7, 6) +1.0, (3, 4) +1.6.
+constexpr int kTileCost = 5;
+constexpr int kMinShare = 6;
 
 struct PrefixArgs {
   const uint16_t *q;
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int lrow = lane >> 4, lch = lane & 15;
-    // ---- The piece at pos: segment, tile, steps [s0, s1).
+    // ---- The piece at pos: segment, tile, stages [s0, s1).
     const int items = a.num_prefixes + a.batch;
     for (;; item += 64) {  // the first segment that ends past pos
       const int i = item + lane;
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
       seg_toks = uniform(line.row_qn[r]);
       q0 = uniform(line.row_q0[r]);
     }
-    const int steps = div_up(len, kStep), cost = steps + kTileCost;
+    const int cost = div_up(len, kStep) + kTileCost;
     const int seg_at = uniform(line.at[item]);
     const int tile = uniform((pos - seg_at) / cost), tile_at = seg_at + tile * cost;
     const int stop = min(end, tile_at + cost);
@@ -802,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 6) prefix_merge_kernel(PrefixArgs a)
 }
 
 // Blocks per kv head: as many as the chip holds, or as the longest line of `tokens` query tokens over rows of
-// `max_pages` fills with kMinShare steps each.
+// `max_pages` fills with kMinShare stages each.
 int plan_blocks(int64_t tokens, int hkv, int64_t max_pages, int slots) {
   const int64_t fill = slots / hkv > 0 ? slots / hkv : 1;
   const int64_t steps = ceil_div(max_pages, kPages) + kTileCost;
@@ -912,7 +914,7 @@ int check_prefix(const void *q, int64_t q_stride_t, int64_t q_stride_h, const vo
   if (num_pages <= 0 || kv_indices_len < 0 || px->indices_len < 0 || kv_indices_len > INT32_MAX / kPageSize ||
       px->indices_len > INT32_MAX / kPageSize)
     return set_error(DELTA_ERR_INVALID, "%s: empty cache or bad table lengths", who);
-  // The line's length (each segment's tiles, at most all tokens', times its steps) and the partials' rows stay below 2^30.
+  // The line's length (each segment's tiles, at most all tokens', times its stages) and the partials' rows stay below 2^30.
   const int64_t steps = ceil_div(kv_indices_len, kPages) + ceil_div(px->indices_len, kPages) +
                         (kTileCost + 1) * ((int64_t)batch + px->num_prefixes);
   if (tokens > 1 << 23 || (ceil_div(tokens * G, kQ) + 1) * steps > 1 << 30 || partial_rows(tokens, hq, hkv, kSlots) > 1 << 30)
