@@ -83,20 +83,23 @@ struct PrefixArgs {
   float sm_scale;
 };
 
-// Pages [first, first + n) of CSR entry i, clamped to the index array.
+// Pages [first, first + n) of CSR entry i, clamped to the index array; no_csr: its end lies before its beginning.
 struct Pages {
   int first, n;
+  bool no_csr;
 };
 __device__ __forceinline__ Pages csr_pages(const int32_t *indptr, int64_t len, int i) {
   int64_t p0 = ld_scalar(indptr, i), p1 = ld_scalar(indptr, i + 1);
+  const bool no_csr = p1 < p0;
   p0 = p0 < 0 ? 0 : (p0 > len ? len : p0);
   p1 = p1 < p0 ? p0 : (p1 > len ? len : p1);
-  return Pages{(int)p0, (int)(p1 - p0)};
+  return Pages{(int)p0, (int)(p1 - p0), no_csr};
 }
 
 struct Row {
   int kv0, pages, len;  // its pages in kv_indices and its tokens, the prefix's included
   int q0, qn;           // query tokens
+  bool no_csr;
 };
 __device__ __forceinline__ Row row_of(const PrefixArgs &a, int r) {
   Row x;
@@ -108,8 +111,10 @@ __device__ __forceinline__ Row row_of(const PrefixArgs &a, int r) {
   x.len = p.n > 0 ? (p.n - 1) * kPageSize + last : 0;
   x.q0 = r;
   x.qn = 1;
+  x.no_csr = p.no_csr;
   if (a.qo_indptr) {
     int q0 = ld_scalar(a.qo_indptr, r), q1 = ld_scalar(a.qo_indptr, r + 1);
+    x.no_csr |= q1 < q0;
     q0 = q0 < 0 ? 0 : (q0 > a.tokens ? a.tokens : q0);
     q1 = q1 < q0 ? q0 : (q1 > a.tokens ? a.tokens : q1);
     x.q0 = q0;
@@ -172,6 +177,7 @@ __device__ __forceinline__ int block_scan(int v, int *sums, int *total) {
 struct Line {
   int *toks;         // [kQ + 4] query tokens of a prefix's tile
   int *sums;         // [4]
+  int *no_csr;       // [1] some table's bounds do not ascend
   int *at;           // [prefixes + rows + 1] where each segment begins (the prefixes, then the rows), and the end
   int *prefix_toks;  // [prefixes] query tokens
   int *prefix_ids;   // [prefixes] first page in prefix_indices
@@ -181,22 +187,26 @@ struct Line {
   int *row_len;      // [rows] own tokens
   int *row_q0, *row_qn;  // [rows] query tokens
   __device__ __forceinline__ Line(int *lds, int prefixes, int rows)
-      : toks(lds), sums(toks + kQ + 4), at(sums + 4), prefix_toks(at + prefixes + rows + 1), prefix_ids(prefix_toks + prefixes),
-        prefix_pages(prefix_ids + prefixes), row_prefix(prefix_pages + prefixes), row_ids(row_prefix + rows),
+      : toks(lds), sums(toks + kQ + 4), no_csr(sums + 4), at(no_csr + 1), prefix_toks(at + prefixes + rows + 1),
+        prefix_ids(prefix_toks + prefixes), prefix_pages(prefix_ids + prefixes), row_prefix(prefix_pages + prefixes), row_ids(row_prefix + rows),
         row_len(row_ids + rows), row_q0(row_len + rows), row_qn(row_q0 + rows) {}
   static size_t bytes(int prefixes, int rows) {
-    return ((size_t)kQ + 8 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
+    return ((size_t)kQ + 9 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
   }
 };
 
+// The line's length; 0 where a table is no CSR: ascending bounds are what keeps the sums below in range.
 template <int G>
 __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line) {
   const int tid = threadIdx.x, P = a.num_prefixes, B = a.batch;
   // (the rows' tables are asked for before the prefixes' have come)
   Row x = row_of(a, tid < B ? tid : 0);
   int want = a.row_prefix[tid < B ? tid : 0];
+  if (tid == 0) *line.no_csr = 0;
+  bool no_csr = false;
   for (int p = tid; p < P; p += kThreads) {
     const Pages pages = csr_pages(a.prefix_indptr, a.prefix_indices_len, p);
+    no_csr |= pages.no_csr;
     line.prefix_toks[p] = 0;
     line.prefix_ids[p] = pages.first;
     line.prefix_pages[p] = pages.n;
@@ -207,6 +217,7 @@ __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line)
       x = row_of(a, r);
       want = a.row_prefix[r];
     }
+    no_csr |= x.no_csr;
     const bool named = want >= 0 && want < P;
     const int n = named ? line.prefix_pages[want] : 0;
     const bool fits = named && !fills_tiles<G>(x.qn) && prefix_fits(a, x, n);
@@ -218,7 +229,9 @@ __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line)
     line.row_q0[r] = x.q0;
     line.row_qn[r] = x.qn;
   }
+  if (no_csr) *line.no_csr = 1;
   __syncthreads();
+  if (*line.no_csr) return 0;
   int end = 0;
   for (int i0 = 0; i0 < P + B; i0 += kThreads) {
     const int i = i0 + tid;

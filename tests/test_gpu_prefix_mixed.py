@@ -103,6 +103,33 @@ def test_captured_prompts_follow_tables_and_queries():
         torch.randn(64, 64, device=DEV).sum().item()
 
 
+@pytest.mark.parametrize("table", ["kv_indptr", "prefix_indptr", "qo"])
+def test_tables_that_do_not_ascend_write_nothing_out_of_place(table):
+    b = Batch(12, 2, [9, 4], [(0, 20, 3), (1, 33, 30), (0, 50, 1), (-1, 60, 20)], seed=49)
+    want = b.want()
+    good = (b.t[table].clone() if table != "qo" else list(b.qo))
+    if table == "qo":
+        b.qo = [0, 33, 3, 34, 54]
+    elif table == "kv_indptr":
+        b.t[table][1:3] = b.t[table][1:3].flip(0)
+    else:
+        b.t[table].copy_(torch.tensor([9, 0, 13], dtype=torch.int32))
+    room, lse = torch.full((60, 12, D), 3.0, dtype=torch.bfloat16, device=DEV), torch.full((60, 12), 4.0, device=DEV)
+    cache = b.cache.clone()
+    K.paged_prefill_prefix(b.q, b.cache, torch.tensor(b.qo, dtype=torch.int32, device=DEV), b.t["kv_indptr"], b.t["kv_indices"],
+                           b.t["last"], b.t["row_prefix"], b.t["prefix_indptr"], b.t["prefix_indices"], max_qo_len=33,
+                           out=room[3:57], lse=lse[3:57])
+    torch.cuda.synchronize()
+    for x, v in ((room, 3), (lse, 4)):
+        assert (x[:3] == v).all() and (x[57:] == v).all()
+    assert torch.equal(b.cache, cache)
+    if table == "qo":
+        b.qo = good
+    else:
+        b.t[table].copy_(good)
+    b.check(b.prefill(), want)
+
+
 def test_two_graphs_share_a_workspace():
     """Replayed in turn on one stream; nothing of one call is kept for the next."""
     bs = [Batch(32, 8, [40], [(0, 30 + i, 1) for i in range(9)], seed=45), Batch(12, 2, [7, 90], [(i % 2, 17 * i, 1) for i in range(20)], seed=46)]
