@@ -88,12 +88,12 @@ struct Pages {
   int first, n;
   bool no_csr;
 };
-__device__ __forceinline__ Pages csr_pages(const int32_t *indptr, int64_t len, int i) {
-  int64_t p0 = ld_scalar(indptr, i), p1 = ld_scalar(indptr, i + 1);
+__device__ __forceinline__ Pages csr_pages(const int32_t *indptr, int len, int i) {
+  int p0 = ld_scalar(indptr, i), p1 = ld_scalar(indptr, i + 1);
   const bool no_csr = p1 < p0;
-  p0 = p0 < 0 ? 0 : (p0 > len ? len : p0);
-  p1 = p1 < p0 ? p0 : (p1 > len ? len : p1);
-  return Pages{(int)p0, (int)(p1 - p0), no_csr};
+  p0 = min(max(p0, 0), len);
+  p1 = min(max(p1, p0), len);
+  return Pages{p0, p1 - p0, no_csr};
 }
 
 struct Row {
@@ -103,9 +103,9 @@ struct Row {
 };
 __device__ __forceinline__ Row row_of(const PrefixArgs &a, int r) {
   Row x;
-  const Pages p = csr_pages(a.kv_indptr, a.kv_indices_len, r);
+  const Pages p = csr_pages(a.kv_indptr, (int)a.kv_indices_len, r);
   int last = ld_scalar(a.last_page_len, r);
-  last = last < 0 ? 0 : (last > kPageSize ? kPageSize : last);
+  last = min(max(last, 0), kPageSize);
   x.kv0 = p.first;
   x.pages = p.n;
   x.len = p.n > 0 ? (p.n - 1) * kPageSize + last : 0;
@@ -115,8 +115,8 @@ __device__ __forceinline__ Row row_of(const PrefixArgs &a, int r) {
   if (a.qo_indptr) {
     int q0 = ld_scalar(a.qo_indptr, r), q1 = ld_scalar(a.qo_indptr, r + 1);
     x.no_csr |= q1 < q0;
-    q0 = q0 < 0 ? 0 : (q0 > a.tokens ? a.tokens : q0);
-    q1 = q1 < q0 ? q0 : (q1 > a.tokens ? a.tokens : q1);
+    q0 = min(max(q0, 0), a.tokens);
+    q1 = min(max(q1, q0), a.tokens);
     x.q0 = q0;
     x.qn = q1 - q0;
   }
@@ -199,24 +199,24 @@ struct Line {
 template <int G>
 __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line) {
   const int tid = threadIdx.x, P = a.num_prefixes, B = a.batch;
-  // (the rows' tables are asked for before the prefixes' have come)
-  Row x = row_of(a, tid < B ? tid : 0);
-  int want = a.row_prefix[tid < B ? tid : 0];
   if (tid == 0) *line.no_csr = 0;
   bool no_csr = false;
-  for (int p = tid; p < P; p += kThreads) {
-    const Pages pages = csr_pages(a.prefix_indptr, a.prefix_indices_len, p);
-    no_csr |= pages.no_csr;
-    line.prefix_toks[p] = 0;
-    line.prefix_ids[p] = pages.first;
-    line.prefix_pages[p] = pages.n;
-  }
-  __syncthreads();
-  for (int r = tid; r < B; r += kThreads) {
-    if (r != tid) {
-      x = row_of(a, r);
-      want = a.row_prefix[r];
+#pragma unroll 1
+  for (int r0 = 0; r0 < B; r0 += kThreads) {
+    const int r = r0 + tid;
+    const Row x = row_of(a, r < B ? r : 0);
+    const int want = a.row_prefix[r < B ? r : 0];
+    if (r0 == 0) {  // (the rows' tables are asked for before the prefixes' have come)
+      for (int p = tid; p < P; p += kThreads) {
+        const Pages pages = csr_pages(a.prefix_indptr, (int)a.prefix_indices_len, p);
+        no_csr |= pages.no_csr;
+        line.prefix_toks[p] = 0;
+        line.prefix_ids[p] = pages.first;
+        line.prefix_pages[p] = pages.n;
+      }
+      __syncthreads();
     }
+    if (r >= B) continue;
     no_csr |= x.no_csr;
     const bool named = want >= 0 && want < P;
     const int n = named ? line.prefix_pages[want] : 0;
