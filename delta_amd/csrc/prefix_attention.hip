@@ -83,23 +83,20 @@ struct PrefixArgs {
   float sm_scale;
 };
 
-// Pages [first, first + n) of CSR entry i, clamped to the index array; no_csr: its end lies before its beginning.
+// Pages [first, first + n) of CSR entry i, clamped to the index array.
 struct Pages {
   int first, n;
-  bool no_csr;
 };
 __device__ __forceinline__ Pages csr_pages(const int32_t *indptr, int len, int i) {
   int p0 = ld_scalar(indptr, i), p1 = ld_scalar(indptr, i + 1);
-  const bool no_csr = p1 < p0;
   p0 = min(max(p0, 0), len);
   p1 = min(max(p1, p0), len);
-  return Pages{p0, p1 - p0, no_csr};
+  return Pages{p0, p1 - p0};
 }
 
 struct Row {
   int kv0, pages, len;  // its pages in kv_indices and its tokens, the prefix's included
   int q0, qn;           // query tokens
-  bool no_csr;
 };
 __device__ __forceinline__ Row row_of(const PrefixArgs &a, int r) {
   Row x;
@@ -111,10 +108,8 @@ __device__ __forceinline__ Row row_of(const PrefixArgs &a, int r) {
   x.len = p.n > 0 ? (p.n - 1) * kPageSize + last : 0;
   x.q0 = r;
   x.qn = 1;
-  x.no_csr = p.no_csr;
   if (a.qo_indptr) {
     int q0 = ld_scalar(a.qo_indptr, r), q1 = ld_scalar(a.qo_indptr, r + 1);
-    x.no_csr |= q1 < q0;
     q0 = min(max(q0, 0), a.tokens);
     q1 = min(max(q1, q0), a.tokens);
     x.q0 = q0;
@@ -151,33 +146,34 @@ __device__ __forceinline__ T *uniform_ptr(T *p) {
                           (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
 }
 
-// Exclusive sum over the block's threads; *total: the block's sum.  `sums` holds 4 ints, free again on return.
-__device__ __forceinline__ int block_scan(int v, int *sums, int *total) {
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
+// Exclusive sum over the block's threads, saturating; *total: the block's sum.  `sums` holds 4 ints, free again on return.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sums, uint32_t *total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int incl = v;
+  uint32_t incl = v;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int x = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += x;
+    const uint32_t x = __shfl_up(incl, off, 64);
+    if (lane >= off) incl = add_sat(incl, x);
   }
   if (lane == 63) sums[wave] = incl;
   __syncthreads();
-  int before = 0, all = 0;
+  uint32_t before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) {
-    before += w < wave ? sums[w] : 0;
-    all += sums[w];
+    before = add_sat(before, w < wave ? sums[w] : 0);
+    all = add_sat(all, sums[w]);
   }
   __syncthreads();
   *total = all;
-  return before + incl - v;
+  return add_sat(before, incl) - v;
 }
 
 // The tables and the line of a kv head's work, in LDS behind the stages.
 struct Line {
   int *toks;         // [kQ + 4] query tokens of a prefix's tile
-  int *sums;         // [4]
-  int *no_csr;       // [1] some table's bounds do not ascend
+  uint32_t *sums;    // [4]
   int *at;           // [prefixes + rows + 1] where each segment begins (the prefixes, then the rows), and the end
   int *prefix_toks;  // [prefixes] query tokens
   int *prefix_ids;   // [prefixes] first page in prefix_indices
@@ -187,20 +183,18 @@ struct Line {
   int *row_len;      // [rows] own tokens
   int *row_q0, *row_qn;  // [rows] query tokens
   __device__ __forceinline__ Line(int *lds, int prefixes, int rows)
-      : toks(lds), sums(toks + kQ + 4), no_csr(sums + 4), at(no_csr + 1), prefix_toks(at + prefixes + rows + 1),
+      : toks(lds), sums(reinterpret_cast<uint32_t *>(toks + kQ + 4)), at(toks + kQ + 8), prefix_toks(at + prefixes + rows + 1),
         prefix_ids(prefix_toks + prefixes), prefix_pages(prefix_ids + prefixes), row_prefix(prefix_pages + prefixes), row_ids(row_prefix + rows),
         row_len(row_ids + rows), row_q0(row_len + rows), row_qn(row_q0 + rows) {}
   static size_t bytes(int prefixes, int rows) {
-    return ((size_t)kQ + 9 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
+    return ((size_t)kQ + 8 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
   }
 };
 
-// The line's length; 0 where a table is no CSR: ascending bounds are what keeps the sums below in range.
+// The line's length; 0 where it would pass 2^30 (only rows that overlap, in tables that do not ascend, come to that).
 template <int G>
 __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line) {
   const int tid = threadIdx.x, P = a.num_prefixes, B = a.batch;
-  if (tid == 0) *line.no_csr = 0;
-  bool no_csr = false;
 #pragma unroll 1
   for (int r0 = 0; r0 < B; r0 += kThreads) {
     const int r = r0 + tid;
@@ -209,7 +203,6 @@ __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line)
     if (r0 == 0) {  // (the rows' tables are asked for before the prefixes' have come)
       for (int p = tid; p < P; p += kThreads) {
         const Pages pages = csr_pages(a.prefix_indptr, (int)a.prefix_indices_len, p);
-        no_csr |= pages.no_csr;
         line.prefix_toks[p] = 0;
         line.prefix_ids[p] = pages.first;
         line.prefix_pages[p] = pages.n;
@@ -217,7 +210,6 @@ __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line)
       __syncthreads();
     }
     if (r >= B) continue;
-    no_csr |= x.no_csr;
     const bool named = want >= 0 && want < P;
     const int n = named ? line.prefix_pages[want] : 0;
     const bool fits = named && !fills_tiles<G>(x.qn) && prefix_fits(a, x, n);
@@ -229,24 +221,26 @@ __device__ __forceinline__ int build_line(const PrefixArgs &a, const Line &line)
     line.row_q0[r] = x.q0;
     line.row_qn[r] = x.qn;
   }
-  if (no_csr) *line.no_csr = 1;
   __syncthreads();
-  if (*line.no_csr) return 0;
-  int end = 0;
+  uint32_t end = 0;
   for (int i0 = 0; i0 < P + B; i0 += kThreads) {
     const int i = i0 + tid;
-    int cost = 0, total;
-    if (i < P)
-      cost = tiles_of<G>(line.prefix_toks[i]) * (div_up(line.prefix_pages[i], kPages) + kTileCost);
-    else if (i < P + B)
-      cost = tiles_of<G>(line.row_qn[i - P]) * (div_up(line.row_len[i - P], kStep) + kTileCost);
-    const int at = end + block_scan(cost, line.sums, &total);
-    if (i < P + B) line.at[i] = at;
-    end += total;
+    uint64_t cost = 0;
+    uint32_t total;
+    if (i < P) {
+      const int toks = min(line.prefix_toks[i], a.tokens);
+      line.prefix_toks[i] = toks;
+      cost = (uint64_t)(uint32_t)tiles_of<G>(toks) * (uint32_t)(div_up(line.prefix_pages[i], kPages) + kTileCost);
+    } else if (i < P + B) {
+      cost = (uint64_t)(uint32_t)tiles_of<G>(line.row_qn[i - P]) * (uint32_t)(div_up(line.row_len[i - P], kStep) + kTileCost);
+    }
+    const uint32_t before = block_scan((uint32_t)(cost < UINT32_MAX ? cost : UINT32_MAX), line.sums, &total);
+    if (i < P + B) line.at[i] = (int)add_sat(end, before);
+    end = add_sat(end, total);
   }
-  if (tid == 0) line.at[P + B] = end;
+  if (tid == 0) line.at[P + B] = (int)end;
   __syncthreads();
-  return end;
+  return end <= 1u << 30 ? (int)end : 0;
 }
 
 template <int DT, int G>
@@ -328,15 +322,16 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
     }
     if (of_prefix) {
       // The tile's tokens out of those of the prefix's rows, row by row.
-      int before = 0, sum;
+      uint32_t before = 0, sum;
+      const int upto = t0 + ntok;
       for (int r0 = 0; r0 < a.batch; r0 += kThreads) {
         const int r = r0 + threadIdx.x;
         const bool mine = r < a.batch && line.row_prefix[r] == item;
         const int qn = mine ? line.row_qn[r] : 0, rq0 = mine ? line.row_q0[r] : 0;
-        const int at = before + block_scan(qn, line.sums, &sum);
-        for (int k = t0 > at ? t0 - at : 0; k < qn && at + k < t0 + ntok; ++k) line.toks[at + k - t0] = rq0 + k;
-        before += sum;
-        if (before >= t0 + ntok) break;
+        const int at = (int)min(add_sat(before, block_scan(qn, line.sums, &sum)), (uint32_t)upto);
+        for (int k = t0 > at ? t0 - at : 0; k < qn && at + k < upto; ++k) line.toks[at + k - t0] = rq0 + k;
+        before = add_sat(before, sum);
+        if (before >= (uint32_t)upto) break;
       }
     }
     __syncthreads();  // the tile's tokens are listed, the piece before is done with the buffers

@@ -571,8 +571,8 @@ int delta_paged_decode_prefix(const delta_shared_prefix_t *prefix, const void *q
  * rows of qo_indptr, causal.  A row's prefix applies where it lies in front of the row's
  * query tokens (16 * pages <= kv_len_b - qo_len_b).  max_qo_len >= every row's query
  * tokens, as for delta_paged_prefill.  o and lse of tokens behind the last row are left as
- * they were.  batch <= 1024.  (Here and above: where an indptr does not ascend, o and lse of
- * the rows' tokens are unspecified; nothing else is read or written out of place.) */
+ * they were.  batch <= 1024.  (Here and above: a row whose bounds do not ascend is an empty
+ * one; qo_indptr has to ascend, or o and lse of the rows' tokens are unspecified.) */
 int delta_paged_prefill_prefix(const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_t,
                                int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
                                const int32_t *qo_indptr, const int32_t *kv_indptr,

@@ -168,3 +168,17 @@ def test_calls_at_the_same_time():
     for w, rs in zip(want, got):
         for r in rs:
             assert torch.equal(r[0], w[0]) and torch.equal(r[1], w[1])
+
+
+def test_rows_behind_the_tables_end_are_empty():
+    """A batch padded with rows of zero bounds: their o is 0, the others' unchanged."""
+    b = Batch(28, 4, [9, 4], [(0, 20, 1), (1, 33, 1), (-1, 60, 1)], seed=50)
+    o, lse = b.decode()
+    pad = lambda t, n: torch.cat([t, torch.zeros(n, dtype=torch.int32, device=DEV)])
+    t = b.t
+    q = torch.cat([b.q, torch.randn(4, 28, D, device=DEV).to(b.q.dtype)])
+    lse2 = torch.zeros(7, 28, device=DEV)
+    o2 = K.paged_decode_prefix(q, b.cache, pad(t["kv_indptr"], 4), t["kv_indices"], pad(t["last"], 4), pad(t["row_prefix"], 4),
+                               pad(t["prefix_indptr"], 3), t["prefix_indices"], max_pages_per_row=8192, lse=lse2)
+    b.check((o2[:3], lse2[:3]), b.want())
+    assert (o2[3:] == 0).all() and (lse2[3:] == -math.inf).all()
