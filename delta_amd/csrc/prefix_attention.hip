@@ -184,8 +184,8 @@ struct Line {
   int *row_q0, *row_qn;  // [rows] query tokens
   __device__ __forceinline__ Line(int *lds, int prefixes, int rows)
       : toks(lds), sums(reinterpret_cast<uint32_t *>(toks + kQ + 4)), at(toks + kQ + 8), prefix_toks(at + prefixes + rows + 1),
-        prefix_ids(prefix_toks + prefixes), prefix_pages(prefix_ids + prefixes), row_prefix(prefix_pages + prefixes), row_ids(row_prefix + rows),
-        row_len(row_ids + rows), row_q0(row_len + rows), row_qn(row_q0 + rows) {}
+        prefix_ids(prefix_toks + prefixes), prefix_pages(prefix_ids + prefixes), row_prefix(prefix_pages + prefixes),
+        row_ids(row_prefix + rows), row_len(row_ids + rows), row_q0(row_len + rows), row_qn(row_q0 + rows) {}
   static size_t bytes(int prefixes, int rows) {
     return ((size_t)kQ + 8 + 4 * (size_t)prefixes + 6 * (size_t)rows + 1) * sizeof(int);
   }
