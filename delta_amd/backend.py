@@ -875,10 +875,10 @@ class LMBackend:
                 req.admit()
                 self.slot_block_table[slot_id].fill_(int(self.scratch_pages[slot_id]))
                 self._sync_slot_block_table(slot_id, req, 0)
+            if finished or placed:
+                self._update_sharing()  # also behind the last ones: no later step may read their prefix
             if not self.scheduler.any_active():
                 break
-            if finished or placed:
-                self._update_sharing()
             self._forward(i)
             if on_step is not None:
                 on_step(self, i)

@@ -1,0 +1,65 @@
+"""The engine's bookkeeping of shared pages without a GPU: an ``LMBackend`` on CPU tables whose model steps are stand-ins."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+import delta_amd.backend as backend
+from delta_amd.backend import LMBackend
+from delta_amd.scheduler import BatchSlots, PagePool
+
+PAGE = 16
+
+
+@pytest.fixture
+def host_engine(monkeypatch):
+    """An engine of ``batch`` slots whose forward hands every active request one token (its prompt is cached by then)."""
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+
+    def make(batch=16, pages=337, hq=4, hkv=2):
+        e = LMBackend.__new__(LMBackend)
+        e.device, e.batch_size, e.pages_per_slot, e.max_length = torch.device("cpu"), batch, pages, (pages - 1) * PAGE
+        e.model = SimpleNamespace(config=SimpleNamespace(n_head=hq, n_local_heads=hkv), layers=[])
+        e.max_num_pages = batch * pages
+        e.page_pool = PagePool(e.max_num_pages, seed=0)
+        e.scheduler = BatchSlots(batch, e.page_pool, verbose=False)
+        e.scratch_pages = torch.arange(e.max_num_pages, e.max_num_pages + batch, dtype=torch.int32)
+        e.slot_block_table = e.scratch_pages[:, None].repeat(1, pages)
+        e.cachelens, e.active = torch.zeros(batch, dtype=torch.int32), torch.zeros(batch, dtype=torch.int32)
+        e._host_lens, e._host_active, e._slot_pages = [0] * batch, [0] * batch, [pages] * batch
+        e.row_prefix = torch.full((batch,), -1, dtype=torch.int32)
+        e.prefix_indptr = torch.zeros(batch // 2 + 1, dtype=torch.int32)
+        e.prefix_indices = torch.zeros(e.max_num_pages, dtype=torch.int32)
+        e.prefix_workspace, e._sharing, e._decode_graph = None, False, None
+        e.page_selector = SimpleNamespace(paged_kv_indptr=None, paged_kv_indices=None, paged_kv_last_page_len=None)
+        e.enable_delta_impl_profile = e.throughput_mode = e.is_main_process = False
+        e.tokenizer, e._step = None, None
+        e.seen = []
+
+        def forward(i):
+            for s in e.scheduler.occupied():
+                r = e.scheduler.request_in(s)
+                old = len(r.pages)
+                r.reserve(len(r.next_input()))
+                e._sync_slot_block_table(s, r, old)
+                r.record(7)
+            e.seen.append(e._sharing)
+
+        e._forward = forward
+        e._compute_prefix = lambda prefix: prefix.reserve()
+        return e
+
+    return make
+
+
+def prompts(n, length=3):
+    return [torch.arange(length) + i for i in range(n)]
+
+
+def test_sharing_ends_with_the_last_sharers(host_engine):
+    """Sixteen rows that end in one step leave no prefix to the steps that follow the loop."""
+    e = host_engine()
+    e.add_requests(prompts(16), 4800 + 6, [], prefix_ids=torch.arange(4800))
+    e.run_scheduler_loop()
+    assert any(e.seen) and e.page_pool.available == e.page_pool.total_pages
+    assert not e._sharing and e._decode_csr().prefix is None
