@@ -830,6 +830,9 @@ class LMBackend:
         try:
             self._profile_cuda_section("delta_prefill_step", lambda: self.model(
                 prefix.tokens.view(1, -1).to(self.device), torch.zeros(1, **i32), qo, ind, ip, last))
+        except BaseException:
+            prefix.drop()  # or the next request would take them for computed
+            raise
         finally:
             self._step = None
 
@@ -869,10 +872,14 @@ class LMBackend:
             for slot_id in finished:
                 self._release_slot(slot_id)
             placed = self.scheduler.fill_free_slots()
-            for slot_id, req in placed:
-                if req.prefix is not None and not req.prefix.pages:
-                    self._compute_prefix(req.prefix)
-                req.admit()
+            for n, (slot_id, req) in enumerate(placed):
+                try:
+                    if req.prefix is not None and not req.prefix.pages:
+                        self._compute_prefix(req.prefix)
+                    req.admit()
+                except BaseException:  # no slot may hold a request without pages
+                    self.scheduler.unplace(placed[n:])
+                    raise
                 self.slot_block_table[slot_id].fill_(int(self.scratch_pages[slot_id]))
                 self._sync_slot_block_table(slot_id, req, 0)
             if finished or placed:

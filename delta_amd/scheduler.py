@@ -95,11 +95,15 @@ class SharedPrefix:
         self.pages = self._pool.take(len(self.tokens) // PAGE_SIZE)
         return self.pages
 
+    def drop(self) -> None:
+        """Give the pages back: nobody needs them any more, or they could not be computed."""
+        self._pool.give_back(self.pages)
+        self.pages = []
+
     def user_finished(self) -> None:
         self.users -= 1
         if self.users == 0:
-            self._pool.give_back(self.pages)
-            self.pages = []
+            self.drop()
 
 
 def shared_prefixes(rows: Dict[int, Sequence[int]]) -> Tuple[Dict[int, int], List[List[int]]]:
@@ -185,9 +189,9 @@ class ServingRequest:
     # -- pages
     def admit(self) -> None:
         """Start serving: one empty page, behind the pages of the prefix (computed by now) if there is one."""
+        own = self._pool.take(1)
         self.state = self.ACTIVE
         self.t_start = time.perf_counter()
-        own = self._pool.take(1)
         self.pages = own
         self.fill = 0
         if self.prefix is not None:
@@ -305,6 +309,12 @@ class BatchSlots:
                 self.slots[s] = req.rid
                 placed.append((s, req))
         return placed
+
+    def unplace(self, placed: Sequence[Tuple[int, ServingRequest]]) -> None:
+        """Requests of ``fill_free_slots`` that could not be admitted go back to the head of the queue."""
+        for s, req in reversed(placed):
+            self.slots[s] = None
+            self.waiting.appendleft(req.rid)
 
     def place(self, req: ServingRequest) -> int:
         """Put an already served request (a fork) into a free slot."""

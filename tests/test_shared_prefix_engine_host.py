@@ -63,3 +63,26 @@ def test_sharing_ends_with_the_last_sharers(host_engine):
     e.run_scheduler_loop()
     assert any(e.seen) and e.page_pool.available == e.page_pool.total_pages
     assert not e._sharing and e._decode_csr().prefix is None
+
+
+def test_a_prefix_that_could_not_be_computed_is_computed_again(host_engine):
+    """A failing forward (out of memory, say) leaves no pages behind that pass for the prefix's K and V."""
+    e = host_engine(batch=2)
+    del e._compute_prefix
+    tries = []
+
+    def model(*a):
+        tries.append(a[0].shape[1])
+        if len(tries) == 1:
+            raise torch.OutOfMemoryError("no room for the prefix")
+
+    e.model = type("Model", (), {"config": e.model.config, "layers": [], "__call__": staticmethod(model)})()
+    e.add_requests(prompts(3), 60, [], prefix_ids=torch.arange(40))
+    px = e.scheduler.requests[0].prefix
+    with pytest.raises(torch.OutOfMemoryError):
+        e.run_scheduler_loop()
+    assert px.pages == [] and e.page_pool.available == e.page_pool.total_pages and e._step is None
+    assert e.scheduler.occupied() == [] and list(e.scheduler.waiting) == [0, 1, 2]  # as before the call
+    e.run_scheduler_loop()
+    assert tries == [32, 32] and all(r.finished for r in e.scheduler.requests)
+    assert e.page_pool.available == e.page_pool.total_pages
