@@ -800,11 +800,15 @@ class LMBackend:
             raise ValueError(f"a fork of {total} tokens needs 1-D input_ids and a max_length in ({total}, "
                              f"{self.max_length}], got {limit}")
         child = parent.fork(len(sched.requests), more, limit, eot_token_ids)
+        try:
+            if child.fill:
+                i32 = dict(dtype=torch.int32, device=self.device)
+                K.copy_pages(self._kv_caches(), torch.tensor(parent.pages[-1:], **i32), torch.tensor(child.pages[-1:], **i32),
+                             tokens=torch.tensor([child.fill], **i32))
+        except BaseException:  # a child without those tokens may not be served
+            self.page_pool.give_back(child.pages)
+            raise
         sched.place(child)
-        if child.fill:
-            i32 = dict(dtype=torch.int32, device=self.device)
-            K.copy_pages(self._kv_caches(), torch.tensor(parent.pages[-1:], **i32), torch.tensor(child.pages[-1:], **i32),
-                         tokens=torch.tensor([child.fill], **i32))
         self.slot_block_table[slot].fill_(int(self.scratch_pages[slot]))
         self._sync_slot_block_table(slot, child, 0)
         self._update_sharing()

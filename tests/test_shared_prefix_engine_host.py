@@ -86,3 +86,25 @@ def test_a_prefix_that_could_not_be_computed_is_computed_again(host_engine):
     e.run_scheduler_loop()
     assert tries == [32, 32] and all(r.finished for r in e.scheduler.requests)
     assert e.page_pool.available == e.page_pool.total_pages
+
+
+def test_a_fork_whose_page_copy_fails_is_not_served(host_engine, monkeypatch):
+    e = host_engine(batch=2)
+    e.add_requests(prompts(1, 5), 60, [])
+
+    def refuse(*a, **kw):
+        raise torch.OutOfMemoryError("no room for the tables")
+
+    monkeypatch.setattr(backend.K, "copy_pages", refuse)
+    tries = []
+
+    def on_step(e, i):
+        if i == 3:
+            pages = e.page_pool.available
+            with pytest.raises(torch.OutOfMemoryError):
+                e.fork_request(0, torch.tensor([1, 2]))
+            tries.append(i)
+            assert e.page_pool.available == pages and len(e.scheduler.requests) == 1 and e.scheduler.occupied() == [0]
+
+    e.run_scheduler_loop(on_step=on_step)
+    assert tries and e.page_pool.available == e.page_pool.total_pages
