@@ -397,8 +397,12 @@ class LMBackend:
         """Full attention of a step whose rows share prefixes: every prefix's pages read once for all its rows."""
         st = self._step
         if st.mode == "prefill":
-            return self._profile_cuda_section("delta_prefill_attention", lambda: K.paged_prefill_prefix(
-                q, kv_cache, st.qo_indptr, st.kv_indptr, st.kv_indices, st.kv_last, *st.prefix, max_qo_len=st.max_qo))
+            try:
+                return self._profile_cuda_section("delta_prefill_attention", lambda: K.paged_prefill_prefix(
+                    q, kv_cache, st.qo_indptr, st.kv_indptr, st.kv_indices, st.kv_last, *st.prefix, max_qo_len=st.max_qo))
+            except torch.OutOfMemoryError:  # no room for the partials: the ordinary launch, from here on in this step
+                st.prefix = None
+                return self.attn_full(q, kv_cache)
 
         def decode():
             x = q
@@ -574,6 +578,14 @@ class LMBackend:
             rows = {s: self.scheduler.request_in(s).pages for s in self.scheduler.occupied()}
         row_prefix, prefixes = shared_prefixes(rows)
         on = self._sharing_pays(prefixes, row_prefix, self.batch_size)
+        if on and self.prefix_workspace is None:
+            cfg = self.model.config
+            try:
+                self.prefix_workspace = torch.empty(
+                    K.prefix_attention_workspace_bytes(self.batch_size, cfg.n_head, cfg.n_local_heads, self.pages_per_slot),
+                    dtype=torch.uint8, device=self.device)
+            except torch.OutOfMemoryError:  # the ordinary launches need none of it
+                on = False
         if on:
             ip = [0, *itertools.accumulate(len(p) for p in prefixes)]
             ip += [ip[-1]] * (self.prefix_indptr.numel() - len(ip))
@@ -581,11 +593,6 @@ class LMBackend:
             self.row_prefix.copy_(torch.tensor([row_prefix.get(s, -1) for s in range(self.batch_size)], dtype=torch.int32))
             self.prefix_indptr.copy_(torch.tensor(ip, dtype=torch.int32))
             self.prefix_indices[:len(flat)].copy_(torch.tensor(flat, dtype=torch.int32))
-            if self.prefix_workspace is None:
-                cfg = self.model.config
-                self.prefix_workspace = torch.empty(
-                    K.prefix_attention_workspace_bytes(self.batch_size, cfg.n_head, cfg.n_local_heads, self.pages_per_slot),
-                    dtype=torch.uint8, device=self.device)
         if on != self._sharing:
             self._sharing = on
             self._decode_graph = None  # captured with the other attention launches

@@ -108,3 +108,43 @@ def test_a_fork_whose_page_copy_fails_is_not_served(host_engine, monkeypatch):
 
     e.run_scheduler_loop(on_step=on_step)
     assert tries and e.page_pool.available == e.page_pool.total_pages
+
+
+def test_prompt_steps_go_on_where_the_partials_find_no_room(host_engine, monkeypatch):
+    """As ``paged_prefill`` does: the ordinary launch attends the same tables."""
+    e = host_engine()
+    calls = []
+
+    def shared(*a, **kw):
+        calls.append("shared")
+        raise torch.OutOfMemoryError("no room for the partials")
+
+    def ordinary(q, cache, *tables, **kw):
+        calls.append("ordinary")
+        return q, tables, kw["max_qo_len"]
+
+    monkeypatch.setattr(backend.K, "paged_prefill_prefix", shared)
+    monkeypatch.setattr(backend.K, "paged_prefill", ordinary)
+    e.workspace = None
+    e._step = backend._StepCSR("prefill", "ip", "ind", "last", 7, qo_indptr="qo", max_qo=5, single_pages=[], prefix=(1, 2, 3))
+    assert e.attn_full("q", "cache") == ("q", ("qo", "ip", "ind", "last"), 5)
+    assert e.attn_full("q", "cache") == ("q", ("qo", "ip", "ind", "last"), 5)  # the next layer does not try again
+    assert calls == ["shared", "ordinary", "ordinary"]
+
+
+def test_decode_steps_go_on_where_the_workspace_finds_no_room(host_engine, monkeypatch):
+    e = host_engine()
+    rows = {s: list(range(300)) + [300 + s] for s in range(16)}
+    empty = torch.empty
+
+    def full(*a, **kw):
+        if kw.get("dtype") is torch.uint8:
+            raise torch.OutOfMemoryError("no room for the workspace")
+        return empty(*a, **kw)
+
+    monkeypatch.setattr(torch, "empty", full)
+    e._update_sharing(rows)
+    assert not e._sharing and e._decode_csr().prefix is None
+    monkeypatch.setattr(torch, "empty", empty)
+    e._update_sharing(rows)
+    assert e._sharing and e.prefix_workspace is not None
