@@ -34,7 +34,7 @@ import os
 import time
 from collections import defaultdict
 from pathlib import Path
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -51,12 +51,40 @@ PAGE_SIZE = 16
 # sharers: 64 MB, what the ordinary launches read in the time that the shared ones take besides their work (8 kv heads: 16
 # rows sharing 256 pages 21 us against 27, 8 sharing 64 14 against 12).
 SHARING_PAYS = 8192
-# Prompt steps: a row of more new (token, q head of a kv head) pairs than this fills tiles of its own, so that sharing spares
-# it nothing, and the ordinary launch sweeps such rows faster (8 kv heads of 4 over 8192 tokens, us shared / ordinary: 64
-# rows of 60-70 660 / 720, 32 of 120-130 620 / 680, 8 of 512 626 / 519, 2 of 2048 719 / 561); and a step of more new tokens
-# than this is no sharers' step (the partials take 1 KiB per token and q head).
+# Prompt steps: rows of more new (token, q head of a kv head) pairs than this fill tiles of their own, so that sharing spares
+# them nothing, and a step of more new tokens than this is no sharers' step (the partials take 1 KiB per token and q head).
+# Whether the others' sharing pays depends on all the step's rows, which one launch attends: ``prompt_step_us``.
 SHARING_PAIRS = 1024
 SHARING_TOKENS = 16384
+
+
+def prompt_step_us(qo_lens: List[int], kv_lens: List[int], spared: int, group: int, hkv: int) -> Tuple[float, float]:
+    """Estimates of a prompt step's attention in one layer, shared and ordinary launch, in us (``spared``: pages that sharing
+    saves, of the rows' ``kv_lens`` tokens).
+
+    Ordinary: rows of one new token are read at about 10 TB/s (page-heads of 8 KiB, mostly from caches where rows share); the
+    others' products run at 2.1 G (pair, token)s per ms, pairs padded to blocks of 128 on ``32 // group * 4`` tokens, but a
+    block sweeps its row's pages at 0.33 us each.  Shared: 1.75 G over whole tiles, a page-head per 1.5 ns, and about 20-28 us
+    of beginnings and merge.  Over 195 steps that spare 64 MB or more (8 kv heads of 4, 4 of 7, 2 of 6; 8-64 rows of 1-250 new
+    tokens over prefixes of 50-1000 pages, alone or beside prompts of 1100-8000) taking the lower estimate costs over 3 % in
+    2 (us 51 / 44, 49 / 43) and misses a gain of over 3 % in 16 (most with 7 q heads per kv head, whose tokens fill the
+    ordinary launch's last round badly); sharing in all of them was over 3 % slower in 108, up to twice the time.  E.g. us
+    shared / ordinary, 8 kv heads of 4: 31 decoding rows over 300 pages 25 / 59, beside a prompt of 2000 tokens 101 / 112, of
+    4000 264 / 200, of 8000 899 / 555; 64 prompts of 20 tokens over 400 pages 191 / 194, of 60 475 / 398, of 120 913 / 763;
+    8 of 60 86 / 140."""
+    ordinary = sweep = single = shared = 0.0
+    tile = 32 // group * 4
+    for q, n in zip(qo_lens, kv_lens):
+        shared += q * group * hkv * (n - q / 4)
+        if q == 1:
+            single += n / PAGE_SIZE * hkv
+        else:
+            ordinary += -(-q // tile) * 128 * hkv * (n - q / 2)
+            sweep = max(sweep, 6 + 0.33 * n / PAGE_SIZE)
+    ordinary = max(ordinary / 2.1e6, sweep) + (12 + 0.65e-3 * single if single else 0)
+    read = (sum(-(-n // PAGE_SIZE) for n in kv_lens) - spared) * hkv
+    shared = max(shared / 1.75e6, 1.5e-3 * read) + 20 + 0.15 * len(qo_lens) + (8 if sweep else 0)
+    return shared, ordinary
 
 
 class _StepCSR:
@@ -561,14 +589,27 @@ class LMBackend:
         return _StepCSR("decode", sel.paged_kv_indptr, sel.paged_kv_indices, sel.paged_kv_last_page_len,
                         self.pages_per_slot, prefix=prefix)
 
-    def _sharing_pays(self, prefixes: List[List[int]], row_prefix: dict, n_rows: int) -> bool:
-        if n_rows > 1024:  # more than the launches take
-            return False
+    def _spared_pages(self, prefixes: List[List[int]], row_prefix: dict) -> int:
         users = [0] * len(prefixes)
         for p in row_prefix.values():
             users[p] += 1
-        spared = sum((n - 1) * len(pages) for n, pages in zip(users, prefixes))
-        return spared * self.model.config.n_local_heads >= SHARING_PAYS
+        return sum((n - 1) * len(pages) for n, pages in zip(users, prefixes))
+
+    def _sharing_pays(self, prefixes: List[List[int]], row_prefix: dict, n_rows: int) -> bool:
+        if n_rows > 1024:  # more than the launches take
+            return False
+        return self._spared_pages(prefixes, row_prefix) * self.model.config.n_local_heads >= SHARING_PAYS
+
+    def _prompt_prefixes(self, rows_pages: List[List[int]], qo_lens: List[int], kv_lens: List[int]):
+        """The prefixes (``shared_prefixes``' result) that a prompt step's rows are served with, or None."""
+        cfg = self.model.config
+        hkv = cfg.n_local_heads
+        group = cfg.n_head // hkv
+        row_prefix, prefixes = shared_prefixes({b: p for b, p in enumerate(rows_pages) if qo_lens[b] * group <= SHARING_PAIRS})
+        if sum(qo_lens) > SHARING_TOKENS or not self._sharing_pays(prefixes, row_prefix, len(rows_pages)):
+            return None
+        shared, ordinary = prompt_step_us(qo_lens, kv_lens, self._spared_pages(prefixes, row_prefix), group, hkv)
+        return (row_prefix, prefixes) if shared < ordinary else None
 
     @torch.inference_mode()
     def _update_sharing(self, rows: Optional[dict] = None) -> None:
@@ -1025,11 +1066,10 @@ class LMBackend:
         row_ip = torch.tensor(kv_indptr, **i32)
         row_ind = torch.tensor(kv_indices, **i32)
         row_last = torch.tensor(rows_last, **i32)
-        cfg = self.model.config
-        group = cfg.n_head // cfg.n_local_heads
-        row_prefix, prefixes = shared_prefixes({b: p for b, p in enumerate(rows_pages) if qo_lens[b] * group <= SHARING_PAIRS})
+        sharing = self._prompt_prefixes(rows_pages, qo_lens, [start + n for start, n in zip(offsets, qo_lens)])
         prefix = None
-        if sum(qo_lens) <= SHARING_TOKENS and self._sharing_pays(prefixes, row_prefix, len(rows_pages)):
+        if sharing is not None:
+            row_prefix, prefixes = sharing
             prefix = (torch.tensor([row_prefix.get(b, -1) for b in range(len(rows_pages))], **i32),
                       torch.tensor([0] + list(itertools.accumulate(len(p) for p in prefixes)), **i32),
                       torch.tensor([p for pages in prefixes for p in pages], **i32))

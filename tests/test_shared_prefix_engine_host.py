@@ -148,3 +148,41 @@ def test_decode_steps_go_on_where_the_workspace_finds_no_room(host_engine, monke
     monkeypatch.setattr(torch, "empty", empty)
     e._update_sharing(rows)
     assert e._sharing and e.prefix_workspace is not None
+
+
+def step(sharers, prefix_pages, longs=()):
+    """Rows of a prompt step: (own cached tokens, new tokens) behind a prefix of so many pages, and beside it rows of none."""
+    pages, qo, lens, at = [], [], [], prefix_pages
+    for own, q in list(sharers) + list(longs):
+        shared = prefix_pages if len(pages) < len(sharers) else 0
+        n = -(-(own + q) // PAGE)
+        pages.append(list(range(shared)) + list(range(at, at + n)))
+        at += n
+        qo.append(q)
+        lens.append(shared * PAGE + own + q)
+    return pages, qo, lens
+
+
+@pytest.mark.parametrize("heads,rows,shared", [  # us shared / ordinary
+    ((32, 8), step([(40, 1)] * 31, 300), True),                    # 25 / 59
+    ((32, 8), step([(40, 1)] * 31, 600, [(0, 1100)]), True),       # 52 / 156
+    ((32, 8), step([(40, 1)] * 31, 600, [(0, 2000)]), True),       # 98 / 179
+    ((32, 8), step([(40, 1)] * 31, 300, [(0, 4000)]), False),      # 264 / 200
+    ((32, 8), step([(40, 1)] * 31, 600, [(0, 8000)]), False),      # 906 / 618
+    ((32, 8), step([(20, 20)] * 31, 300, [(0, 4000)]), False),     # 300 / 225
+    ((32, 8), step([(0, 20)] * 31, 300, [(0, 2000)] * 4), False),  # 341 / 244
+    ((28, 4), step([(40, 1)] * 31, 600, [(0, 4000)]), False),      # 237 / 190
+    ((12, 2), step([(40, 1)] * 31, 600, [(0, 8000)]), False),      # 365 / 252
+    ((12, 2), step([(40, 1)] * 15, 1000, [(0, 2000)]), True),      # 55 / 94
+    ((32, 8), step([(0, 60)] * 8, 400), True),                     # 86 / 140
+    ((32, 8), step([(0, 20)] * 32, 400), True),                    # 105 / 138
+    ((32, 8), step([(0, 60)] * 64, 400), False),                   # 475 / 398
+    ((32, 8), step([(0, 250)] * 64, 200), False),                  # 1026 / 868
+    ((32, 8), step([(0, 20)] * 64, 50), False),                    # 61 / 33
+    ((28, 4), step([(0, 60)] * 64, 100), False),                   # 169 / 117
+])
+def test_prompt_steps_share_where_that_is_faster(host_engine, heads, rows, shared):
+    """Rows that gain nothing from sharing weigh against those that do: one launch attends them all."""
+    pages, qo, lens = rows
+    e = host_engine(batch=len(qo), hq=heads[0], hkv=heads[1])
+    assert (e._prompt_prefixes(pages, qo, lens) is not None) == shared
