@@ -48,14 +48,30 @@ from .scheduler import BatchSlots, PagePool, ServingRequest, SharedPrefix, share
 
 PAGE_SIZE = 16
 # Page-heads (a page of one kv head, 8 KiB) that sharing has to spare a layer's attention before its rows are served as
-# sharers: 64 MB, what the ordinary launches read in the time that the shared ones take besides their work (8 kv heads: 16
-# rows sharing 256 pages 21 us against 27, 8 sharing 64 14 against 12).
+# sharers: 64 MB, and more of them the more (row, kv head) pairs there are (``sharing_pays_from``).
 SHARING_PAYS = 8192
 # Prompt steps: rows of more new (token, q head of a kv head) pairs than this fill tiles of their own, so that sharing spares
 # them nothing, and a step of more new tokens than this is no sharers' step (the partials take 1 KiB per token and q head).
 # Whether the others' sharing pays depends on all the step's rows, which one launch attends: ``prompt_step_us``.
 SHARING_PAIRS = 1024
 SHARING_TOKENS = 16384
+
+
+def sharing_pays_from(rows: int, hkv: int, max_pages: int) -> float:
+    """Page-heads from which on decode steps of ``rows`` rows planned for ``max_pages`` share.
+
+    Each row's own pages are a piece of work of their own in the shared launch, which takes RoPE and the KV append in one more
+    launch, so the break-even rises with the (row, kv head) pairs: measured in captured engine steps with sharing on and off,
+    own parts of 20-3000 tokens, it lies at 14-18 k for 64 pairs, 18-22 k for 128, 25-29 k for 256, 42-47 k for 512, 50-55 k
+    for 1024 (us a layer more with sharing, 64 rows of 8 kv heads: +15 at 8.6 k, +9 at 25 k, +3 at 41 k, -2 at 49 k, -7 at 66 k;
+    32 rows of 2: +8 at 8.2 k, +2 at 12 k, +1 at 16 k, -3 at 25 k; rows whose own parts are long and ragged gain earlier, by
+    1-6 us).  Where the ordinary launch cuts the rows of 256 pairs or more into units (a large ``max_pages``) sharing gains
+    from the start (64 rows of 8 over 9000 tokens' pages: -8 to -74 at 8.6 k).  Below 64 pairs the plan of the ordinary launch
+    decides (32 pairs at 9 k: +6 where a slot holds 337 pages, +2 with 563, 0 with 751, -8 with 1251): 8192 for all."""
+    pairs = rows * hkv
+    if pairs >= 256 and K.decode_num_splits(rows, hkv, max_pages) > 1:
+        return SHARING_PAYS
+    return SHARING_PAYS * (max(pairs, 32) / 32) ** 0.58
 
 
 def prompt_step_us(qo_lens: List[int], kv_lens: List[int], spared: int, group: int, hkv: int) -> Tuple[float, float]:
@@ -598,7 +614,8 @@ class LMBackend:
     def _sharing_pays(self, prefixes: List[List[int]], row_prefix: dict, n_rows: int) -> bool:
         if n_rows > 1024:  # more than the launches take
             return False
-        return self._spared_pages(prefixes, row_prefix) * self.model.config.n_local_heads >= SHARING_PAYS
+        hkv = self.model.config.n_local_heads
+        return self._spared_pages(prefixes, row_prefix) * hkv >= sharing_pays_from(n_rows, hkv, self.pages_per_slot)
 
     def _prompt_prefixes(self, rows_pages: List[List[int]], qo_lens: List[int], kv_lens: List[int]):
         """The prefixes (``shared_prefixes``' result) that a prompt step's rows are served with, or None."""
@@ -606,9 +623,10 @@ class LMBackend:
         hkv = cfg.n_local_heads
         group = cfg.n_head // hkv
         row_prefix, prefixes = shared_prefixes({b: p for b, p in enumerate(rows_pages) if qo_lens[b] * group <= SHARING_PAIRS})
-        if sum(qo_lens) > SHARING_TOKENS or not self._sharing_pays(prefixes, row_prefix, len(rows_pages)):
+        spared = self._spared_pages(prefixes, row_prefix)
+        if len(rows_pages) > 1024 or sum(qo_lens) > SHARING_TOKENS or spared * hkv < SHARING_PAYS:
             return None
-        shared, ordinary = prompt_step_us(qo_lens, kv_lens, self._spared_pages(prefixes, row_prefix), group, hkv)
+        shared, ordinary = prompt_step_us(qo_lens, kv_lens, spared, group, hkv)
         return (row_prefix, prefixes) if shared < ordinary else None
 
     @torch.inference_mode()

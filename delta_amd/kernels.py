@@ -114,6 +114,11 @@ def decode_workspace_bytes(batch: int, hq: int, hkv: int, max_pages: int) -> int
     return int(_lib.query("delta_paged_decode_workspace_bytes", batch, hq, hkv, max_pages))
 
 
+def decode_num_splits(batch: int, hkv: int, max_pages: int) -> int:
+    """Units that ``paged_decode`` cuts a row of ``max_pages`` pages into."""
+    return int(_lib.query("delta_decode_num_splits", batch, hkv, max_pages))
+
+
 @dataclass
 class DecodeAppend:
     """The decode token's RoPE and KV append, fused into a ``paged_decode`` launch

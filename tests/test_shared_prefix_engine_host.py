@@ -186,3 +186,27 @@ def test_prompt_steps_share_where_that_is_faster(host_engine, heads, rows, share
     pages, qo, lens = rows
     e = host_engine(batch=len(qo), hq=heads[0], hkv=heads[1])
     assert (e._prompt_prefixes(pages, qo, lens) is not None) == shared
+
+
+@pytest.mark.parametrize("rows,heads,capacity,shared,on", [  # us a layer more (-: less) in captured steps that share
+    (8, (32, 8), 9000, 147, False),   # +4.0 to -0.5 over own parts of 20 to 3000 tokens
+    (8, (32, 8), 9000, 293, True),    # -0.2 to -2.8
+    (16, (32, 8), 9000, 69, False),   # +2.0 to +5.2
+    (16, (32, 8), 9000, 205, True),   # -1.8 to -6.2
+    (32, (32, 8), 5000, 50, False),   # +3.6 to +9.3
+    (32, (32, 8), 5000, 130, True),   # -7.8 at 166, +2.2 to -3.8 at 100
+    (64, (32, 8), 5000, 49, False),   # +5.1 to +8.9
+    (64, (32, 8), 5000, 98, True),    # -0.9 to -3.9
+    (64, (32, 8), 9000, 17, True),    # -8 to -74: the ordinary launch cuts these rows
+    (128, (32, 8), 3000, 33, False),  # +4.5 to +8.8
+    (64, (28, 4), 9000, 49, False),   # -2.6 to +10.9
+    (64, (28, 4), 9000, 163, True),   # -4.4 to -19.7
+    (32, (12, 2), 9000, 133, False),  # -1.2 to +8.0
+    (64, (12, 2), 4500, 66, False),   # +5.5 to +8.4
+    (128, (12, 2), 9000, 49, False),  # -1.0 to +9.7
+    (128, (12, 2), 16000, 162, True), # -5.2 to -20.2
+])
+def test_decode_steps_share_where_that_is_faster(host_engine, rows, heads, capacity, shared, on):
+    e = host_engine(batch=rows, pages=capacity // PAGE + 1, hq=heads[0], hkv=heads[1])
+    e._update_sharing({s: list(range(shared)) + [100000 + s] for s in range(rows)})
+    assert e._sharing == on
