@@ -191,7 +191,8 @@ class LMBackend:
         self.timer = None
         self._compiled = False
         self._step: Optional[_StepCSR] = None
-        self._decode_graph: Optional[torch.cuda.CUDAGraph] = None
+        self._decode_graphs: dict = {}  # sharing on / off -> captured step
+        self._sharing = False
         self._decode_graph_on_chip = False  # the planner path the captured step runs
         self._decode_graph_failed: Optional[str] = None
         self._decode_graph_stats = defaultdict(int)
@@ -320,7 +321,7 @@ class LMBackend:
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
         self._pinned_tokens = torch.zeros(B, dtype=torch.long).pin_memory()
         # Rows that share their first pages (``_update_sharing``): each slot's prefix and the prefixes' pages, read by a
-        # captured step at every replay; switching them on or off captures it again.
+        # captured step at every replay; the steps that share and those that do not are captured each once.
         self.row_prefix = torch.full((B,), -1, **i32)
         self.prefix_indptr = torch.zeros(B // 2 + 1, **i32)
         self.prefix_indices = torch.zeros(max(self.max_num_pages, 1), **i32)
@@ -652,9 +653,7 @@ class LMBackend:
             self.row_prefix.copy_(torch.tensor([row_prefix.get(s, -1) for s in range(self.batch_size)], dtype=torch.int32))
             self.prefix_indptr.copy_(torch.tensor(ip, dtype=torch.int32))
             self.prefix_indices[:len(flat)].copy_(torch.tensor(flat, dtype=torch.int32))
-        if on != self._sharing:
-            self._sharing = on
-            self._decode_graph = None  # captured with the other attention launches
+        self._sharing = on  # (each side has a captured step of its own)
 
     def _decode_body(self, advance: bool):
         """One decode step for all slots; only device work (capturable)."""
@@ -675,6 +674,19 @@ class LMBackend:
         if advance:
             self.cachelens.add_(self.active)
         return tokens
+
+    @property
+    def _decode_graph(self) -> Optional[torch.cuda.CUDAGraph]:
+        """The captured step of the attention launches that are in use, shared or ordinary: a batch that crosses the line
+        comes back to the one it had (two eager steps and a capture otherwise).  Setting it to None drops both."""
+        return self._decode_graphs.get(self._sharing)
+
+    @_decode_graph.setter
+    def _decode_graph(self, graph) -> None:
+        if graph is None:
+            self._decode_graphs = {}
+        else:
+            self._decode_graphs[self._sharing] = graph
 
     def _capture_decode_graph(self):
         t0 = time.perf_counter()
@@ -725,7 +737,7 @@ class LMBackend:
         before running when a row would need more pages than its slot holds."""
         self._check_decode_budget(n)
         use_graph = self.enable_cuda_graph_decode if use_graph is None else use_graph
-        if self._decode_graph is not None and self._decode_graph_on_chip != self._plan_on_chip():
+        if self._decode_graphs and self._decode_graph_on_chip != self._plan_on_chip():
             self._decode_graph = None  # captured with the other planner path (the debug flag moved)
         if use_graph and self._decode_graph is None and self._decode_graph_failed is None:
             try:

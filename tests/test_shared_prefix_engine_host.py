@@ -210,3 +210,23 @@ def test_decode_steps_share_where_that_is_faster(host_engine, rows, heads, capac
     e = host_engine(batch=rows, pages=capacity // PAGE + 1, hq=heads[0], hkv=heads[1])
     e._update_sharing({s: list(range(shared)) + [100000 + s] for s in range(rows)})
     assert e._sharing == on
+
+
+def test_crossing_the_line_keeps_both_captured_steps(host_engine):
+    """A batch that fills and drains around it goes back to the step that it had captured; what else changes drops both."""
+    e = host_engine()
+    sharers = {s: list(range(300)) + [300 + s] for s in range(16)}
+    alone = {s: [s] for s in range(16)}
+    e._update_sharing(alone)
+    assert e._decode_graph is None
+    e._decode_graph = "ordinary"
+    e._update_sharing(sharers)
+    assert e._sharing and e._decode_graph is None
+    e._decode_graph = "shared"
+    for rows, graph in ((alone, "ordinary"), (sharers, "shared"), (sharers, "shared"), (alone, "ordinary")):
+        e._update_sharing(rows)
+        assert e._decode_graph == graph
+    e._decode_graph = None
+    assert e._decode_graph is None
+    e._update_sharing(sharers)
+    assert e._decode_graph is None
