@@ -36,6 +36,7 @@
 // without any of them 84.
 #include "delta_common.h"
 #include "mfma32.h"
+#include <math.h>
 
 namespace delta {
 
@@ -875,13 +876,20 @@ void launch(const PrefixArgs &a, int G, hipStream_t stream) {
     launch_merge<DT, 1>(a, rows, stream);
 }
 
-// Whether a decode batch is too small for sharing to pay: one row, or rows that are read in the time that the launches
-// here take besides their work (about 8 us: the line, the pieces' beginnings, the merge).  The ordinary launch reads every
-// row, pages that rows share mostly from the L2 and the Infinity Cache.  (us here / ordinary, 8 kv heads of 4: 4 rows of 2100
-// tokens, 34 MB of K and V, 13.6 / 11.4; 8 of 1100, 36 MB, 13.9 / 11.9; 16 of 4170, 270 MB, 21 / 27; 2 kv heads of 6: 2 of 550, 1
-// MB, 12.5 / 9.5; one row of 4200, 8 kv heads, 15 / 10.8.)
+// Whether a decode batch is too small for sharing to pay: one row, or rows that are read in the time that the launches here take
+// besides their work (the line, the merge, and a piece's beginning for every row's own pages: 8 us for few rows, 20 for 1024 (row,
+// kv head) pairs).  The ordinary launch reads every row, pages that rows share mostly from the L2 and the Infinity Cache.  What
+// the rows share is known on the device only, so the rule goes by all that they may read, planned; us here / ordinary at rows
+// that share four fifths of it, bf16, the line at 8192 page-heads (of 8 KiB) up to 32 pairs, 18.3 k for 128, 41 k for 512:
+//   8 kv heads of 4: 8 rows, 8 k 15.4 / 14.4, 16 k 17.8 / 19.2; 16 rows, 16 k 18.1 / 18.1, 33 k 22.1 / 29.9; 32 rows, 16 k 20.8 /
+//   15.5, 33 k 24.9 / 26.9; 64 rows, 8 k 24.6 / 8.8, 33 k 28.8 / 23.0, 49 k 33.5 / 32.7, 66 k 37.0 / 41.9; 128 rows, 49 k 39.1 /
+//   33.3, 66 k 41.5 / 42.5; 2 of 6: 16 rows, 8 k 17.7 / 14.7, 16 k 20.2 / 21.3; 64 rows, 16 k 22.5 / 19.0, 33 k 26.9 / 32.1; 256
+//   rows, 33 k 33.9 / 26.7, 66 k 40.8 / 45.4; 8 of 1: 64 rows, 16 k 17.6 / 12.3, 33 k 20.3 / 21.1.
+// (The ordinary launch takes at most 16 kv heads.)
 bool decode_alone(int64_t rows, int hkv, int64_t max_pages) {
-  return hkv <= 16 && (rows == 1 || rows * hkv * max_pages <= 8192);  // page-heads of 8 KiB: 64 MB
+  if (hkv > 16 || rows > kMaxRows) return false;
+  const double pairs = (double)(rows * hkv);
+  return rows == 1 || pairs * (double)max_pages <= 8192.0 * pow(pairs > 32 ? pairs / 32 : 1.0, 0.58);
 }
 // And a prompt step: the ordinary launch has one block sweep a row's pages for each of its tiles, 0.33 us a page, so only
 // where all rows together are short (3 prompts of up to 17 tokens over 304, 60 pages: 16.7 / 11.4; 2 of up to 20 over 1024, 132
