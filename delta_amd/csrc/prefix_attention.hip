@@ -891,10 +891,12 @@ bool decode_alone(int64_t rows, int hkv, int64_t max_pages) {
   const double pairs = (double)(rows * hkv);
   return rows == 1 || pairs * (double)max_pages <= 8192.0 * pow(pairs > 32 ? pairs / 32 : 1.0, 0.58);
 }
-// And a prompt step: the ordinary launch has one block sweep a row's pages for each of its tiles, 0.33 us a page, so only
-// where all rows together are short (3 prompts of up to 17 tokens over 304, 60 pages: 16.7 / 11.4; 2 of up to 20 over 1024, 132
-// pages: 17.4 / 26.7).
-bool prefill_alone(int64_t pages) { return pages <= 64; }
+// And a prompt step: the ordinary launch has one block sweep a row's pages for each of its tiles, 6 us and 0.3 a page whatever the
+// number of rows, the launches here take 15-40 us whatever the pages.  The host knows the rows' pages in all only, so a single row
+// of up to 32, several of up to 64 together (us here / ordinary, 8 kv heads of 4, 7 new tokens: one row of 30 pages 15.4 / 14.6, of
+// 40 15.6 / 17.0, of 62 15.8 / 24.2; 2 rows of 31 16.4 / 14.6, 3 of 21 18.1 / 12.3, 4 of 16 19.3 / 9.8; past 64 two rows of 46 15.7 /
+// 19.4, but 32 of 20 31.1 / 11.3: who knows that the longest row is that short takes delta_paged_prefill).
+bool prefill_alone(int64_t pages, int batch) { return pages <= (batch == 1 ? 32 : 64); }
 
 size_t prefix_workspace_bytes(int64_t tokens, int hq, int hkv, int64_t max_pages) {
   const size_t n = workspace_bytes_for(tokens, hq, hkv, plan_blocks(tokens, hkv, max_pages, kSlots));
@@ -1039,7 +1041,7 @@ extern "C" DELTA_EXPORT int delta_paged_prefill_prefix(
                                      num_kv_heads, head_dim, dtype, kv_indices_len > 1 ? kv_indices_len : 1, workspace,
                                      workspace_bytes, who);
   if (rc != DELTA_OK || batch <= 0 || num_tokens <= 0) return rc;
-  if (delta::prefill_alone(kv_indices_len) && !((uintptr_t)o & 7u) && o_stride_t % 4 == 0 && o_stride_h % 4 == 0)
+  if (delta::prefill_alone(kv_indices_len, batch) && !((uintptr_t)o & 7u) && o_stride_t % 4 == 0 && o_stride_h % 4 == 0)
     return delta_paged_prefill(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices,
                                kv_indices_len, kv_last_page_len, o, o_stride_t, o_stride_h, lse, batch, num_qo_heads,
                                num_kv_heads, head_dim, dtype, sm_scale, max_qo_len, stream);

@@ -394,10 +394,10 @@ def _call_on(dev: torch.device, name: str, *args) -> None:
 
 
 def _prefix_call(name: str, q, kv_cache, B: int, tables: tuple, prefix: tuple, out, lse, workspace, max_pages: int,
-                 sm_scale: Optional[float], tail: tuple) -> torch.Tensor:
+                 sm_scale: Optional[float], tail: tuple, alone: Optional[int] = None) -> torch.Tensor:
     """What the two attention calls over shared prefixes have in common: checks, outputs, workspace, the call.
     ``tables`` are the row tables in the entry point's order, the page indices next to last; ``tail`` the arguments
-    between the batch and the head counts."""
+    between the batch and the head counts.  ``alone``: max_qo_len of prompts that the ordinary launch attends faster."""
     indices, row_prefix, p_indptr, p_indices = tables[-2], *prefix
     dev = _check_cuda(q, kv_cache, *tables, *prefix, out, lse, workspace)
     _check_cache(kv_cache)
@@ -411,6 +411,13 @@ def _prefix_call(name: str, q, kv_cache, B: int, tables: tuple, prefix: tuple, o
         raise ValueError("out must match q's shape/dtype with unit inner stride")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
         raise ValueError(f"lse must be contiguous fp32 [{q.shape[0]}, {hq}]")
+    scale = _DEFAULT_SCALE if sm_scale is None else float(sm_scale)
+    if alone is not None and out.data_ptr() % 8 == 0 and out.stride(0) % 4 == 0 and out.stride(1) % 4 == 0:
+        _call_on(dev, "delta_paged_prefill_rows", q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(),
+                 kv_cache.shape[0], *[t.data_ptr() for t in tables[:-1]], indices.numel(), tables[-1].data_ptr(),
+                 out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), B, hq, hkv, HEAD_DIM, _DTYPES[q.dtype], scale,
+                 alone, q.shape[0], 0, 0, 0, None, 0)
+        return out
     need = prefix_attention_workspace_bytes(q.shape[0], hq, hkv, max_pages)
     if workspace is None:  # of this call: safe on any stream, in any capture
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -421,8 +428,7 @@ def _prefix_call(name: str, q, kv_cache, B: int, tables: tuple, prefix: tuple, o
     _call_on(dev, name, ctypes.byref(px), q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), kv_cache.shape[0],
              *[t.data_ptr() for t in tables[:-1]], indices.numel(), tables[-1].data_ptr(), out.data_ptr(), out.stride(0),
              out.stride(1), _ptr(lse), B, *tail[0], hq, hkv, HEAD_DIM, _DTYPES[q.dtype],
-             _DEFAULT_SCALE if sm_scale is None else float(sm_scale), *tail[1], workspace.data_ptr(),
-             workspace.numel() * workspace.element_size())
+             scale, *tail[1], workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return out
 
 
@@ -446,18 +452,22 @@ def paged_decode_prefix(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torc
 def paged_prefill_prefix(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor,
                          kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, row_prefix: torch.Tensor,
                          prefix_indptr: torch.Tensor, prefix_indices: torch.Tensor, *, max_qo_len: int,
-                         sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-                         lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         max_pages_per_row: Optional[int] = None, sm_scale: Optional[float] = None,
+                         out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``paged_prefill`` for prompts that continue shared prefixes (``delta_paged_prefill_prefix``); q/out
     [nnz, Hq, 128], the prefixes as in ``paged_decode_prefix``.
 
     A row's prefix applies where it ends before the row's query tokens.  ``max_qo_len`` is at least the longest row's
     count of them, as for ``paged_prefill``, which is as fast or faster where the rows bring several hundred tokens each
-    (sharing spares reads, not products).  ``out`` and ``lse`` of tokens behind the last row are left as they were."""
+    (sharing spares reads, not products).  ``max_pages_per_row``, where the caller knows it, is the most pages of a row: up
+    to 40 the ordinary launch attends the rows (32 rows of 20 pages 11 us, shared 31).  ``out`` and ``lse`` of tokens behind
+    the last row are left as they were."""
     _check_i32("qo_indptr", qo_indptr, 1)
     return _prefix_call("delta_paged_prefill_prefix", q, kv_cache, qo_indptr.numel() - 1,
                         (qo_indptr, kv_indptr, kv_indices, kv_last_page_len), (row_prefix, prefix_indptr, prefix_indices),
-                        out, lse, workspace, kv_indices.numel(), sm_scale, ((q.shape[0], int(max_qo_len)), ()))
+                        out, lse, workspace, kv_indices.numel(), sm_scale, ((q.shape[0], int(max_qo_len)), ()),
+                        int(max_qo_len) if max_pages_per_row is not None and max_pages_per_row <= 40 else None)
 
 
 def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, *,

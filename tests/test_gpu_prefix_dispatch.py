@@ -39,3 +39,31 @@ def test_decode_past_the_line_is_shared(rows, heads, prefix):
         got = b.decode(max_pages_per_row=planned)
         b.check(got, b.want())
         assert torch.equal(got[0], b.decode(max_pages_per_row=8192)[0])
+
+
+def test_prompts_of_short_rows_run_on_the_ordinary_launch():
+    """Where the caller says how long the rows are; the same results where it does not, and where the rows are longer or out
+    only fits the shared launch."""
+    b = Batch(32, 8, [18], [(0, 3 + i % 9, 1 + i % 3) for i in range(32)] + [(-1, 30, 20), (-2, 0, 4)], seed=3)
+    t, most = exact_tables(b)
+    assert most <= 40 and t["kv_indices"].numel() > 64
+    want = b.want()
+    got = b.prefill(max_pages_per_row=most)
+    b.check(got, want)
+    ordinary = K.paged_prefill(b.q, b.cache, i32(b.qo), t["kv_indptr"], t["kv_indices"], t["last"], max_qo_len=20)
+    assert torch.equal(got[0], ordinary)
+    shared = b.prefill()
+    b.check(shared, want)
+    far = b.prefill(max_pages_per_row=41)
+    assert torch.equal(far[0], shared[0]) and torch.equal(far[1], shared[1])
+    wide = torch.full((b.q.shape[0], 33 * D + 2), 2.0, dtype=torch.bfloat16, device=DEV)
+    o = torch.as_strided(wide, b.q.shape, (33 * D + 2, D, 1), 2)
+    assert torch.equal(b.prefill(max_pages_per_row=most, out=o)[0], shared[0])
+    assert (wide[:, :2] == 2).all() and (wide[:, 2 + 32 * D:] == 2).all()
+
+
+@pytest.mark.parametrize("rows,pages", [(1, 32), (1, 33), (3, 21), (4, 16), (5, 13)])
+def test_few_pages_in_all_on_either_side_of_the_line(rows, pages):
+    b = Batch(12, 2, [pages - 1], [(0, 5 + i, 5) for i in range(rows)], seed=rows)
+    exact_tables(b)
+    b.check(b.prefill(), b.want())
