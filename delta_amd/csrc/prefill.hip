@@ -101,6 +101,7 @@ struct PrefillArgs {
   float *lse;
   int batch, hq, hkv;
   int64_t num_tokens;     // query tokens of all rows, -1: not known
+  int token_limit;        // no row's tokens reach past it
   int decode_rows;        // rows of one query token, their pages (for the choice of the blocks only)
   int64_t decode_pages;
   int skip_single;  // rows of one query token are run_decode_rows'
@@ -115,7 +116,10 @@ struct RowBounds {
 };
 __device__ __forceinline__ RowBounds row_bounds(const PrefillArgs &a, int r) {
   if (r >= a.batch) return RowBounds{0, 0, 0, 0, 0};
-  return RowBounds{a.qo_indptr[r], a.qo_indptr[r + 1], a.kv_indptr[r], a.kv_indptr[r + 1], a.last_page_len[r]};
+  RowBounds x{a.qo_indptr[r], a.qo_indptr[r + 1], a.kv_indptr[r], a.kv_indptr[r + 1], a.last_page_len[r]};
+  x.q0 = min(max(x.q0, 0), a.token_limit);
+  x.q1 = min(max(x.q1, 0), a.token_limit);
+  return x;
 }
 __device__ __forceinline__ RowBounds bounds_of_lane(const RowBounds &x, int l) {
   return RowBounds{__builtin_amdgcn_readlane(x.q0, l), __builtin_amdgcn_readlane(x.q1, l),
@@ -619,6 +623,7 @@ int run_prefill(const void *q, int64_t q_stride_t, int64_t q_stride_h, const voi
   a.hkv = num_kv_heads;
   a.sm_scale = sm_scale;
   a.num_tokens = num_tokens;
+  a.token_limit = num_tokens >= 0 && num_tokens < INT32_MAX ? (int)num_tokens : INT32_MAX;
   a.decode_rows = decode_rows;
   a.decode_pages = decode_pages;
   a.skip_single = workspace != nullptr;

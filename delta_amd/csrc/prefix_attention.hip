@@ -1042,9 +1042,10 @@ extern "C" DELTA_EXPORT int delta_paged_prefill_prefix(
                                      workspace_bytes, who);
   if (rc != DELTA_OK || batch <= 0 || num_tokens <= 0) return rc;
   if (delta::prefill_alone(kv_indices_len, batch) && !((uintptr_t)o & 7u) && o_stride_t % 4 == 0 && o_stride_h % 4 == 0)
-    return delta_paged_prefill(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices,
-                               kv_indices_len, kv_last_page_len, o, o_stride_t, o_stride_h, lse, batch, num_qo_heads,
-                               num_kv_heads, head_dim, dtype, sm_scale, max_qo_len, stream);
+    return delta_paged_prefill_rows(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices,
+                                    kv_indices_len, kv_last_page_len, o, o_stride_t, o_stride_h, lse, batch, num_qo_heads,
+                                    num_kv_heads, head_dim, dtype, sm_scale, max_qo_len, num_tokens, 0, 0, 0, nullptr, 0,
+                                    stream);
   return delta::run_prefix(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices,
                            kv_indices_len, kv_last_page_len, prefix, o, o_stride_t, o_stride_h, lse, batch, num_tokens,
                            num_qo_heads, num_kv_heads, dtype, sm_scale, kv_indices_len > 1 ? kv_indices_len : 1, workspace, stream,

@@ -67,3 +67,23 @@ def test_few_pages_in_all_on_either_side_of_the_line(rows, pages):
     b = Batch(12, 2, [pages - 1], [(0, 5 + i, 5) for i in range(rows)], seed=rows)
     exact_tables(b)
     b.check(b.prefill(), b.want())
+
+
+@pytest.mark.parametrize("hint", [None, 40])
+def test_short_prompts_whose_bounds_leave_the_tokens_write_nothing_out_of_place(hint):
+    """As on the shared launch: a table that does not fit q ends at its first and last token."""
+    b = Batch(12, 2, [9, 4], [(0, 20, 3), (1, 33, 30), (0, 50, 1), (-1, 60, 20)], seed=49)
+    t, most = exact_tables(b)
+    assert t["kv_indices"].numel() <= 64
+    room, lse = torch.full((400, 12, D), 3.0, dtype=torch.bfloat16, device=DEV), torch.full((400, 12), 4.0, device=DEV)
+    want = b.want()
+    for qo in ([0, 3, 33, 34, 154], [-100, 3, 33, 34, 54], [0, 3, 33, 34, 54]):
+        room.fill_(3.0)
+        lse.fill_(4.0)
+        K.paged_prefill_prefix(b.q, b.cache, i32(qo), t["kv_indptr"], t["kv_indices"], t["last"], t["row_prefix"],
+                               t["prefix_indptr"], t["prefix_indices"], max_qo_len=160, max_pages_per_row=hint,
+                               out=room[160:214], lse=lse[160:214])
+        torch.cuda.synchronize()
+        for x, v in ((room, 3), (lse, 4)):
+            assert (x[:160] == v).all() and (x[214:] == v).all()
+    b.check((room[160:214], lse[160:214]), want)
