@@ -13,8 +13,10 @@
 // pairs, in that order, are cut into tiles of 128, its pages into stages of 32 tokens.  The stages of
 // all tiles of a kv head form one line, kTileCost more per tile for what a tile costs besides them, and
 // block i of the head's `blocks` takes the i-th equal share of it: so the chip's block slots (two per CU)
-// finish together whatever the lengths are (to +-8 %), and a tile is cut only where a share ends.  The lengths are only on
-// the device: every block derives the same line from the tables (build_line, 1.7-2.0 us).
+// finish about together whatever the lengths are (8-13 % apart in the large cases), and a tile is cut only where a share ends.
+// Only a long prompt's own tokens are shared out badly: a tile is charged its row's whole length, of which its causal mask leaves
+// the first ones little (one prompt of 8000 tokens beside 31 decoding rows over 4800: 899 us, the ordinary launch 555).  The
+// lengths are only on the device: every block derives the same line from the tables (build_line, 1.7-2.0 us).
 //   A whole tile of a row without a prefix writes o and lse.  Any other one writes un-normalised partials
 // (m, l, a): a whole tile at its token's place, a cut one into its block's two buffers (a block's first piece may
 // end a cut tile, its last may begin one); the merge kernel joins them per (token, q head).  No atomics: the same call
@@ -27,11 +29,11 @@
 // The S of a stage are computed under the softmax of the stage before.  Tiles of up to 64 pairs (a decode row's own pages
 // have G) have 16 to a wave, on 16x16 MFMA tiles.
 //
-// What bounds it.  Decode reads: 128 rows of 1050 own tokens over a prefix of 16384, 8 kv heads of 5: 632 MB in 148 us, 4.3
-// TB/s (97 us at the 6.5 TB/s of a bare read; the ordinary launch, which reads the prefix for every row, 752); 32 rows of 530
+// What bounds it.  Decode reads: 128 rows of 1050 own tokens over a prefix of 16384, 8 kv heads of 5: 632 MB in 144 us, 4.4
+// TB/s (97 us at the 6.5 TB/s of a bare read; the ordinary launch, which reads the prefix for every row, 754); 32 rows of 530
 // over 8192: 33 us against 17 and 101; the line, the pieces' beginnings (2-4 us each) and the merge (6 us with its launch) are
-// the rest.  Prompts compute: 32 prompts of 34 tokens over 8192, 8 kv heads of 4: 196 us, 0.70 PFLOP/s, 1.0 in the loop
-// (1.06 us a stage of two blocks; 116 us at the 1.19 of an 8192^3 product; the ordinary launch 217).  In the loop no single
+// the rest.  Prompts compute: 32 prompts of 34 tokens over 8192, 8 kv heads of 4: 199 us, 0.69 PFLOP/s, 1.0 in the loop
+// (1.06 us a stage of two blocks; 116 us at the 1.19 of an 8192^3 product; the ordinary launch 216).  In the loop no single
 // unit is the bound: without the exponentials it would take 95 % of its time, without V's fragments 94, without K's 97,
 // without any of them 84.
 #include "delta_common.h"
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_kernel(PrefixArg
   const int total = uniform(build_line<G>(a, line));
   int share = uniform(div_up(total, a.blocks));
   share = share < kMinShare ? kMinShare : share;
-  int pos = blk * share;  // (total < 2^30: checked on the host)
+  int pos = blk * share;  // (total <= 2^30: build_line)
   const int end = min(total, pos + share);
 
   // Loads: K and V rows go straight to LDS, 1 KiB (4 rows of this head) per load.  16-byte chunk ch of K row r sits at

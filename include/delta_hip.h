@@ -556,7 +556,10 @@ size_t delta_prefix_attention_workspace_bytes(int64_t tokens, int num_qo_heads, 
  * rounding: the softmax is summed in another order), with each prefix's K and V read once
  * for all its rows instead of once per row.  Row b's prefix applies where its pages fit in
  * the row (16 * pages <= kv_len_b); a row it does not fit attends its own CSR alone, and so
- * does every row of a batch too small for sharing to pay.  max_pages_per_row is the planned
+ * does every row of a batch too small for sharing to pay: one row, or at most 8192 * (pairs /
+ * 32)^0.58 planned page-heads (pairs = batch * kv heads, 32 at least; page-heads = pairs *
+ * max_pages_per_row).  How much the rows share is on the device: a caller whose rows share
+ * less than that is better served by delta_paged_decode.  max_pages_per_row is the planned
  * maximum of the rows' pages (a longer row is still covered whole).  batch <= 1024.  No
  * counterpart in the reference. */
 int delta_paged_decode_prefix(const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_b,
@@ -572,7 +575,9 @@ int delta_paged_decode_prefix(const delta_shared_prefix_t *prefix, const void *q
  * rows of qo_indptr, causal.  A row's prefix applies where it lies in front of the row's
  * query tokens (16 * pages <= kv_len_b - qo_len_b).  max_qo_len >= every row's query
  * tokens, as for delta_paged_prefill.  o and lse of tokens behind the last row are left as
- * they were.  batch <= 1024.  (Here and above: a row whose bounds do not ascend is an empty
+ * they were.  batch <= 1024.  Calls of at most 64 pages in all (one row: 32) run on the
+ * ordinary launch; a caller who knows that no row has more than 40 pages is better served by
+ * delta_paged_prefill.  (Here and above: a row whose bounds do not ascend is an empty
  * one; qo_indptr has to ascend, or o and lse of the rows' tokens are unspecified.) */
 int delta_paged_prefill_prefix(const delta_shared_prefix_t *prefix, const void *q, int64_t q_stride_t,
                                int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
