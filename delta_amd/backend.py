@@ -637,7 +637,8 @@ class LMBackend:
         if rows is None:
             rows = {s: self.scheduler.request_in(s).pages for s in self.scheduler.occupied()}
         row_prefix, prefixes = shared_prefixes(rows)
-        on = self._sharing_pays(prefixes, row_prefix, self.batch_size)
+        shares = not self.enable_selective_cache or "full" in self.layer_roles  # (planner and subset layers never do)
+        on = shares and self._sharing_pays(prefixes, row_prefix, self.batch_size)
         if on and self.prefix_workspace is None:
             cfg = self.model.config
             try:

@@ -442,7 +442,8 @@ def paged_decode_prefix(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torc
 
     ``row_prefix`` (int32 [B]) names each row's prefix, -1 for none; prefix p's full pages are
     ``prefix_indices[prefix_indptr[p]:prefix_indptr[p + 1]]``, and the rows' CSR lists them too, first.  A row that
-    its prefix does not fit in attends its own CSR alone.  At most 1024 rows and prefixes.  ``workspace``
+    its prefix does not fit in attends its own CSR alone, and so do all rows of a small batch (``decode_alone`` in
+    csrc/prefix_attention.hip).  At most 1024 rows and prefixes.  ``workspace``
     (``prefix_attention_workspace_bytes``) is allocated for the call where none is given."""
     return _prefix_call("delta_paged_decode_prefix", q, kv_cache, q.shape[0], (kv_indptr, kv_indices, kv_last_page_len),
                         (row_prefix, prefix_indptr, prefix_indices), out, lse, workspace, int(max_pages_per_row), sm_scale,

@@ -34,6 +34,7 @@ def host_engine(monkeypatch):
         e.page_selector = SimpleNamespace(paged_kv_indptr=None, paged_kv_indices=None, paged_kv_last_page_len=None)
         e.enable_delta_impl_profile = e.throughput_mode = e.is_main_process = False
         e.tokenizer, e._step = None, None
+        e.enable_selective_cache, e.layer_roles = False, ["full"] * 4
         e.seen = []
 
         def forward(i):
@@ -230,3 +231,16 @@ def test_crossing_the_line_keeps_both_captured_steps(host_engine):
     assert e._decode_graph is None
     e._update_sharing(sharers)
     assert e._decode_graph is None
+
+
+@pytest.mark.parametrize("selective,roles,on", [
+    (False, ["plan", "subset"], True),  # every layer attends everything
+    (True, ["full", "plan", "subset"], True),
+    (True, ["plan", "subset", "subset"], False),
+])
+def test_decode_steps_without_a_layer_that_shares_are_captured_once(host_engine, selective, roles, on):
+    """Planner and subset layers keep their launches: with no other, sharing changes nothing but the captures."""
+    e = host_engine()
+    e.enable_selective_cache, e.layer_roles = selective, roles
+    e._update_sharing({s: list(range(300)) + [300 + s] for s in range(16)})
+    assert e._sharing == on
