@@ -67,7 +67,8 @@ def sharing_pays_from(rows: int, hkv: int, max_pages: int) -> float:
     32 rows of 2: +8 at 8.2 k, +2 at 12 k, +1 at 16 k, -3 at 25 k; rows whose own parts are long and ragged gain earlier, by
     1-6 us).  Where the ordinary launch cuts the rows of 256 pairs or more into units (a large ``max_pages``) sharing gains
     from the start (64 rows of 8 over 9000 tokens' pages: -8 to -74 at 8.6 k).  Below 64 pairs the plan of the ordinary launch
-    decides (32 pairs at 9 k: +6 where a slot holds 337 pages, +2 with 563, 0 with 751, -8 with 1251): 8192 for all."""
+    decides (32 pairs at 9 k: +6 where a slot holds 337 pages, +2 with 563, 0 with 751, -8 with 1251): 8192 for all.
+    ``decode_alone`` in csrc/prefix_attention.hip draws the same line for all that rows may read."""
     pairs = rows * hkv
     if pairs >= 256 and K.decode_num_splits(rows, hkv, max_pages) > 1:
         return SHARING_PAYS

@@ -894,7 +894,7 @@ bool decode_alone(int64_t rows, int hkv, int64_t max_pages) {
   return rows == 1 || pairs * (double)max_pages <= 8192.0 * pow(pairs > 32 ? pairs / 32 : 1.0, 0.58);
 }
 // And a prompt step: the ordinary launch has one block sweep a row's pages for each of its tiles, 6 us and 0.3 a page whatever the
-// number of rows, the launches here take 15-40 us whatever the pages.  The host knows the rows' pages in all only, so a single row
+// number of rows, the launches here take 15-50 us whatever the pages.  The host knows the rows' pages in all only, so a single row
 // of up to 32, several of up to 64 together (us here / ordinary, 8 kv heads of 4, 7 new tokens: one row of 30 pages 15.4 / 14.6, of
 // 40 15.6 / 17.0, of 62 15.8 / 24.2; 2 rows of 31 16.4 / 14.6, 3 of 21 18.1 / 12.3, 4 of 16 19.3 / 9.8; past 64 two rows of 46 15.7 /
 // 19.4, but 32 of 20 31.1 / 11.3: who knows that the longest row is that short takes delta_paged_prefill).

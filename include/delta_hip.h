@@ -214,8 +214,8 @@ int delta_paged_prefill(const void *q, int64_t q_stride_t, int64_t q_stride_h,
                         float sm_scale, int max_qo_len, delta_stream_t stream);
 
 /* delta_paged_prefill with what the caller knows of the step; the same o and lse.
- *   num_tokens        query tokens of all rows (>= qo_indptr[batch]): it bounds the grid, and no bound of qo_indptr is
- *                     followed past it
+ *   num_tokens        query tokens of all rows (>= qo_indptr[batch]): it bounds the grid, and without a workspace no
+ *                     bound of qo_indptr is followed past it
  *   decode_rows       rows of exactly one query token, decode_pages their pages in total, decode_max_pages
  *                     those of the longest one (for the launch plan: no result depends on them)
  *   workspace         NULL, or delta_paged_prefill_rows_workspace_bytes bytes, 256-byte aligned: the rows
