@@ -81,11 +81,12 @@ def prompt_step_us(qo_lens: List[int], kv_lens: List[int], spared: int, group: i
 
     Ordinary: rows of one new token are read at about 10 TB/s (page-heads of 8 KiB, mostly from caches where rows share); the
     others' products run at 2.1 G (pair, token)s per ms, pairs padded to blocks of 128 on ``32 // group * 4`` tokens, but a
-    block sweeps its row's pages at 0.33 us each.  Shared: 1.75 G over whole tiles, a page-head per 1.5 ns, and about 20-28 us
+    block sweeps its row's pages at 0.33 us each.  Shared: 1.75 G over whole tiles, a page-head per 1.5 ns, and about 16-28 us
     of beginnings and merge.  Over 195 steps that spare 64 MB or more (8 kv heads of 4, 4 of 7, 2 of 6; 8-64 rows of 1-250 new
     tokens over prefixes of 50-1000 pages, alone or beside prompts of 1100-8000) taking the lower estimate costs over 3 % in
-    2 (us 51 / 44, 49 / 43) and misses a gain of over 3 % in 16 (most with 7 q heads per kv head, whose tokens fill the
-    ordinary launch's last round badly); sharing in all of them was over 3 % slower in 108, up to twice the time.  E.g. us
+    2 (us 51 / 44, 49 / 43) and misses a gain of over 3 % in 15 (most with 7 q heads per kv head, whose tokens fill the
+    ordinary launch's last round badly); sharing in all of them was over 3 % slower in 108, up to twice the time.  Of 96 drawn
+    steps, groups of 1-8, it makes none slower, misses 4; sharing all was slower in 11.  E.g. us
     shared / ordinary, 8 kv heads of 4: 31 decoding rows over 300 pages 25 / 59, beside a prompt of 2000 tokens 101 / 112, of
     4000 264 / 200, of 8000 899 / 555; 64 prompts of 20 tokens over 400 pages 191 / 194, of 60 475 / 398, of 120 913 / 763;
     8 of 60 86 / 140."""
@@ -100,7 +101,7 @@ def prompt_step_us(qo_lens: List[int], kv_lens: List[int], spared: int, group: i
             sweep = max(sweep, 6 + 0.33 * n / PAGE_SIZE)
     ordinary = max(ordinary / 2.1e6, sweep) + (12 + 0.65e-3 * single if single else 0)
     read = (sum(-(-n // PAGE_SIZE) for n in kv_lens) - spared) * hkv
-    shared = max(shared / 1.75e6, 1.5e-3 * read) + 20 + 0.15 * len(qo_lens) + (8 if sweep else 0)
+    shared = max(shared / 1.75e6, 1.5e-3 * read) + 16 + 0.15 * len(qo_lens) + (12 if sweep else 0)
     return shared, ordinary
 
 
