@@ -44,6 +44,27 @@ class SharedPrefixC(ctypes.Structure):
 
 
 _SP = ctypes.POINTER(SharedPrefixC)
+
+
+class RotaryC(ctypes.Structure):
+    """``delta_rotary_t``: the pairs' turns per position, what of the head they cover and in which layout."""
+    _fields_ = [("turns", c_void_p), ("rotary_dim", c_int), ("interleaved", c_int), ("factor", c_float)]
+
+
+class HeadNormC(ctypes.Structure):
+    """``delta_head_norm_t``: the RMS norm of each head of q and k."""
+    _fields_ = [("q_weight", c_void_p), ("k_weight", c_void_p), ("eps", c_float)]
+
+
+class ScoreRuleC(ctypes.Structure):
+    """``delta_score_rule_t``: what attention does to a score, and the keys a token sees."""
+    _fields_ = [("softcap", c_float), ("slopes", c_void_p), ("window", c_int), ("kv_begin", c_void_p),
+                ("kv_end", c_void_p)]
+
+
+_RO = ctypes.POINTER(RotaryC)
+_HN = ctypes.POINTER(HeadNormC)
+_SR = ctypes.POINTER(ScoreRuleC)
 # name -> (restype, argtypes); one entry per function declared in include/delta_hip.h
 SIGNATURES = {
     "delta_last_error": (ctypes.c_char_p, []),
@@ -132,6 +153,20 @@ SIGNATURES = {
         c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, c_size_t, _P]),
     "delta_paged_prefill_prefix": (c_int, [
         _SP, _P, c_int64, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int64, _P,
+        c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
+    "delta_qk_norm_rope": (c_int, [
+        _RO, _HN, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int, c_int, c_int, c_int, c_int,
+        c_int, _P]),
+    "delta_qk_norm_rope_append": (c_int, [
+        _RO, _HN, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, c_int64, _P, _P,
+        c_int, c_int, c_int, c_int, c_int, c_int, _P]),
+    "delta_paged_decode_rule_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "delta_paged_decode_rule": (c_int, [
+        _SR, _P, c_int64, c_int64, _P, c_int64, _P, _P, c_int64, _P, _P, c_int64, c_int64, _P,
+        c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, c_size_t, _P]),
+    "delta_paged_prefill_rule_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int]),
+    "delta_paged_prefill_rule": (c_int, [
+        _SR, _P, c_int64, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int64, _P,
         c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
     "delta_copy_pages": (c_int, [
         ctypes.POINTER(_P), c_int, c_int64, c_int, c_int, c_int, _P, _P, _P, c_int64, _P]),

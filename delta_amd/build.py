@@ -21,7 +21,7 @@ LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["capi.hip", "paged_decode.hip", "page_score.hip", "page_select.hip",
            "page_metadata.hip", "kv_rope.hip", "step_utils.hip",
            "skinny_gemm.hip", "rows_gemm.hip", "prefill.hip",
-           "prefix_attention.hip", "page_copy.hip"]
+           "prefix_attention.hip", "page_copy.hip", "norm_rope.hip", "rule_prefill.hip"]
 
 COMPILE_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",

@@ -32,6 +32,7 @@
 #include <type_traits>
 
 #include "delta_common.h"
+#include "score_rule.h"
 
 namespace delta {
 
@@ -94,6 +95,7 @@ struct DecodeArgs {
   // largest softmax probability over the head's G q heads, [batch][hkv][tokmax_stride_h].
   float *tokmax;
   int64_t tokmax_stride_b, tokmax_stride_h;
+  RuleArgs rule;  // RULE launches
 };
 
 struct RowInfo {
@@ -101,8 +103,13 @@ struct RowInfo {
   int np;
   int kv_len;
   int last;  // last_page_len clamped to [0, 16]
+  int lo;    // RULE: the first page's tokens in front of the row's first key
+  int qpos;  // RULE: the query's position, counted as kv_len is
 };
 
+// RULE: the row as the pages from its first key's to its last key's, positions counted from the first of them; no
+// key at all is an empty row.
+template <bool RULE = false>
 __device__ __forceinline__ RowInfo row_info(const DecodeArgs &a, int b) {
   const int64_t ilen = a.kv_indices_len;
   int64_t p0 = a.kv_indptr[b];
@@ -116,6 +123,17 @@ __device__ __forceinline__ RowInfo row_info(const DecodeArgs &a, int b) {
   r.np = (int)(p1 - p0);
   r.kv_len = r.np > 0 ? (r.np - 1) * kPageSize + last : 0;
   r.last = last;
+  if constexpr (RULE) {
+    int lo, hi;
+    key_range(a.rule, b, r.kv_len - 1, r.kv_len, &lo, &hi);
+    const int page0 = lo / kPageSize;
+    r.np = hi > lo ? (hi + kPageSize - 1) / kPageSize - page0 : 0;
+    r.p0 = r.np > 0 ? p0 + page0 : p0;
+    r.qpos = r.kv_len - 1 - page0 * kPageSize;
+    r.lo = lo % kPageSize;
+    r.kv_len = r.np > 0 ? hi - page0 * kPageSize : 0;
+    r.last = r.np > 0 ? r.kv_len - (r.np - 1) * kPageSize : 0;
+  }
   return r;
 }
 
@@ -155,10 +173,10 @@ typedef __attribute__((address_space(3))) s4_t lds_s4_t;
 // nsplit) of them (its last unit takes any pages past units * chunk, so a row longer than the
 // planned maximum is still covered), numbered row by row.
 // (ROWS: a row of another token count has one unit, which exits; the others as many as their pages need.)
-template <bool ROWS = false>
+template <bool ROWS = false, bool RULE = false>
 __device__ __forceinline__ int units_of(const DecodeArgs &a, int b) {
   if (ROWS && a.q_rows[b + 1] - a.q_rows[b] != 1) return 1;
-  const RowInfo r = row_info(a, b);
+  const RowInfo r = row_info<RULE>(a, b);
   const int n = (r.np + a.chunk - 1) / a.chunk;
   return n < 1 ? 1 : (!ROWS && n > a.nsplit ? a.nsplit : n);
 }
@@ -182,6 +200,7 @@ __device__ __forceinline__ int64_t part_slot(const DecodeArgs &a, int b, int64_t
 // key per row, (pages << 9) | (511 - row), and keeps every row's bounds in LDS, so the chosen
 // row's come from there.  `lds` holds 5 B + 1 ints; the block's waves leave in step, so the LDS
 // is free afterwards.  Returns the row; *ri gets its bounds.
+template <bool RULE = false>
 __device__ int balanced_row(const DecodeArgs &a, int y, int *lds, RowInfo *ri) {
   const int B = a.batch;
   int64_t *p0 = reinterpret_cast<int64_t *>(lds);  // [B] (the dynamic LDS starts 16-byte aligned)
@@ -191,7 +210,7 @@ __device__ int balanced_row(const DecodeArgs &a, int y, int *lds, RowInfo *ri) {
   int *win = lds + 5 * B;
   if (threadIdx.x == 0) *win = y;  // replaced by the ranking below (kept in range regardless)
   for (int r = threadIdx.x; r < B; r += blockDim.x) {
-    const RowInfo x = row_info(a, r);
+    const RowInfo x = row_info<RULE>(a, r);
     // Distinct keys (the row in the low bits); page counts past 2^21 - 1 rank as equal.
     key[r] = ((x.np < (1 << 21) ? x.np : (1 << 21) - 1) << 9) | (511 - r);
     np[r] = x.np;
@@ -218,6 +237,7 @@ __device__ int balanced_row(const DecodeArgs &a, int y, int *lds, RowInfo *ri) {
   x.np = np[b];
   x.last = last[b];
   x.kv_len = x.np > 0 ? (x.np - 1) * kPageSize + x.last : 0;
+  if constexpr (RULE) x = row_info<true>(a, b);  // its range too
   *ri = x;
   __syncthreads();
   return b;
@@ -229,12 +249,12 @@ __device__ int balanced_row(const DecodeArgs &a, int y, int *lds, RowInfo *ri) {
 // the plan), row b at F + b, F = the number of full units.  Blocks start in grid order, so the
 // short last units of a ragged batch fill the launch's tail instead of whole units of the last
 // rows.  A running inclusive scan over 64 rows at a time; false past the last unit.
-template <bool ROWS = false>
+template <bool ROWS = false, bool RULE = false>
 __device__ __forceinline__ bool find_unit(const DecodeArgs &a, int u, int lane, int *row, int *split, int *nu) {
   int base = 0;
   for (int r0 = 0; r0 < a.batch; r0 += 64) {
     const int r = r0 + lane;
-    const int n = r < a.batch ? units_of<ROWS>(a, r) - 1 : 0;  // full units of row r
+    const int n = r < a.batch ? units_of<ROWS, RULE>(a, r) - 1 : 0;  // full units of row r
     int incl = n;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -256,7 +276,7 @@ __device__ __forceinline__ bool find_unit(const DecodeArgs &a, int u, int lane, 
   const int b = u - base;  // the last units, one per row
   if (b >= a.batch) return false;
   *row = b;
-  *nu = units_of<ROWS>(a, b);
+  *nu = units_of<ROWS, RULE>(a, b);
   *split = *nu - 1;
   return true;
 }
@@ -331,12 +351,13 @@ __device__ __forceinline__ void part_store(float *p, float v) {
 }
 
 template <int DT, int G, bool WITH_V, bool WITH_DUMP, bool ROPE, bool TOKMAX = false, bool AGENT_PARTS = false,
-          bool ROWS = false>
+          bool ROWS = false, bool RULE = false>
 __device__ __forceinline__ void decode_split_body(const DecodeArgs &a, float *smem) {
   // No FMA contraction: every instantiation (with or without the dump) rounds the softmax
   // arguments identically, so P -- rounded to the KV dtype for the P.V MFMA -- is the same.
 #pragma clang fp contract(off)
   static_assert(!TOKMAX || (!WITH_DUMP && (WITH_V || !ROPE)), "TOKMAX: the K-only scorer or the on-chip planner");
+  static_assert(!RULE || (WITH_V && !WITH_DUMP && !ROPE && !TOKMAX && !ROWS), "RULE: plain attention launches");
   constexpr bool REGV = TOKMAX && WITH_V;  // P.V with V in registers (no V tiles)
   using E = Elem<DT>;
   using M16 = Mfma16<DT>;
@@ -374,22 +395,22 @@ __device__ __forceinline__ void decode_split_body(const DecodeArgs &a, float *sm
         b = uniform(unit / a.nsplit);
         split = uniform(unit - b * a.nsplit);
       }
-      ri = row_info(a, b);
+      ri = row_info<RULE>(a, b);
       nu = (ri.np + a.chunk - 1) / a.chunk;
       nu = nu < 1 ? 1 : (nu > a.nsplit ? a.nsplit : nu);
       if (split >= nu) return;  // whole block
     } else {
-      if (!find_unit<ROWS>(a, unit, lane, &b, &split, &nu)) return;  // past the last unit: whole block
-      ri = row_info(a, b);
+      if (!find_unit<ROWS, RULE>(a, unit, lane, &b, &split, &nu)) return;  // past the last unit: whole block
+      ri = row_info<RULE>(a, b);
     }
     j0 = split * a.chunk;
     j1 = split == nu - 1 ? ri.np : min(ri.np, j0 + a.chunk);
   } else {
     if (a.bal_w > 0) {
-      b = balanced_row(a, blockIdx.y, reinterpret_cast<int *>(smem), &ri);
+      b = balanced_row<RULE>(a, blockIdx.y, reinterpret_cast<int *>(smem), &ri);
     } else {
       b = blockIdx.y;
-      ri = row_info(a, b);
+      ri = row_info<RULE>(a, b);
     }
     j1 = ri.np;
   }
@@ -468,6 +489,7 @@ __device__ __forceinline__ void decode_split_body(const DecodeArgs &a, float *sm
   for (int n = 0; n < 8; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const float sm_scale = a.sm_scale;
+  const float slope = RULE && a.rule.slopes && t < G ? a.rule.slopes[h * G + t] : 0.f;
   const int first = j0 + rslot;
   const int count = first < j1 ? (j1 - first + R - 1) / R : 0;
 
@@ -605,7 +627,8 @@ __device__ __forceinline__ void decode_split_body(const DecodeArgs &a, float *sm
       const int vlim = ok ? ri.kv_len - j * kPageSize : 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t keep = 4 * i + c < vlim ? 0xffffffffu : 0u;
+        const bool in = 4 * i + c < vlim && (!RULE || j > 0 || 4 * i + c >= ri.lo);
+        const uint32_t keep = in ? 0xffffffffu : 0u;
         const u32x4 w = vr[i] & u32x4{keep, keep, keep, keep};
         const int trow = 8 * (i & 1) + 4 * (c >> 1) + 2 * (i >> 1) + (c & 1);
         st128(vt + trow * kVStride + 8 * t, w);
@@ -634,6 +657,18 @@ __device__ __forceinline__ void decode_split_body(const DecodeArgs &a, float *sm
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       x[r] = (ok && tok0 + 8 * (r >> 1) + (r & 1) < ri.kv_len) ? S[r] * sm_scale : -INFINITY;
+    if constexpr (RULE) {
+      // The rule's scores, each of its parts for the whole launch or not at all.
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = S[r] * sm_scale;
+      if (a.rule.softcap > 0.f) cap_scores(x, a.rule, 1.f, 1.f);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tok = tok0 + 8 * (r >> 1) + (r & 1);
+        if (a.rule.slopes) x[r] = fmaf(-slope, fabsf((float)(ri.qpos - tok)), x[r]);
+        if (!ok || tok >= ri.kv_len || tok < ri.lo) x[r] = -INFINITY;
+      }
+    }
     const int slot = gi % kDumpSlots;
     if (TOKMAX && t < G && j < a.dump_pages) {
       float *dl = smem + tokmax_lds_header<G>() + (j * G + t) * kPageSize + 2 * c;
@@ -959,11 +994,11 @@ __device__ __forceinline__ void decode_split_body(const DecodeArgs &a, float *sm
     const int hq = hh * G + g;
     if (a.nsplit == 1) {
       if (WITH_V) {
-        const float ov = L > 0.f ? A / L : 0.f;
+        const float ov = (RULE ? L != 0.f : L > 0.f) ? A / L : 0.f;  // (RULE: NaN scores stay NaN)
         a.o[(int64_t)b * a.o_stride_b + (int64_t)hq * a.o_stride_h + dd] = (uint16_t)E::from_float(ov);
       }
       if (dd == 0 && a.lse != nullptr)
-        a.lse[(int64_t)b * a.hq + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+        a.lse[(int64_t)b * a.hq + hq] = (RULE ? L != 0.f : L > 0.f) ? (M + log2f(L)) * kLn2 : -INFINITY;
       if (TOKMAX) smem[tokmax_lds_header<G>() - 16 + g] = L > 0.f ? M + log2f(L) : -INFINITY;
     } else {
       const int64_t pidx = ((int64_t)pslot * a.hkv + hh) * G + g;
@@ -1001,6 +1036,12 @@ __global__ void __launch_bounds__(kMaxWaves * 64) paged_decode_subset_kernel(Dec
   extern __shared__ float smem[];
   decode_split_body<DT, G, true, false, ROPE, false, true>(a, smem);
 }
+// Attention under a score rule (score_rule.h).
+template <int DT, int G>
+__global__ void __launch_bounds__(kMaxWaves * 64) paged_decode_rule_kernel(DecodeArgs a) {
+  extern __shared__ float smem[];
+  decode_split_body<DT, G, true, false, false, false, true, false, true>(a, smem);
+}
 template <int DT, int G, bool ROPE>
 __global__ void __launch_bounds__(kMaxWaves * 64) paged_decode_plan_kernel(DecodeArgs a) {
   extern __shared__ float smem[];
@@ -1032,7 +1073,7 @@ __global__ void __launch_bounds__(kMaxWaves * 64) paged_decode_plan_tokmax_kerne
 // sit at (row, split), so each group's first batch issues its loads with the row bounds, not
 // after them (splits the row does not have weigh nothing).  ROWS: the slots follow from the row bounds;
 // past the row's units its last one's slot is read.
-template <int DT, bool ROWS>
+template <int DT, bool ROWS, bool RULE = false>
 __global__ void __launch_bounds__(kMergeGroups * kHeadDim) decode_merge_kernel(DecodeArgs a, int G) {
   using E = Elem<DT>;
   __shared__ float s_m[kMergeGroups], s_l[kMergeGroups], s_a[kMergeGroups][kHeadDim];
@@ -1047,7 +1088,7 @@ __global__ void __launch_bounds__(kMergeGroups * kHeadDim) decode_merge_kernel(D
     orow = a.q_rows[b];
     if (a.q_rows[b + 1] - orow != 1) return;  // whole block
   }
-  const int nu = units_of<ROWS>(a, b);
+  const int nu = units_of<ROWS, RULE>(a, b);
   const int64_t first_page = ROWS ? row_info(a, b).p0 : 0;
   const int64_t stride = (int64_t)a.hkv * G;  // partial rows per slot
   // Batches of 16 splits whose loads all issue together (weight 0 past the row's last split;
@@ -1104,8 +1145,9 @@ __global__ void __launch_bounds__(kMergeGroups * kHeadDim) decode_merge_kernel(D
     }
     M = MM;
   }
-  a.o[(int64_t)orow * a.o_stride_b + (int64_t)hq * a.o_stride_h + dd] = (uint16_t)E::from_float(L > 0.f ? A / L : 0.f);
-  if (dd == 0 && a.lse != nullptr) a.lse[(int64_t)orow * a.hq + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+  const bool some = RULE ? L != 0.f : L > 0.f;  // (RULE: NaN scores stay NaN)
+  a.o[(int64_t)orow * a.o_stride_b + (int64_t)hq * a.o_stride_h + dd] = (uint16_t)E::from_float(some ? A / L : 0.f);
+  if (dd == 0 && a.lse != nullptr) a.lse[(int64_t)orow * a.hq + hq] = some ? (M + log2f(L)) * kLn2 : -INFINITY;
 }
 
 // lse-only merge (scorer path without V): one 64-lane wave per (row, q head), lanes over units.
@@ -1136,7 +1178,7 @@ __global__ void __launch_bounds__(256) decode_merge_lse_kernel(DecodeArgs a, int
   if (lane == 0) a.lse[idx] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
 }
 
-enum Mode { kAttn = 0, kAttnDump = 1, kScoreOnly = 2, kAttnSubset = 3, kScoreTokmax = 4, kAttnTokmax = 5 };
+enum Mode { kAttn = 0, kAttnDump = 1, kScoreOnly = 2, kAttnSubset = 3, kScoreTokmax = 4, kAttnTokmax = 5, kAttnRule = 6 };
 
 template <int DT, int G>
 void launch_split(const DecodeArgs &a, int waves, int mode, hipStream_t stream) {
@@ -1173,6 +1215,9 @@ void launch_split(const DecodeArgs &a, int waves, int mode, hipStream_t stream) 
         hipLaunchKernelGGL((paged_decode_subset_kernel<DT, G, true>), grid, block, lds(sm_attn), stream, a);
       else
         hipLaunchKernelGGL((paged_decode_subset_kernel<DT, G, false>), grid, block, lds(sm_attn), stream, a);
+      break;
+    case kAttnRule:
+      hipLaunchKernelGGL((paged_decode_rule_kernel<DT, G>), grid, block, lds(sm_attn), stream, a);
       break;
     case kAttnDump:
       if (rope)
@@ -1378,14 +1423,14 @@ size_t decode_workspace_bytes(int batch, int hq, int nsplit, bool with_acc) {
 }
 
 // Shared validation + launch used by the attention and the scorer entry points.
-int run_decode(const void *q, int64_t q_stride_b, int64_t q_stride_h, const void *kv_cache,
-               int64_t num_pages, const int32_t *kv_indptr, const int32_t *kv_indices,
-               int64_t kv_indices_len, const int32_t *kv_last_page_len, void *o,
-               int64_t o_stride_b, int64_t o_stride_h, float *lse, float *dump,
-               int64_t dump_stride_b, int64_t dump_stride_h, int batch, int hq, int hkv,
-               int head_dim, int dtype, float sm_scale, int max_pages, int mode,
-               void *workspace, size_t workspace_bytes, hipStream_t stream, const char *who,
-               const delta_decode_append_t *ap) {
+static int run_decode_any(const void *q, int64_t q_stride_b, int64_t q_stride_h, const void *kv_cache,
+                          int64_t num_pages, const int32_t *kv_indptr, const int32_t *kv_indices,
+                          int64_t kv_indices_len, const int32_t *kv_last_page_len, void *o,
+                          int64_t o_stride_b, int64_t o_stride_h, float *lse, float *dump,
+                          int64_t dump_stride_b, int64_t dump_stride_h, int batch, int hq, int hkv,
+                          int head_dim, int dtype, float sm_scale, int max_pages, int mode,
+                          void *workspace, size_t workspace_bytes, hipStream_t stream, const char *who,
+                          const delta_decode_append_t *ap, const RuleArgs *rule) {
   clear_error();
   if (batch <= 0) return DELTA_OK;
   if (head_dim != kHeadDim) return set_error(DELTA_ERR_INVALID, "%s: head_dim must be 128 (got %d)", who, head_dim);
@@ -1470,6 +1515,7 @@ int run_decode(const void *q, int64_t q_stride_b, int64_t q_stride_h, const void
   a.offsets = a.ap_indptr = a.ap_indices = nullptr;
   a.ap_indices_len = 0;
   a.rcp_scale = a.log2_theta = a.smooth_a = a.smooth_b = 0.f;
+  a.rule = rule ? *rule : RuleArgs{};
   if (ap) {
     if (mode == kScoreOnly || mode == kScoreTokmax)
       return set_error(DELTA_ERR_INVALID, "%s: the scorer takes no append", who);
@@ -1521,7 +1567,14 @@ int run_decode(const void *q, int64_t q_stride_b, int64_t q_stride_h, const void
     launch_split_g<DELTA_FP16>(a, G, waves, mode, stream);
   int rc = check_launch(who);
   if (rc || a.nsplit == 1) return rc;
-  if (with_acc) {
+  if (with_acc && mode == kAttnRule) {
+    if (dtype == DELTA_BF16)
+      hipLaunchKernelGGL((decode_merge_kernel<DELTA_BF16, false, true>), dim3(batch * hq),
+                         dim3(kHeadDim * merge_groups(a.nsplit)), 0, stream, a, G);
+    else
+      hipLaunchKernelGGL((decode_merge_kernel<DELTA_FP16, false, true>), dim3(batch * hq),
+                         dim3(kHeadDim * merge_groups(a.nsplit)), 0, stream, a, G);
+  } else if (with_acc) {
     if (dtype == DELTA_BF16)
       hipLaunchKernelGGL((decode_merge_kernel<DELTA_BF16, false>), dim3(batch * hq), dim3(kHeadDim * merge_groups(a.nsplit)), 0,
                          stream, a, G);
@@ -1533,6 +1586,20 @@ int run_decode(const void *q, int64_t q_stride_b, int64_t q_stride_h, const void
     hipLaunchKernelGGL(decode_merge_lse_kernel, dim3((n + 3) / 4), dim3(256), 0, stream, a, G);
   }
   return check_launch(who);
+}
+
+int run_decode(const void *q, int64_t q_stride_b, int64_t q_stride_h, const void *kv_cache,
+               int64_t num_pages, const int32_t *kv_indptr, const int32_t *kv_indices,
+               int64_t kv_indices_len, const int32_t *kv_last_page_len, void *o,
+               int64_t o_stride_b, int64_t o_stride_h, float *lse, float *dump,
+               int64_t dump_stride_b, int64_t dump_stride_h, int batch, int hq, int hkv,
+               int head_dim, int dtype, float sm_scale, int max_pages, int mode,
+               void *workspace, size_t workspace_bytes, hipStream_t stream, const char *who,
+               const delta_decode_append_t *ap) {
+  return run_decode_any(q, q_stride_b, q_stride_h, kv_cache, num_pages, kv_indptr, kv_indices, kv_indices_len,
+                        kv_last_page_len, o, o_stride_b, o_stride_h, lse, dump, dump_stride_b, dump_stride_h, batch, hq,
+                        hkv, head_dim, dtype, sm_scale, max_pages, mode, workspace, workspace_bytes, stream, who, ap,
+                        nullptr);
 }
 
 // The rows of exactly one query token of a prompt step (delta_paged_prefill_rows): decode attention of
@@ -1648,6 +1715,33 @@ extern "C" DELTA_EXPORT int delta_paged_decode(const void *q, int64_t q_stride_b
                            dump_stride_h, batch, num_qo_heads, num_kv_heads, head_dim, dtype, sm_scale,
                            max_pages_per_row, mode, workspace, workspace_bytes, (hipStream_t)stream,
                            "delta_paged_decode", nullptr);
+}
+
+extern "C" DELTA_EXPORT size_t delta_paged_decode_rule_workspace_bytes(int batch, int num_qo_heads, int num_kv_heads,
+                                                                       int max_pages_per_row, int window) {
+  if (batch <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0) return 0;
+  const int pages = delta::rule_pages(window, max_pages_per_row);
+  return delta_paged_decode_workspace_bytes(batch, num_qo_heads, num_kv_heads, pages > 0 ? pages : 1);
+}
+
+extern "C" DELTA_EXPORT int delta_paged_decode_rule(const delta_score_rule_t *rule, const void *q, int64_t q_stride_b,
+                                                    int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+                                                    const int32_t *kv_indptr, const int32_t *kv_indices,
+                                                    int64_t kv_indices_len, const int32_t *kv_last_page_len, void *o,
+                                                    int64_t o_stride_b, int64_t o_stride_h, float *lse, int batch,
+                                                    int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
+                                                    float sm_scale, int max_pages_per_row, void *workspace,
+                                                    size_t workspace_bytes, delta_stream_t stream) {
+  const char *who = "delta_paged_decode_rule";
+  delta::clear_error();
+  if (batch <= 0) return DELTA_OK;
+  delta::RuleArgs r;
+  const int rc = delta::rule_args(rule, &r, who);
+  if (rc) return rc;
+  return delta::run_decode_any(q, q_stride_b, q_stride_h, kv_cache, num_pages, kv_indptr, kv_indices, kv_indices_len,
+                               kv_last_page_len, o, o_stride_b, o_stride_h, lse, nullptr, 0, 0, batch, num_qo_heads,
+                               num_kv_heads, head_dim, dtype, sm_scale, delta::rule_pages(r.window, max_pages_per_row),
+                               delta::kAttnRule, workspace, workspace_bytes, (hipStream_t)stream, who, nullptr, &r);
 }
 
 extern "C" DELTA_EXPORT int delta_paged_decode_subset(const void *q, int64_t q_stride_b, int64_t q_stride_h,

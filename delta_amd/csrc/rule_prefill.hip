@@ -1,0 +1,711 @@
+// Attention of several new tokens a row over the paged cache under a score rule (score_rule.h): scores capped by a tanh, a
+// bias that falls with the distance, and of each query token's keys a range [lo, hi) only (causal, a window, packed
+// documents, a prefix seen as a whole).  The cache already holds the new tokens; query i of row b sits at position
+// kv_len_b - qo_len_b + i.
+//
+// Work decomposition, on the 32x32 MFMA tiles of the causal prompt kernel (prefill.hip): a block is PW waves of one (row, kv
+// head) and a run of query tokens; each wave owns 32 query rows, the (token, q head) pairs of TW = 32 / G tokens, with its q
+// in registers.  The block sweeps the keys that any of its tokens sees, 64 at a time from the first one's step to the last
+// one's; K and V go from global memory straight to LDS.  Per wave and step S^T = K Q^T, the rule on the scores in registers,
+// the online softmax, O^T += V^T P^T.  Steps that all the wave's rows see whole take no masks, steps that none of them sees
+// are left out.
+//
+// Few tokens over a long cache are too few blocks: the tile's steps are cut into parts, each a block of its own that writes
+// its sums (acc, m, l) to the workspace, and a second launch joins them.  How many parts is a matter of all rows' lengths,
+// which only the device knows: every block adds up the call's work W (tiles x steps) and cuts rows that are longer than
+// 1.5 C steps into parts of about C = W hkv / kTargetBlocks, at least kMinSteps.  So a decode row beside short prompts is
+// cut, and equal long prompts are not.
+//
+// A key that a mask leaves out has no part in the result, whatever it holds.  Its score is replaced and its p is 0, but 0
+// times a V of infinity or NaN is NaN in the product of the whole tile, so a row that ends with sums that are not finite is
+// summed again key by key over its own keys alone (slow_row): nothing for finite caches.
+#include "delta_common.h"
+#include "mfma32.h"
+#include "score_rule.h"
+
+namespace delta {
+namespace {
+
+constexpr int kSub = 2;                // 32-token sub-tiles per step
+constexpr int kKvStep = 32 * kSub;     // keys per step
+constexpr int kPgStep = kKvStep / 16;  // pages per step
+constexpr int kTileB = kKvStep * 256;  // bytes of a step's K (or V) tile: 64 rows of 256 bytes
+constexpr int kTargetBlocks = 512;     // two 4-wave blocks for each CU
+constexpr int kMinSteps = 8;           // a part's steps, at least
+constexpr int kMaxParts = 1024;
+constexpr int kSplitWaves = 4;         // waves of a block where rows may be cut
+
+struct RulePrefillArgs {
+  const uint16_t *q;
+  int64_t q_stride_t, q_stride_h;
+  const uint16_t *kv;
+  int64_t num_pages;
+  const int32_t *qo_indptr, *kv_indptr, *kv_indices;
+  int64_t kv_indices_len;
+  const int32_t *last_page_len;
+  uint16_t *o;
+  int64_t o_stride_t, o_stride_h;
+  float *lse;
+  int batch, hq, hkv, G;
+  int token_limit;  // query tokens of all rows
+  int row_tiles;    // the most tiles a row has (of max_qo_len tokens)
+  int max_cut;      // units of cut rows that the workspace holds, 0: no row is cut
+  float sm_scale;
+  RuleArgs rule;
+  float2 *part_ml;  // [unit][hkv][wave][32 rows]
+  f32x4 *part_acc;  // [unit][hkv][wave][16][64 lanes], the accumulators as the lanes hold them
+};
+
+struct RowBounds {
+  int q0, q1, p0, np, kv_len;
+};
+__device__ __forceinline__ RowBounds row_bounds(const RulePrefillArgs &a, int r) {
+  if (r >= a.batch) return RowBounds{0, 0, 0, 0, 0};
+  RowBounds x;
+  x.q0 = min(max(a.qo_indptr[r], 0), a.token_limit);
+  x.q1 = min(max(a.qo_indptr[r + 1], 0), a.token_limit);
+  const int64_t ilen = a.kv_indices_len;
+  int64_t p0 = a.kv_indptr[r], p1 = a.kv_indptr[r + 1];
+  p0 = p0 < 0 ? 0 : (p0 > ilen ? ilen : p0);
+  p1 = p1 < p0 ? p0 : (p1 > ilen ? ilen : p1);
+  int lp = a.last_page_len[r];
+  lp = lp < 0 ? 0 : (lp > kPageSize ? kPageSize : lp);
+  x.p0 = (int)p0;
+  x.np = (int)(p1 - p0);
+  x.kv_len = x.np > 0 ? (x.np - 1) * kPageSize + lp : 0;
+  return x;
+}
+__device__ __forceinline__ RowBounds bounds_of_lane(const RowBounds &x, int l) {
+  return RowBounds{__builtin_amdgcn_readlane(x.q0, l), __builtin_amdgcn_readlane(x.q1, l),
+                   __builtin_amdgcn_readlane(x.p0, l), __builtin_amdgcn_readlane(x.np, l),
+                   __builtin_amdgcn_readlane(x.kv_len, l)};
+}
+
+// One block's work: part `part` of `parts` of a row's tile.
+struct Unit {
+  RowBounds row;
+  int tile, part, parts;
+};
+
+// Unit u of a kv head, the cut rows' first (their parts, tile by tile), then the others' tiles row by row, a row's last
+// tile first (in a causal row it sees the most keys); false past the last one.
+__device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int u, int lane, Unit *unit) {
+  auto tiles_of = [&](const RowBounds &x) {
+    const int qn = x.q1 - x.q0;
+    return qn <= 0 ? 0 : min((qn + BT - 1) / BT, a.row_tiles);
+  };
+  auto steps_of = [&](const RowBounds &x) {  // of one tile, at most
+    const int span = a.rule.window > 0 && a.rule.window < x.kv_len - BT ? a.rule.window + BT : x.kv_len;
+    return (span + kKvStep - 1) / kKvStep;
+  };
+  int C = 0;
+  if (a.max_cut > 0) {
+    float w = 0.f;  // (an estimate; every block of the launch gets the same one)
+    for (int r0 = 0; r0 < a.batch; r0 += 64) {
+      const RowBounds x = row_bounds(a, r0 + lane);
+      w += (float)tiles_of(x) * (float)steps_of(x);
+    }
+    for (int off = 32; off > 0; off >>= 1) w += shfl_xor(w, off);
+    w = w * (float)a.hkv * (1.f / kTargetBlocks);
+    C = w < (float)kMinSteps ? kMinSteps : w > 1e8f ? 100000000 : (int)w + 1;
+    C = uniform(C);
+  }
+  auto parts_of = [&](const RowBounds &x) {
+    const int s = steps_of(x);
+    return C > 0 && s > C + C / 2 ? min((s + C - 1) / C, kMaxParts) : 1;
+  };
+  int base = 0;
+  for (int pass = C > 0 ? 0 : 1; pass < 2; ++pass) {
+    for (int r0 = 0; r0 < a.batch; r0 += 64) {
+      const RowBounds mine = row_bounds(a, r0 + lane);
+      const int parts = parts_of(mine);
+      const int n = (parts > 1) == (pass == 0) ? tiles_of(mine) * parts : 0;
+      int incl = n;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += v;
+      }
+      const uint64_t m = __ballot(base + incl > u);
+      if (m != 0) {
+        const int l = __builtin_ctzll(m);
+        unit->row = bounds_of_lane(mine, l);
+        unit->parts = __builtin_amdgcn_readlane(parts, l);
+        const int at = base + __builtin_amdgcn_readlane(incl, l) - 1 - u;  // from the row's last unit
+        unit->tile = at / unit->parts;
+        unit->part = unit->parts - 1 - (at - unit->tile * unit->parts);
+        return true;
+      }
+      base += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  return false;
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+  for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
+  return uniform(v);
+}
+__device__ __forceinline__ int wave_max(int v) {
+  for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
+  return uniform(v);
+}
+
+template <int DT, int PW>
+__global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePrefillArgs a) {
+#pragma clang fp contract(off)
+  using E = Elem<DT>;
+  using MF = Mfma32<DT>;
+  constexpr bool kLate = PW == 8;   // the second wave of each SIMD runs half a step behind
+  constexpr int kBufs = kLate ? 4 : 2;
+  constexpr int kPgWave = 16 / PW;  // pages a wave loads rows of, per step
+  __shared__ __attribute__((aligned(1024))) char tiles[kBufs][2 * kTileB];
+
+  const int G = a.G, TW = 32 / G, BT = PW * TW;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int hl = lane >> 5, n = lane & 31;
+  const int h = blockIdx.x;
+  const int u = (int)(blockIdx.z * gridDim.y + blockIdx.y);
+  Unit un;
+  if (!find_unit(a, BT, u, lane, &un)) return;  // whole block
+  const int64_t q0 = un.row.q0;
+  const int qn = un.row.q1 - un.row.q0, np = un.row.np, kv_len = un.row.kv_len;
+  const int btok0 = un.tile * BT;
+  const int tok0 = __builtin_amdgcn_readfirstlane(btok0 + wave * TW);
+
+  // This lane's query row n = (token tt, head g) and its keys [lo, hi).
+  const int tt = n / G, g = n - tt * G;
+  const bool row_ok = n < TW * G && tok0 + tt < qn;
+  const int qpos = kv_len - qn + tok0 + tt;
+  u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
+  if (row_ok) {
+    // With a negative scale q's signs are flipped (the scale below is then positive).  The xor also makes the loads
+    // complete here, before the kv loop.
+    const uint32_t flip = a.sm_scale < 0.f ? 0x80008000u : 0u;
+    const uint16_t *qp = a.q + (q0 + tok0 + tt) * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = ld128(qp + 16 * ks) ^ u32x4{flip, flip, flip, flip};
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = u32x4{0u, 0u, 0u, 0u};
+  }
+  int lo = 0, hi = 0;
+  if (row_ok) {
+    key_range(a.rule, q0 + tok0 + tt, qpos, kv_len, &lo, &hi);
+    if (hi <= lo) lo = hi = 0;
+  }
+  // The wave's rows together: the first and last key any of them sees, and the keys that all of them see.
+  const int any0 = wave_min(hi > lo ? lo : INT32_MAX), any1 = wave_max(hi);
+  const int all0 = wave_max(row_ok ? lo : 0), all1 = wave_min(row_ok ? hi : INT32_MAX);
+  // The block's tokens together.
+  int blo = INT32_MAX, bhi = 0;
+  for (int t0 = btok0; t0 < min(btok0 + BT, qn); t0 += 64) {
+    const int tk = t0 + lane;
+    if (tk < min(btok0 + BT, qn)) {
+      int l2, h2;
+      key_range(a.rule, q0 + tk, kv_len - qn + tk, kv_len, &l2, &h2);
+      if (h2 > l2) {
+        blo = min(blo, l2);
+        bhi = max(bhi, h2);
+      }
+    }
+  }
+  blo = wave_min(blo);
+  bhi = wave_max(bhi);
+  // The block's steps [s0, s1) (its part of them) and the wave's.
+  int s0 = 0, s1 = 0;
+  if (bhi > blo) {
+    s0 = blo / kKvStep;
+    s1 = (bhi + kKvStep - 1) / kKvStep;
+    if (un.parts > 1) {
+      const int per = (s1 - s0 + un.parts - 1) / un.parts;
+      s0 += un.part * per;
+      s1 = min(s1, s0 + per);
+    }
+  }
+  const int w0 = any1 > 0 ? max(s0, any0 / kKvStep) : 0, w1 = any1 > 0 ? min(s1, (any1 + kKvStep - 1) / kKvStep) : 0;
+
+  // Step loads (as in prefill.hip): 1 KiB a load, 4 rows of this head; 16-byte chunk ch of K row r at slot ch ^ (r % 16),
+  // of V row r at ch ^ 4 (r % 4).
+  const uint32_t row_bytes = (uint32_t)a.hkv * kHeadDim * 2;
+  const uint32_t page_bytes = 2 * kPageSize * row_bytes;
+  const int wv = uniform((int)(threadIdx.x >> 6));
+  const int lrow = lane >> 4, lch = lane & 15;
+  const uint32_t koff = (4 * (wv & 3) + lrow) * row_bytes + 16 * (lch ^ (4 * (wv & 3) + lrow));
+  const uint32_t voff = (kPageSize + 4 * (wv & 3) + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&tiles[0][0] + wv * 1024;
+  const char *const kvh = reinterpret_cast<const char *>(a.kv) + (int64_t)h * (kHeadDim * 2);
+  const int32_t *const row_ids = a.kv_indices + un.row.p0;
+  auto page_bad = [&](int pid) { return pid < 0 || (int64_t)pid >= a.num_pages; };
+  // Ids outside the cache are looked for once over the part's pages; steps of a row without any take its ids as they are.
+  bool row_bad = false;
+  for (int i = s0 * kPgStep; i < s1 * kPgStep && i < np; i += 64)
+    row_bad |= __ballot(i + lane < np && i + lane < s1 * kPgStep && page_bad(row_ids[i + lane < np ? i + lane : 0])) != 0;
+  auto bad_of = [&](int j) {  // bit i: page i of step j lies outside the cache
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < kPgStep; ++i) {
+      const int pg = kPgStep * j + i;
+      r |= (pg < np && page_bad(ld_scalar(row_ids, pg < np ? pg : np - 1)) ? 1u : 0u) << i;
+    }
+    return r;
+  };
+  const uint32_t last_pg = (uint32_t)(np - 1);  // (steps exist only where pages do)
+  uint32_t id[kPgWave];                         // of the step issued next; pages past the row repeat its last one
+  auto load_ids = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < kPgWave; ++i) {
+      const uint32_t pg = (uint32_t)(kPgStep * j + i * (PW / 4) + (wv >> 2));
+      id[i] = (uint32_t)ld_scalar(row_ids, pg < last_pg ? pg : last_pg);
+    }
+  };
+  auto issue = [&](int j, int i) {
+    const uint32_t dst = lds0 + (uint32_t)(j % kBufs) * (2 * kTileB) + i * (PW / 4) * 4096;
+    const uint32_t pid = row_bad && page_bad((int)id[i]) ? 0u : id[i];
+    const char *pg = kvh + (uint64_t)pid * page_bytes;
+    load_lds_1k(dst, pg, koff);
+    load_lds_1k(dst + kTileB, pg, voff);
+  };
+  auto issue_step = [&](int j) {  // step j's loads, then the ids of step j + 1
+#pragma unroll
+    for (int i = 0; i < kPgWave; ++i) issue(j, i);
+    load_ids(j + 1);
+  };
+  if (s0 < s1) {
+    load_ids(s0);
+    issue_step(s0);
+    if (kLate && s0 + 1 < s1) issue_step(s0 + 1);
+  }
+  uint32_t bad = 0;  // bad_of(j)
+
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+  const float scale = fabsf(a.sm_scale), scale2 = scale * kLog2e;
+  const bool capped = a.rule.softcap > 0.f, leaning = a.rule.slopes != nullptr;
+  // Scores that the rule changes leave it in log2 units; others keep the scale for the exponent's fma.
+  const bool scaled = capped || leaning || scale2 == 0.f;
+  const float xs = scaled ? 1.f : scale2;
+  const float slope2 = leaning && row_ok ? a.rule.slopes[h * G + g] * kLog2e : 0.f;
+  uint32_t kfo[8];  // K fragment of k-slice ks: row 32 sb + n, chunk 2 ks + hl
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) kfo[ks] = (uint32_t)(n * 256 + 16 * ((2 * ks + hl) ^ (n & 15)));
+  const int q16 = lane >> 4, t16 = lane & 15;
+  uint32_t vfo[4];  // transposed V reads
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+    vfo[dt] = (uint32_t)(kTileB + (4 * hl + (t16 >> 2)) * 256 +
+                         16 * ((4 * dt + 2 * (q16 & 1) + ((t16 & 3) >> 1)) ^ (4 * (t16 >> 2))) + 8 * (t16 & 1));
+
+  // One step for the wave: S^T = K Q^T, the rule, the online softmax and P^T packed into pc.
+  auto score_step = [&](int j, const char *tk, u32x4 (&pc)[2 * kSub]) {
+    f32x16 S[kSub];
+#pragma unroll
+    for (int sb = 0; sb < kSub; ++sb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[sb][i] = 0.f;
+    auto kfrag = [&](int sb, int ks) { return *reinterpret_cast<const u32x4 *>(tk + kfo[ks] + sb * 8192); };
+    u32x4 kq[4][kSub];  // three k-slices ahead of the MFMAs; the fences keep the reads from sinking to their uses
+#pragma unroll
+    for (int s = 0; s < 3; ++s)
+#pragma unroll
+      for (int sb = 0; sb < kSub; ++sb) kq[s][sb] = kfrag(sb, s);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      if (ks + 3 < 8) {
+#pragma unroll
+        for (int sb = 0; sb < kSub; ++sb) kq[(ks + 3) % 4][sb] = kfrag(sb, ks + 3);
+      }
+#pragma unroll
+      for (int sb = 0; sb < kSub; ++sb) S[sb] = MF::run(kq[ks % 4][sb], qf[ks], S[sb]);
+      if (!kLate && ks < kPgWave && j + 1 < s1) issue(j + 1, ks);  // the next step's loads go out under the MFMAs
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!kLate && j + 1 < s1) load_ids(j + 2);
+    __builtin_amdgcn_s_setprio(0);
+    const int kv0 = j * kKvStep;
+    const bool full = kv0 >= all0 && kv0 + kKvStep <= all1 && bad == 0;
+    constexpr int NX = 16 * kSub;
+    float x[NX];
+#pragma unroll
+    for (int i = 0; i < NX; ++i) x[i] = S[i >> 4][i & 15];
+    auto key = [&](int i) { return 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3); };  // + kv0 + 4 hl
+    if (capped) {
+      cap_scores(x, a.rule, scale, kLog2e);
+    } else if (scaled) {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) x[i] *= scale2;
+    }
+    if (leaning) {
+      const float d0 = (float)(qpos - kv0 - 4 * hl);
+#pragma unroll
+      for (int i = 0; i < NX; ++i) x[i] = fmaf(-slope2, fabsf(d0 - (float)key(i)), x[i]);
+    }
+    float pm = -INFINITY;
+    if (!full) {
+      const int l0 = lo - kv0 - 4 * hl, h0 = hi - kv0 - 4 * hl;
+#pragma unroll
+      for (int i = 0; i < NX; ++i)
+        x[i] = key(i) >= l0 && key(i) < h0 && ((bad >> (2 * (i >> 4) + ((i & 15) >> 3))) & 1u) == 0 ? x[i] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < NX; ++i) pm = fmaxf(pm, x[i]);
+    // m is the row's reference maximum: it moves only when a score exceeds it by more than 8 (a factor of 2^8).
+    const float smax = halves_max(pm) * xs;
+    float alpha = 1.f;
+    if (smax > m + 8.f) {  // also the first finite score of the row (m = -inf)
+      alpha = fast_exp2(m - smax);
+      m = smax;
+    }
+    const float nm = m == -INFINITY ? 0.f : -m;
+    float ps = 0.f;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      x[i] = fast_exp2(fmaf(x[i], xs, nm));
+      ps += x[i];
+    }
+    l = l * alpha + ps;  // this half's keys; the halves are summed once at the end
+    if (__ballot(alpha != 1.f)) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+    }
+#pragma unroll
+    for (int cc = 0; cc < 2 * kSub; ++cc)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) pc[cc][w] = pack2<DT>(x[8 * cc + 2 * w], x[8 * cc + 2 * w + 1]);
+  };
+  // O^T += V^T P^T of a step whose P^T is in pc.
+  auto pv_step = [&](const char *tk, const u32x4 (&pc)[2 * kSub]) {
+    auto vfrag = [&](int i) {  // V^T fragment of chunk i / 4, d tile i % 4
+      const char *rd = tk + vfo[i % 4] + (i / 4) * 4096;
+      const ps4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)rd);
+      const ps4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ps4_t *)(rd + 2048));
+      u32x4 va;
+      va[0] = (uint32_t)(uint16_t)v0[0] | ((uint32_t)(uint16_t)v0[1] << 16);
+      va[1] = (uint32_t)(uint16_t)v0[2] | ((uint32_t)(uint16_t)v0[3] << 16);
+      va[2] = (uint32_t)(uint16_t)v1[0] | ((uint32_t)(uint16_t)v1[1] << 16);
+      va[3] = (uint32_t)(uint16_t)v1[2] | ((uint32_t)(uint16_t)v1[3] << 16);
+      return va;
+    };
+    constexpr int kAhead = 4;  // fragments read ahead of their MFMAs
+    u32x4 vq[kAhead + 1];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) vq[i] = vfrag(i);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < 8 * kSub; ++i) {
+      if (i + kAhead < 8 * kSub) vq[(i + kAhead) % (kAhead + 1)] = vfrag(i + kAhead);
+      acc[i % 4] = MF::run(vq[i % (kAhead + 1)], pc[i / 4], acc[i % 4]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  const bool late = kLate && wave >= PW / 2;
+  u32x4 pcar[2 * kSub];
+  for (int j = s0; s0 < s1 && j < s1 + (kLate ? 1 : 0); ++j) {
+    // Step j's loads have landed when at most the next step's (kLate: four) are pending.
+    if (kLate && j + 1 < s1)
+      wait_loads<2 * kPgWave>();
+    else
+      wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (row_bad) bad = j < s1 ? bad_of(j) : 0u;
+    if (j < s1 && (j * kKvStep < blo || (j + 1) * kKvStep > bhi || bad != 0)) {
+      // V rows that no token of the block sees, and of pages outside the cache, meet p = 0 but may hold NaN/Inf: zeros.
+      constexpr int kTpr = PW;  // threads per row
+      const int r = (int)threadIdx.x / kTpr, at = j * kKvStep + r;
+      if (at < blo || at >= bhi || ((bad >> (r >> 4)) & 1u)) {
+        char *vr = &tiles[j % kBufs][kTileB + r * 256 + 256 / kTpr * ((int)threadIdx.x % kTpr)];
+#pragma unroll
+        for (int i = 0; i < 16 / kTpr; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
+    const bool mine = j >= w0 && j < w1;
+    if (kLate ? j + 2 < s1 : !mine && j + 1 < s1) issue_step(kLate ? j + 2 : j + 1);
+    if (late) {
+      if (j - 1 >= w0 && j - 1 < w1) pv_step(&tiles[(j - 1) % kBufs][0], pcar);
+      if (mine) score_step(j, &tiles[j % kBufs][0], pcar);
+    } else if (mine) {
+      u32x4 pc[2 * kSub];
+      score_step(j, &tiles[j % kBufs][0], pc);
+      pv_step(&tiles[j % kBufs][0], pc);
+    }
+  }
+
+  l = halves_sum(l);
+  // Rows whose sums are not finite though their scores are: slow_row's.
+  bool odd = false;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) odd |= !(fabsf(acc[dt][i]) < INFINITY);
+  const uint64_t om = __ballot(odd && row_ok && l < INFINITY);
+  const uint32_t odd_rows = (uint32_t)om | (uint32_t)(om >> 32);
+  const bool sums_ok = ((odd_rows >> n) & 1u) == 0;
+  const int64_t pslot = ((int64_t)u * a.hkv + h) * PW + wave;  // (cut rows: u < a.max_cut)
+  if (un.parts > 1 && u >= a.max_cut) return;
+  uint16_t *const orow = a.o + (q0 + tok0 + tt) * a.o_stride_t + (int64_t)(h * G + g) * a.o_stride_h;
+  if (un.parts > 1) {
+    if (hl == 0) a.part_ml[pslot * 32 + n] = float2{m, l};
+    if (w0 < w1 && sums_ok) {  // (l = 0 of a wave without steps: the join takes no sums)
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        a.part_acc[(pslot * 16 + c) * 64 + lane] = f32x4{acc[c >> 2][4 * (c & 3)], acc[c >> 2][4 * (c & 3) + 1],
+                                                         acc[c >> 2][4 * (c & 3) + 2], acc[c >> 2][4 * (c & 3) + 3]};
+    }
+  } else if (row_ok) {
+    // Normalise and write: lane l holds O[row l%32][32 dt + 8 (i / 4) + 4 hl + i % 4].  (l is NaN where a score is.)
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int c = 0; c < 16 && sums_ok; ++c) {
+      uint2 w;
+      w.x = pack2<DT>(acc[c >> 2][4 * (c & 3)] * inv, acc[c >> 2][4 * (c & 3) + 1] * inv);
+      w.y = pack2<DT>(acc[c >> 2][4 * (c & 3) + 2] * inv, acc[c >> 2][4 * (c & 3) + 3] * inv);
+      *reinterpret_cast<uint2 *>(orow + 4 * hl + 32 * (c >> 2) + 8 * (c & 3)) = w;
+    }
+    if (a.lse && hl == 0) a.lse[(q0 + tok0 + tt) * a.hq + h * G + g] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  }
+
+  // slow_row: the sums again, key by key, over the row's own keys.
+  for (uint32_t rows = odd_rows; rows != 0; rows &= rows - 1) {
+    const int rn = __builtin_ctz(rows);
+    const int rlo = max(__builtin_amdgcn_readlane(lo, rn), s0 * kKvStep), rhi = min(__builtin_amdgcn_readlane(hi, rn), s1 * kKvStep);
+    const float rm = readlane(m, rn), rl = readlane(l, rn), rs = readlane(slope2, rn);
+    const int rt = rn / G, rg = rn - rt * G, rpos = __builtin_amdgcn_readlane(qpos, rn);
+    const uint16_t *qp = a.q + (q0 + tok0 + rt) * a.q_stride_t + (int64_t)(h * G + rg) * a.q_stride_h;
+    float o0 = 0.f, o1 = 0.f;  // d = 2 lane, 2 lane + 1
+    for (int c0 = rlo; c0 < rhi; c0 += 64) {
+      const int k = c0 + lane;
+      int pid = k < rhi && k / kPageSize < np ? row_ids[k / kPageSize] : -1;
+      if (page_bad(pid)) pid = -1;
+      float x[1] = {0.f};
+      if (pid >= 0) {
+        const uint32_t *kp = reinterpret_cast<const uint32_t *>(kvh + (uint64_t)pid * page_bytes + (k % kPageSize) * row_bytes);
+        for (int d = 0; d < 64; ++d) {
+          const uint32_t kw = kp[d], qw = reinterpret_cast<const uint32_t *>(qp)[d];
+          x[0] = fmaf(E::lo(kw), E::lo(qw), x[0]);
+          x[0] = fmaf(E::hi(kw), E::hi(qw), x[0]);
+        }
+      }
+      if (capped)
+        cap_scores(x, a.rule, a.sm_scale, kLog2e);
+      else
+        x[0] *= a.sm_scale * kLog2e;
+      if (leaning) x[0] = fmaf(-rs, fabsf((float)(rpos - k)), x[0]);
+      const float p = fast_exp2(x[0] - rm);
+      for (uint64_t keys = __ballot(pid >= 0); keys != 0; keys &= keys - 1) {
+        const int kl = __builtin_ctzll(keys);
+        const float pk = readlane(p, kl);
+        const uint64_t kpid = (uint32_t)__builtin_amdgcn_readlane(pid, kl);
+        const uint32_t vw = reinterpret_cast<const uint32_t *>(kvh + kpid * page_bytes +
+                                                               (uint32_t)(kPageSize + (c0 + kl) % kPageSize) * row_bytes)[lane];
+        o0 = fmaf(pk, E::lo(vw), o0);
+        o1 = fmaf(pk, E::hi(vw), o1);
+      }
+    }
+    if (un.parts > 1) {
+      // element d of the row: chunk d / 8, lane 32 ((d % 8) / 4) + n, component d % 4
+      const int d = 2 * lane;
+      float *dst = reinterpret_cast<float *>(a.part_acc + (pslot * 16 + d / 8) * 64 + 32 * (d % 8 / 4) + rn) + d % 4;
+      dst[0] = o0;
+      dst[1] = o1;
+    } else {
+      const float inv = 1.f / rl;
+      uint32_t *dst = reinterpret_cast<uint32_t *>(a.o + (q0 + tok0 + rt) * a.o_stride_t + (int64_t)(h * G + rg) * a.o_stride_h);
+      dst[lane] = pack2<DT>(o0 * inv, o1 * inv);
+    }
+  }
+}
+
+// Joins the parts of cut rows: the blocks of a tile's parts share its (wave, chunk) pairs, a wave each, whose lanes hold
+// the rows as the accumulators did.
+template <int DT>
+__global__ void __launch_bounds__(kSplitWaves * 64) rule_join_kernel(RulePrefillArgs a) {
+  constexpr int PW = kSplitWaves;
+  const int G = a.G, TW = 32 / G, BT = PW * TW;
+  const int lane = threadIdx.x & 63, hl = lane >> 5, n = lane & 31;
+  const int h = blockIdx.x, u = (int)(blockIdx.z * gridDim.y + blockIdx.y);
+  Unit un;
+  if (!find_unit(a, BT, u, lane, &un) || un.parts == 1) return;
+  const int qn = un.row.q1 - un.row.q0, btok0 = un.tile * BT;
+  const int waves = min(PW, (qn - btok0 + TW - 1) / TW);
+  const int64_t first = u - un.part;
+  for (int task = un.part * PW + uniform((int)(threadIdx.x >> 6)); task < waves * 16; task += un.parts * PW) {
+    const int w = task >> 4, c = task & 15;
+    float M = -INFINITY, L = 0.f;
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < un.parts; s0 += 8) {
+      float2 ml[8];
+      f32x4 av[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t at = ((first + min(s0 + i, un.parts - 1)) * a.hkv + h) * PW + w;
+        ml[i] = a.part_ml[at * 32 + n];
+        av[i] = a.part_acc[(at * 16 + c) * 64 + lane];
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+      const float ref = top == -INFINITY ? 0.f : top, al = fast_exp2(M - ref);
+      L *= al;
+      A = A * al;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (s0 + i < un.parts && ml[i].y != 0.f) {  // a part without keys wrote no sums
+          const float sc = fast_exp2(ml[i].x - ref);
+          L = fmaf(ml[i].y, sc, L);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) A[e] = fmaf(av[i][e], sc, A[e]);
+        }
+      }
+      M = top;
+    }
+    const int tt = n / G, g = n - tt * G, tok = btok0 + w * TW + tt;
+    if (n < TW * G && tok < qn) {
+      const int64_t t = un.row.q0 + tok;
+      const float inv = L != 0.f ? 1.f / L : 0.f;
+      uint2 o;
+      o.x = pack2<DT>(A[0] * inv, A[1] * inv);
+      o.y = pack2<DT>(A[2] * inv, A[3] * inv);
+      *reinterpret_cast<uint2 *>(a.o + t * a.o_stride_t + (int64_t)(h * G + g) * a.o_stride_h + 4 * hl + 8 * c) = o;
+      if (a.lse && c == 0 && hl == 0) a.lse[t * a.hq + h * G + g] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+    }
+  }
+}
+
+// Tiles of BT tokens that rows of num_tokens tokens in all, max_qo_len each at most, have at most.
+int64_t tiles_bound(int64_t num_tokens, int batch, int max_qo_len, int BT) {
+  const int64_t slots = (int64_t)batch * ceil_div(max_qo_len, BT);
+  const int64_t most = (num_tokens + (int64_t)batch * (BT - 1)) / BT;
+  return slots < most ? slots : most;
+}
+
+// Units of cut rows (a kv head's), at most; 0 where no row can be cut.  A cut row has s > 1.5 C steps, so its tiles' parts
+// are at most s / C + 1 < (5 / 3) s / C each, and W hkv <= C kTargetBlocks.
+int64_t cut_bound(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len, int64_t kv_indices_len, int window) {
+  const int BT = kSplitWaves * (32 / G);
+  const int64_t keys = kv_indices_len * kPageSize, span = window > 0 && window + (int64_t)BT < keys ? window + (int64_t)BT : keys;
+  const int64_t steps = ceil_div(span, kKvStep);
+  if (steps <= kMinSteps + kMinSteps / 2) return 0;
+  const int64_t tiles = tiles_bound(num_tokens, batch, max_qo_len, BT);
+  if (batch == 1 && tiles * hkv >= kTargetBlocks) return 0;  // C >= steps
+  const int64_t by_work = ceil_div(5 * kTargetBlocks, 3 * (int64_t)hkv) + 1;
+  const int64_t by_size = tiles * ceil_div(steps, kMinSteps);
+  return by_work < by_size ? by_work : by_size;
+}
+
+size_t part_bytes(int64_t units, int hkv) {
+  const size_t per = (size_t)kSplitWaves * 32 * (sizeof(float2) + kHeadDim * sizeof(float));
+  return (units * hkv * per + 255) & ~(size_t)255;
+}
+
+template <int DT>
+int launch_rule(RulePrefillArgs a, int64_t num_tokens, int max_qo_len, hipStream_t stream, const char *who) {
+  const int TW = 32 / a.G;
+  // Whole prompts that fill the chip nearly twice over in 4-wave blocks run 8-wave ones (prefill.hip, wide_blocks).
+  const bool wide = a.max_cut == 0 && a.hkv * ceil_div(max_qo_len, 4 * TW) >= 850;
+  const int BT = TW * (wide ? 8 : 4);
+  a.row_tiles = (int)ceil_div(max_qo_len, BT);
+  const int64_t units = a.max_cut + tiles_bound(num_tokens, a.batch, max_qo_len, BT), y = units < 32768 ? units : 32768;
+  const dim3 grid((unsigned)a.hkv, (unsigned)y, (unsigned)ceil_div(units, y));
+  if (wide)
+    hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 8>), grid, dim3(512), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 4>), grid, dim3(256), 0, stream, a);
+  const int rc = check_launch(who);
+  if (rc || a.max_cut == 0) return rc;
+  hipLaunchKernelGGL((rule_join_kernel<DT>), dim3((unsigned)a.hkv, (unsigned)a.max_cut), dim3(kSplitWaves * 64), 0, stream, a);
+  return check_launch(who);
+}
+
+}  // namespace
+}  // namespace delta
+
+extern "C" DELTA_EXPORT size_t delta_paged_prefill_rule_workspace_bytes(int64_t num_tokens, int batch, int num_qo_heads,
+                                                                        int num_kv_heads, int max_qo_len,
+                                                                        int64_t kv_indices_len, int window) {
+  using namespace delta;
+  if (num_tokens <= 0 || batch <= 0 || max_qo_len <= 0 || num_kv_heads <= 0 || num_qo_heads < num_kv_heads ||
+      num_qo_heads % num_kv_heads || num_qo_heads / num_kv_heads > kMaxGroup || kv_indices_len <= 0)
+    return 0;
+  const int64_t units = cut_bound(num_tokens, batch, num_kv_heads, num_qo_heads / num_kv_heads, max_qo_len, kv_indices_len, window);
+  return units > 0 ? part_bytes(units, num_kv_heads) : 0;
+}
+
+extern "C" DELTA_EXPORT int delta_paged_prefill_rule(const delta_score_rule_t *rule, const void *q, int64_t q_stride_t,
+                                                     int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+                                                     const int32_t *qo_indptr, const int32_t *kv_indptr,
+                                                     const int32_t *kv_indices, int64_t kv_indices_len,
+                                                     const int32_t *kv_last_page_len, void *o, int64_t o_stride_t,
+                                                     int64_t o_stride_h, float *lse, int batch, int64_t num_tokens,
+                                                     int max_qo_len, int num_qo_heads, int num_kv_heads, int head_dim,
+                                                     int dtype, float sm_scale, void *workspace, size_t workspace_bytes,
+                                                     delta_stream_t stream) {
+  using namespace delta;
+  clear_error();
+  const char *who = "delta_paged_prefill_rule";
+  if (batch <= 0 || num_tokens <= 0 || max_qo_len <= 0) return DELTA_OK;
+  if (head_dim != kHeadDim) return set_error(DELTA_ERR_INVALID, "%s: head_dim must be 128", who);
+  if (num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads)
+    return set_error(DELTA_ERR_INVALID, "%s: num_qo_heads must be a multiple of num_kv_heads", who);
+  const int G = num_qo_heads / num_kv_heads;
+  if (G > kMaxGroup) return set_error(DELTA_ERR_INVALID, "%s: group size %d > %d unsupported", who, G, kMaxGroup);
+  if (dtype != DELTA_BF16 && dtype != DELTA_FP16) return set_error(DELTA_ERR_INVALID, "%s: bad dtype", who);
+  RulePrefillArgs a = {};
+  const int rc = rule_args(rule, &a.rule, who);
+  if (rc) return rc;
+  if (!q || !kv_cache || !qo_indptr || !kv_indptr || !kv_indices || !kv_last_page_len || !o)
+    return set_error(DELTA_ERR_INVALID, "%s: null pointer", who);
+  if (((uintptr_t)q | (uintptr_t)kv_cache) & 15u || (q_stride_t % 8) || (q_stride_h % 8))
+    return set_error(DELTA_ERR_INVALID, "%s: q and kv_cache 16-byte aligned, q strides multiples of 8", who);
+  if (((uintptr_t)o & 7u) || (o_stride_t % 4) || (o_stride_h % 4))
+    return set_error(DELTA_ERR_INVALID, "%s: o 8-byte aligned with strides in multiples of 4", who);
+  if (num_pages <= 0 || kv_indices_len < 0) return set_error(DELTA_ERR_INVALID, "%s: empty cache", who);
+  if (num_tokens > 1 << 23 || batch > 1 << 20 || num_kv_heads > 1 << 12 || kv_indices_len > 1 << 26)
+    return set_error(DELTA_ERR_INVALID, "%s: more than 2^23 tokens, 2^20 rows, 2^12 kv heads or 2^26 pages", who);
+  a.q = (const uint16_t *)q;
+  a.q_stride_t = q_stride_t;
+  a.q_stride_h = q_stride_h;
+  a.kv = (const uint16_t *)kv_cache;
+  a.num_pages = num_pages;
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_indices_len = kv_indices_len;
+  a.last_page_len = kv_last_page_len;
+  a.o = (uint16_t *)o;
+  a.o_stride_t = o_stride_t;
+  a.o_stride_h = o_stride_h;
+  a.lse = lse;
+  a.batch = batch;
+  a.hq = num_qo_heads;
+  a.hkv = num_kv_heads;
+  a.G = G;
+  a.token_limit = (int)num_tokens;
+  a.sm_scale = sm_scale;
+  const int64_t cut = cut_bound(num_tokens, batch, num_kv_heads, G, max_qo_len, kv_indices_len, a.rule.window);
+  if (cut > 0) {
+    const size_t need = part_bytes(cut, num_kv_heads);
+    if (!workspace || workspace_bytes < need)
+      return set_error(DELTA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+    if ((uintptr_t)workspace & 255u) return set_error(DELTA_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
+    a.max_cut = (int)cut;
+    a.part_acc = (f32x4 *)workspace;
+    a.part_ml = (float2 *)(a.part_acc + (size_t)cut * num_kv_heads * kSplitWaves * 16 * 64);
+  }
+  if (dtype == DELTA_BF16) return launch_rule<DELTA_BF16>(a, num_tokens, max_qo_len, (hipStream_t)stream, who);
+  return launch_rule<DELTA_FP16>(a, num_tokens, max_qo_len, (hipStream_t)stream, who);
+}

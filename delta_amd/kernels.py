@@ -471,6 +471,275 @@ def paged_prefill_prefix(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: tor
                         int(max_qo_len) if max_pages_per_row is not None and max_pages_per_row <= 40 else None)
 
 
+@dataclass(frozen=True)
+class Rotary:
+    """A position rotation of each head's first ``rotary_dim`` elements (``delta_rotary_t``), made by ``rotary`` once
+    per model and device: ``turns`` (int64 [rotary_dim / 2]) is each pair's turn per position as a fraction of 2^64."""
+    turns: torch.Tensor
+    rotary_dim: int
+    interleaved: bool
+    factor: float
+    c: _lib.RotaryC
+
+
+def rotary_frequencies(rotary_dim: int, *, rope_theta: float = 1e4, rope_scale: float = 1.0,
+                       low_freq_factor: Optional[float] = None, high_freq_factor: Optional[float] = None,
+                       old_context_len: Optional[float] = None, scaling: Optional[str] = None, beta_fast: float = 32.0,
+                       beta_slow: float = 1.0):
+    """(radians per position of each pair, factor on what is rotated) of a scaling, in 64 bits.
+
+    With f_j = rope_theta^(-2j / rotary_dim), s = rope_scale and r_j = old_context_len f_j / (2 pi), the turns over the
+    trained context:
+      ``linear``  f_j / s
+      ``ntk``     f_j of the base rope_theta s^(rotary_dim / (rotary_dim - 2)): the first pair's kept, the last one's / s
+      ``llama31`` f_j / s where r_j <= low_freq_factor, f_j where r_j >= high_freq_factor, between them linear in r_j
+      ``yarn``    the same between beta_slow and beta_fast turns, and a factor of 0.1 ln(s) + 1 (s > 1) on q and k
+    Without ``scaling``: ``llama31`` where both frequency factors are given, as for ``rope``, else ``linear``."""
+    if rotary_dim % 2 or not 2 <= rotary_dim <= HEAD_DIM:
+        raise ValueError(f"rotary_dim must be even and in [2, {HEAD_DIM}], got {rotary_dim}")
+    if not rope_theta > 0 or not rope_scale > 0 or math.isinf(rope_theta) or math.isinf(rope_scale):
+        raise ValueError("rope_theta and rope_scale must be positive and finite")
+    if scaling is None:
+        scaling = "llama31" if low_freq_factor is not None and high_freq_factor is not None else "linear"
+    theta, factor = float(rope_theta), 1.0
+    if scaling == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("ntk scaling needs a rotary_dim over 2")
+        theta *= rope_scale ** (rotary_dim / (rotary_dim - 2))
+    freqs = [theta ** (-2.0 * j / rotary_dim) for j in range(rotary_dim // 2)]
+    if scaling == "linear":
+        freqs = [f / rope_scale for f in freqs]
+    elif scaling in ("llama31", "yarn"):
+        lo, hi = (low_freq_factor, high_freq_factor) if scaling == "llama31" else (beta_slow, beta_fast)
+        if lo is None or hi is None or not hi > lo > 0 or old_context_len is None or not old_context_len > 0:
+            raise ValueError(f"{scaling} scaling needs old_context_len and 0 < low < high turns")
+        keep = [min(max((old_context_len * f / (2 * math.pi) - lo) / (hi - lo), 0.0), 1.0) for f in freqs]
+        freqs = [f / rope_scale * (1 - k) + f * k for f, k in zip(freqs, keep)]
+        if scaling == "yarn" and rope_scale > 1:
+            factor = 0.1 * math.log(rope_scale) + 1.0
+    elif scaling != "ntk":
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return freqs, factor
+
+
+def rotary(rotary_dim: int = HEAD_DIM, *, interleaved: bool = False, device=None,
+           frequencies: Optional[Sequence[float]] = None, factor: Optional[float] = None, **scaling) -> Rotary:
+    """The rotation that ``qk_norm_rope`` and ``qk_norm_rope_append`` apply; keep it for all layers and steps.
+
+    Pairs (2j, 2j + 1) where ``interleaved``, else (j, j + rotary_dim / 2).  ``scaling``: the arguments of
+    ``rotary_frequencies``; or ``frequencies``, each pair's radians per position, as they are.  ``factor`` replaces the
+    scaling's."""
+    if frequencies is None:
+        freqs, f = rotary_frequencies(rotary_dim, **scaling)
+    else:
+        freqs, f = [float(x) for x in frequencies], 1.0
+        if scaling:
+            raise ValueError("frequencies are taken as they are: no scaling beside them")
+        if rotary_dim % 2 or not 2 <= rotary_dim <= HEAD_DIM or len(freqs) != rotary_dim // 2:
+            raise ValueError(f"{rotary_dim // 2} frequencies for an even rotary_dim in [2, {HEAD_DIM}], got {len(freqs)}")
+        if not all(math.isfinite(x) for x in freqs):
+            raise ValueError("frequencies must be finite")
+    f = f if factor is None else float(factor)
+    if not math.isfinite(f):
+        raise ValueError("factor must be finite")
+    turns = [int(math.ldexp(math.fmod(x / (2 * math.pi), 1.0), 64)) % (1 << 64) for x in freqs]
+    t = torch.tensor([v - (1 << 64) if v >> 63 else v for v in turns], dtype=torch.int64, device=device or "cuda")
+    return Rotary(t, rotary_dim, bool(interleaved), f, _lib.RotaryC(t.data_ptr(), rotary_dim, int(bool(interleaved)), f))
+
+
+def _norm_rope_args(q, k, indptr, offsets, rot, q_weight, k_weight, eps, *others):
+    """Device, row count and the C structures of the two norm + rotation calls, after their common checks."""
+    dev = q.device
+    for t in (q, k, indptr, offsets, *others, q_weight, k_weight, None if rot is None else rot.turns):
+        if t is not None and (not t.is_cuda or t.device != dev):
+            _check_cuda(t, device=dev)
+    dtype = q.dtype
+    _dtype_code(q)
+    for name, t in (("q", q), ("k", k)):
+        s = t.stride()
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or s[2] != 1 or (s[1] != HEAD_DIM and t.shape[1] != 1) or s[0] % 8 \
+                or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be [nnz, heads, 128] with contiguous heads and 16-byte aligned rows")
+        if t.dtype != dtype:
+            raise TypeError("q and k must share a dtype")
+    if k.shape[0] != q.shape[0]:
+        raise ValueError("q and k token counts differ")
+    B = indptr.numel() - 1
+    if B < 0:
+        raise ValueError("indptr needs >= 1 entries")
+    _check_i32("indptr", indptr)
+    _check_i32("offsets", offsets, B)
+    norm = None
+    if q_weight is not None or k_weight is not None:
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is None or w.dtype != dtype or w.numel() != HEAD_DIM or not w.is_contiguous() or w.data_ptr() % 16:
+                raise ValueError(f"{name} must be a contiguous, 16-byte aligned [128] tensor of q's dtype (both weights or none)")
+        norm = ctypes.byref(_lib.HeadNormC(q_weight.data_ptr(), k_weight.data_ptr(), float(eps)))
+    return dev, B, None if rot is None else ctypes.byref(rot.c), norm
+
+
+def _rows_like(name: str, out: Optional[torch.Tensor], ref: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(ref.shape, dtype=ref.dtype, device=ref.device)
+    s = out.stride()
+    if out.shape != ref.shape or out.dtype != ref.dtype or s[2] != 1 or (s[1] != HEAD_DIM and ref.shape[1] != 1) \
+            or s[0] % 8 or out.data_ptr() % 16:
+        raise ValueError(f"{name} must match its input's shape and dtype with contiguous heads and 16-byte aligned rows")
+    return out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, indptr: torch.Tensor, offsets: torch.Tensor,
+                 rotary: Optional[Rotary], *, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None):
+    """RMS norm of each head (with ``q_weight`` and ``k_weight``, [128] each) and rotation by the token's position, in
+    fp32, rounded once (``delta_qk_norm_rope``); returns (q_out, k_out), which may be q and k themselves.
+
+    Token i of row b (rows from ``indptr``) is at position ``offsets[b] + i - indptr[b]``; tokens of no row are left
+    as they were."""
+    dev, B, rot, norm = _norm_rope_args(q, k, indptr, offsets, rotary, q_weight, k_weight, eps, q_out, k_out)
+    q_out, k_out = _rows_like("q_out", q_out, q), _rows_like("k_out", k_out, k)
+    _call_on(dev, "delta_qk_norm_rope", rot, norm, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), q_out.data_ptr(),
+             q_out.stride(0), k_out.data_ptr(), k_out.stride(0), indptr.data_ptr(), offsets.data_ptr(), q.shape[0], B,
+             q.shape[1], k.shape[1], HEAD_DIM, _DTYPES[q.dtype])
+    return q_out, k_out
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_indptr: torch.Tensor,
+                        offsets: torch.Tensor, kv_cache: torch.Tensor, kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
+                        kv_last_page_len: torch.Tensor, rotary: Optional[Rotary], *,
+                        q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                        eps: float = 1e-6, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``qk_norm_rope`` then ``append_kv`` of its keys and of ``v`` in one launch (``delta_qk_norm_rope_append``);
+    returns the rotated q (``q_out``, which may be q itself)."""
+    dev, B, rot, norm = _norm_rope_args(q, k, kv_append_indptr, offsets, rotary, q_weight, k_weight, eps, v, kv_cache,
+                                        kv_indices, kv_indptr, kv_last_page_len, q_out)
+    _check_cache(kv_cache)
+    s = v.stride()
+    if k.shape[1] != kv_cache.shape[3] or v.shape != k.shape or s[2] != 1 or (s[1] != HEAD_DIM and v.shape[1] != 1) \
+            or s[0] % 8 or v.data_ptr() % 16:
+        raise ValueError(f"k and v must be [nnz, {kv_cache.shape[3]}, 128] with contiguous heads and 16-byte aligned rows")
+    if v.dtype != q.dtype or kv_cache.dtype != q.dtype:
+        raise TypeError("q, k, v and kv_cache must share a dtype")
+    _check_i32("kv_indices", kv_indices)
+    _check_i32("kv_indptr", kv_indptr, B + 1)
+    _check_i32("kv_last_page_len", kv_last_page_len, B)
+    q_out = _rows_like("q_out", q_out, q)
+    _call_on(dev, "delta_qk_norm_rope_append", rot, norm, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
+             s[0], q_out.data_ptr(), q_out.stride(0), kv_append_indptr.data_ptr(), offsets.data_ptr(), kv_cache.data_ptr(),
+             kv_cache.shape[0], kv_indices.data_ptr(), kv_indices.numel(), kv_indptr.data_ptr(),
+             kv_last_page_len.data_ptr(), q.shape[0], B, q.shape[1], k.shape[1], HEAD_DIM, _DTYPES[q.dtype])
+    return q_out
+
+
+@dataclass(frozen=True)
+class ScoreRule:
+    """What attention does to the score ``x = q.k * sm_scale`` of a query token at position ``pos`` and a key
+    (``delta_score_rule_t``), in this order:
+
+    * ``softcap`` c > 0: ``c * tanh(x / c)``;
+    * ``slopes`` (fp32 [Hq]): ``x - slopes[h] * |pos - key|``;
+    * ``window`` w > 0: keys in front of ``pos - w + 1`` are left out;
+    * ``kv_begin`` (int32 [tokens]): keys in front of ``kv_begin[token]`` are left out -- for documents packed into a
+      row each token's first key of its own document;
+    * ``kv_end`` (int32 [tokens]): keys from ``kv_end[token]`` on are left out, instead of those behind ``pos`` -- a prefix
+      seen as a whole is ``max(pos + 1, prefix length)``.
+
+    Key positions count from the row's first cached token.  A token that sees no key gets o = 0 and lse = -inf."""
+    softcap: float = 0.0
+    slopes: Optional[torch.Tensor] = None
+    window: int = 0
+    kv_begin: Optional[torch.Tensor] = None
+    kv_end: Optional[torch.Tensor] = None
+
+
+def _rule_call(name: str, q, kv_cache, B: int, tables: tuple, rule: ScoreRule, out, lse, workspace, need, sm_scale,
+               tail: tuple) -> torch.Tensor:
+    """What the two attention calls under a score rule have in common: checks, outputs, workspace, the call.  ``tables``
+    are the row tables in the entry point's order, the page indices next to last; ``need`` sizes the workspace; ``tail``
+    the arguments between the batch and the head counts, and those behind the scale."""
+    dev = q.device
+    slopes, begin, end = rule.slopes, rule.kv_begin, rule.kv_end
+    for t in (q, kv_cache, *tables, slopes, begin, end, out, lse, workspace):
+        if t is not None and (not t.is_cuda or t.device != dev):
+            _check_cuda(t, device=dev)
+    _check_cache(kv_cache)
+    hq, hkv = _check_heads(q, kv_cache)
+    T, indices = q.shape[0], tables[-2]
+    _check_i32("kv_indptr", tables[-3], B + 1)
+    _check_i32("kv_indices", indices)
+    _check_i32("kv_last_page_len", tables[-1], B)
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != hq or not slopes.is_contiguous()):
+        raise ValueError(f"slopes must be contiguous fp32 [{hq}]")
+    if begin is not None:
+        _check_i32("kv_begin", begin, T)
+    if end is not None:
+        _check_i32("kv_end", end, T)
+    if not 0 <= rule.window < 1 << 31:
+        raise ValueError(f"window must be 0 (none) or a positive int32, got {rule.window}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out must match q's shape/dtype with unit inner stride")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous fp32 [{T}, {hq}]")
+    need = need(hq, hkv, rule.window)
+    if workspace is None:  # of this call: safe on any stream, in any capture
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace too small: {need} bytes needed")
+    c = _lib.ScoreRuleC(rule.softcap, _ptr(slopes), rule.window, _ptr(begin), _ptr(end))
+    _call_on(dev, name, ctypes.byref(c), q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), kv_cache.shape[0],
+             *[t.data_ptr() for t in tables[:-1]], indices.numel(), tables[-1].data_ptr(), out.data_ptr(), out.stride(0),
+             out.stride(1), _ptr(lse), B, *tail[0], hq, hkv, HEAD_DIM, _DTYPES[q.dtype],
+             _DEFAULT_SCALE if sm_scale is None else float(sm_scale), *tail[1], _ptr(workspace),
+             0 if workspace is None else workspace.numel() * workspace.element_size())
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def decode_rule_workspace_bytes(batch: int, hq: int, hkv: int, max_pages: int, window: int = 0) -> int:
+    """Bytes of ``paged_decode_rule``'s workspace."""
+    return int(_lib.query("delta_paged_decode_rule_workspace_bytes", batch, hq, hkv, max_pages, window))
+
+
+@functools.lru_cache(maxsize=1024)
+def prefill_rule_workspace_bytes(tokens: int, batch: int, hq: int, hkv: int, max_qo_len: int, pages: int,
+                                 window: int = 0) -> int:
+    """Bytes of ``paged_prefill_rule``'s workspace (``pages``: entries of its ``kv_indices``)."""
+    return int(_lib.query("delta_paged_prefill_rule_workspace_bytes", tokens, batch, hq, hkv, max_qo_len, pages, window))
+
+
+def paged_decode_rule(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                      kv_last_page_len: torch.Tensor, rule: ScoreRule, *, max_pages_per_row: int,
+                      sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                      lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_decode`` under a score rule (``delta_paged_decode_rule``): one query token per row, the last of its cached
+    ones; only the pages of keys that the rule leaves in are read.
+
+    ``workspace`` (``decode_rule_workspace_bytes``) is allocated for the call where none is given."""
+    B, mp = q.shape[0], int(max_pages_per_row)
+    return _rule_call("delta_paged_decode_rule", q, kv_cache, B, (kv_indptr, kv_indices, kv_last_page_len), rule, out, lse,
+                      workspace, lambda hq, hkv, w: decode_rule_workspace_bytes(B, hq, hkv, mp, w), sm_scale, ((), (mp,)))
+
+
+def paged_prefill_rule(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor,
+                       kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, rule: ScoreRule, *, max_qo_len: int,
+                       sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                       lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_prefill`` under a score rule (``delta_paged_prefill_rule``); q/out [nnz, Hq, 128], row b's last
+    ``qo_indptr[b + 1] - qo_indptr[b]`` cached tokens its query tokens, ``max_qo_len`` at least the longest row's count.
+
+    ``out`` and ``lse`` of tokens behind the last row are left as they were.  ``workspace``
+    (``prefill_rule_workspace_bytes``) is allocated for the call where none is given."""
+    _check_i32("qo_indptr", qo_indptr, 1)
+    B, T, mq, pages = qo_indptr.numel() - 1, q.shape[0], int(max_qo_len), kv_indices.numel()
+    return _rule_call("delta_paged_prefill_rule", q, kv_cache, B, (qo_indptr, kv_indptr, kv_indices, kv_last_page_len),
+                      rule, out, lse, workspace, lambda hq, hkv, w: prefill_rule_workspace_bytes(T, B, hq, hkv, mq, pages, w),
+                      sm_scale, ((T, mq), ()))
+
+
 def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, *,
                tokens: Optional[torch.Tensor] = None) -> None:
     """Copy pages in place inside each of ``caches`` (one per layer, one shape) in one launch (``delta_copy_pages``):

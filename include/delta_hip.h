@@ -601,6 +601,109 @@ int delta_copy_pages(void *const *caches, int num_caches, int64_t num_pages, int
                      int head_dim, int dtype, const int32_t *src, const int32_t *dst,
                      const int32_t *tokens, int64_t num_copies, delta_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Norms and rotation of queries and keys; attention under a score rule       */
+/* ------------------------------------------------------------------------ */
+
+/* A rotation of each head's first rotary_dim elements (even, <= 128; 0: none) by the token's
+ * position.  Pair j (j < rotary_dim / 2) is (2j, 2j + 1) where interleaved != 0, else
+ * (j, j + rotary_dim / 2).  turns[j] is the pair's turn per position as a fraction of 2^64
+ * (device memory): frequency f in radians is f / (2 pi) 2^64 mod 2^64, so angles are exact for
+ * every position.  factor multiplies what is rotated (1, or a long-context scaling's). */
+typedef struct delta_rotary {
+  const uint64_t *turns; /* [rotary_dim / 2] */
+  int rotary_dim;
+  int interleaved;
+  float factor;
+} delta_rotary_t;
+
+/* RMS norm of each head before its rotation: y = x rsqrt(mean(x^2) + eps) w, w [128] of the
+ * tensors' dtype, 16-byte aligned; q and k have weights of their own. */
+typedef struct delta_head_norm {
+  const void *q_weight;
+  const void *k_weight;
+  float eps;
+} delta_head_norm_t;
+
+/* Norms (norm NULL: none) and rotation (rotary NULL: none) of q [nnz, num_qo_heads, 128] and
+ * k [nnz, num_kv_heads, 128], in fp32, rounded once, into q_out and k_out (which may alias
+ * q and k).  Token i of row b (rows from indptr [batch + 1]) is at position
+ * offsets[b] + i - indptr[b]; tokens of no row are left as they were.  Token strides in
+ * elements, multiples of 8, heads contiguous, 16-byte aligned.  nnz <= 2^23. */
+int delta_qk_norm_rope(const delta_rotary_t *rotary, const delta_head_norm_t *norm, const void *q,
+                       int64_t q_stride, const void *k, int64_t k_stride, void *q_out,
+                       int64_t q_out_stride, void *k_out, int64_t k_out_stride,
+                       const int32_t *indptr, const int32_t *offsets, int nnz, int batch,
+                       int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
+                       delta_stream_t stream);
+
+/* delta_qk_norm_rope whose keys go, with v [nnz, num_kv_heads, 128], into the paged cache, at
+ * the slots delta_append_kv would use (a token without a valid slot appends nothing). */
+int delta_qk_norm_rope_append(const delta_rotary_t *rotary, const delta_head_norm_t *norm,
+                              const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                              const void *v, int64_t v_stride, void *q_out, int64_t q_out_stride,
+                              const int32_t *kv_append_indptr, const int32_t *offsets,
+                              void *kv_cache, int64_t num_pages, const int32_t *kv_indices,
+                              int64_t kv_indices_len, const int32_t *kv_indptr,
+                              const int32_t *kv_last_page_len, int nnz, int batch,
+                              int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
+                              delta_stream_t stream);
+
+/* What attention does to the score x = q.k sm_scale of a query token at position pos and a key:
+ *   softcap c > 0      x <- c tanh(x / c)                       (0: none)
+ *   slopes [num_qo_heads] fp32, or NULL
+ *                      x <- x - slopes[h] |pos - key|
+ *   window w > 0       keys in front of pos - w + 1 are left out (0: none)
+ *   kv_begin [tokens] int32, or NULL
+ *                      keys in front of kv_begin[token] are left out: documents packed into a
+ *                      row are each token's first key of its own document
+ *   kv_end [tokens] int32, or NULL
+ *                      keys from kv_end[token] on are left out, instead of those behind pos: a
+ *                      prefix seen as a whole is max(pos + 1, prefix length)
+ * in that order, tokens numbered as the rows of q.  Key positions count from the row's first
+ * cached token; none past kv_len is seen.  A token that sees no key gets o = 0 and lse = -inf.
+ * What is left out has no part in o and lse, whatever it holds (infinities and NaN too). */
+typedef struct delta_score_rule {
+  float softcap;
+  const float *slopes;
+  int window;
+  const int32_t *kv_begin;
+  const int32_t *kv_end;
+} delta_score_rule_t;
+
+/* delta_paged_decode under a score rule: one query token per row, at position kv_len_b - 1.
+ * Only the pages that hold keys the rule leaves in are read.  max_pages_per_row is the planned
+ * maximum of the rows' pages (a longer row is still covered whole).  workspace:
+ * delta_paged_decode_rule_workspace_bytes, 256-byte aligned (0 bytes: may be NULL). */
+size_t delta_paged_decode_rule_workspace_bytes(int batch, int num_qo_heads, int num_kv_heads,
+                                               int max_pages_per_row, int window);
+int delta_paged_decode_rule(const delta_score_rule_t *rule, const void *q, int64_t q_stride_b,
+                            int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+                            const int32_t *kv_indptr, const int32_t *kv_indices,
+                            int64_t kv_indices_len, const int32_t *kv_last_page_len, void *o,
+                            int64_t o_stride_b, int64_t o_stride_h, float *lse, int batch,
+                            int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
+                            float sm_scale, int max_pages_per_row, void *workspace,
+                            size_t workspace_bytes, delta_stream_t stream);
+
+/* delta_paged_prefill under a score rule: num_tokens query tokens in rows of qo_indptr (tokens
+ * behind the last row are left as they were), max_qo_len >= every row's query tokens.  Rows of
+ * few tokens over long caches are cut over their keys and joined by a second launch.
+ * workspace: delta_paged_prefill_rule_workspace_bytes, 256-byte aligned (0 bytes: may be
+ * NULL).  At most 2^23 tokens, 2^20 rows, 2^12 kv heads and 2^26 entries of kv_indices. */
+size_t delta_paged_prefill_rule_workspace_bytes(int64_t num_tokens, int batch, int num_qo_heads,
+                                                int num_kv_heads, int max_qo_len,
+                                                int64_t kv_indices_len, int window);
+int delta_paged_prefill_rule(const delta_score_rule_t *rule, const void *q, int64_t q_stride_t,
+                             int64_t q_stride_h, const void *kv_cache, int64_t num_pages,
+                             const int32_t *qo_indptr, const int32_t *kv_indptr,
+                             const int32_t *kv_indices, int64_t kv_indices_len,
+                             const int32_t *kv_last_page_len, void *o, int64_t o_stride_t,
+                             int64_t o_stride_h, float *lse, int batch, int64_t num_tokens,
+                             int max_qo_len, int num_qo_heads, int num_kv_heads, int head_dim,
+                             int dtype, float sm_scale, void *workspace, size_t workspace_bytes,
+                             delta_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
