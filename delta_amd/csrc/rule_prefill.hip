@@ -19,6 +19,8 @@
 // A key that a mask leaves out has no part in the result, whatever it holds.  Its score is replaced and its p is 0, but 0
 // times a V of infinity or NaN is NaN in the product of the whole tile, so a row that ends with sums that are not finite is
 // summed again key by key over its own keys alone (slow_row): nothing for finite caches.
+#include <type_traits>
+
 #include "delta_common.h"
 #include "mfma32.h"
 #include "score_rule.h"
@@ -34,6 +36,21 @@ constexpr int kTargetBlocks = 512;     // two 4-wave blocks for each CU
 constexpr int kMinSteps = 8;           // a part's steps, at least
 constexpr int kMaxParts = 1024;
 constexpr int kSplitWaves = 4;         // waves of a block where rows may be cut
+
+// What the rule does to the scores, a kernel each (a branch in the step costs the instructions that the compiler moves out
+// of it): nothing, a cap alone, slopes alone, anything.  kCappedRef: a cap alone, and the exponents' reference is a
+// constant.
+enum ScoreMode { kPlain = 0, kCapped = 1, kCappedRef = 2, kLeaning = 3, kAny = 4 };
+
+// A cap c alone: c tanh(y), y = x s / c, in log2 units is xs r + xo with r = -1 / (1 + e^(2 y)), xs = 2 c log2 e and
+// xo = c log2 e; off by 2^-22 c, so for caps up to kQuickCap (1.5e-5) and smaller ones alone.  (tanh as a polynomial of x,
+// one multiply-add a degree, took 739 us where this takes 670: a step's exponentials and reciprocals cost two issue slots
+// each, no more.)
+constexpr float kQuickCap = 64.f;
+struct CapArgs {
+  float k, xs, xo;  // k = 2 log2 e s / c
+  float ref;        // kCappedRef: the reference, log2 units
+};
 
 struct RulePrefillArgs {
   const uint16_t *q;
@@ -52,6 +69,7 @@ struct RulePrefillArgs {
   int max_cut;      // units of cut rows that the workspace holds, 0: no row is cut
   float sm_scale;
   RuleArgs rule;
+  CapArgs cap;
   float2 *part_ml;  // [unit][hkv][wave][32 rows]
   f32x4 *part_acc;  // [unit][hkv][wave][16][64 lanes], the accumulators as the lanes hold them
 };
@@ -151,7 +169,7 @@ __device__ __forceinline__ int wave_max(int v) {
   return uniform(v);
 }
 
-template <int DT, int PW>
+template <int DT, int PW, int SM>
 __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePrefillArgs a) {
 #pragma clang fp contract(off)
   using E = Elem<DT>;
@@ -252,33 +270,37 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   };
   const uint32_t last_pg = (uint32_t)(np - 1);  // (steps exist only where pages do)
   uint32_t id[kPgWave];                         // of the step issued next; pages past the row repeat its last one
-  auto load_ids = [&](int j) {
+  int next_ids = 0;
+  auto load_ids = [&](int j) { next_ids = row_ids[min((uint32_t)(kPgStep * j + (lane & 3)), last_pg)]; };
+  auto take_ids = [&]() {
+    const int v = page_bad(next_ids) ? 0 : next_ids;
 #pragma unroll
-    for (int i = 0; i < kPgWave; ++i) {
-      const uint32_t pg = (uint32_t)(kPgStep * j + i * (PW / 4) + (wv >> 2));
-      id[i] = (uint32_t)ld_scalar(row_ids, pg < last_pg ? pg : last_pg);
-    }
+    for (int i = 0; i < kPgWave; ++i) id[i] = (uint32_t)__builtin_amdgcn_readlane(v, i * (PW / 4) + (wv >> 2));
   };
   auto issue = [&](int j, int i) {
-    const uint32_t dst = lds0 + (uint32_t)(j % kBufs) * (2 * kTileB) + i * (PW / 4) * 4096;
-    const uint32_t pid = row_bad && page_bad((int)id[i]) ? 0u : id[i];
-    const char *pg = kvh + (uint64_t)pid * page_bytes;
+    const uint32_t dst = lds0 + (uint32_t)(j & (kBufs - 1)) * (2 * kTileB) + i * (PW / 4) * 4096;
+    const char *pg = kvh + (uint64_t)id[i] * page_bytes;
     load_lds_1k(dst, pg, koff);
     load_lds_1k(dst + kTileB, pg, voff);
   };
   auto issue_step = [&](int j) {  // step j's loads, then the ids of step j + 1
 #pragma unroll
     for (int i = 0; i < kPgWave; ++i) issue(j, i);
-    load_ids(j + 1);
   };
   if (s0 < s1) {
     load_ids(s0);
+    take_ids();
+    load_ids(s0 + 1);
     issue_step(s0);
-    if (kLate && s0 + 1 < s1) issue_step(s0 + 1);
+    if (kLate && s0 + 1 < s1) {
+      take_ids();
+      load_ids(s0 + 2);
+      issue_step(s0 + 1);
+    }
   }
   uint32_t bad = 0;  // bad_of(j)
 
-  float m = -INFINITY, l = 0.f;
+  float m = SM == kCappedRef ? a.cap.ref : -INFINITY, l = 0.f;
   f32x16 acc[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
@@ -286,10 +308,12 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
     for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
   const float scale = fabsf(a.sm_scale), scale2 = scale * kLog2e;
   const bool capped = a.rule.softcap > 0.f, leaning = a.rule.slopes != nullptr;
-  // Scores that the rule changes leave it in log2 units; others keep the scale for the exponent's fma.
-  const bool scaled = capped || leaning || scale2 == 0.f;
-  const float xs = scaled ? 1.f : scale2;
+  // Scores leave the rule in log2 units but for kPlain, which keeps the scale for the exponent's fma.
+  const float xs = SM == kPlain || SM == kLeaning ? scale2 : SM == kAny ? 1.f : a.cap.xs;
+  float xo = SM == kCapped || SM == kCappedRef ? a.cap.xo : 0.f;  // (kLeaning: of the step)
+  const int first_pos = kv_len - qn + tok0;  // the wave's first query's position
   const float slope2 = leaning && row_ok ? a.rule.slopes[h * G + g] * kLog2e : 0.f;
+  const float lean = slope2 / scale2;  // kLeaning: the slope in units of the unscaled scores
   uint32_t kfo[8];  // K fragment of k-slice ks: row 32 sb + n, chunk 2 ks + hl
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) kfo[ks] = (uint32_t)(n * 256 + 16 * ((2 * ks + hl) ^ (n & 15)));
@@ -326,7 +350,6 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       if (!kLate && ks < kPgWave && j + 1 < s1) issue(j + 1, ks);  // the next step's loads go out under the MFMAs
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (!kLate && j + 1 < s1) load_ids(j + 2);
     __builtin_amdgcn_s_setprio(0);
     const int kv0 = j * kKvStep;
     const bool full = kv0 >= all0 && kv0 + kKvStep <= all1 && bad == 0;
@@ -335,16 +358,32 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
 #pragma unroll
     for (int i = 0; i < NX; ++i) x[i] = S[i >> 4][i & 15];
     auto key = [&](int i) { return 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3); };  // + kv0 + 4 hl
-    if (capped) {
-      cap_scores(x, a.rule, scale, kLog2e);
-    } else if (scaled) {
+    if constexpr (SM == kCapped || SM == kCappedRef) {
 #pragma unroll
-      for (int i = 0; i < NX; ++i) x[i] *= scale2;
-    }
-    if (leaning) {
+      for (int i = 0; i < NX; ++i) x[i] = __builtin_amdgcn_rcpf(-1.f - fast_exp2(x[i] * a.cap.k));
+    } else if constexpr (SM == kLeaning) {
       const float d0 = (float)(qpos - kv0 - 4 * hl);
+      if (kv0 + kKvStep - 1 <= first_pos) {  // no key behind a query: -lean (d0 - key), its -lean d0 a constant of the row
 #pragma unroll
-      for (int i = 0; i < NX; ++i) x[i] = fmaf(-slope2, fabsf(d0 - (float)key(i)), x[i]);
+        for (int i = 0; i < NX; ++i) x[i] = fmaf(lean, (float)key(i), x[i]);
+        xo = -slope2 * d0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < NX; ++i) x[i] = fmaf(-lean, fabsf(d0 - (float)key(i)), x[i]);
+        xo = 0.f;
+      }
+    } else if constexpr (SM == kAny) {
+      if (capped) {
+        cap_scores(x, a.rule, scale, kLog2e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NX; ++i) x[i] *= scale2;
+      }
+      if (leaning) {
+        const float d0 = (float)(qpos - kv0 - 4 * hl);
+#pragma unroll
+        for (int i = 0; i < NX; ++i) x[i] = fmaf(-slope2, fabsf(d0 - (float)key(i)), x[i]);
+      }
     }
     float pm = -INFINITY;
     if (!full) {
@@ -353,28 +392,37 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       for (int i = 0; i < NX; ++i)
         x[i] = key(i) >= l0 && key(i) < h0 && ((bad >> (2 * (i >> 4) + ((i & 15) >> 3))) & 1u) == 0 ? x[i] : -INFINITY;
     }
-#pragma unroll
-    for (int i = 0; i < NX; ++i) pm = fmaxf(pm, x[i]);
-    // m is the row's reference maximum: it moves only when a score exceeds it by more than 8 (a factor of 2^8).
-    const float smax = halves_max(pm) * xs;
-    float alpha = 1.f;
-    if (smax > m + 8.f) {  // also the first finite score of the row (m = -inf)
-      alpha = fast_exp2(m - smax);
-      m = smax;
-    }
-    const float nm = m == -INFINITY ? 0.f : -m;
     float ps = 0.f;
+    if constexpr (SM == kCappedRef) {
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      x[i] = fast_exp2(fmaf(x[i], xs, nm));
-      ps += x[i];
-    }
-    l = l * alpha + ps;  // this half's keys; the halves are summed once at the end
-    if (__ballot(alpha != 1.f)) {
+      for (int i = 0; i < NX; ++i) {
+        x[i] = fast_exp2(fmaf(x[i], xs, xo - m));
+        ps += x[i];
+      }
+      l += ps;
+    } else {
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
+      for (int i = 0; i < NX; ++i) pm = fmaxf(pm, x[i]);
+      // m is the row's reference maximum: it moves only when a score exceeds it by more than 8 (a factor of 2^8).
+      const float smax = halves_max(fmaf(pm, xs, xo));
+      float alpha = 1.f;
+      if (smax > m + 8.f) {  // also the first finite score of the row (m = -inf)
+        alpha = fast_exp2(m - smax);
+        m = smax;
+      }
+      const float nm = m == -INFINITY ? 0.f : xo - m;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+      for (int i = 0; i < NX; ++i) {
+        x[i] = fast_exp2(fmaf(x[i], xs, nm));
+        ps += x[i];
+      }
+      l = l * alpha + ps;  // this half's keys; the halves are summed once at the end
+      if (__ballot(alpha != 1.f)) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+      }
     }
 #pragma unroll
     for (int cc = 0; cc < 2 * kSub; ++cc)
@@ -414,7 +462,7 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   for (int j = s0; s0 < s1 && j < s1 + (kLate ? 1 : 0); ++j) {
     // Step j's loads have landed when at most the next step's (kLate: four) are pending.
     if (kLate && j + 1 < s1)
-      wait_loads<2 * kPgWave>();
+      wait_loads<2 * kPgWave + 1>();
     else
       wait_loads<0>();
     __builtin_amdgcn_s_barrier();
@@ -434,7 +482,11 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       asm volatile("" ::: "memory");
     }
     const bool mine = j >= w0 && j < w1;
-    if (kLate ? j + 2 < s1 : !mine && j + 1 < s1) issue_step(kLate ? j + 2 : j + 1);
+    if (kLate ? j + 2 < s1 : j + 1 < s1) {
+      take_ids();
+      load_ids(kLate ? j + 3 : j + 2);
+      if (kLate || !mine) issue_step(kLate ? j + 2 : j + 1);
+    }
     if (late) {
       if (j - 1 >= w0 && j - 1 < w1) pv_step(&tiles[(j - 1) % kBufs][0], pcar);
       if (mine) score_step(j, &tiles[j % kBufs][0], pcar);
@@ -607,6 +659,25 @@ int64_t cut_bound(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len,
   return by_work < by_size ? by_work : by_size;
 }
 
+// How the kernel treats the scores, and for a cap alone its constants.
+int score_mode(RulePrefillArgs &a, int dtype) {
+  const double scale = fabs((double)a.sm_scale);
+  if (!(scale > 0)) return kAny;
+  if (!(a.rule.softcap > 0.f)) return !a.rule.slopes ? kPlain : scale > 1e-10 ? kLeaning : kAny;
+  if (a.rule.slopes) return kAny;
+  if (a.rule.softcap > kQuickCap) return kAny;
+  const double c2 = a.rule.softcap * 1.4426950408889634;
+  a.cap.k = (float)(2 * 1.4426950408889634 * scale / a.rule.softcap);
+  a.cap.xs = (float)(2 * c2);
+  a.cap.xo = (float)c2;
+  if (!(a.cap.k < INFINITY)) return kAny;
+  // Scores lie within c2 of 0, so with p = 2^(score - ref) in [2^-125, 2^60] no maximum is needed: every p is a normal
+  // number of fp32 and bf16, and the sums stay below 2^77 max|v|.
+  const double top = 2 * c2 - 125 > 0 ? 2 * c2 - 125 : 0;
+  a.cap.ref = (float)(c2 - top);
+  return dtype == DELTA_BF16 && top <= 60 ? kCappedRef : kCapped;
+}
+
 size_t part_bytes(int64_t units, int hkv) {
   const size_t per = (size_t)kSplitWaves * 32 * (sizeof(float2) + kHeadDim * sizeof(float));
   return (units * hkv * per + 255) & ~(size_t)255;
@@ -621,10 +692,20 @@ int launch_rule(RulePrefillArgs a, int64_t num_tokens, int max_qo_len, hipStream
   a.row_tiles = (int)ceil_div(max_qo_len, BT);
   const int64_t units = a.max_cut + tiles_bound(num_tokens, a.batch, max_qo_len, BT), y = units < 32768 ? units : 32768;
   const dim3 grid((unsigned)a.hkv, (unsigned)y, (unsigned)ceil_div(units, y));
-  if (wide)
-    hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 8>), grid, dim3(512), 0, stream, a);
-  else
-    hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 4>), grid, dim3(256), 0, stream, a);
+  auto launch = [&](auto sm) {
+    constexpr int SM = decltype(sm)::value;
+    if (wide)
+      hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 8, SM>), grid, dim3(512), 0, stream, a);
+    else
+      hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 4, SM>), grid, dim3(256), 0, stream, a);
+  };
+  switch (score_mode(a, DT)) {
+    case kPlain: launch(std::integral_constant<int, kPlain>()); break;
+    case kCapped: launch(std::integral_constant<int, kCapped>()); break;
+    case kCappedRef: launch(std::integral_constant<int, kCappedRef>()); break;
+    case kLeaning: launch(std::integral_constant<int, kLeaning>()); break;
+    default: launch(std::integral_constant<int, kAny>()); break;
+  }
   const int rc = check_launch(who);
   if (rc || a.max_cut == 0) return rc;
   hipLaunchKernelGGL((rule_join_kernel<DT>), dim3((unsigned)a.hkv, (unsigned)a.max_cut), dim3(kSplitWaves * 64), 0, stream, a);
