@@ -175,18 +175,10 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
       st128(a.cache + ((((int64_t)pid * 2 + is_v) * kPageSize + slot) * a.hkv + hk) * kHeadDim + 8 * t, out);
     }
   };
-  // Every lane of a wave goes through a pass that any of its heads has: the lane permutes read their neighbours.
-  const int first_of_wave = uniform(first - (lane >> 4));
 #pragma unroll
-  for (int p = 0; p < kPre; ++p) {
-    if (first_of_wave + p * step >= nh) return;
-    const int h = first + p * step;
-    if (h < nh) one(h, pre[p]);
-  }
-  for (int p = kPre; first_of_wave + p * step < nh; ++p) {
-    const int h = first + p * step;
-    if (h < nh) one(h, ld128(src(h) + 8 * t));
-  }
+  for (int p = 0; p < kPre; ++p)
+    if (first + p * step < nh) one(first + p * step, pre[p]);
+  for (int h = first + kPre * step; h < nh; h += step) one(h, ld128(src(h) + 8 * t));
 }
 
 // Blocks over a token's heads: one pass each until the chip's block slots are filled, then one block a token, whose
@@ -292,7 +284,7 @@ extern "C" DELTA_EXPORT int delta_qk_norm_rope_append(const delta_rotary_t *rota
   const int rc = common(a, rotary, norm, q, q_stride, k, k_stride, q_out, q_out_stride, kv_append_indptr, offsets, nnz,
                         batch, num_qo_heads, num_kv_heads, head_dim, dtype, who);
   if (rc) return rc;
-  if (!v || !kv_cache || !kv_indices || !kv_indptr || !kv_last_page_len)
+  if (!v || !kv_cache || (!kv_indices && kv_indices_len > 0) || !kv_indptr || !kv_last_page_len)
     return set_error(DELTA_ERR_INVALID, "%s: null pointer", who);
   if ((((uintptr_t)v | (uintptr_t)kv_cache) & 15u) || (v_stride % 8))
     return set_error(DELTA_ERR_INVALID, "%s: v and kv_cache 16-byte aligned, v stride a multiple of 8", who);

@@ -547,45 +547,55 @@ def rotary(rotary_dim: int = HEAD_DIM, *, interleaved: bool = False, device=None
     return Rotary(t, rotary_dim, bool(interleaved), f, _lib.RotaryC(t.data_ptr(), rotary_dim, int(bool(interleaved)), f))
 
 
-def _norm_rope_args(q, k, indptr, offsets, rot, q_weight, k_weight, eps, *others):
-    """Device, row count and the C structures of the two norm + rotation calls, after their common checks."""
-    dev = q.device
-    for t in (q, k, indptr, offsets, *others, q_weight, k_weight, None if rot is None else rot.turns):
-        if t is not None and (not t.is_cuda or t.device != dev):
-            _check_cuda(t, device=dev)
-    dtype = q.dtype
-    _dtype_code(q)
-    for name, t in (("q", q), ("k", k)):
-        s = t.stride()
-        if t.dim() != 3 or t.shape[2] != HEAD_DIM or s[2] != 1 or (s[1] != HEAD_DIM and t.shape[1] != 1) or s[0] % 8 \
-                or t.data_ptr() % 16:
-            raise ValueError(f"{name} must be [nnz, heads, 128] with contiguous heads and 16-byte aligned rows")
-        if t.dtype != dtype:
-            raise TypeError("q and k must share a dtype")
-    if k.shape[0] != q.shape[0]:
-        raise ValueError("q and k token counts differ")
-    B = indptr.numel() - 1
-    if B < 0:
-        raise ValueError("indptr needs >= 1 entries")
-    _check_i32("indptr", indptr)
-    _check_i32("offsets", offsets, B)
-    norm = None
-    if q_weight is not None or k_weight is not None:
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is None or w.dtype != dtype or w.numel() != HEAD_DIM or not w.is_contiguous() or w.data_ptr() % 16:
-                raise ValueError(f"{name} must be a contiguous, 16-byte aligned [128] tensor of q's dtype (both weights or none)")
-        norm = ctypes.byref(_lib.HeadNormC(q_weight.data_ptr(), k_weight.data_ptr(), float(eps)))
-    return dev, B, None if rot is None else ctypes.byref(rot.c), norm
+# The calls below take a few microseconds on the GPU, so what they check on the host they check in as few steps as that
+# takes: one condition over all of it, and only where that fails the checks that say what is wrong.
+def _launch(index: int, name: str, *args) -> None:
+    """``_lib.call`` on GPU ``index``'s current stream."""
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _rows_like(name: str, out: Optional[torch.Tensor], ref: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(ref.shape, dtype=ref.dtype, device=ref.device)
-    s = out.stride()
-    if out.shape != ref.shape or out.dtype != ref.dtype or s[2] != 1 or (s[1] != HEAD_DIM and ref.shape[1] != 1) \
-            or s[0] % 8 or out.data_ptr() % 16:
-        raise ValueError(f"{name} must match its input's shape and dtype with contiguous heads and 16-byte aligned rows")
-    return out
+def _same_gpu(first: torch.Tensor, *tensors) -> int:
+    """The GPU that all the tensors (None: left out) are on."""
+    index = first.get_device()
+    if index < 0:
+        _check_cuda(first)
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _check_cuda(t, device=first.device)
+    return index
+
+
+def _head_rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: Optional[int] = None, rows: Optional[int] = None):
+    """(rows, heads, row stride) of [rows, heads, 128] with contiguous heads and 16-byte aligned rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1 or (stride[1] != HEAD_DIM and shape[1] != 1) \
+            or stride[0] % 8 or t.data_ptr() % 16 or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [nnz, {heads or 'heads'}, 128] with contiguous heads and 16-byte aligned rows")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, as q, is {t.dtype}")
+    if rows is not None and shape[0] != rows:
+        raise ValueError(f"{name} holds {shape[0]} tokens, q {rows}")
+    return shape[0], shape[1], stride[0]
+
+
+def _norm_c(dtype, q_weight, k_weight, eps):
+    if q_weight is None and k_weight is None:
+        return None
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None or w.dtype is not dtype or w.numel() != HEAD_DIM or not w.is_contiguous() or w.data_ptr() % 16:
+            raise ValueError(f"{name} must be a contiguous, 16-byte aligned [128] tensor of q's dtype (both weights or none)")
+    return ctypes.byref(_lib.HeadNormC(q_weight.data_ptr(), k_weight.data_ptr(), eps))
+
+
+def _i32_tables(*named) -> None:
+    """``_check_i32`` of (name, tensor, least entries), for each."""
+    for name, t, n in named:
+        if t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous():
+            _check_i32(name, t, n)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, indptr: torch.Tensor, offsets: torch.Tensor,
@@ -597,11 +607,19 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, indptr: torch.Tensor, offsets
 
     Token i of row b (rows from ``indptr``) is at position ``offsets[b] + i - indptr[b]``; tokens of no row are left
     as they were."""
-    dev, B, rot, norm = _norm_rope_args(q, k, indptr, offsets, rotary, q_weight, k_weight, eps, q_out, k_out)
-    q_out, k_out = _rows_like("q_out", q_out, q), _rows_like("k_out", k_out, k)
-    _call_on(dev, "delta_qk_norm_rope", rot, norm, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), q_out.data_ptr(),
-             q_out.stride(0), k_out.data_ptr(), k_out.stride(0), indptr.data_ptr(), offsets.data_ptr(), q.shape[0], B,
-             q.shape[1], k.shape[1], HEAD_DIM, _DTYPES[q.dtype])
+    gpu = _same_gpu(q, k, indptr, offsets, q_weight, k_weight, q_out, k_out, None if rotary is None else rotary.turns)
+    dtype = q.dtype
+    code = _dtype_code(q)
+    T, hq, qs = _head_rows("q", q, dtype)
+    _, hkv, ks = _head_rows("k", k, dtype, None, T)
+    B = indptr.numel() - 1
+    _i32_tables(("indptr", indptr, 1), ("offsets", offsets, B))
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    k_out = torch.empty_like(k) if k_out is None else k_out
+    qos, kos = _head_rows("q_out", q_out, dtype, hq, T)[2], _head_rows("k_out", k_out, dtype, hkv, T)[2]
+    _launch(gpu, "delta_qk_norm_rope", None if rotary is None else rotary.c, _norm_c(dtype, q_weight, k_weight, eps),
+            q.data_ptr(), qs, k.data_ptr(), ks, q_out.data_ptr(), qos, k_out.data_ptr(), kos, indptr.data_ptr(),
+            offsets.data_ptr(), T, B, hq, hkv, HEAD_DIM, code)
     return q_out, k_out
 
 
@@ -612,27 +630,30 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_ap
                         eps: float = 1e-6, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``qk_norm_rope`` then ``append_kv`` of its keys and of ``v`` in one launch (``delta_qk_norm_rope_append``);
     returns the rotated q (``q_out``, which may be q itself)."""
-    dev, B, rot, norm = _norm_rope_args(q, k, kv_append_indptr, offsets, rotary, q_weight, k_weight, eps, v, kv_cache,
-                                        kv_indices, kv_indptr, kv_last_page_len, q_out)
+    gpu = _same_gpu(q, k, v, kv_append_indptr, offsets, kv_cache, kv_indices, kv_indptr, kv_last_page_len, q_weight, k_weight,
+                    q_out, None if rotary is None else rotary.turns)
+    dtype = q.dtype
+    code = _dtype_code(q)
     _check_cache(kv_cache)
-    s = v.stride()
-    if k.shape[1] != kv_cache.shape[3] or v.shape != k.shape or s[2] != 1 or (s[1] != HEAD_DIM and v.shape[1] != 1) \
-            or s[0] % 8 or v.data_ptr() % 16:
-        raise ValueError(f"k and v must be [nnz, {kv_cache.shape[3]}, 128] with contiguous heads and 16-byte aligned rows")
-    if v.dtype != q.dtype or kv_cache.dtype != q.dtype:
-        raise TypeError("q, k, v and kv_cache must share a dtype")
-    _check_i32("kv_indices", kv_indices)
-    _check_i32("kv_indptr", kv_indptr, B + 1)
-    _check_i32("kv_last_page_len", kv_last_page_len, B)
-    q_out = _rows_like("q_out", q_out, q)
-    _call_on(dev, "delta_qk_norm_rope_append", rot, norm, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
-             s[0], q_out.data_ptr(), q_out.stride(0), kv_append_indptr.data_ptr(), offsets.data_ptr(), kv_cache.data_ptr(),
-             kv_cache.shape[0], kv_indices.data_ptr(), kv_indices.numel(), kv_indptr.data_ptr(),
-             kv_last_page_len.data_ptr(), q.shape[0], B, q.shape[1], k.shape[1], HEAD_DIM, _DTYPES[q.dtype])
+    if kv_cache.dtype is not dtype:
+        raise TypeError(f"kv_cache must be {dtype}, as q, is {kv_cache.dtype}")
+    pages, _, _, hkv, _ = kv_cache.shape
+    T, hq, qs = _head_rows("q", q, dtype)
+    ks, vs = _head_rows("k", k, dtype, hkv, T)[2], _head_rows("v", v, dtype, hkv, T)[2]
+    B = kv_append_indptr.numel() - 1
+    _i32_tables(("kv_append_indptr", kv_append_indptr, 1), ("offsets", offsets, B), ("kv_indices", kv_indices, 0),
+                ("kv_indptr", kv_indptr, B + 1), ("kv_last_page_len", kv_last_page_len, B))
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    qos = _head_rows("q_out", q_out, dtype, hq, T)[2]
+    _launch(gpu, "delta_qk_norm_rope_append", None if rotary is None else rotary.c,
+            _norm_c(dtype, q_weight, k_weight, eps), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+            q_out.data_ptr(), qos, kv_append_indptr.data_ptr(), offsets.data_ptr(), kv_cache.data_ptr(), pages,
+            kv_indices.data_ptr(), kv_indices.numel(), kv_indptr.data_ptr(), kv_last_page_len.data_ptr(), T, B, hq, hkv,
+            HEAD_DIM, code)
     return q_out
 
 
-@dataclass(frozen=True)
+@dataclass
 class ScoreRule:
     """What attention does to the score ``x = q.k * sm_scale`` of a query token at position ``pos`` and a key
     (``delta_score_rule_t``), in this order:
@@ -653,48 +674,51 @@ class ScoreRule:
     kv_end: Optional[torch.Tensor] = None
 
 
-def _rule_call(name: str, q, kv_cache, B: int, tables: tuple, rule: ScoreRule, out, lse, workspace, need, sm_scale,
-               tail: tuple) -> torch.Tensor:
-    """What the two attention calls under a score rule have in common: checks, outputs, workspace, the call.  ``tables``
-    are the row tables in the entry point's order, the page indices next to last; ``need`` sizes the workspace; ``tail``
-    the arguments between the batch and the head counts, and those behind the scale."""
-    dev = q.device
-    slopes, begin, end = rule.slopes, rule.kv_begin, rule.kv_end
-    for t in (q, kv_cache, *tables, slopes, begin, end, out, lse, workspace):
-        if t is not None and (not t.is_cuda or t.device != dev):
-            _check_cuda(t, device=dev)
+def _rule_call(name: str, q, kv_cache, B: int, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, rule: ScoreRule, out,
+               lse, workspace, size, sm_scale, longest: int) -> torch.Tensor:
+    """What the two attention calls under a score rule have in common: checks, outputs, workspace, the call.  ``size`` is
+    the workspace's query of the head counts and the window, ``longest`` the call's maximum over the rows."""
+    slopes, begin, end, window = rule.slopes, rule.kv_begin, rule.kv_end, rule.window
+    gpu = _same_gpu(q, kv_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, slopes, begin, end, out, lse, workspace)
     _check_cache(kv_cache)
     hq, hkv = _check_heads(q, kv_cache)
-    T, indices = q.shape[0], tables[-2]
-    _check_i32("kv_indptr", tables[-3], B + 1)
-    _check_i32("kv_indices", indices)
-    _check_i32("kv_last_page_len", tables[-1], B)
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != hq or not slopes.is_contiguous()):
+    T = q.shape[0]
+    _i32_tables(("kv_indptr", kv_indptr, B + 1), ("kv_indices", kv_indices, 0), ("kv_last_page_len", kv_last_page_len, B))
+    if slopes is not None and (slopes.dtype is not torch.float32 or slopes.numel() != hq or not slopes.is_contiguous()):
         raise ValueError(f"slopes must be contiguous fp32 [{hq}]")
     if begin is not None:
         _check_i32("kv_begin", begin, T)
     if end is not None:
         _check_i32("kv_end", end, T)
-    if not 0 <= rule.window < 1 << 31:
-        raise ValueError(f"window must be 0 (none) or a positive int32, got {rule.window}")
+    if not 0 <= window < 1 << 31:
+        raise ValueError(f"window must be 0 (none) or a positive int32, got {window}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.stride(2) != 1:
         raise ValueError("out must match q's shape/dtype with unit inner stride")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+    ot, oh, _ = out.stride()
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (T, hq) or not lse.is_contiguous()):
         raise ValueError(f"lse must be contiguous fp32 [{T}, {hq}]")
-    need = need(hq, hkv, rule.window)
+    need = size(hq, hkv, window)
     if workspace is None:  # of this call: safe on any stream, in any capture
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.numel() * workspace.element_size() < need:
-        raise ValueError(f"workspace too small: {need} bytes needed")
-    c = _lib.ScoreRuleC(rule.softcap, _ptr(slopes), rule.window, _ptr(begin), _ptr(end))
-    _call_on(dev, name, ctypes.byref(c), q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), kv_cache.shape[0],
-             *[t.data_ptr() for t in tables[:-1]], indices.numel(), tables[-1].data_ptr(), out.data_ptr(), out.stride(0),
-             out.stride(1), _ptr(lse), B, *tail[0], hq, hkv, HEAD_DIM, _DTYPES[q.dtype],
-             _DEFAULT_SCALE if sm_scale is None else float(sm_scale), *tail[1], _ptr(workspace),
-             0 if workspace is None else workspace.numel() * workspace.element_size())
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+        if nbytes < need:
+            raise ValueError(f"workspace too small: {need} bytes needed")
+        need = nbytes
+    qt, qh, _ = q.stride()
+    args = (_lib.ScoreRuleC(rule.softcap, _ptr(slopes), window, _ptr(begin), _ptr(end)), q.data_ptr(), qt, qh,
+            kv_cache.data_ptr(), kv_cache.shape[0])
+    tables = (kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), out.data_ptr(),
+              ot, oh, _ptr(lse), B)
+    scale = _DEFAULT_SCALE if sm_scale is None else float(sm_scale)
+    ws = _ptr(workspace), need
+    if qo_indptr is None:
+        _launch(gpu, name, *args, *tables, hq, hkv, HEAD_DIM, _DTYPES[q.dtype], scale, longest, *ws)
+    else:
+        _launch(gpu, name, *args, qo_indptr.data_ptr(), *tables, T, longest, hq, hkv, HEAD_DIM, _DTYPES[q.dtype], scale, *ws)
     return out
 
 
@@ -720,8 +744,8 @@ def paged_decode_rule(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torch.
 
     ``workspace`` (``decode_rule_workspace_bytes``) is allocated for the call where none is given."""
     B, mp = q.shape[0], int(max_pages_per_row)
-    return _rule_call("delta_paged_decode_rule", q, kv_cache, B, (kv_indptr, kv_indices, kv_last_page_len), rule, out, lse,
-                      workspace, lambda hq, hkv, w: decode_rule_workspace_bytes(B, hq, hkv, mp, w), sm_scale, ((), (mp,)))
+    return _rule_call("delta_paged_decode_rule", q, kv_cache, B, None, kv_indptr, kv_indices, kv_last_page_len, rule, out,
+                      lse, workspace, lambda hq, hkv, w: decode_rule_workspace_bytes(B, hq, hkv, mp, w), sm_scale, mp)
 
 
 def paged_prefill_rule(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor,
@@ -733,11 +757,11 @@ def paged_prefill_rule(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch
 
     ``out`` and ``lse`` of tokens behind the last row are left as they were.  ``workspace``
     (``prefill_rule_workspace_bytes``) is allocated for the call where none is given."""
-    _check_i32("qo_indptr", qo_indptr, 1)
+    _i32_tables(("qo_indptr", qo_indptr, 1))
     B, T, mq, pages = qo_indptr.numel() - 1, q.shape[0], int(max_qo_len), kv_indices.numel()
-    return _rule_call("delta_paged_prefill_rule", q, kv_cache, B, (qo_indptr, kv_indptr, kv_indices, kv_last_page_len),
-                      rule, out, lse, workspace, lambda hq, hkv, w: prefill_rule_workspace_bytes(T, B, hq, hkv, mq, pages, w),
-                      sm_scale, ((T, mq), ()))
+    return _rule_call("delta_paged_prefill_rule", q, kv_cache, B, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, rule,
+                      out, lse, workspace, lambda hq, hkv, w: prefill_rule_workspace_bytes(T, B, hq, hkv, mq, pages, w),
+                      sm_scale, mq)
 
 
 def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, *,
