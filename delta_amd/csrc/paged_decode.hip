@@ -1440,7 +1440,7 @@ static int run_decode_any(const void *q, int64_t q_stride_b, int64_t q_stride_h,
   if (G > kMaxGroup) return set_error(DELTA_ERR_INVALID, "%s: group size %d > %d unsupported", who, G, kMaxGroup);
   if (hkv > kMaxWaves) return set_error(DELTA_ERR_INVALID, "%s: num_kv_heads %d > %d unsupported", who, hkv, kMaxWaves);
   if (dtype != DELTA_BF16 && dtype != DELTA_FP16) return set_error(DELTA_ERR_INVALID, "%s: dtype must be bf16 or fp16", who);
-  if (!q || !kv_cache || !kv_indptr || !kv_indices || !kv_last_page_len)
+  if (!q || !kv_cache || !kv_indptr || (!kv_indices && !(rule && kv_indices_len == 0)) || !kv_last_page_len)
     return set_error(DELTA_ERR_INVALID, "%s: null input pointer", who);
   // `dump` is the [batch][hkv][stride_h] per-token maxima output of the TOKMAX modes
   const bool tokmax = mode == kScoreTokmax || mode == kAttnTokmax;
@@ -1498,6 +1498,16 @@ static int run_decode_any(const void *q, int64_t q_stride_b, int64_t q_stride_h,
     a.hb = 1;
     a.direct = kPacked;
     waves = kHeadMajorWaves;
+    a.chunk = max_pages;
+  }
+  // Few pairs and rows of 5-32 pages under a rule (short contexts, windows up to 500): 16 waves of at most two pages each
+  // and no second launch (us split and merged / 16 waves; 2 pairs of 6 q heads 16 pages 7.7 / 6.9, 32 pages 9.6 / 9.0; 128
+  // pairs of 4 8.0 / 7.1, 12.6 / 11.8; 240 pairs of 5 8.5 / 8.2, 18.2 / 13.9; 63 pages 11.2 / 12.4 and 17.0 / 18.6).
+  if (mode == kAttnRule && (int64_t)batch * hkv < kHeadMajorPairs && max_pages > 4 && max_pages <= 32) {
+    a.nsplit = 1;
+    a.hb = 1;
+    a.direct = kPacked;
+    waves = kMaxWaves;
     a.chunk = max_pages;
   }
   // Unsplit head-major launches with more blocks than CUs deal ragged rows to CUs evenly.
