@@ -35,6 +35,7 @@ constexpr int kTileB = kKvStep * 256;  // bytes of a step's K (or V) tile: 64 ro
 constexpr int kTargetBlocks = 512;     // two 4-wave blocks for each CU
 constexpr int kMinSteps = 8;           // a part's steps, at least
 constexpr int kMaxParts = 1024;
+constexpr int kJoin = 16;              // parts whose sums the join loads together
 constexpr int kSplitWaves = 4;         // waves of a block where rows may be cut
 
 // What the rule does to the scores, a kernel each (a branch in the step costs the instructions that the compiler moves out
@@ -71,6 +72,7 @@ struct RulePrefillArgs {
   RuleArgs rule;
   CapArgs cap;
   float2 *part_ml;  // [unit][hkv][wave][32 rows]
+  float *part_le;   // likewise
   f32x4 *part_acc;  // [unit][hkv][wave][16][64 lanes], the accumulators as the lanes hold them
 };
 
@@ -116,6 +118,7 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
     const int span = a.rule.window > 0 && a.rule.window < x.kv_len - BT ? a.rule.window + BT : x.kv_len;
     return (span + kKvStep - 1) / kKvStep;
   };
+  const int lanes = a.batch > 32 ? 64 : a.batch > 8 ? 32 : a.batch > 2 ? 8 : 2;  // that hold rows (sums stop there)
   int C = 0;
   if (a.max_cut > 0) {
     float w = 0.f;  // (an estimate; every block of the launch gets the same one)
@@ -123,10 +126,9 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
       const RowBounds x = row_bounds(a, r0 + lane);
       w += (float)tiles_of(x) * (float)steps_of(x);
     }
-    for (int off = 32; off > 0; off >>= 1) w += shfl_xor(w, off);
-    w = w * (float)a.hkv * (1.f / kTargetBlocks);
+    for (int off = lanes >> 1; off > 0; off >>= 1) w += shfl_xor(w, off);
+    w = readlane(w, 0) * (float)a.hkv * (1.f / kTargetBlocks);
     C = w < (float)kMinSteps ? kMinSteps : w > 1e8f ? 100000000 : (int)w + 1;
-    C = uniform(C);
   }
   auto parts_of = [&](const RowBounds &x) {
     const int s = steps_of(x);
@@ -139,12 +141,11 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
       const int parts = parts_of(mine);
       const int n = (parts > 1) == (pass == 0) ? tiles_of(mine) * parts : 0;
       int incl = n;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
+      for (int off = 1; off < lanes; off <<= 1) {
         const int v = __shfl_up(incl, off, 64);
         if (lane >= off) incl += v;
       }
-      const uint64_t m = __ballot(base + incl > u);
+      const uint64_t m = __ballot(base + incl > u);  // (the first such lane is a row's)
       if (m != 0) {
         const int l = __builtin_ctzll(m);
         unit->row = bounds_of_lane(mine, l);
@@ -154,19 +155,36 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
         unit->part = unit->parts - 1 - (at - unit->tile * unit->parts);
         return true;
       }
-      base += __builtin_amdgcn_readlane(incl, 63);
+      base += __builtin_amdgcn_readlane(incl, lanes - 1);
     }
   }
   return false;
 }
 
-__device__ __forceinline__ int wave_min(int v) {
-  for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
-  return uniform(v);
+// c + the sum of two packed 16-bit values, in fp32
+template <int DT>
+__device__ __forceinline__ float add2(uint32_t v, float c) {
+  if constexpr (DT == DELTA_BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v), __builtin_bit_cast(b2, 0x3f803f80u), c, false);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v), __builtin_bit_cast(h2, 0x3c003c00u), c, false);
+  }
 }
-__device__ __forceinline__ int wave_max(int v) {
-  for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
-  return uniform(v);
+
+// Over a wave: the 16-lane rows by DPP, the four rows by permlane swaps.
+template <bool MAX>
+__device__ __forceinline__ int wave_extreme(int v) {
+  auto pick = [](int a, int b) { return MAX ? max(a, b) : min(a, b); };
+  v = pick(v, dpp_i<0xB1>(v));
+  v = pick(v, dpp_i<0x4E>(v));
+  v = pick(v, dpp_i<0x141>(v));
+  v = pick(v, dpp_i<0x140>(v));
+  auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = pick((int)a[0], (int)a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return uniform(pick((int)b[0], (int)b[1]));
 }
 
 template <int DT, int PW, int SM>
@@ -197,12 +215,9 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   const int qpos = kv_len - qn + tok0 + tt;
   u32x4 qf[8];  // B operand of S^T = K Q^T: d = 16 ks + 8 hl + [0, 8)
   if (row_ok) {
-    // With a negative scale q's signs are flipped (the scale below is then positive).  The xor also makes the loads
-    // complete here, before the kv loop.
-    const uint32_t flip = a.sm_scale < 0.f ? 0x80008000u : 0u;
     const uint16_t *qp = a.q + (q0 + tok0 + tt) * a.q_stride_t + (int64_t)(h * G + g) * a.q_stride_h + 8 * hl;
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qf[ks] = ld128(qp + 16 * ks) ^ u32x4{flip, flip, flip, flip};
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = ld128(qp + 16 * ks);
   } else {
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) qf[ks] = u32x4{0u, 0u, 0u, 0u};
@@ -212,24 +227,38 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
     key_range(a.rule, q0 + tok0 + tt, qpos, kv_len, &lo, &hi);
     if (hi <= lo) lo = hi = 0;
   }
-  // The wave's rows together: the first and last key any of them sees, and the keys that all of them see.
-  const int any0 = wave_min(hi > lo ? lo : INT32_MAX), any1 = wave_max(hi);
-  const int all0 = wave_max(row_ok ? lo : 0), all1 = wave_min(row_ok ? hi : INT32_MAX);
-  // The block's tokens together.
-  int blo = INT32_MAX, bhi = 0;
-  for (int t0 = btok0; t0 < min(btok0 + BT, qn); t0 += 64) {
-    const int tk = t0 + lane;
-    if (tk < min(btok0 + BT, qn)) {
-      int l2, h2;
-      key_range(a.rule, q0 + tk, kv_len - qn + tk, kv_len, &l2, &h2);
-      if (h2 > l2) {
-        blo = min(blo, l2);
-        bhi = max(bhi, h2);
+  // The wave's rows together: the first and last key any of them sees, and the keys that all of them see; and the block's
+  // tokens together.  Without bounds of their own the tokens' ranges move up with them: the first and last one's say it all.
+  const int wtok1 = min(tok0 + TW, qn), btok1 = min(btok0 + BT, qn);
+  int any0, any1, all0, all1, blo, bhi;
+  if (!a.rule.kv_begin && !a.rule.kv_end) {
+    int unused;
+    key_range(a.rule, 0, kv_len - qn + tok0, kv_len, &any0, &all1);
+    key_range(a.rule, 0, kv_len - qn + wtok1 - 1, kv_len, &all0, &any1);
+    if (wtok1 <= tok0) any1 = 0;
+    key_range(a.rule, 0, kv_len - qn + btok0, kv_len, &blo, &unused);
+    key_range(a.rule, 0, kv_len - qn + btok1 - 1, kv_len, &unused, &bhi);
+  } else {
+    any0 = wave_extreme<false>(hi > lo ? lo : INT32_MAX);
+    any1 = wave_extreme<true>(hi);
+    all0 = wave_extreme<true>(row_ok ? lo : 0);
+    all1 = wave_extreme<false>(row_ok ? hi : INT32_MAX);
+    blo = INT32_MAX;
+    bhi = 0;
+    for (int t0 = btok0; t0 < btok1; t0 += 64) {
+      const int tk = t0 + lane;
+      if (tk < btok1) {
+        int l2, h2;
+        key_range(a.rule, q0 + tk, kv_len - qn + tk, kv_len, &l2, &h2);
+        if (h2 > l2) {
+          blo = min(blo, l2);
+          bhi = max(bhi, h2);
+        }
       }
     }
+    blo = wave_extreme<false>(blo);
+    bhi = wave_extreme<true>(bhi);
   }
-  blo = wave_min(blo);
-  bhi = wave_max(bhi);
   // The block's steps [s0, s1) (its part of them) and the wave's.
   int s0 = 0, s1 = 0;
   if (bhi > blo) {
@@ -255,10 +284,6 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   const char *const kvh = reinterpret_cast<const char *>(a.kv) + (int64_t)h * (kHeadDim * 2);
   const int32_t *const row_ids = a.kv_indices + un.row.p0;
   auto page_bad = [&](int pid) { return pid < 0 || (int64_t)pid >= a.num_pages; };
-  // Ids outside the cache are looked for once over the part's pages; steps of a row without any take its ids as they are.
-  bool row_bad = false;
-  for (int i = s0 * kPgStep; i < s1 * kPgStep && i < np; i += 64)
-    row_bad |= __ballot(i + lane < np && i + lane < s1 * kPgStep && page_bad(row_ids[i + lane < np ? i + lane : 0])) != 0;
   auto bad_of = [&](int j) {  // bit i: page i of step j lies outside the cache
     uint32_t r = 0;
 #pragma unroll
@@ -298,9 +323,22 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       issue_step(s0 + 1);
     }
   }
+  // With a negative scale q's signs are flipped (the scale below is then positive).  The xor also makes q's loads, in flight
+  // beside the first keys', complete here, before the kv loop.
+  const uint32_t flip = a.sm_scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) qf[ks] ^= u32x4{flip, flip, flip, flip};
+  // Ids outside the cache are looked for once over the part's pages; steps of a row without any take its ids as they are.
+  bool row_bad = false;
+  for (int i = s0 * kPgStep; i < s1 * kPgStep && i < np; i += 64)
+    row_bad |= __ballot(i + lane < np && i + lane < s1 * kPgStep && page_bad(row_ids[i + lane < np ? i + lane : 0])) != 0;
   uint32_t bad = 0;  // bad_of(j)
 
-  float m = SM == kCappedRef ? a.cap.ref : -INFINITY, l = 0.f;
+  // p is rounded to 16 bits for its product with V.  A row is divided by l, which in steps with masks adds up the rounded
+  // p: a row of one key is that key's v, and a few keys' weights add up to 1.  Over whole steps the roundings of 64 keys and
+  // more average out, and l takes the fp32 p as le does, the sum for the lse (rounded ones there as well took 8192 tokens
+  // with a cap from 613 to 627 us).
+  float m = SM == kCappedRef ? a.cap.ref : -INFINITY, l = 0.f, le = 0.f;
   f32x16 acc[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
@@ -392,20 +430,18 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       for (int i = 0; i < NX; ++i)
         x[i] = key(i) >= l0 && key(i) < h0 && ((bad >> (2 * (i >> 4) + ((i & 15) >> 3))) & 1u) == 0 ? x[i] : -INFINITY;
     }
-    float ps = 0.f;
+    float alpha = 1.f, pe = 0.f;
     if constexpr (SM == kCappedRef) {
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
         x[i] = fast_exp2(fmaf(x[i], xs, xo - m));
-        ps += x[i];
+        pe += x[i];
       }
-      l += ps;
     } else {
 #pragma unroll
       for (int i = 0; i < NX; ++i) pm = fmaxf(pm, x[i]);
       // m is the row's reference maximum: it moves only when a score exceeds it by more than 8 (a factor of 2^8).
       const float smax = halves_max(fmaf(pm, xs, xo));
-      float alpha = 1.f;
       if (smax > m + 8.f) {  // also the first finite score of the row (m = -inf)
         alpha = fast_exp2(m - smax);
         m = smax;
@@ -414,9 +450,8 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
         x[i] = fast_exp2(fmaf(x[i], xs, nm));
-        ps += x[i];
+        pe += x[i];
       }
-      l = l * alpha + ps;  // this half's keys; the halves are summed once at the end
       if (__ballot(alpha != 1.f)) {
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
@@ -428,6 +463,16 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
     for (int cc = 0; cc < 2 * kSub; ++cc)
 #pragma unroll
       for (int w = 0; w < 4; ++w) pc[cc][w] = pack2<DT>(x[8 * cc + 2 * w], x[8 * cc + 2 * w + 1]);
+    float ps = pe;
+    if (!full) {
+      ps = 0.f;
+#pragma unroll
+      for (int cc = 0; cc < 2 * kSub; ++cc)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) ps = add2<DT>(pc[cc][w], ps);
+    }
+    l = l * alpha + ps;  // this half's keys; the halves are summed once at the end
+    le = le * alpha + pe;
   };
   // O^T += V^T P^T of a step whose P^T is in pc.
   auto pv_step = [&](const char *tk, const u32x4 (&pc)[2 * kSub]) {
@@ -498,6 +543,7 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   }
 
   l = halves_sum(l);
+  le = halves_sum(le);
   // Rows whose sums are not finite though their scores are: slow_row's.
   bool odd = false;
 #pragma unroll
@@ -512,6 +558,7 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   uint16_t *const orow = a.o + (q0 + tok0 + tt) * a.o_stride_t + (int64_t)(h * G + g) * a.o_stride_h;
   if (un.parts > 1) {
     if (hl == 0) a.part_ml[pslot * 32 + n] = float2{m, l};
+    if (a.lse && hl == 0) a.part_le[pslot * 32 + n] = le;
     if (w0 < w1 && sums_ok) {  // (l = 0 of a wave without steps: the join takes no sums)
 #pragma unroll
       for (int c = 0; c < 16; ++c)
@@ -528,17 +575,17 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       w.y = pack2<DT>(acc[c >> 2][4 * (c & 3) + 2] * inv, acc[c >> 2][4 * (c & 3) + 3] * inv);
       *reinterpret_cast<uint2 *>(orow + 4 * hl + 32 * (c >> 2) + 8 * (c & 3)) = w;
     }
-    if (a.lse && hl == 0) a.lse[(q0 + tok0 + tt) * a.hq + h * G + g] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (a.lse && hl == 0) a.lse[(q0 + tok0 + tt) * a.hq + h * G + g] = l != 0.f ? (m + log2f(le)) * kLn2 : -INFINITY;
   }
 
   // slow_row: the sums again, key by key, over the row's own keys.
   for (uint32_t rows = odd_rows; rows != 0; rows &= rows - 1) {
     const int rn = __builtin_ctz(rows);
     const int rlo = max(__builtin_amdgcn_readlane(lo, rn), s0 * kKvStep), rhi = min(__builtin_amdgcn_readlane(hi, rn), s1 * kKvStep);
-    const float rm = readlane(m, rn), rl = readlane(l, rn), rs = readlane(slope2, rn);
+    const float rm = readlane(m, rn), rs = readlane(slope2, rn);
     const int rt = rn / G, rg = rn - rt * G, rpos = __builtin_amdgcn_readlane(qpos, rn);
     const uint16_t *qp = a.q + (q0 + tok0 + rt) * a.q_stride_t + (int64_t)(h * G + rg) * a.q_stride_h;
-    float o0 = 0.f, o1 = 0.f;  // d = 2 lane, 2 lane + 1
+    float rl = 0.f, o0 = 0.f, o1 = 0.f;  // d = 2 lane, 2 lane + 1
     for (int c0 = rlo; c0 < rhi; c0 += 64) {
       const int k = c0 + lane;
       int pid = k < rhi && k / kPageSize < np ? row_ids[k / kPageSize] : -1;
@@ -561,6 +608,7 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       for (uint64_t keys = __ballot(pid >= 0); keys != 0; keys &= keys - 1) {
         const int kl = __builtin_ctzll(keys);
         const float pk = readlane(p, kl);
+        rl += pk;
         const uint64_t kpid = (uint32_t)__builtin_amdgcn_readlane(pid, kl);
         const uint32_t vw = reinterpret_cast<const uint32_t *>(kvh + kpid * page_bytes +
                                                                (uint32_t)(kPageSize + (c0 + kl) % kPageSize) * row_bytes)[lane];
@@ -574,6 +622,7 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       float *dst = reinterpret_cast<float *>(a.part_acc + (pslot * 16 + d / 8) * 64 + 32 * (d % 8 / 4) + rn) + d % 4;
       dst[0] = o0;
       dst[1] = o1;
+      if (lane == 0) a.part_ml[pslot * 32 + rn].y = rl;
     } else {
       const float inv = 1.f / rl;
       uint32_t *dst = reinterpret_cast<uint32_t *>(a.o + (q0 + tok0 + rt) * a.o_stride_t + (int64_t)(h * G + rg) * a.o_stride_h);
@@ -597,28 +646,33 @@ __global__ void __launch_bounds__(kSplitWaves * 64) rule_join_kernel(RulePrefill
   const int64_t first = u - un.part;
   for (int task = un.part * PW + uniform((int)(threadIdx.x >> 6)); task < waves * 16; task += un.parts * PW) {
     const int w = task >> 4, c = task & 15;
-    float M = -INFINITY, L = 0.f;
+    const bool want_lse = a.lse && c == 0;
+    float M = -INFINITY, L = 0.f, LE = 0.f;
     f32x4 A = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < un.parts; s0 += 8) {
-      float2 ml[8];
-      f32x4 av[8];
+    for (int s0 = 0; s0 < un.parts; s0 += kJoin) {
+      float2 ml[kJoin];
+      float le[kJoin];
+      f32x4 av[kJoin];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kJoin; ++i) {
         const int64_t at = ((first + min(s0 + i, un.parts - 1)) * a.hkv + h) * PW + w;
         ml[i] = a.part_ml[at * 32 + n];
+        le[i] = want_lse ? a.part_le[at * 32 + n] : 0.f;
         av[i] = a.part_acc[(at * 16 + c) * 64 + lane];
       }
       float top = M;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+      for (int i = 0; i < kJoin; ++i) top = fmaxf(top, ml[i].x);
       const float ref = top == -INFINITY ? 0.f : top, al = fast_exp2(M - ref);
       L *= al;
+      LE *= al;
       A = A * al;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kJoin; ++i) {
         if (s0 + i < un.parts && ml[i].y != 0.f) {  // a part without keys wrote no sums
           const float sc = fast_exp2(ml[i].x - ref);
           L = fmaf(ml[i].y, sc, L);
+          LE = fmaf(le[i], sc, LE);
 #pragma unroll
           for (int e = 0; e < 4; ++e) A[e] = fmaf(av[i][e], sc, A[e]);
         }
@@ -633,7 +687,7 @@ __global__ void __launch_bounds__(kSplitWaves * 64) rule_join_kernel(RulePrefill
       o.x = pack2<DT>(A[0] * inv, A[1] * inv);
       o.y = pack2<DT>(A[2] * inv, A[3] * inv);
       *reinterpret_cast<uint2 *>(a.o + t * a.o_stride_t + (int64_t)(h * G + g) * a.o_stride_h + 4 * hl + 8 * c) = o;
-      if (a.lse && c == 0 && hl == 0) a.lse[t * a.hq + h * G + g] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+      if (want_lse && hl == 0) a.lse[t * a.hq + h * G + g] = L != 0.f ? (M + log2f(LE)) * kLn2 : -INFINITY;
     }
   }
 }
@@ -679,7 +733,7 @@ int score_mode(RulePrefillArgs &a, int dtype) {
 }
 
 size_t part_bytes(int64_t units, int hkv) {
-  const size_t per = (size_t)kSplitWaves * 32 * (sizeof(float2) + kHeadDim * sizeof(float));
+  const size_t per = (size_t)kSplitWaves * 32 * (sizeof(float2) + sizeof(float) + kHeadDim * sizeof(float));
   return (units * hkv * per + 255) & ~(size_t)255;
 }
 
@@ -702,7 +756,7 @@ int launch_rule(RulePrefillArgs a, int64_t num_tokens, int max_qo_len, hipStream
   switch (score_mode(a, DT)) {
     case kPlain: launch(std::integral_constant<int, kPlain>()); break;
     case kCapped: launch(std::integral_constant<int, kCapped>()); break;
-    case kCappedRef: launch(std::integral_constant<int, kCappedRef>()); break;
+    case kCappedRef: if constexpr (DT == DELTA_BF16) launch(std::integral_constant<int, kCappedRef>()); break;
     case kLeaning: launch(std::integral_constant<int, kLeaning>()); break;
     default: launch(std::integral_constant<int, kAny>()); break;
   }
@@ -748,7 +802,7 @@ extern "C" DELTA_EXPORT int delta_paged_prefill_rule(const delta_score_rule_t *r
   RulePrefillArgs a = {};
   const int rc = rule_args(rule, &a.rule, who);
   if (rc) return rc;
-  if (!q || !kv_cache || !qo_indptr || !kv_indptr || !kv_indices || !kv_last_page_len || !o)
+  if (!q || !kv_cache || !qo_indptr || !kv_indptr || (!kv_indices && kv_indices_len > 0) || !kv_last_page_len || !o)
     return set_error(DELTA_ERR_INVALID, "%s: null pointer", who);
   if (((uintptr_t)q | (uintptr_t)kv_cache) & 15u || (q_stride_t % 8) || (q_stride_h % 8))
     return set_error(DELTA_ERR_INVALID, "%s: q and kv_cache 16-byte aligned, q strides multiples of 8", who);
@@ -786,6 +840,7 @@ extern "C" DELTA_EXPORT int delta_paged_prefill_rule(const delta_score_rule_t *r
     a.max_cut = (int)cut;
     a.part_acc = (f32x4 *)workspace;
     a.part_ml = (float2 *)(a.part_acc + (size_t)cut * num_kv_heads * kSplitWaves * 16 * 64);
+    a.part_le = (float *)(a.part_ml + (size_t)cut * num_kv_heads * kSplitWaves * 32);
   }
   if (dtype == DELTA_BF16) return launch_rule<DELTA_BF16>(a, num_tokens, max_qo_len, (hipStream_t)stream, who);
   return launch_rule<DELTA_FP16>(a, num_tokens, max_qo_len, (hipStream_t)stream, who);

@@ -1,12 +1,14 @@
 """Attention under score rules (capped, leaning by distance, windows, documents, prefixes) against a plain 64-bit
 implementation, at the sizes, tables and masks where it can go wrong.
 
-Tolerances.  P is rounded to the cache's type for P.V (half a step u = eps / 2 of each p), o once more.  A score is an fp32
+Tolerances.  P is rounded to the cache's type for P.V, each p_k to p_k (1 + d_k) with |d_k| <= u = eps / 2.  Divided by the
+sum of the p_k that is off by sum p_k |d_k v_k| <= u A, divided by the rounded ones' sum by sum p_k |d_k (v_k - want)| <=
+u (A + |want|); o is rounded once more.  A score is an fp32
 sum of 128 exact products, off by at most 128 * 2^-24 of D = max sum |q_i k_i| * scale; the cap adds 2^-21 of the cap, and
 the four roundings on the way to the exponent (scale, cap or bias, log2 e, maximum) 2^-21 of X, the largest |score| + |bias|
 among the keys that weigh anything.  e = 2^-17 D + 2^-21 (cap + X) moves every p, and the sum of p, by a factor of at most
 1 + 2 e together; exp2 and the sum add 2^-20.  With A = softmax . |v| in 64 bits:
-    |o - want| <= A (u + 2 e + 2^-20) + u |want| + n 2^-25 max|v| (fp16 only: p below its normal range)
+    |o - want| <= A (u + 2 e + 2^-20) + 2 u |want| + n 2^-25 max|v| (fp16 only: p below its normal range)
     |lse - want| <= e + 2^-20 + 2^-21 |want|."""
 import math
 import random
@@ -142,7 +144,7 @@ class Batch:
         assert torch.equal(lse.isnan(), nan) and o[nan].isnan().all()
         fin = wo.isfinite()
         assert torch.equal(o.isfinite() & ~nan[..., None], fin & ~nan[..., None]), "finite where it should not be, or the reverse"
-        tol = A * (u + 2 * e + 2.0 ** -20) + u * wo.abs() + (nv * 2.0 ** -25 if o.dtype == torch.float16 else 0.0) + 1e-30
+        tol = A * (u + 2 * e + 2.0 ** -20) + 2 * u * wo.abs() + (nv * 2.0 ** -25 if o.dtype == torch.float16 else 0.0) + 1e-30
         bad = fin & ((o.double() - wo).abs() > tol)
         assert not bad.any(), f"o off at {bad.nonzero()[:4].tolist()}: {(o.double() - wo)[bad].abs().max():.3e}"
         empty = wl == -math.inf
@@ -248,6 +250,54 @@ def test_long_prompts_in_wide_blocks(kind):
     b = Batch(32, 8, rows, "bf16", seed=5, q_std=3.0)
     rule = rule_of(kind, 32, rows)
     b.check(b.prefill(rule), b.want(rule))
+
+
+def test_more_query_tokens_than_cached_ones():
+    """Positions in front of the cache see nothing; rows without a page, and tables without any."""
+    rows = [(3, 10), (40, 5), (0, 4), (200, 230)]
+    b = Batch(12, 2, rows, seed=17)
+    for rule in (K.ScoreRule(), K.ScoreRule(softcap=9.0, window=2 ** 31 - 1), K.ScoreRule(window=5, slopes=slopes(12))):
+        b.check(b.prefill(rule), b.want(rule))
+    for call, rows in (("prefill", [(0, 3), (0, 1)]), ("decode", [(0, 1), (0, 1)])):
+        b = Batch(12, 2, rows, seed=17)
+        b.tables = (b.tables[0], i32([]), b.tables[2])
+        o, lse = getattr(b, call)(K.ScoreRule(softcap=9.0))
+        assert not o.any() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("kind", ["none", "cap", "slopes", "all"])
+def test_one_key_gives_its_value(kind, dtype):
+    """A token that sees one key: its weight is 1 whatever its score, so o is that key's v to the bit."""
+    rows = [(300, 300), (2500, 7), (40, 1)]
+    b = Batch(12, 2, rows, dtype, seed=19, q_std=3.0)
+    r = rule_of(kind, 12, rows)
+    rng = random.Random(19)
+    key = [rng.randint(0, p) for p in b.pos]
+    rule = K.ScoreRule(softcap=r.softcap, slopes=r.slopes, kv_begin=i32(key), kv_end=i32([k + 1 for k in key]))
+    row = [i for i, (_, n) in enumerate(rows) for _ in range(n)]
+    page = torch.tensor([b.pages[i][k // PAGE] for i, k in zip(row, key)], device=DEV)
+    v = b.cache[page, 1, torch.tensor(key, device=DEV) % PAGE].repeat_interleave(6, 1)
+    assert torch.equal(b.prefill(rule)[0], v)
+    assert torch.equal(b.prefill(rule, lse=None)[0], v)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_without_the_lse(kind):
+    for rows in (ROWS, [(9000, 40), (7000, 1)]):
+        b = Batch(28, 4, rows, "bf16", seed=20)
+        rule = rule_of(kind, 28, rows)
+        o, lse = b.prefill(rule)
+        assert torch.equal(o, b.prefill(rule, lse=None)[0])
+
+
+@pytest.mark.parametrize("tokens", [65, 80, 81, 300, 512, 513])
+@pytest.mark.parametrize("hq,hkv,batch", [(12, 2, 3), (40, 8, 30), (16, 2, 1)])
+def test_single_tokens_of_short_rows(hq, hkv, batch, tokens):
+    rows = [(max(1, tokens - 37 * i), 1) for i in range(batch)]
+    b = Batch(hq, hkv, rows, seed=18)
+    rule = K.ScoreRule(softcap=30.0, slopes=slopes(hq), window=tokens - 3)
+    b.check(b.decode(rule), b.want(rule))
 
 
 def test_masks_that_leave_nothing():
