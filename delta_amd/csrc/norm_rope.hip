@@ -12,8 +12,10 @@
 // are in the lane, half pairs R / 16 lanes away (where R / 2 is no multiple of 8, an element's partner is read again).
 // A wave finds the token's row by a ballot over the row bounds, its lane j computes pair j's (cos, sin) and the group
 // takes the pairs of its elements by lane permutes: no LDS and no barrier, every wave runs on its own.
-// What bounds it: memory for prompts (q, k, v read once and written once); for a decode step the chain row bounds ->
-// position and page -> store.
+// What bounds it: memory for prompts (q, k, v read once and written once: 8192 tokens of 32 + 8 heads 46.8 us from and to
+// HBM, 4.3 TB/s where a copy reaches 5.1); for a decode step the chain row bounds -> position and page -> store (one token
+// 3.6 us, 128 tokens 4.4).  At six waves a SIMD the interleaved layout takes 43 us
+// where it took 50, at eight the half layout spills.
 #include "delta_common.h"
 #include "mfma32.h"
 
@@ -23,6 +25,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kGroups = kThreads / 16;  // heads of a block's pass
 constexpr int kPre = 4;                 // passes whose loads go out before the row is known
+
+// q, k and v as they come in are read here for the last time: past the caches, which keeps what is written in them for the
+// attention behind (with it, 8 rows of 512 tokens 74.3 us, 75.2 with ordinary loads; stores past the caches as well make
+// this kernel 10% faster and the two together 3% slower).
+__device__ __forceinline__ u32x4 ld_once(const uint16_t *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+}
 
 struct NormRopeArgs {
   const uint16_t *q, *k, *v;  // v NULL: no append
@@ -44,7 +53,7 @@ struct NormRopeArgs {
 };
 
 template <int DT, bool INTER>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
+__global__ void __launch_bounds__(kThreads, 6) norm_rope_kernel(NormRopeArgs a) {
   using E = Elem<DT>;
   const int i = blockIdx.x;
   const int lane = threadIdx.x & 63, t = lane & 15;
@@ -58,7 +67,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
   u32x4 pre[kPre];
 #pragma unroll
   for (int p = 0; p < kPre; ++p)
-    if (first + p * step < nh) pre[p] = ld128(src(first + p * step) + 8 * t);
+    if (first + p * step < nh) pre[p] = ld_once(src(first + p * step) + 8 * t);
   const uint64_t turn = lane < a.pairs ? a.turns[lane] : 0;
 
   // The token's row; a token behind the last row is left alone.
@@ -178,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
 #pragma unroll
   for (int p = 0; p < kPre; ++p)
     if (first + p * step < nh) one(first + p * step, pre[p]);
-  for (int h = first + kPre * step; h < nh; h += step) one(h, ld128(src(h) + 8 * t));
+  for (int h = first + kPre * step; h < nh; h += step) one(h, ld_once(src(h) + 8 * t));
 }
 
 // Blocks over a token's heads: one pass each until the chip's block slots are filled, then one block a token, whose
