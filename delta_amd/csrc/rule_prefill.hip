@@ -12,9 +12,9 @@
 //
 // Few tokens over a long cache are too few blocks: the tile's steps are cut into parts, each a block of its own that writes
 // its sums (acc, m, l) to the workspace, and a second launch joins them.  How many parts is a matter of all rows' lengths,
-// which only the device knows: every block adds up the call's work W (tiles x steps) and cuts rows that are longer than
-// 1.5 C steps into parts of about C = W hkv / kTargetBlocks, at least kMinSteps.  So a decode row beside short prompts is
-// cut, and equal long prompts are not.
+// which only the device knows: every block adds up the call's work W (tiles x steps), and with C = W hkv / kTargetBlocks
+// steps (at least kMinSteps; up to kLoneSteps twice as many) a row of s steps is cut into s / C parts (row_parts).  So a decode row beside short prompts is cut, equal
+// long prompts are not, and the cut rows' parts are kTargetBlocks blocks at most.
 //
 // A key that a mask leaves out has no part in the result, whatever it holds.  Its score is replaced and its p is 0, but 0
 // times a V of infinity or NaN is NaN in the product of the whole tile, so a row that ends with sums that are not finite is
@@ -33,7 +33,8 @@ constexpr int kKvStep = 32 * kSub;     // keys per step
 constexpr int kPgStep = kKvStep / 16;  // pages per step
 constexpr int kTileB = kKvStep * 256;  // bytes of a step's K (or V) tile: 64 rows of 256 bytes
 constexpr int kTargetBlocks = 512;     // two 4-wave blocks for each CU
-constexpr int kMinSteps = 8;           // a part's steps, at least
+constexpr int kMinSteps = 4;           // a part's steps, at least
+constexpr float kLoneSteps = 8;        // up to so many, one block for each CU
 constexpr int kMaxParts = 1024;
 constexpr int kJoin = 16;              // parts whose sums the join loads together
 constexpr int kSplitWaves = 4;         // waves of a block where rows may be cut
@@ -73,8 +74,17 @@ struct RulePrefillArgs {
   CapArgs cap;
   float2 *part_ml;  // [unit][hkv][wave][32 rows]
   float *part_le;   // likewise
+  int *any_cut;     // whether any row is: else the join has nothing to do
   f32x4 *part_acc;  // [unit][hkv][wave][16][64 lanes], the accumulators as the lanes hold them
 };
+
+// Parts of a row of s steps, `longer`: than the call's mean.  A step takes about 1.5 us in a block with a CU of its own and
+// 2.4 in each of two, a cut's end and join 8 us: three parts gain from 14 steps on.  Two parts of like rows (that fill 2/3 of
+// the CUs uncut) gain nothing: 192 blocks of 32 steps 55 us, 384 of 16 65.
+__host__ __device__ __forceinline__ int row_parts(int s, int C, bool longer) {
+  const int p = s / C;
+  return s < 14 || p < 2 || (p == 2 && (s < 24 || !longer)) ? 1 : p < kMaxParts ? p : kMaxParts;
+}
 
 struct RowBounds {
   int q0, q1, p0, np, kv_len;
@@ -119,27 +129,38 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
     return (span + kKvStep - 1) / kKvStep;
   };
   const int lanes = a.batch > 32 ? 64 : a.batch > 8 ? 32 : a.batch > 2 ? 8 : 2;  // that hold rows (sums stop there)
+  const RowBounds head = row_bounds(a, lane);  // (of most calls all rows: loaded once)
+  auto rows_at = [&](int r0) { return r0 == 0 ? head : row_bounds(a, r0 + lane); };
   int C = 0;
+  float mean = 0.f;
   if (a.max_cut > 0) {
-    float w = 0.f;  // (an estimate; every block of the launch gets the same one)
+    float w = 0.f, t = 0.f;  // (estimates; every block of the launch gets the same ones)
     for (int r0 = 0; r0 < a.batch; r0 += 64) {
-      const RowBounds x = row_bounds(a, r0 + lane);
+      const RowBounds x = rows_at(r0);
+      t += (float)tiles_of(x);
       w += (float)tiles_of(x) * (float)steps_of(x);
     }
-    for (int off = lanes >> 1; off > 0; off >>= 1) w += shfl_xor(w, off);
-    w = readlane(w, 0) * (float)a.hkv * (1.f / kTargetBlocks);
-    C = w < (float)kMinSteps ? kMinSteps : w > 1e8f ? 100000000 : (int)w + 1;
+    for (int off = lanes >> 1; off > 0; off >>= 1) {
+      w += shfl_xor(w, off);
+      t += shfl_xor(t, off);
+    }
+    w = readlane(w, 0);
+    mean = w / readlane(t, 0);
+    w *= (float)a.hkv * (1.f / kTargetBlocks);
+    w = fmaxf(fmaxf(w, fminf(2.f * w, kLoneSteps)), kMinSteps);
+    C = w > 1e8f ? 100000000 : (int)ceilf(w);
   }
   auto parts_of = [&](const RowBounds &x) {
     const int s = steps_of(x);
-    return C > 0 && s > C + C / 2 ? min((s + C - 1) / C, kMaxParts) : 1;
+    return C > 0 ? row_parts(s, C, (float)s > 1.5f * mean) : 1;
   };
   int base = 0;
   for (int pass = C > 0 ? 0 : 1; pass < 2; ++pass) {
     for (int r0 = 0; r0 < a.batch; r0 += 64) {
-      const RowBounds mine = row_bounds(a, r0 + lane);
+      const RowBounds mine = rows_at(r0);
       const int parts = parts_of(mine);
       const int n = (parts > 1) == (pass == 0) ? tiles_of(mine) * parts : 0;
+      if (__ballot(n > 0) == 0) continue;
       int incl = n;
       for (int off = 1; off < lanes; off <<= 1) {
         const int v = __shfl_up(incl, off, 64);
@@ -203,7 +224,9 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   const int h = blockIdx.x;
   const int u = (int)(blockIdx.z * gridDim.y + blockIdx.y);
   Unit un;
-  if (!find_unit(a, BT, u, lane, &un)) return;  // whole block
+  const bool work = find_unit(a, BT, u, lane, &un);
+  if (a.max_cut > 0 && u == 0 && h == 0 && threadIdx.x == 0) *a.any_cut = work && un.parts > 1;  // (cut rows come first)
+  if (!work) return;  // whole block
   const int64_t q0 = un.row.q0;
   const int qn = un.row.q1 - un.row.q0, np = un.row.np, kv_len = un.row.kv_len;
   const int btok0 = un.tile * BT;
@@ -635,6 +658,7 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
 // the rows as the accumulators did.
 template <int DT>
 __global__ void __launch_bounds__(kSplitWaves * 64) rule_join_kernel(RulePrefillArgs a) {
+  if (*a.any_cut == 0) return;
   constexpr int PW = kSplitWaves;
   const int G = a.G, TW = 32 / G, BT = PW * TW;
   const int lane = threadIdx.x & 63, hl = lane >> 5, n = lane & 31;
@@ -699,17 +723,16 @@ int64_t tiles_bound(int64_t num_tokens, int batch, int max_qo_len, int BT) {
   return slots < most ? slots : most;
 }
 
-// Units of cut rows (a kv head's), at most; 0 where no row can be cut.  A cut row has s > 1.5 C steps, so its tiles' parts
-// are at most s / C + 1 < (5 / 3) s / C each, and W hkv <= C kTargetBlocks.
+// Units of cut rows (a kv head's), at most; 0 where no row can be cut.
 int64_t cut_bound(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len, int64_t kv_indices_len, int window) {
   const int BT = kSplitWaves * (32 / G);
   const int64_t keys = kv_indices_len * kPageSize, span = window > 0 && window + (int64_t)BT < keys ? window + (int64_t)BT : keys;
   const int64_t steps = ceil_div(span, kKvStep);
-  if (steps <= kMinSteps + kMinSteps / 2) return 0;
+  if (row_parts((int)steps, kMinSteps, true) == 1) return 0;
   const int64_t tiles = tiles_bound(num_tokens, batch, max_qo_len, BT);
   if (batch == 1 && tiles * hkv >= kTargetBlocks) return 0;  // C >= steps
-  const int64_t by_work = ceil_div(5 * kTargetBlocks, 3 * (int64_t)hkv) + 1;
-  const int64_t by_size = tiles * ceil_div(steps, kMinSteps);
+  const int64_t by_work = kTargetBlocks / hkv + 1;            // (C hkv parts <= W hkv <= C kTargetBlocks)
+  const int64_t by_size = tiles * (steps / kMinSteps);
   return by_work < by_size ? by_work : by_size;
 }
 
@@ -734,7 +757,7 @@ int score_mode(RulePrefillArgs &a, int dtype) {
 
 size_t part_bytes(int64_t units, int hkv) {
   const size_t per = (size_t)kSplitWaves * 32 * (sizeof(float2) + sizeof(float) + kHeadDim * sizeof(float));
-  return (units * hkv * per + 255) & ~(size_t)255;
+  return (units * hkv * per + sizeof(int) + 255) & ~(size_t)255;
 }
 
 template <int DT>
@@ -841,6 +864,7 @@ extern "C" DELTA_EXPORT int delta_paged_prefill_rule(const delta_score_rule_t *r
     a.part_acc = (f32x4 *)workspace;
     a.part_ml = (float2 *)(a.part_acc + (size_t)cut * num_kv_heads * kSplitWaves * 16 * 64);
     a.part_le = (float *)(a.part_ml + (size_t)cut * num_kv_heads * kSplitWaves * 32);
+    a.any_cut = (int *)(a.part_le + (size_t)cut * num_kv_heads * kSplitWaves * 32);
   }
   if (dtype == DELTA_BF16) return launch_rule<DELTA_BF16>(a, num_tokens, max_qo_len, (hipStream_t)stream, who);
   return launch_rule<DELTA_FP16>(a, num_tokens, max_qo_len, (hipStream_t)stream, who);
