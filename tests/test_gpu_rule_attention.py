@@ -244,6 +244,17 @@ def test_cut_rows(rows, kind):
     assert torch.equal(first[0], rest[0]) and torch.equal(first[1], rest[1])
 
 
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (12, 2), (5, 5)])
+@pytest.mark.parametrize("rows", [[(831, 1)], [(832, 1)], [(833, 3)], [(896, 40)], [(1535, 2)] * 6, [(1537, 9)] * 9,
+                                  [(1100, 20)] * 24, [(1600, 4)] + [(100, 4)] * 30, [(3000, 1)] + [(40, 3)] * 70,
+                                  [(30, 2)] * 64 + [(2500, 30), (0, 0), (70, 70), (4000, 1)]])
+def test_around_the_least_cuts(rows, hq, hkv):
+    """Row lengths and batches where the rows begin to be cut, batches that take more than one pass over the rows."""
+    b = Batch(hq, hkv, rows, "bf16", seed=21)
+    for rule in (K.ScoreRule(softcap=30.0), K.ScoreRule(window=1024, slopes=slopes(hq))):
+        b.check(b.prefill(rule), b.want(rule))
+
+
 @pytest.mark.parametrize("kind", ["cap", "slopes", "docs", "prefix"])
 def test_long_prompts_in_wide_blocks(kind):
     rows = [(3600, 3600)]
