@@ -114,12 +114,16 @@ __device__ __forceinline__ RowBounds bounds_of_lane(const RowBounds &x, int l) {
 // One block's work: part `part` of `parts` of a row's tile.
 struct Unit {
   RowBounds row;
-  int tile, part, parts;
+  int h, tile, part, parts;
+  int slot;  // of a cut row's unit in the workspace
 };
 
-// Unit u of a kv head, the cut rows' first (their parts, tile by tile), then the others' tiles row by row, a row's last
-// tile first (in a causal row it sees the most keys); false past the last one.
-__device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int u, int lane, Unit *unit) {
+// Unit (u, h) of the launch, h the kv head: the cut rows' first, then the others' tiles row by row, a row's last tile first
+// (in a causal row it sees the most keys); false past the last one.  Consecutive blocks go to the eight XCDs in turn, so a
+// cut row's blocks are dealt out in groups of eight (part, head) pairs, whose tiles follow one another eight blocks apart: the
+// tiles of a part read its keys from one L2 (groups of 7 over 65548 keys: 48 tokens fetch 139 MB, not 372; 32 tokens 63 us, not
+// 67).
+__device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int u, int h, int lane, Unit *unit) {
   auto tiles_of = [&](const RowBounds &x) {
     const int qn = x.q1 - x.q0;
     return qn <= 0 ? 0 : min((qn + BT - 1) / BT, a.row_tiles);
@@ -158,8 +162,8 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
   for (int pass = C > 0 ? 0 : 1; pass < 2; ++pass) {
     for (int r0 = 0; r0 < a.batch; r0 += 64) {
       const RowBounds mine = rows_at(r0);
-      const int parts = parts_of(mine);
-      const int n = (parts > 1) == (pass == 0) ? tiles_of(mine) * parts : 0;
+      const int parts = parts_of(mine), tiles = tiles_of(mine);
+      const int n = (parts > 1) == (pass == 0) ? tiles * parts : 0;
       if (__ballot(n > 0) == 0) continue;
       int incl = n;
       for (int off = 1; off < lanes; off <<= 1) {
@@ -171,9 +175,24 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
         const int l = __builtin_ctzll(m);
         unit->row = bounds_of_lane(mine, l);
         unit->parts = __builtin_amdgcn_readlane(parts, l);
-        const int at = base + __builtin_amdgcn_readlane(incl, l) - 1 - u;  // from the row's last unit
-        unit->tile = at / unit->parts;
-        unit->part = unit->parts - 1 - (at - unit->tile * unit->parts);
+        const int nt = __builtin_amdgcn_readlane(tiles, l), end = base + __builtin_amdgcn_readlane(incl, l);
+        unit->h = h;
+        unit->tile = end - 1 - u;  // from the row's last
+        unit->part = unit->slot = 0;
+        if (unit->parts > 1) {
+          const int start = end - nt * unit->parts;
+          unit->tile = 0;
+          unit->part = u - start;
+          if (nt > 1) {
+            const int rel = (u - start) * a.hkv + h, group = rel / (8 * nt), r = rel - group * 8 * nt;
+            const int wide = min(8, unit->parts * a.hkv - 8 * group);
+            unit->tile = r / wide;
+            const int pair = 8 * group + r - unit->tile * wide;
+            unit->part = pair / a.hkv;
+            unit->h = pair - unit->part * a.hkv;
+          }
+          unit->slot = start + unit->tile * unit->parts + unit->part;
+        }
         return true;
       }
       base += __builtin_amdgcn_readlane(incl, lanes - 1);
@@ -221,12 +240,12 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   const int G = a.G, TW = 32 / G, BT = PW * TW;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int hl = lane >> 5, n = lane & 31;
-  const int h = blockIdx.x;
   const int u = (int)(blockIdx.z * gridDim.y + blockIdx.y);
   Unit un;
-  const bool work = find_unit(a, BT, u, lane, &un);
-  if (a.max_cut > 0 && u == 0 && h == 0 && threadIdx.x == 0) *a.any_cut = work && un.parts > 1;  // (cut rows come first)
+  const bool work = find_unit(a, BT, u, (int)blockIdx.x, lane, &un);
+  if (a.max_cut > 0 && u == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = work && un.parts > 1;  // (cut rows come first)
   if (!work) return;  // whole block
+  const int h = un.h;
   const int64_t q0 = un.row.q0;
   const int qn = un.row.q1 - un.row.q0, np = un.row.np, kv_len = un.row.kv_len;
   const int btok0 = un.tile * BT;
@@ -576,8 +595,8 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   const uint64_t om = __ballot(odd && row_ok && l < INFINITY);
   const uint32_t odd_rows = (uint32_t)om | (uint32_t)(om >> 32);
   const bool sums_ok = ((odd_rows >> n) & 1u) == 0;
-  const int64_t pslot = ((int64_t)u * a.hkv + h) * PW + wave;  // (cut rows: u < a.max_cut)
-  if (un.parts > 1 && u >= a.max_cut) return;
+  const int64_t pslot = ((int64_t)un.slot * a.hkv + h) * PW + wave;
+  if (un.parts > 1 && un.slot >= a.max_cut) return;  // (no call's cut rows are that many)
   uint16_t *const orow = a.o + (q0 + tok0 + tt) * a.o_stride_t + (int64_t)(h * G + g) * a.o_stride_h;
   if (un.parts > 1) {
     if (hl == 0) a.part_ml[pslot * 32 + n] = float2{m, l};
@@ -662,12 +681,13 @@ __global__ void __launch_bounds__(kSplitWaves * 64) rule_join_kernel(RulePrefill
   constexpr int PW = kSplitWaves;
   const int G = a.G, TW = 32 / G, BT = PW * TW;
   const int lane = threadIdx.x & 63, hl = lane >> 5, n = lane & 31;
-  const int h = blockIdx.x, u = (int)(blockIdx.z * gridDim.y + blockIdx.y);
+  const int u = (int)(blockIdx.z * gridDim.y + blockIdx.y);
   Unit un;
-  if (!find_unit(a, BT, u, lane, &un) || un.parts == 1) return;
+  if (!find_unit(a, BT, u, (int)blockIdx.x, lane, &un) || un.parts == 1) return;
+  const int h = un.h;
   const int qn = un.row.q1 - un.row.q0, btok0 = un.tile * BT;
   const int waves = min(PW, (qn - btok0 + TW - 1) / TW);
-  const int64_t first = u - un.part;
+  const int64_t first = un.slot - un.part;
   for (int task = un.part * PW + uniform((int)(threadIdx.x >> 6)); task < waves * 16; task += un.parts * PW) {
     const int w = task >> 4, c = task & 15;
     const bool want_lse = a.lse && c == 0;
