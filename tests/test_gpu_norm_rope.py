@@ -264,6 +264,7 @@ def test_cache_offsets_past_32_bits():
     assert torch.equal(cache[66000, 1, :4], s.v[16:]) and not cache[66000, :, 4:].any() and not cache[:66000].any()
 
 
+@torch.inference_mode()  # as the engine captures: torch's graph state must not change mode between captures
 def test_graphs_and_streams():
     s = Step(28, 4, ROWS, seed=14)
     rot, _ = make(128, False)

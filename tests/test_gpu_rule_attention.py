@@ -457,6 +457,7 @@ def test_cache_offsets_past_32_bits(single):
 
 
 @pytest.mark.parametrize("single", [False, True])
+@torch.inference_mode()  # as the engine captures: torch's graph state must not change mode between captures
 def test_graphs_and_streams(single):
     """Two captured calls that share a workspace, replayed with eager work between, and a call on a stream of its own."""
     rows = [(5000, 1), (300, 1)] if single else [(5000, 20), (300, 70)]
