@@ -10,11 +10,14 @@
 // the online softmax, O^T += V^T P^T.  Steps that all the wave's rows see whole take no masks, steps that none of them sees
 // are left out.
 //
+// Calls of a few hundred blocks run them with two sets of four waves, every other step each (TWO, two_sided).
+//
 // Few tokens over a long cache are too few blocks: the tile's steps are cut into parts, each a block of its own that writes
 // its sums (acc, m, l) to the workspace, and a second launch joins them.  How many parts is a matter of all rows' lengths,
 // which only the device knows: every block adds up the call's work W (tiles x steps), and with C = W hkv / kTargetBlocks
-// steps (at least kMinSteps; up to kLoneSteps twice as many) a row of s steps is cut into s / C parts (row_parts).  So a decode row beside short prompts is cut, equal
-// long prompts are not, and the cut rows' parts are kTargetBlocks blocks at most.
+// steps (at least kMinSteps; up to kLoneSteps twice as many) a row of s steps is cut into s / C parts (row_parts).  So a
+// decode row beside short prompts is cut, equal long prompts are not, and the cut rows' parts are kTargetBlocks blocks at
+// most.
 //
 // A key that a mask leaves out has no part in the result, whatever it holds.  Its score is replaced and its p is 0, but 0
 // times a V of infinity or NaN is NaN in the product of the whole tile, so a row that ends with sums that are not finite is
@@ -39,11 +42,12 @@ constexpr int kSub = 2;                // 32-token sub-tiles per step
 constexpr int kKvStep = 32 * kSub;     // keys per step
 constexpr int kPgStep = kKvStep / 16;  // pages per step
 constexpr int kTileB = kKvStep * 256;  // bytes of a step's K (or V) tile: 64 rows of 256 bytes
-constexpr int kTargetBlocks = 512;     // two 4-wave blocks for each CU
+constexpr int kTargetBlocks = 512;     // two 4-wave blocks for each CU (TWO: half as many)
 constexpr int kMinSteps = 4;           // a part's steps, at least
-constexpr float kLoneSteps = 8;        // up to so many, one block for each CU
+constexpr int kLoneSteps = 8;          // up to so many, one block for each CU
 constexpr int kMaxParts = 1024;
 constexpr int kJoin = 16;              // parts whose sums the join loads together
+constexpr int kTwoFrom = 128, kTwoTo = 450;  // blocks of a call that are TWO (two_sided)
 constexpr int kSplitWaves = 4;         // waves of a block where rows may be cut
 
 // What the rule does to the scores, a kernel each (a branch in the step costs the instructions that the compiler moves out
@@ -76,6 +80,7 @@ struct RulePrefillArgs {
   int token_limit;  // query tokens of all rows
   int row_tiles;    // the most tiles a row has (of max_qo_len tokens)
   int max_cut;      // units of cut rows that the workspace holds, 0: no row is cut
+  bool two;         // blocks are TWO
   float sm_scale;
   RuleArgs rule;
   CapArgs cap;
@@ -158,7 +163,7 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
     w = readlane(w, 0);
     mean = w / readlane(t, 0);
     w *= (float)a.hkv * (1.f / kTargetBlocks);
-    w = fmaxf(fmaxf(w, fminf(2.f * w, kLoneSteps)), kMinSteps);
+    w = a.two ? fmaxf(2.f * w, (float)kLoneSteps) : fmaxf(fmaxf(w, fminf(2.f * w, (float)kLoneSteps)), (float)kMinSteps);
     C = w > 1e8f ? 100000000 : (int)ceilf(w);
   }
   auto parts_of = [&](const RowBounds &x) {
@@ -234,18 +239,21 @@ __device__ __forceinline__ int wave_extreme(int v) {
   return uniform(pick((int)b[0], (int)b[1]));
 }
 
-template <int DT, int PW, int SM>
-__global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePrefillArgs a) {
+template <int DT, int PW, bool TWO, int SM>
+__global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_kernel(RulePrefillArgs a) {
 #pragma clang fp contract(off)
+  static_assert(!TWO || PW == 4, "TWO: 4-wave tiles");
   using E = Elem<DT>;
   using MF = Mfma32<DT>;
   constexpr bool kLate = PW == 8;   // the second wave of each SIMD runs half a step behind
   constexpr int kBufs = kLate ? 4 : 2;
   constexpr int kPgWave = 16 / PW;  // pages a wave loads rows of, per step
-  __shared__ __attribute__((aligned(1024))) char tiles[kBufs][2 * kTileB];
+  constexpr int kStride = TWO ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) char lds[kStride * kBufs][2 * kTileB];
 
   const int G = a.G, TW = 32 / G, BT = PW * TW;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = (threadIdx.x >> 6) & (PW - 1), lane = threadIdx.x & 63;
+  const int side = TWO ? uniform((int)(threadIdx.x >> 8)) : 0;  // TWO: the block's first or second four waves
   const int hl = lane >> 5, n = lane & 31;
   const int u = (int)(blockIdx.z * gridDim.y + blockIdx.y);
   Unit un;
@@ -325,11 +333,11 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
   // of V row r at ch ^ 4 (r % 4).
   const uint32_t row_bytes = (uint32_t)a.hkv * kHeadDim * 2;
   const uint32_t page_bytes = 2 * kPageSize * row_bytes;
-  const int wv = uniform((int)(threadIdx.x >> 6));
+  const int wv = uniform(wave);
   const int lrow = lane >> 4, lch = lane & 15;
   const uint32_t koff = (4 * (wv & 3) + lrow) * row_bytes + 16 * (lch ^ (4 * (wv & 3) + lrow));
   const uint32_t voff = (kPageSize + 4 * (wv & 3) + lrow) * row_bytes + 16 * (lch ^ (4 * lrow));
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&tiles[0][0] + wv * 1024;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&lds[side * kBufs][0] + wv * 1024;
   const char *const kvh = reinterpret_cast<const char *>(a.kv) + (int64_t)h * (kHeadDim * 2);
   const int32_t *const row_ids = a.kv_indices + un.row.p0;
   auto page_bad = [&](int pid) { return pid < 0 || (int64_t)pid >= a.num_pages; };
@@ -351,8 +359,10 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
 #pragma unroll
     for (int i = 0; i < kPgWave; ++i) id[i] = (uint32_t)__builtin_amdgcn_readlane(v, i * (PW / 4) + (wv >> 2));
   };
+  auto buf = [&](int j) { return (uint32_t)(j / kStride & (kBufs - 1)); };  // of the side's buffers
+  auto tile = [&](int j) { return &lds[side * kBufs + buf(j)][0]; };
   auto issue = [&](int j, int i) {
-    const uint32_t dst = lds0 + (uint32_t)(j & (kBufs - 1)) * (2 * kTileB) + i * (PW / 4) * 4096;
+    const uint32_t dst = lds0 + buf(j) * (2 * kTileB) + i * (PW / 4) * 4096;
     const char *pg = kvh + (uint64_t)id[i] * page_bytes;
     load_lds_1k(dst, pg, koff);
     load_lds_1k(dst + kTileB, pg, voff);
@@ -361,11 +371,11 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
 #pragma unroll
     for (int i = 0; i < kPgWave; ++i) issue(j, i);
   };
-  if (s0 < s1) {
-    load_ids(s0);
+  if (s0 + side < s1) {
+    load_ids(s0 + side);
     take_ids();
-    load_ids(s0 + 1);
-    issue_step(s0);
+    load_ids(s0 + side + kStride);
+    issue_step(s0 + side);
     if (kLate && s0 + 1 < s1) {
       take_ids();
       load_ids(s0 + 2);
@@ -434,7 +444,7 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       }
 #pragma unroll
       for (int sb = 0; sb < kSub; ++sb) S[sb] = MF::run(kq[ks % 4][sb], qf[ks], S[sb]);
-      if (!kLate && ks < kPgWave && j + 1 < s1) issue(j + 1, ks);  // the next step's loads go out under the MFMAs
+      if (!kLate && ks < kPgWave && j + kStride < s1) issue(j + kStride, ks);  // the next step's loads go out under the MFMAs
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
@@ -553,7 +563,8 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
 
   const bool late = kLate && wave >= PW / 2;
   u32x4 pcar[2 * kSub];
-  for (int j = s0; s0 < s1 && j < s1 + (kLate ? 1 : 0); ++j) {
+  for (int j0 = s0; s0 < s1 && j0 < s1 + (kLate ? 1 : 0); j0 += kStride) {
+    const int j = j0 + side;
     // Step j's loads have landed when at most the next step's (kLate: four) are pending.
     if (kLate && j + 1 < s1)
       wait_loads<2 * kPgWave + 1>();
@@ -561,13 +572,17 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (row_bad) bad = j < s1 ? bad_of(j) : 0u;
-    if (j < s1 && (j * kKvStep < blo || (j + 1) * kKvStep > bhi || bad != 0)) {
+    uint32_t bad0 = 0;  // of the block's step or two
+    if (row_bad) {
+      bad = j < s1 ? bad_of(j) : 0u;
+      bad0 = TWO ? bad_of(j0) | bad_of(j0 + 1) : bad;
+    }
+    if (j0 < s1 && (j0 * kKvStep < blo || (j0 + kStride) * kKvStep > bhi || bad0 != 0)) {
       // V rows that no token of the block sees, and of pages outside the cache, meet p = 0 but may hold NaN/Inf: zeros.
       constexpr int kTpr = PW;  // threads per row
-      const int r = (int)threadIdx.x / kTpr, at = j * kKvStep + r;
-      if (at < blo || at >= bhi || ((bad >> (r >> 4)) & 1u)) {
-        char *vr = &tiles[j % kBufs][kTileB + r * 256 + 256 / kTpr * ((int)threadIdx.x % kTpr)];
+      const int t = (int)threadIdx.x & (PW * 64 - 1), r = t / kTpr, at = j * kKvStep + r;
+      if (j < s1 && (at < blo || at >= bhi || ((bad >> (r >> 4)) & 1u))) {
+        char *vr = tile(j) + kTileB + r * 256 + 256 / kTpr * (t % kTpr);
 #pragma unroll
         for (int i = 0; i < 16 / kTpr; ++i) st128(vr + 16 * i, u32x4{0u, 0u, 0u, 0u});
       }
@@ -576,23 +591,51 @@ __global__ void __launch_bounds__(PW * 64, 2) paged_prefill_rule_kernel(RulePref
       asm volatile("" ::: "memory");
     }
     const bool mine = j >= w0 && j < w1;
-    if (kLate ? j + 2 < s1 : j + 1 < s1) {
+    constexpr int kNext = kLate ? 2 : kStride;  // the step whose loads go out
+    if (j + kNext < s1) {
       take_ids();
-      load_ids(kLate ? j + 3 : j + 2);
-      if (kLate || !mine) issue_step(kLate ? j + 2 : j + 1);
+      load_ids(j + kNext + kStride);
+      if (kLate || !mine) issue_step(j + kNext);
     }
     if (late) {
-      if (j - 1 >= w0 && j - 1 < w1) pv_step(&tiles[(j - 1) % kBufs][0], pcar);
-      if (mine) score_step(j, &tiles[j % kBufs][0], pcar);
+      if (j - 1 >= w0 && j - 1 < w1) pv_step(tile(j - 1), pcar);
+      if (mine) score_step(j, tile(j), pcar);
     } else if (mine) {
       u32x4 pc[2 * kSub];
-      score_step(j, &tiles[j % kBufs][0], pc);
-      pv_step(&tiles[j % kBufs][0], pc);
+      score_step(j, tile(j), pc);
+      pv_step(tile(j), pc);
     }
   }
 
   l = halves_sum(l);
   le = halves_sum(le);
+  if constexpr (TWO) {  // the second four waves' sums, through the LDS that held the tiles, to the first four's
+    f32x4 *const xa = reinterpret_cast<f32x4 *>(&lds[0][0]);   // [wave][16][64 lanes]
+    float *const xs = reinterpret_cast<float *>(xa + PW * 16 * 64);  // [wave][3][64 lanes]
+    __syncthreads();
+    if (side == 1) {
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        xa[(wave * 16 + c) * 64 + lane] = f32x4{acc[c >> 2][4 * (c & 3)], acc[c >> 2][4 * (c & 3) + 1],
+                                                acc[c >> 2][4 * (c & 3) + 2], acc[c >> 2][4 * (c & 3) + 3]};
+      xs[(wave * 3 + 0) * 64 + lane] = m;
+      xs[(wave * 3 + 1) * 64 + lane] = l;
+      xs[(wave * 3 + 2) * 64 + lane] = le;
+    }
+    __syncthreads();
+    if (side == 1) return;
+    const float m1 = xs[(wave * 3 + 0) * 64 + lane], top = fmaxf(m, m1), ref = top == -INFINITY ? 0.f : top;
+    const float f0 = fast_exp2(m - ref), f1 = fast_exp2(m1 - ref);
+    l = l * f0 + xs[(wave * 3 + 1) * 64 + lane] * f1;
+    le = le * f0 + xs[(wave * 3 + 2) * 64 + lane] * f1;
+    m = top;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const f32x4 v = xa[(wave * 16 + c) * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[c >> 2][4 * (c & 3) + i] = acc[c >> 2][4 * (c & 3) + i] * f0 + v[i] * f1;
+    }
+  }
   // Rows whose sums are not finite though their scores are: slow_row's.
   bool odd = false;
 #pragma unroll
@@ -750,16 +793,28 @@ int64_t tiles_bound(int64_t num_tokens, int batch, int max_qo_len, int BT) {
   return slots < most ? slots : most;
 }
 
+// Calls whose blocks have a CU each, or nearly, and are too many to be cut are bound by the longest one's steps: there a
+// block's keys are swept by two sets of four waves, every other step each, whose sums are added at the end (us one set / two;
+// prompts of 8 kv heads of 4: 512 tokens, 128 blocks 19.9 / 19.1, 1024 34 / 29, 1536, 384 blocks 48 / 40, 1800, 452 55 / 52; of 8
+// of 5: 1200, 400 blocks 41 / 38, 1536, 512 48 / 50; 24 rows of 24 tokens over 4096, 192 blocks 110 / 100).  Fewer blocks are
+// better cut (16 tokens over 1600, 8 blocks 20.4 / 22.3), a single step is quicker with one set (9.6 / 11.1).
+bool two_sided(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len) {
+  const int64_t blocks = tiles_bound(num_tokens, batch, max_qo_len, kSplitWaves * (32 / G)) * hkv;
+  return blocks >= kTwoFrom && blocks <= kTwoTo;
+}
+
 // Units of cut rows (a kv head's), at most; 0 where no row can be cut.
 int64_t cut_bound(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len, int64_t kv_indices_len, int window) {
   const int BT = kSplitWaves * (32 / G);
+  const bool two = two_sided(num_tokens, batch, hkv, G, max_qo_len);
+  const int target = two ? kTargetBlocks / 2 : kTargetBlocks, least = two ? kLoneSteps : kMinSteps;
   const int64_t keys = kv_indices_len * kPageSize, span = window > 0 && window + (int64_t)BT < keys ? window + (int64_t)BT : keys;
   const int64_t steps = ceil_div(span, kKvStep);
-  if (row_parts((int)steps, kMinSteps, true) == 1) return 0;
+  if (row_parts((int)steps, least, true) == 1) return 0;
   const int64_t tiles = tiles_bound(num_tokens, batch, max_qo_len, BT);
-  if (batch == 1 && tiles * hkv >= kTargetBlocks) return 0;  // C >= steps
-  const int64_t by_work = kTargetBlocks / hkv + 1;            // (C hkv parts <= W hkv <= C kTargetBlocks)
-  const int64_t by_size = tiles * (steps / kMinSteps);
+  if (batch == 1 && tiles * hkv >= target) return 0;  // C >= steps
+  const int64_t by_work = target / hkv + 1;             // (C hkv parts <= W hkv <= C target)
+  const int64_t by_size = tiles * (steps / least);
   return by_work < by_size ? by_work : by_size;
 }
 
@@ -791,7 +846,8 @@ template <int DT>
 int launch_rule(RulePrefillArgs a, int64_t num_tokens, int max_qo_len, hipStream_t stream, const char *who) {
   const int TW = 32 / a.G;
   // Whole prompts that fill the chip nearly twice over in 4-wave blocks run 8-wave ones (prefill.hip, wide_blocks).
-  const bool wide = a.max_cut == 0 && a.hkv * ceil_div(max_qo_len, 4 * TW) >= 850;
+  a.two = two_sided(num_tokens, a.batch, a.hkv, a.G, max_qo_len);
+  const bool wide = !a.two && a.max_cut == 0 && a.hkv * ceil_div(max_qo_len, 4 * TW) >= 850;
   const int BT = TW * (wide ? 8 : 4);
   a.row_tiles = (int)ceil_div(max_qo_len, BT);
   const int64_t units = a.max_cut + tiles_bound(num_tokens, a.batch, max_qo_len, BT), y = units < 32768 ? units : 32768;
@@ -799,9 +855,11 @@ int launch_rule(RulePrefillArgs a, int64_t num_tokens, int max_qo_len, hipStream
   auto launch = [&](auto sm) {
     constexpr int SM = decltype(sm)::value;
     if (wide)
-      hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 8, SM>), grid, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 8, false, SM>), grid, dim3(512), 0, stream, a);
+    else if (a.two)
+      hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 4, true, SM>), grid, dim3(512), 0, stream, a);
     else
-      hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 4, SM>), grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((paged_prefill_rule_kernel<DT, 4, false, SM>), grid, dim3(256), 0, stream, a);
   };
   switch (score_mode(a, DT)) {
     case kPlain: launch(std::integral_constant<int, kPlain>()); break;

@@ -255,6 +255,41 @@ def test_around_the_least_cuts(rows, hq, hkv):
         b.check(b.prefill(rule), b.want(rule))
 
 
+# calls of 128 to 450 blocks: whole prompts, chunks, a long row that is cut beside short ones, rows of one step and none
+FEW_HUNDRED = [[(700, 700)], [(400, 30)] * 30, [(1500, 40)] * 10 + [(6000, 1), (3000, 20)], [(0, 0), (1, 1), (63, 63), (64, 64)] * 12,
+               [(129, 65), (190, 33), (65, 1)] * 8]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", FEW_HUNDRED)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_calls_of_a_few_hundred_blocks(rows, kind, dtype):
+    b = Batch(32, 8, rows, dtype, seed=22, q_std=3.0)
+    rule = rule_of(kind, 32, rows)
+    b.check(b.prefill(rule), b.want(rule))
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+@pytest.mark.parametrize("rows", [[(700, 700)], [(1500, 40)] * 10 + [(6000, 8), (3000, 20)]])
+def test_a_few_hundred_blocks_beside_anything(rows, what):
+    """Values that windows and documents leave out, and pages outside the cache."""
+    b = Batch(32, 8, rows, seed=23)
+    rng = random.Random(23)
+    for pages in b.pages:
+        for at in rng.sample(range(len(pages)), len(pages) // 4):
+            b.cache[pages[at], 1, rng.randrange(PAGE), :, rng.randrange(D)] = what
+    seen = K.ScoreRule(window=30, softcap=20.0)
+    got, want = b.prefill(seen), b.want(seen)
+    assert torch.equal(got[0].isfinite(), want[0].isfinite())
+    assert torch.equal(got[1].isfinite(), want[1].isfinite())
+    b = Batch(32, 8, rows, seed=24)
+    for pages in b.pages:
+        for at in rng.sample(range(len(pages)), len(pages) // 5):
+            b.tables[1][sum(len(x) for x in b.pages[:b.pages.index(pages)]) + at] = pages[at] = rng.choice([-1, 1 << 30])
+    for rule in (K.ScoreRule(), K.ScoreRule(softcap=30.0, slopes=slopes(32))):
+        b.check(b.prefill(rule), b.want(rule))
+
+
 @pytest.mark.parametrize("kind", ["cap", "slopes", "docs", "prefix"])
 def test_long_prompts_in_wide_blocks(kind):
     rows = [(3600, 3600)]
