@@ -414,6 +414,19 @@ def test_pages_outside_the_cache_are_dropped(single):
         b.check(b.decode(rule) if single else b.prefill(rule), b.want(rule))
 
 
+@pytest.mark.parametrize("padded", [30, 2900, 2992, 3008, 3009, 9000])
+def test_few_tokens_of_many_planned(padded):
+    """A query buffer planned for more tokens than the rows have, up to more than the pages hold."""
+    b = Batch(12, 2, [(2990, 7), (9, 2)], seed=25)
+    q = torch.zeros(padded, 12, D, dtype=b.dtype, device=DEV)
+    q[:9] = b.q
+    rule = K.ScoreRule(softcap=30.0)
+    for most in (7, padded):
+        o, lse = torch.full_like(q, 5.0), torch.full((padded, 12), 5.0, device=DEV)
+        b.check(b.prefill(rule, q=q, out=o, lse=lse, max_qo_len=most), b.want(rule))
+        assert (o[9:] == 5.0).all() and (lse[9:] == 5.0).all()
+
+
 def test_tokens_behind_the_last_row_stay():
     b = Batch(12, 2, [(40, 40), (900, 3)], seed=10)
     q = torch.cat([b.q, torch.full((9, 12, D), math.nan, dtype=b.dtype, device=DEV)])
