@@ -636,6 +636,14 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
       for (int i = 0; i < 4; ++i) acc[c >> 2][4 * (c & 3) + i] = acc[c >> 2][4 * (c & 3) + i] * f0 + v[i] * f1;
     }
   }
+  // A row that saw no key (l = 0; one that saw any has a weight of 1 or more, with kCappedRef of 2^-125) holds 0 times the
+  // values that its wave's other rows saw, NaN where those are NaN or infinity.
+  if (l == 0.f) {
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+  }
   // Rows whose sums are not finite though their scores are: slow_row's.
   bool odd = false;
 #pragma unroll

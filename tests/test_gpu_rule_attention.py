@@ -563,3 +563,33 @@ def test_drawn(seed):
                        window=rng.choice([0, 0, rng.randint(1, 2000)]),
                        kv_begin=rng.choice([None, documents(rows, seed)]), kv_end=rng.choice([None, prefixes(rows, seed)]))
     b.check(b.prefill(rule), b.want(rule))
+
+
+# (q heads, kv heads, rows, planned tokens): one set of waves to a block, two, eight waves to a block, cut rows
+BLOCKS = [(8, 2, [(300, 40), (70, 70), (20, 31)], 70), (32, 8, [(700, 700), (9, 14)], 700), (32, 8, [(290, 200), (5, 9)], 4000),
+          (28, 4, [(5000, 40), (90, 90)], 90)]
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+@pytest.mark.parametrize("kind", ["none", "cap", "slopes", "all"])
+@pytest.mark.parametrize("blocks", range(len(BLOCKS)))
+def test_tokens_without_keys_beside_anything(blocks, kind, what):
+    """Tokens that see no key (bounds, positions in front of the cache, pages outside it) among tokens whose values are NaN or
+    infinity: 0 and -inf, as beside finite values."""
+    hq, hkv, rows, most = BLOCKS[blocks]
+    rng = random.Random(blocks)
+    for dtype in ("bf16", "fp16"):
+        b = Batch(hq, hkv, rows, dtype, seed=30, q_std=3.0)
+        r = rule_of(kind if kind != "all" else "cap", hq, rows)
+        n = rows[0][0]
+        for s in range(n % 7, n, 9):
+            b.cache[b.pages[0][s // PAGE], 1, s % PAGE, :, rng.randrange(D)] = what
+        b.cache[b.pages[-1][0], 1, 1] = what
+        bad = n // PAGE - 1  # a page outside the cache, and tokens that see nothing else
+        b.pages[0][bad] = b.tables[1][bad] = -1
+        begin = [p + 1 if i % 3 == 0 else PAGE * bad if i % 3 == 1 else 0 for i, p in enumerate(b.pos)]
+        end = [0 if i % 4 == 0 else PAGE * bad + PAGE if i % 3 == 1 else p + 1 for i, p in enumerate(b.pos)]
+        for kb, ke in ((begin, None), (begin, end), (None, end), (None, None)):
+            rule = K.ScoreRule(softcap=r.softcap, slopes=slopes(hq) if kind in ("slopes", "all") else None,
+                               kv_begin=kb and i32(kb), kv_end=ke and i32(ke))
+            b.check(b.prefill(rule, max_qo_len=most), b.want(rule))
