@@ -470,7 +470,10 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
         xo = 0.f;
       }
     } else if constexpr (SM == kAny) {
-      if (capped) {
+      if (a.cap.k > 0.f) {  // a cap up to kQuickCap
+#pragma unroll
+        for (int i = 0; i < NX; ++i) x[i] = fmaf(a.cap.xs, __builtin_amdgcn_rcpf(-1.f - fast_exp2(x[i] * a.cap.k)), a.cap.xo);
+      } else if (capped) {
         cap_scores(x, a.rule, scale, kLog2e);
       } else {
 #pragma unroll
@@ -834,13 +837,14 @@ int score_mode(RulePrefillArgs &a, int dtype) {
   const double scale = fabs((double)a.sm_scale);
   if (!(scale > 0)) return kAny;
   if (!(a.rule.softcap > 0.f)) return !a.rule.slopes ? kPlain : scale > 1e-10 ? kLeaning : kAny;
-  if (a.rule.slopes) return kAny;
   if (a.rule.softcap > kQuickCap) return kAny;
   const double c2 = a.rule.softcap * 1.4426950408889634;
-  a.cap.k = (float)(2 * 1.4426950408889634 * scale / a.rule.softcap);
+  const float k = (float)(2 * 1.4426950408889634 * scale / a.rule.softcap);
+  if (!(k < INFINITY)) return kAny;
+  a.cap.k = k;
   a.cap.xs = (float)(2 * c2);
   a.cap.xo = (float)c2;
-  if (!(a.cap.k < INFINITY)) return kAny;
+  if (a.rule.slopes) return kAny;
   // Scores lie within c2 of 0, so with p = 2^(score - ref) in [2^-125, 2^60] no maximum is needed: every p is a normal
   // number of fp32 and bf16, and the sums stay below 2^77 max|v|.
   const double top = 2 * c2 - 125 > 0 ? 2 * c2 - 125 : 0;

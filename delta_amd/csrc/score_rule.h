@@ -36,8 +36,10 @@ __device__ __forceinline__ float tanh_ratio(float u) {
 }
 
 // x <- unit c tanh(x in / c) for a wave's N scores a lane (in: the scale that x still lacks; unit: log2 e for scores in
-// log2 units, else 1).  c - 2 c / (1 + e^(2 y)) is off by 2^-22 c, whatever the score; where no score of the wave's
-// passes c / 2 the polynomial keeps the error relative to the score, so a cap far above the scores costs them nothing.
+// log2 units, else 1).  c - 2 c / (1 + e^(2 y)) is off by 2^-22 c, whatever the score: it is for scores past c / 2, and the
+// polynomial, whose error is relative to the score, for the others, so a cap far above the scores costs them nothing.  Each
+// score's form is its own matter, since those beside it may be hidden keys'; where no score of the wave's passes c / 2 the first
+// form is left out.
 template <int N>
 __device__ __forceinline__ void cap_scores(float (&x)[N], const RuleArgs &r, float in, float unit) {
   const float ky = in * r.rcp_cap, kx = in * unit;
@@ -53,7 +55,11 @@ __device__ __forceinline__ void cap_scores(float (&x)[N], const RuleArgs &r, flo
   } else {
     const float k2 = 2.f * kLog2e * ky, c = r.softcap * unit;
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = fmaf(-2.f * c, __builtin_amdgcn_rcpf(1.f + fast_exp2(x[i] * k2)), c);
+    for (int i = 0; i < N; ++i) {
+      const float y = x[i] * ky, near = (x[i] * kx) * tanh_ratio(y * y);
+      const float far = fmaf(-2.f * c, __builtin_amdgcn_rcpf(1.f + fast_exp2(x[i] * k2)), c);
+      x[i] = fabsf(y) > 0.5f ? far : near;
+    }
   }
 }
 

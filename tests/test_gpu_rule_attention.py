@@ -593,3 +593,45 @@ def test_tokens_without_keys_beside_anything(blocks, kind, what):
             rule = K.ScoreRule(softcap=r.softcap, slopes=slopes(hq) if kind in ("slopes", "all") else None,
                                kv_begin=kb and i32(kb), kv_end=ke and i32(ke))
             b.check(b.prefill(rule, max_qo_len=most), b.want(rule))
+
+
+def far_cap(want, cap):
+    """A cap far above the scores: no error that grows with it."""
+    want[3] = want[3] - 2.0 ** -21 * cap
+    return want
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("cap", [1e3, 1e4, 1e20])
+@pytest.mark.parametrize("size", [math.inf, -math.inf, "max"])
+@pytest.mark.parametrize("single", [False, True])
+def test_large_caps_beside_hidden_keys_of_any_size(single, size, cap, dtype):
+    """Keys behind a row's end, in front of its first one and in place of a page outside the cache have no part in how the
+    scores of the others are capped."""
+    rows = [(300, 1), (41, 1), (200, 1)] if single else [(300, 40), (41, 41), (200, 5)]
+    b = Batch(8, 2, rows, dtype, seed=31, q_std=3.0, stale=0.0, first_page=1, num_pages=40)
+    b.cache[0] = 0.0
+    call, size = b.decode if single else b.prefill, torch.finfo(DT[dtype]).max if size == "max" else size
+    b.tables[1][sum(len(p) for p in b.pages[:2]) + 4] = b.pages[2][4] = -1
+    begin = i32([251 if i < rows[0][1] else 0 for i in range(b.T)])
+    rules = [K.ScoreRule(softcap=cap, kv_begin=begin), K.ScoreRule(softcap=cap, kv_begin=begin, slopes=slopes(8))]
+    want = [far_cap(b.want(rule), cap) for rule in rules]  # (of the values that are seen)
+    b.cache[b.pages[0][-1], 0, 300 % PAGE:, :, 5] = size
+    b.cache[b.pages[1][-1], 0, 41 % PAGE:, :, 5] = size
+    b.cache[b.pages[0][250 // PAGE], 0, 250 % PAGE, :, 7] = size
+    b.cache[0, 0, :, :, 9] = size
+    for rule, w in zip(rules, want):
+        b.check(call(rule), w)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("cap", [1e3, 1e6])
+@pytest.mark.parametrize("single", [False, True])
+def test_large_caps_beside_tokens_and_heads_of_larger_scores(single, cap, dtype):
+    """Scores about the cap in some tokens and heads; the small ones beside them keep an error of their own size."""
+    rows = [(300, 1), (41, 1)] if single else [(300, 40), (41, 41)]
+    b = Batch(8, 2, rows, dtype, seed=32, q_std=3.0)
+    b.q[::3, ::4] *= cap / 20
+    rule = K.ScoreRule(softcap=cap)
+    call = b.decode if single else b.prefill
+    b.check(call(rule), far_cap(b.want(rule), cap))
