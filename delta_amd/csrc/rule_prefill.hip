@@ -64,6 +64,7 @@ struct CapArgs {
   float k, xs, xo;  // k = 2 log2 e s / c
   float ref;        // kCappedRef: the reference, log2 units
 };
+constexpr float kLeastSum = 0x1p-64f;  // kCappedRef: of p over a row's keys; below it products with small values are lost
 
 struct RulePrefillArgs {
   const uint16_t *q;
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
       for (int i = 0; i < 4; ++i) acc[c >> 2][4 * (c & 3) + i] = acc[c >> 2][4 * (c & 3) + i] * f0 + v[i] * f1;
     }
   }
-  // A row that saw no key (l = 0; one that saw any has a weight of 1 or more, with kCappedRef of 2^-125) holds 0 times the
+  // A row that saw no key (l = 0; one that saw any has a weight of 1 or more, with kCappedRef of 2^-93) holds 0 times the
   // values that its wave's other rows saw, NaN where those are NaN or infinity.
   if (l == 0.f) {
 #pragma unroll
@@ -647,8 +648,8 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
   }
-  // Rows whose sums are not finite though their scores are: slow_row's.
-  bool odd = false;
+  // Rows whose sums are not finite though their scores are, or too small: slow_row's.
+  bool odd = SM == kCappedRef && l != 0.f && l < kLeastSum;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -681,14 +682,14 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
     if (a.lse && hl == 0) a.lse[(q0 + tok0 + tt) * a.hq + h * G + g] = l != 0.f ? (m + log2f(le)) * kLn2 : -INFINITY;
   }
 
-  // slow_row: the sums again, key by key, over the row's own keys.
+  // slow_row: the sums again, key by key, over the row's own keys, beside their own maximum.
   for (uint32_t rows = odd_rows; rows != 0; rows &= rows - 1) {
     const int rn = __builtin_ctz(rows);
     const int rlo = max(__builtin_amdgcn_readlane(lo, rn), s0 * kKvStep), rhi = min(__builtin_amdgcn_readlane(hi, rn), s1 * kKvStep);
-    const float rm = readlane(m, rn), rs = readlane(slope2, rn);
+    const float rs = readlane(slope2, rn);
     const int rt = rn / G, rg = rn - rt * G, rpos = __builtin_amdgcn_readlane(qpos, rn);
     const uint16_t *qp = a.q + (q0 + tok0 + rt) * a.q_stride_t + (int64_t)(h * G + rg) * a.q_stride_h;
-    float rl = 0.f, o0 = 0.f, o1 = 0.f;  // d = 2 lane, 2 lane + 1
+    float rm = -INFINITY, rl = 0.f, o0 = 0.f, o1 = 0.f;  // d = 2 lane, 2 lane + 1
     for (int c0 = rlo; c0 < rhi; c0 += 64) {
       const int k = c0 + lane;
       int pid = k < rhi && k / kPageSize < np ? row_ids[k / kPageSize] : -1;
@@ -707,7 +708,15 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
       else
         x[0] *= a.sm_scale * kLog2e;
       if (leaning) x[0] = fmaf(-rs, fabsf((float)(rpos - k)), x[0]);
-      const float p = fast_exp2(x[0] - rm);
+      const float top = fmaxf(rm, rows4_max(row16_max(pid >= 0 ? x[0] : -INFINITY)));
+      if (top > rm) {
+        const float al = fast_exp2(rm - top);
+        rl *= al;
+        o0 *= al;
+        o1 *= al;
+        rm = top;
+      }
+      const float p = fast_exp2(x[0] - (rm == -INFINITY ? 0.f : rm));
       for (uint64_t keys = __ballot(pid >= 0); keys != 0; keys &= keys - 1) {
         const int kl = __builtin_ctzll(keys);
         const float pk = readlane(p, kl);
@@ -725,9 +734,10 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
       float *dst = reinterpret_cast<float *>(a.part_acc + (pslot * 16 + d / 8) * 64 + 32 * (d % 8 / 4) + rn) + d % 4;
       dst[0] = o0;
       dst[1] = o1;
-      if (lane == 0) a.part_ml[pslot * 32 + rn].y = rl;
+      if (lane == 0) a.part_ml[pslot * 32 + rn] = float2{rm, rl};
+      if (a.lse && lane == 0) a.part_le[pslot * 32 + rn] = rl;
     } else {
-      const float inv = 1.f / rl;
+      const float inv = rl != 0.f ? 1.f / rl : 0.f;
       uint32_t *dst = reinterpret_cast<uint32_t *>(a.o + (q0 + tok0 + rt) * a.o_stride_t + (int64_t)(h * G + rg) * a.o_stride_h);
       dst[lane] = pack2<DT>(o0 * inv, o1 * inv);
     }
@@ -765,16 +775,16 @@ __global__ void __launch_bounds__(kSplitWaves * 64) rule_join_kernel(RulePrefill
         le[i] = want_lse ? a.part_le[at * 32 + n] : 0.f;
         av[i] = a.part_acc[(at * 16 + c) * 64 + lane];
       }
-      float top = M;
+      float top = M;  // the largest part's m + log2 l: no part's sums weigh more than its values
 #pragma unroll
-      for (int i = 0; i < kJoin; ++i) top = fmaxf(top, ml[i].x);
+      for (int i = 0; i < kJoin; ++i) top = fmaxf(top, ml[i].y != 0.f ? ml[i].x + __builtin_amdgcn_logf(ml[i].y) : -INFINITY);
       const float ref = top == -INFINITY ? 0.f : top, al = fast_exp2(M - ref);
       L *= al;
       LE *= al;
       A = A * al;
 #pragma unroll
       for (int i = 0; i < kJoin; ++i) {
-        if (s0 + i < un.parts && ml[i].y != 0.f) {  // a part without keys wrote no sums
+        if (s0 + i < un.parts && ml[i].y != 0.f) {  // (a part without keys wrote no sums)
           const float sc = fast_exp2(ml[i].x - ref);
           L = fmaf(ml[i].y, sc, L);
           LE = fmaf(le[i], sc, LE);
@@ -845,11 +855,12 @@ int score_mode(RulePrefillArgs &a, int dtype) {
   a.cap.xs = (float)(2 * c2);
   a.cap.xo = (float)c2;
   if (a.rule.slopes) return kAny;
-  // Scores lie within c2 of 0, so with p = 2^(score - ref) in [2^-125, 2^60] no maximum is needed: every p is a normal
-  // number of fp32 and bf16, and the sums stay below 2^77 max|v|.
-  const double top = 2 * c2 - 125 > 0 ? 2 * c2 - 125 : 0;
+  // Scores lie within c2 of 0, so with p = 2^(score - ref) in [2^-64, 2^92] (caps over 54: from 2^-93 on) no maximum is needed:
+  // every p is a normal number of fp32 and bf16, and so are its products with values of 2^-40 to 2^20 and their sums.  Rows
+  // whose largest p is below 2^-64 (kLeastSum: a cap over 54, all scores below -44) or whose sums overflow are slow_row's.
+  const double top = 2 * c2 - 64 < 0 ? 0 : 2 * c2 - 64 < 92 ? 2 * c2 - 64 : 92;
   a.cap.ref = (float)(c2 - top);
-  return dtype == DELTA_BF16 && top <= 60 ? kCappedRef : kCapped;
+  return dtype == DELTA_BF16 ? kCappedRef : kCapped;
 }
 
 size_t part_bytes(int64_t units, int hkv) {

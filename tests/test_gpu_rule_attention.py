@@ -635,3 +635,47 @@ def test_large_caps_beside_tokens_and_heads_of_larger_scores(single, cap, dtype)
     rule = K.ScoreRule(softcap=cap)
     call = b.decode if single else b.prefill
     b.check(call(rule), far_cap(b.want(rule), cap))
+
+
+def saturate(b, sign, cap, scale):
+    """Scores of about sign * cap throughout, values of about `scale`."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(33)
+    u = torch.empty(b.hkv, D, device=DEV).normal_(0, 1, generator=g).sign()
+    b.cache[:, 0] = (u + 0.3 * b.cache[:, 0].float()).to(b.dtype)
+    b.cache[:, 1] *= scale
+    far = torch.linspace(0.1, 0.35, b.T, device=DEV)[:, None, None] * cap  # raw scores from 1.1 to 4 caps
+    b.q = (sign * far * u.repeat_interleave(b.hq // b.hkv, 0) + 0.3 * b.q.float()).to(b.dtype)
+
+
+@pytest.mark.parametrize("power", [-40, -20, -10, 0, 20, 40, 60, 100])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("cap", [30.0, 45.0, 50.0, 64.0, 65.0])
+def test_scores_at_the_cap(cap, sign, power):
+    """Rows whose every score is about -cap or cap, where p is smallest and largest beside a constant reference, with values from
+    small to large: one set of waves, two, eight waves, cut rows, tokens of one key."""
+    dtypes = ["bf16", "fp16"] if -10 <= power <= 0 else ["bf16"]
+    for dtype in dtypes:
+        for hq, hkv, rows, most in BLOCKS:
+            b = Batch(hq, hkv, [(n, min(n, q)) for n, q in rows], dtype, seed=34, stale=0.0)
+            saturate(b, sign, cap, 2.0 ** power)
+            rule = K.ScoreRule(softcap=cap)
+            b.check(b.prefill(rule, max_qo_len=most), b.want(rule))
+        key = [p * 5 // 7 for p in b.pos]
+        rule = K.ScoreRule(softcap=cap, kv_begin=i32(key), kv_end=i32([k + 1 for k in key]))
+        row = [i for i, (_, n) in enumerate(b.rows) for _ in range(n)]
+        page = torch.tensor([b.pages[i][k // PAGE] for i, k in zip(row, key)], device=DEV)
+        v = b.cache[page, 1, torch.tensor(key, device=DEV) % PAGE].repeat_interleave(hq // hkv, 1)
+        assert torch.equal(b.prefill(rule)[0], v)
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_parts_of_a_row_at_both_ends_of_the_cap(sign):
+    """A cut row of which some keys score -64 and others, in other parts, anything: the parts' sums have references of their own."""
+    for power in (-30, 0, 60):
+        b = Batch(28, 4, [(6000, 12), (3000, 5)], seed=35, stale=0.0)
+        saturate(b, -1, 64.0, 2.0 ** power)
+        pages = torch.tensor(b.pages[0][40:90], device=DEV)  # 800 keys
+        b.cache[pages, 0] *= -0.02 if sign < 0 else -1.0
+        rule = K.ScoreRule(softcap=64.0)
+        b.check(b.prefill(rule), b.want(rule))
