@@ -229,3 +229,31 @@ def test_wrappers_refuse_host_tensors():
         K.paged_decode_rule(q, cache, ip, one, one, K.ScoreRule(), max_pages_per_row=1)
     with pytest.raises(ValueError, match="GPU tensors"):
         K.paged_prefill_rule(q, cache, ip, ip, one, one, K.ScoreRule(), max_qo_len=1)
+
+
+@pytest.mark.parametrize("dim,theta,context,scale", [(128, 1e6, 32768, 4.0), (128, 5e5, 8192, 16.0), (64, 1e4, 4096, 16.0), (96, 1e4, 64, 4.0),
+                                                     (128, 1e6, 1 << 20, 2.0)])
+def test_yarn_over_the_pairs(dim, theta, context, scale):
+    """The blend linear in the pair's index between the last pair of at least 32 turns and the first of at most one, as yarn
+    checkpoints have it, found here by counting each pair's turns."""
+    args = dict(rope_theta=theta, rope_scale=scale, old_context_len=float(context), scaling="yarn")
+    got, factor = K.rotary_frequencies(dim, ramp="pairs", **args)
+    plain, _ = K.rotary_frequencies(dim, rope_theta=theta)
+    turns = [context * theta ** (-2 * j / dim) / (2 * math.pi) for j in range(dim)]
+    first, last = max([j for j in range(dim) if turns[j] >= 32], default=0), min([j for j in range(dim) if turns[j] <= 1], default=dim - 1)
+    assert factor == pytest.approx(0.1 * math.log(scale) + 1)
+    for j, (f, g) in enumerate(zip(plain, got)):
+        slow = min(max((j - first) / (last - first), 0), 1)
+        assert g == pytest.approx(f * ((1 - slow) + slow / scale), rel=1e-12)
+    same, _ = K.rotary_frequencies(dim, ramp="turns", **args)
+    assert same == K.rotary_frequencies(dim, **args)[0] and same != got
+
+
+@pytest.mark.parametrize("args,match", [
+    (dict(ramp="index"), "ramp must be"), (dict(ramp="pairs"), "ramp must be"),
+    (dict(ramp="pairs", scaling="llama31", low_freq_factor=1.0, high_freq_factor=4.0, old_context_len=10.0), "ramp must be"),
+    (dict(ramp="pairs", scaling="yarn"), "old_context_len"), (dict(ramp="pairs", scaling="yarn", old_context_len=10.0, rope_theta=1.0), "over 1"),
+])
+def test_ramp_refusals(args, match):
+    with pytest.raises(ValueError, match=match):
+        K.rotary_frequencies(128, **args)
