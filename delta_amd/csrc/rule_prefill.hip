@@ -824,16 +824,21 @@ bool two_sided(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len) {
   return blocks >= kTwoFrom && blocks <= kTwoTo;
 }
 
-// Units of cut rows (a kv head's), at most; 0 where no row can be cut, or none is likely to gain: a row holds its new tokens
-// and what the page table has room for beyond all rows' new ones (12 prompts of 166 tokens of 8 kv heads of 5 30.6 us
-// with the join's launch, 27.4 without).
+// Units of cut rows (a kv head's), at most; 0 where no row can be cut, or, in a call of whole prompts, none would gain: there the
+// page table has room for the new tokens and the rest of the rows' last pages, and no row is longer than max_qo_len (12 prompts of
+// 166 tokens of 8 kv heads of 5 30.6 us with the join's launch, 27.4 without).  Of num_tokens, which may be padded, at
+// most max_qo_len a row are new ones: padding alone does not make a call one of whole prompts.
 int64_t cut_bound(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len, int64_t kv_indices_len, int window) {
   const int BT = kSplitWaves * (32 / G);
   const bool two = two_sided(num_tokens, batch, hkv, G, max_qo_len);
   const int target = two ? kTargetBlocks / 2 : kTargetBlocks, least = two ? kLoneSteps : kMinSteps;
   const int64_t keys = kv_indices_len * kPageSize, span = window > 0 && window + (int64_t)BT < keys ? window + (int64_t)BT : keys;
-  const int64_t steps = ceil_div(span, kKvStep), likely = max_qo_len + keys - num_tokens;
-  if (keys >= num_tokens && row_parts((int)ceil_div(likely < span ? likely : span, kKvStep), least, true) == 1) return 0;
+  const int64_t steps = ceil_div(span, kKvStep), most = (int64_t)batch * max_qo_len;
+  const int64_t room = keys - (num_tokens < most ? num_tokens : most);
+  if (room >= 0 && room <= (int64_t)batch * (kPageSize - 1)) {
+    const int64_t longest = max_qo_len + room < span ? max_qo_len + room : span;
+    if (row_parts((int)ceil_div(longest, kKvStep), least, true) == 1) return 0;
+  }
   if (row_parts((int)steps, least, true) == 1) return 0;
   const int64_t tiles = tiles_bound(num_tokens, batch, max_qo_len, BT);
   if (batch == 1 && tiles * hkv >= target) return 0;  // C >= steps

@@ -257,3 +257,13 @@ def test_yarn_over_the_pairs(dim, theta, context, scale):
 def test_ramp_refusals(args, match):
     with pytest.raises(ValueError, match=match):
         K.rotary_frequencies(128, **args)
+
+
+def test_padded_token_buffers_are_cut_all_the_same(lib):
+    """Few real tokens over a long cache (max_qo_len tokens a row at most) in a buffer of more: what a buffer of the real size needs."""
+    p = lib.delta_paged_prefill_rule_workspace_bytes
+    for batch, most, pages in ((2, 7, 189), (1, 64, 563), (16, 1, 4096), (4, 40, 300)):
+        for tokens in range(batch * most, 40 * pages, 37):
+            assert p(tokens, batch, 12, 2, most, pages, 0) > 0 and p(tokens, batch, 32, 8, most, pages, 0) > 0, (tokens, batch, most, pages)
+    for batch, most, tokens in ((12, 166, 12 * 166), (3, 40, 70), (30, 400, 30 * 400)):  # whole prompts are not
+        assert p(tokens, batch, 40, 8, most, sum(-(-tokens // batch // 16) for _ in range(batch)), 0) == 0
