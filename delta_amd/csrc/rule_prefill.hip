@@ -91,7 +91,7 @@ struct RulePrefillArgs {
   f32x4 *part_acc;  // [unit][hkv][wave][16][64 lanes], the accumulators as the lanes hold them
 };
 
-// Parts of a row of s steps, `longer`: than the call's mean.  A step takes about 1.5 us in a block with a CU of its own and
+// Parts of a row of s steps, `longer`: than 1.5 times the call's mean.  A step takes about 1.5 us in a block with a CU of its own and
 // 2.4 in each of two, a cut's end and join 8 us: three parts gain from 14 steps on.  Two parts of like rows (that fill 2/3 of
 // the CUs uncut) gain nothing: 192 blocks of 32 steps 55 us, 384 of 16 65.
 __host__ __device__ __forceinline__ int row_parts(int s, int C, bool longer) {
@@ -148,28 +148,30 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
   const int lanes = a.batch > 32 ? 64 : a.batch > 8 ? 32 : a.batch > 2 ? 8 : 2;  // that hold rows (sums stop there)
   const RowBounds head = row_bounds(a, lane);  // (of most calls all rows: loaded once)
   auto rows_at = [&](int r0) { return r0 == 0 ? head : row_bounds(a, r0 + lane); };
+  // Whole numbers, up to 2^47 tile steps: the kernel and its join, each block of both, cut alike.
   int C = 0;
-  float mean = 0.f;
+  uint64_t w = 0;
+  uint32_t t = 0;
   if (a.max_cut > 0) {
-    float w = 0.f, t = 0.f;  // (estimates; every block of the launch gets the same ones)
     for (int r0 = 0; r0 < a.batch; r0 += 64) {
       const RowBounds x = rows_at(r0);
-      t += (float)tiles_of(x);
-      w += (float)tiles_of(x) * (float)steps_of(x);
+      t += (uint32_t)tiles_of(x);
+      w += (uint64_t)tiles_of(x) * (uint32_t)steps_of(x);
     }
     for (int off = lanes >> 1; off > 0; off >>= 1) {
-      w += shfl_xor(w, off);
-      t += shfl_xor(t, off);
+      w += (uint64_t)__shfl_xor((unsigned long long)w, off, 64);
+      t += (uint32_t)__shfl_xor((int)t, off, 64);
     }
-    w = readlane(w, 0);
-    mean = w / readlane(t, 0);
-    w *= (float)a.hkv * (1.f / kTargetBlocks);
-    w = a.two ? fmaxf(2.f * w, (float)kLoneSteps) : fmaxf(fmaxf(w, fminf(2.f * w, (float)kLoneSteps)), (float)kMinSteps);
-    C = w > 1e8f ? 100000000 : (int)ceilf(w);
+    w = (uint64_t)(uint32_t)uniform((int)(w >> 32)) << 32 | (uint32_t)uniform((int)w);
+    t = (uint32_t)uniform((int)t);
+    const uint64_t wh = w * (uint32_t)a.hkv, one = (wh + kTargetBlocks - 1) / kTargetBlocks, two = (2 * wh + kTargetBlocks - 1) / kTargetBlocks;
+    const uint64_t lone = kLoneSteps, least = kMinSteps;
+    const uint64_t c = a.two ? max(two, lone) : max(max(one, min(two, lone)), least);
+    C = c > 100000000 ? 100000000 : (int)c;
   }
   auto parts_of = [&](const RowBounds &x) {
     const int s = steps_of(x);
-    return C > 0 ? row_parts(s, C, (float)s > 1.5f * mean) : 1;
+    return C > 0 ? row_parts(s, C, 2 * (uint64_t)(uint32_t)s * t > 3 * w) : 1;
   };
   int base = 0;
   for (int pass = C > 0 ? 0 : 1; pass < 2; ++pass) {

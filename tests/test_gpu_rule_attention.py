@@ -679,3 +679,42 @@ def test_parts_of_a_row_at_both_ends_of_the_cap(sign):
         b.cache[pages, 0] *= -0.02 if sign < 0 else -1.0
         rule = K.ScoreRule(softcap=64.0)
         b.check(b.prefill(rule), b.want(rule))
+
+
+def test_rows_cut_in_a_call_of_very_many_steps():
+    """A row of 400000 pages cut in three beside prompts of 2^24 tile steps and more, the same pages over and over: as the row
+    alone, which is cut in some hundred.
+
+    A part adds up to 34000 sums of 64 keys, each addition off by 2^-24 of the sum: 2^-8.9 of l, le and every element's A at most,
+    beside what the file's head counts (scores to 2^-16: D < 16, cap 30)."""
+    pages = 32768
+    g = torch.Generator(device=DEV)
+    g.manual_seed(36)
+    cache = torch.empty(pages, 2, PAGE, 1, D, dtype=torch.bfloat16, device=DEV).normal_(0, 1, generator=g)
+    cache[:, 1] += 1.0
+    rows = [(400000, 5)] + [(pages, 700)] * 48 + [(1, 1)]
+    kv = indptr([n for n, _ in rows])
+    table = torch.arange(kv[-1], dtype=torch.int32, device=DEV) % pages
+    qo = indptr([n for _, n in rows])
+    q = torch.empty(qo[-1], 8, D, dtype=torch.bfloat16, device=DEV).normal_(0, 1, generator=g)
+    rule = K.ScoreRule(softcap=30.0)
+
+    def call(r0, r1):
+        t = slice(qo[r0], qo[r1])
+        most, n = max(n for _, n in rows[r0:r1]), q[t].shape[0]
+        lse = torch.empty(n, 8, device=DEV)
+        ids = table[kv[r0]:kv[r1]]
+        need = K.prefill_rule_workspace_bytes(n, r1 - r0, 8, 1, most, ids.numel())
+        ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)  # (NaN)
+        o = K.paged_prefill_rule(q[t], cache, i32([x - qo[r0] for x in qo[r0:r1 + 1]]), i32([x - kv[r0] for x in kv[r0:r1 + 1]]), ids,
+                                 i32([PAGE] * (r1 - r0)), rule, max_qo_len=most, lse=lse, workspace=ws)
+        return o.double(), lse.double(), need
+
+    o, lse, need = call(0, len(rows))
+    assert need > 0
+    for r in (0, 7, 49):
+        alone, lone, _ = call(r, r + 1)
+        t = slice(qo[r], qo[r + 1])
+        A, off = alone.abs().max() + 3.0, 2.0 ** -8.9  # (E|v - 1| < 1; one key's |v| is below its own |o| + 3)
+        assert (o[t] - alone).abs().max() <= 2 * (A * (2.0 ** -8 + 2.0 ** -15 + 2 * off) + 2.0 ** -7 * A)
+        assert (lse[t] - lone).abs().max() <= 2 * (2.0 ** -13 + off + 2.0 ** -21 * 60)
