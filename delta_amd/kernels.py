@@ -753,7 +753,8 @@ def paged_decode_rule(q: torch.Tensor, kv_cache: torch.Tensor, kv_indptr: torch.
                       sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                       lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``paged_decode`` under a score rule (``delta_paged_decode_rule``): one query token per row, the last of its cached
-    ones; only the pages of keys that the rule leaves in are read.
+    ones; only the pages of keys that the rule leaves in are read.  At most 16 kv heads, as ``paged_decode``; more of them are
+    ``paged_prefill_rule``'s, with ``max_qo_len=1``.
 
     ``workspace`` (``decode_rule_workspace_bytes``) is allocated for the call where none is given."""
     B, mp = q.shape[0], int(max_pages_per_row)

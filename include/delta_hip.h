@@ -673,7 +673,8 @@ typedef struct delta_score_rule {
 
 /* delta_paged_decode under a score rule: one query token per row, at position kv_len_b - 1.
  * Only the pages that hold keys the rule leaves in are read.  max_pages_per_row is the planned
- * maximum of the rows' pages (a longer row is still covered whole).  workspace:
+ * maximum of the rows' pages (a longer row is still covered whole).  At most 16 kv heads, as
+ * delta_paged_decode; more of them are delta_paged_prefill_rule's, with max_qo_len 1.  workspace:
  * delta_paged_decode_rule_workspace_bytes, 256-byte aligned (0 bytes: may be NULL). */
 size_t delta_paged_decode_rule_workspace_bytes(int batch, int num_qo_heads, int num_kv_heads,
                                                int max_pages_per_row, int window);

@@ -718,3 +718,13 @@ def test_rows_cut_in_a_call_of_very_many_steps():
         A, off = alone.abs().max() + 3.0, 2.0 ** -8.9  # (E|v - 1| < 1; one key's |v| is below its own |o| + 3)
         assert (o[t] - alone).abs().max() <= 2 * (A * (2.0 ** -8 + 2.0 ** -15 + 2 * off) + 2.0 ** -7 * A)
         assert (lse[t] - lone).abs().max() <= 2 * (2.0 ** -13 + off + 2.0 ** -21 * 60)
+
+
+@pytest.mark.parametrize("hq,hkv", [(32, 32), (40, 40), (68, 17)])
+def test_single_tokens_of_many_kv_heads(hq, hkv):
+    """More kv heads than the decode call takes: refused there, a prompt call of one token a row."""
+    b = Batch(hq, hkv, SINGLE, seed=37, q_std=3.0)
+    rule = K.ScoreRule(slopes=slopes(hq), window=700)
+    with pytest.raises(RuntimeError, match="num_kv_heads .* > 16 unsupported"):
+        b.decode(rule)
+    b.check(b.prefill(rule, max_qo_len=1), b.want(rule))

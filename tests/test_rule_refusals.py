@@ -267,3 +267,10 @@ def test_padded_token_buffers_are_cut_all_the_same(lib):
             assert p(tokens, batch, 12, 2, most, pages, 0) > 0 and p(tokens, batch, 32, 8, most, pages, 0) > 0, (tokens, batch, most, pages)
     for batch, most, tokens in ((12, 166, 12 * 166), (3, 40, 70), (30, 400, 30 * 400)):  # whole prompts are not
         assert p(tokens, batch, 40, 8, most, sum(-(-tokens // batch // 16) for _ in range(batch)), 0) == 0
+
+
+@NO_GPU
+@pytest.mark.parametrize("hkv", [17, 32, 40])
+def test_decode_of_more_than_16_kv_heads(hkv):
+    """Refused by the decode call, with every other argument right, and by name."""
+    rejects("delta_paged_decode_rule", decode(hq=hkv, hkv=hkv), f"num_kv_heads {hkv} > 16 unsupported")
