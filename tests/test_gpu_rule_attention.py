@@ -728,3 +728,31 @@ def test_single_tokens_of_many_kv_heads(hq, hkv):
     with pytest.raises(RuntimeError, match="num_kv_heads .* > 16 unsupported"):
         b.decode(rule)
     b.check(b.prefill(rule, max_qo_len=1), b.want(rule))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kind", ["none", "cap", "slopes", "window", "docs"])
+@pytest.mark.parametrize("rows", [[(700, 700)], [(1500, 40)] * 10 + [(6000, 8), (3000, 20)]])
+def test_values_beside_anything_in_a_few_hundred_blocks(rows, kind, what, dtype):
+    """Two sets of waves to a block: rows that are summed again, because of values that they do not see, against 64 bits."""
+    b = Batch(32, 8, rows, dtype, seed=38, q_std=3.0)
+    rng = random.Random(38)
+    for pages, (n, qn) in zip(b.pages, rows):
+        for s in rng.sample(range(n - qn // 2 - 8, n - 1), 5) + [n // 3]:
+            b.cache[pages[s // PAGE], 1, s % PAGE, :, rng.randrange(D)] = what
+    rule = {"none": K.ScoreRule(), "cap": K.ScoreRule(softcap=30.0), "slopes": K.ScoreRule(slopes=slopes(32)),
+            "window": K.ScoreRule(window=30, softcap=20.0), "docs": K.ScoreRule(kv_begin=documents(rows, 38))}[kind]
+    got, want = b.prefill(rule), b.want(rule)
+    assert 0.5 < want[0].isfinite().double().mean() < 1
+    b.check(got, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_single_tokens_by_either_call(kind):
+    for hq, hkv, dtype in ((12, 2, "bf16"), (40, 8, "fp16")):
+        b = Batch(hq, hkv, SINGLE, dtype, seed=39, q_std=4.0)
+        rule = rule_of(kind, hq, SINGLE)
+        want = b.want(rule)
+        b.check(b.prefill(rule), want)
+        b.check(b.decode(rule), want)
