@@ -64,7 +64,6 @@ struct CapArgs {
   float k, xs, xo;  // k = 2 log2 e s / c
   float ref;        // kCappedRef: the reference, log2 units
 };
-constexpr float kLeastSum = 0x1p-64f;  // kCappedRef: of p over a row's keys; below it products with small values are lost
 
 struct RulePrefillArgs {
   const uint16_t *q;
@@ -642,7 +641,7 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
       for (int i = 0; i < 4; ++i) acc[c >> 2][4 * (c & 3) + i] = acc[c >> 2][4 * (c & 3) + i] * f0 + v[i] * f1;
     }
   }
-  // A row that saw no key (l = 0; one that saw any has a weight of 1 or more, with kCappedRef of 2^-93) holds 0 times the
+  // A row that saw no key (l = 0; one that saw any has a weight of 1 or more, with kCappedRef of 2^-64) holds 0 times the
   // values that its wave's other rows saw, NaN where those are NaN or infinity.
   if (l == 0.f) {
 #pragma unroll
@@ -650,8 +649,8 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
   }
-  // Rows whose sums are not finite though their scores are, or too small: slow_row's.
-  bool odd = SM == kCappedRef && l != 0.f && l < kLeastSum;
+  // Rows whose sums are not finite though their scores are: slow_row's.
+  bool odd = false;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -862,12 +861,12 @@ int score_mode(RulePrefillArgs &a, int dtype) {
   a.cap.xs = (float)(2 * c2);
   a.cap.xo = (float)c2;
   if (a.rule.slopes) return kAny;
-  // Scores lie within c2 of 0, so with p = 2^(score - ref) in [2^-64, 2^92] (caps over 54: from 2^-93 on) no maximum is needed:
-  // every p is a normal number of fp32 and bf16, and so are its products with values of 2^-40 to 2^20 and their sums.  Rows
-  // whose largest p is below 2^-64 (kLeastSum: a cap over 54, all scores below -44) or whose sums overflow are slow_row's.
-  const double top = 2 * c2 - 64 < 0 ? 0 : 2 * c2 - 64 < 92 ? 2 * c2 - 64 : 92;
+  // Scores lie within c2 of 0, so with p = 2^(score - ref) in [2^-64, 2^92] (caps up to 54) no maximum is needed: every p is a
+  // normal number of fp32 and bf16, and so are its products with values of 2^-40 to 2^20 and their sums (the matrix unit drops
+  // smaller products; rows whose sums overflow are slow_row's).  Larger caps take the running maximum.
+  const double top = 2 * c2 - 64 > 0 ? 2 * c2 - 64 : 0;
   a.cap.ref = (float)(c2 - top);
-  return dtype == DELTA_BF16 ? kCappedRef : kCapped;
+  return dtype == DELTA_BF16 && top <= 92 ? kCappedRef : kCapped;
 }
 
 size_t part_bytes(int64_t units, int hkv) {

@@ -650,7 +650,7 @@ def saturate(b, sign, cap, scale):
 
 @pytest.mark.parametrize("power", [-40, -20, -10, 0, 20, 40, 60, 100])
 @pytest.mark.parametrize("sign", [-1, 1])
-@pytest.mark.parametrize("cap", [30.0, 45.0, 50.0, 64.0, 65.0])
+@pytest.mark.parametrize("cap", [30.0, 45.0, 50.0, 54.0, 55.0, 64.0, 65.0])
 def test_scores_at_the_cap(cap, sign, power):
     """Rows whose every score is about -cap or cap, where p is smallest and largest beside a constant reference, with values from
     small to large: one set of waves, two, eight waves, cut rows, tokens of one key."""
