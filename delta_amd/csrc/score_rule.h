@@ -56,6 +56,8 @@ __device__ __forceinline__ void cap_scores(float (&x)[N], const RuleArgs &r, flo
     const float k2 = 2.f * kLog2e * ky, c = r.softcap * unit;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+      // (what both branches compute alike stays in each: moved in front of them it takes a register a score)
+      asm volatile("" : "+v"(x[i]));
       const float y = x[i] * ky, near = (x[i] * kx) * tanh_ratio(y * y);
       const float far = fmaf(-2.f * c, __builtin_amdgcn_rcpf(1.f + fast_exp2(x[i] * k2)), c);
       x[i] = fabsf(y) > 0.5f ? far : near;
