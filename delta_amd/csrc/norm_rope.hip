@@ -13,9 +13,9 @@
 // A wave finds the token's row by a ballot over the row bounds, its lane j computes pair j's (cos, sin) and the group
 // takes the pairs of its elements by lane permutes: no LDS and no barrier, every wave runs on its own.
 // What bounds it: memory for prompts (q, k, v read once and written once: 8192 tokens of 32 + 8 heads 46.8 us from and to
-// HBM, 4.3 TB/s where a copy reaches 5.1); for a decode step the chain row bounds -> position and page -> store (one token
-// 3.6 us, 128 tokens 4.4).  At six waves a SIMD the interleaved layout takes 43 us
-// where it took 50, at eight the half layout spills.
+// HBM, 4.3 TB/s where a copy reaches 5.1; 44 us in a replayed graph, part of its inputs still in the caches); for a decode
+// step the chain row bounds -> position and page -> store (one token 3.6 us, 128 tokens 4.4).  At six waves a SIMD the interleaved
+// layout takes 43 us where it took 50, at eight the half layout spills.
 #include "delta_common.h"
 #include "mfma32.h"
 

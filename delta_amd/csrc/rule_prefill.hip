@@ -21,10 +21,11 @@
 //
 // A key that a mask leaves out has no part in the result, whatever it holds.  Its score is replaced and its p is 0, but 0
 // times a V of infinity or NaN is NaN in the product of the whole tile, so a row that ends with sums that are not finite is
-// summed again key by key over its own keys alone (slow_row): nothing for finite caches.
+// summed again key by key over its own keys alone, beside their maximum (slow_row): nothing for finite caches.
 //
-// What bounds it: the card's power for long prompts.  8192 tokens of 32 + 8 heads under a cap take 612 us, 0.90 PFLOP/s (an
-// 8192^3 product 1.22; without a rule 527, slopes 584): the clock falls to 1.86 GHz where matrix and ordinary instructions
+// What bounds it: the card's power for long prompts.  8192 tokens of 32 + 8 heads under a cap of 50 take 612 us in a replayed
+// graph, 0.90 PFLOP/s (an 8192^3 product 1.22; no rule 522, slopes 573; the cap in fp16 671, of 55 to 64 in bf16 662, with slopes 765, of
+// 100 723): the clock falls to 1.86 GHz where matrix and ordinary instructions
 // run together (1.7 the former alone, 2.3 the latter), so fewer idle cycles bring little: waves that interleave one
 // sub-tile's MFMAs with another's softmax took 623-632.  Page ids by vector loads and readlane (scalar loads in flight make
 // every LDS wait a full one): 666 -> 630.  A block's start, four dependent loads, is 3 us, its step 1.5 us alone on a CU and
@@ -123,6 +124,18 @@ __device__ __forceinline__ RowBounds bounds_of_lane(const RowBounds &x, int l) {
                    __builtin_amdgcn_readlane(x.kv_len, l)};
 }
 
+// Over a wave: the 16-lane rows by DPP, the four rows by permlane swaps.
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+  v += (uint32_t)dpp_i<0xB1>((int)v);
+  v += (uint32_t)dpp_i<0x4E>((int)v);
+  v += (uint32_t)dpp_i<0x141>((int)v);
+  v += (uint32_t)dpp_i<0x140>((int)v);
+  auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = a[0] + a[1];
+  auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return (uint32_t)uniform((int)(b[0] + b[1]));
+}
+
 // One block's work: part `part` of `parts` of a row's tile.
 struct Unit {
   RowBounds row;
@@ -144,7 +157,7 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
     const int span = a.rule.window > 0 && a.rule.window < x.kv_len - BT ? a.rule.window + BT : x.kv_len;
     return (span + kKvStep - 1) / kKvStep;
   };
-  const int lanes = a.batch > 32 ? 64 : a.batch > 8 ? 32 : a.batch > 2 ? 8 : 2;  // that hold rows (sums stop there)
+  const int lanes = a.batch > 32 ? 64 : a.batch > 8 ? 32 : a.batch > 2 ? 8 : 2;  // that hold rows (prefix sums stop there)
   const RowBounds head = row_bounds(a, lane);  // (of most calls all rows: loaded once)
   auto rows_at = [&](int r0) { return r0 == 0 ? head : row_bounds(a, r0 + lane); };
   // Whole numbers, up to 2^47 tile steps: the kernel and its join, each block of both, cut alike.
@@ -157,13 +170,11 @@ __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int 
       t += (uint32_t)tiles_of(x);
       w += (uint64_t)tiles_of(x) * (uint32_t)steps_of(x);
     }
-    for (int off = lanes >> 1; off > 0; off >>= 1) {
-      w += (uint64_t)__shfl_xor((unsigned long long)w, off, 64);
-      t += (uint32_t)__shfl_xor((int)t, off, 64);
-    }
-    w = (uint64_t)(uint32_t)uniform((int)(w >> 32)) << 32 | (uint32_t)uniform((int)w);
-    t = (uint32_t)uniform((int)t);
-    const uint64_t wh = w * (uint32_t)a.hkv, one = (wh + kTargetBlocks - 1) / kTargetBlocks, two = (2 * wh + kTargetBlocks - 1) / kTargetBlocks;
+    // (64 lanes' lower 26 bits add up below 2^32)
+    w = ((uint64_t)wave_sum((uint32_t)(w >> 26)) << 26) + wave_sum((uint32_t)w & 0x3ffffffu);
+    t = wave_sum(t);
+    const uint64_t wh = w * (uint32_t)a.hkv, one = (wh + kTargetBlocks - 1) / kTargetBlocks;
+    const uint64_t two = (2 * wh + kTargetBlocks - 1) / kTargetBlocks;
     const uint64_t lone = kLoneSteps, least = kMinSteps;
     const uint64_t c = a.two ? max(two, lone) : max(max(one, min(two, lone)), least);
     C = c > 100000000 ? 100000000 : (int)c;
@@ -227,7 +238,7 @@ __device__ __forceinline__ float add2(uint32_t v, float c) {
   }
 }
 
-// Over a wave: the 16-lane rows by DPP, the four rows by permlane swaps.
+// Likewise the largest or least value.
 template <bool MAX>
 __device__ __forceinline__ int wave_extreme(int v) {
   auto pick = [](int a, int b) { return MAX ? max(a, b) : min(a, b); };
@@ -570,7 +581,9 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
   u32x4 pcar[2 * kSub];
   for (int j0 = s0; s0 < s1 && j0 < s1 + (kLate ? 1 : 0); j0 += kStride) {
     const int j = j0 + side;
-    // Step j's loads have landed when at most the next step's (kLate: four) are pending.
+    // Step j's loads have landed when at most the next step's (kLate: four, and an id load in front of them) are pending.  (kLate:
+    // take_ids below waits for these too, the compiler counting the id load behind loads that it does not see: the second
+    // stage is under way during the barrier alone.)
     if (kLate && j + 1 < s1)
       wait_loads<2 * kPgWave + 1>();
     else
@@ -641,15 +654,8 @@ __global__ void __launch_bounds__(PW * (TWO ? 128 : 64), 2) paged_prefill_rule_k
       for (int i = 0; i < 4; ++i) acc[c >> 2][4 * (c & 3) + i] = acc[c >> 2][4 * (c & 3) + i] * f0 + v[i] * f1;
     }
   }
-  // A row that saw no key (l = 0; one that saw any has a weight of 1 or more, with kCappedRef of 2^-64) holds 0 times the
-  // values that its wave's other rows saw, NaN where those are NaN or infinity.
-  if (l == 0.f) {
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
-  }
-  // Rows whose sums are not finite though their scores are: slow_row's.
+  // Rows whose sums are not finite though their scores are: slow_row's.  (Among them rows without a key, l = 0, whose sums are 0 times
+  // values that their wave's other rows saw: nothing to add up there, and 0.)
   bool odd = false;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
@@ -818,8 +824,9 @@ int64_t tiles_bound(int64_t num_tokens, int batch, int max_qo_len, int BT) {
 // Calls whose blocks have a CU each, or nearly, and are too many to be cut are bound by the longest one's steps: there a
 // block's keys are swept by two sets of four waves, every other step each, whose sums are added at the end (us one set / two;
 // prompts of 8 kv heads of 4: 512 tokens, 128 blocks 19.9 / 19.1, 1024 34 / 29, 1536, 384 blocks 48 / 40, 1800, 452 55 / 52; of 8
-// of 5: 1200, 400 blocks 41 / 38, 1536, 512 48 / 50; 24 rows of 24 tokens over 4096, 192 blocks 110 / 100).  Fewer blocks are
-// better cut (16 tokens over 1600, 8 blocks 20.4 / 22.3), a single step is quicker with one set (9.6 / 11.1).
+// of 5: 1200, 400 blocks 41 / 38, 1536, 512 48 / 50; 24 rows of 24 tokens over 4096, 192 blocks 110 / 100).  The two cross
+// between 450 and 512 blocks, in groups of 4 and 5; others were not measured.  Fewer blocks are better cut (16 tokens over
+// 1600, 8 blocks 20.4 / 22.3), a single step is quicker with one set (9.6 / 11.1).
 bool two_sided(int64_t num_tokens, int batch, int hkv, int G, int max_qo_len) {
   const int64_t blocks = tiles_bound(num_tokens, batch, max_qo_len, kSplitWaves * (32 / G)) * hkv;
   return blocks >= kTwoFrom && blocks <= kTwoTo;
