@@ -146,7 +146,7 @@ struct Unit {
 // Unit (u, h) of the launch, h the kv head: the cut rows' first, then the others' tiles row by row, a row's last tile first
 // (in a causal row it sees the most keys); false past the last one.  Consecutive blocks go to the eight XCDs in turn, so a
 // cut row's blocks are dealt out in groups of eight (part, head) pairs, whose tiles follow one another eight blocks apart: the
-// tiles of a part read its keys from one L2 (groups of 7 over 65548 keys: 48 tokens fetch 139 MB, not 372; 32 tokens 63 us, not
+// tiles of a part read its keys from one L2 (groups of 7 over 65548 keys: 48 tokens fetch 142 MB, not 381; 32 tokens 63 us, not
 // 67).
 __device__ __forceinline__ bool find_unit(const RulePrefillArgs &a, int BT, int u, int h, int lane, Unit *unit) {
   auto tiles_of = [&](const RowBounds &x) {
